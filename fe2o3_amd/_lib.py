@@ -51,6 +51,18 @@ class Fe2o3KernelResources(C.Structure):
     ]
 
 
+class Fe2o3KvCacheV1(C.Structure):
+    """A paged key-value cache: arrays, strides and sizes (112 bytes)."""
+
+    _fields_ = [("k", C.c_void_p), ("k_len", C.c_uint64), ("v", C.c_void_p),
+                ("v_len", C.c_uint64), ("k_scale", C.c_void_p), ("k_scale_len", C.c_uint64),
+                ("v_scale", C.c_void_p), ("v_scale_len", C.c_uint64),
+                ("page_stride", C.c_uint64), ("token_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("format", C.c_uint32), ("pages", C.c_uint32),
+                ("page_size", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32),
+                ("reserved", C.c_uint32)]
+
+
 # ---- exact LDS GEMM lifecycle records (fe2o3_lds_gemm_slice1_*) ----------------------
 
 u8, c_char = C.c_uint8, C.c_char
@@ -288,6 +300,14 @@ SIGNATURES = {
         i32, [vp, u64, vp, u64, vp, u64, vp, u64, vp]),
     "fe2o3_flash_attention_fwd": (
         i32, [vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, u32, u32, u32, u32, i32, f32, vp]),
+    "fe2o3_kv_cache_write": (
+        i32, [C.POINTER(Fe2o3KvCacheV1), vp, u64, vp, u64, vp, u64, u32, u64, u64, vp]),
+    "fe2o3_kv_cache_read": (
+        i32, [C.POINTER(Fe2o3KvCacheV1), vp, u64, vp, u64, vp, u64, vp, u64, u32, u32, u32, u64,
+              u64, vp]),
+    "fe2o3_paged_attention_decode": (
+        i32, [C.POINTER(Fe2o3KvCacheV1), vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64,
+              u32, u32, u32, u32, u64, u32, f32, vp]),
     "fe2o3_moe_top2_route_f32_t8_e4_k2_c4_v1": (
         i32, [vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp]),
     "fe2o3_moe_top2_route": (

@@ -1,0 +1,697 @@
+// paged_attn.hip -- attention of one new token per sequence over a paged
+// key-value cache, for gfx950.
+//
+//   s_j = scale q.k_j,  o = sum_j e^(s_j - m) v_j / sum_j e^(s_j - m)
+//
+// over a sequence's keys, for the `group` query heads that share a KV head at
+// once: K and V are read once for all of them.  With group <= 16 that is 2
+// group flops a byte of bf16 cache, so the bound is memory and the MFMAs'
+// unused rows cost nothing.
+//
+// A wave works on tiles of 32 keys of its own, with no barrier among waves:
+//   * K and V rows come to registers with 16-byte loads, adjacent lanes on
+//     adjacent pieces of a row, a tile (bf16, 128 wide) or more ahead of their
+//     use.  Lane l looks up the page of key l % 32; its offset reaches the
+//     lanes that load the row by a lane permutation, so pages of any size and
+//     place cost the same.
+//   * They pass through LDS of the wave's own as bf16 (codes are widened on the
+//     way, exactly), chunks XOR-permuted per row, into the MFMAs' layouts.
+//   * S^T = K Q^T with v_mfma_f32_16x16x32_bf16: row m of key block b is key
+//     8 (m / 4) + 4 b + m % 4, so that lane l holds query row l % 16 and the
+//     eight keys 8 (l / 16) .. + 7, and the probabilities are the second
+//     operand of O^T += V^T P^T as they stand; V^T comes by transposing LDS
+//     reads.  The softmax is the prompt kernel's: exponentials against a
+//     running reference that is raised only when a tile exceeds it by 2^8.
+//   * An e4m3 cache's K scales multiply the scores, its V scales the
+//     probabilities before they are rounded to bf16 for the MFMA.
+// A workgroup's waves take every fourth tile of a run of tiles and add their
+// sums in LDS when the run or the sequence ends.
+//
+// The tiles of all sequences and KV heads, one behind another, are dealt in
+// equal runs to as many workgroups as the device holds, so that one long
+// sequence fills it as well as many, and mixed lengths leave no tail.  Each
+// workgroup finds its run from the lengths.  A run that a sequence's head
+// does not fit into leaves its sums in the workspace; paged_join_kernel adds
+// those of each head in the order of the keys.
+#include "common.hpp"
+#include "internal.hpp"
+#include "kv_cache.hpp"
+
+namespace {
+
+using namespace fe2o3;
+using kv_cache::View;
+
+constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
+constexpr uint32_t kKeys = 32;              // keys per tile
+constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
+constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
+constexpr uint32_t kGridX = 1u << 22;       // a grid holds fewer than 2^32 threads a dimension
+constexpr uint32_t kBlockRows = 64;         // query heads that one pass over K and V serves
+
+struct Args {
+  View cache;
+  const uint16_t* q;
+  const uint32_t *table, *lengths;
+  uint16_t* o;
+  float* lse;
+  uint4* records;  // workspace: the head that each workgroup's run leaves unfinished,
+  float* stats;    // reference and sum, [workgroup][2][rows][2],
+  float* sums;     // and weighted V, [workgroup][2][rows][head_dim]
+  uint64_t q_stride;
+  uint32_t seqs, q_heads, group, blocks_per_head, rows;  // rows: per block, at most kBlockRows
+  uint32_t table_cols, max_length, window;
+  float scale_log2;
+};
+
+// keys [first, end) of a sequence and its tiles, one at least
+struct Span {
+  uint32_t first, end, tile0, tiles;
+};
+FE2O3_DEVICE Span span_of(const Args& a, uint32_t length) {
+  Span s;
+  s.end = min(length, a.max_length);
+  s.first = a.window != 0u && s.end > a.window ? s.end - a.window : 0u;
+  s.tile0 = s.first / kKeys;
+  s.tiles = max((s.end + kKeys - 1u) / kKeys - s.tile0, 1u);
+  return s;
+}
+
+// LDS rows of 2 D bytes, 16-byte chunk c of row r at c ^ swz(r).  K is read 8
+// rows at once, r % 4 and bit 3 apart, two chunks each; V as 4 rows of 2 chunks
+// for each of the lane groups, whose rows differ in bit 3 within half a wave:
+// either way 16 chunks in 16 different places of 256 bytes.
+template <int D>
+FE2O3_DEVICE uint32_t swz(uint32_t r) {
+  if constexpr (D == 128) return 2u * ((r & 3u) | (r >> 1 & 4u));
+  else return 2u * ((r >> 1 & 1u) | (r >> 2 & 2u));
+}
+
+FE2O3_DEVICE uint64_t shfl64(uint64_t v, uint32_t lane) {
+  const uint32_t lo = (uint32_t)__shfl((int)(uint32_t)v, (int)lane, 64);
+  const uint32_t hi = (uint32_t)__shfl((int)(uint32_t)(v >> 32), (int)lane, 64);
+  return lo | (uint64_t)hi << 32;
+}
+
+FE2O3_DEVICE uint32_t wave_sum_u32(uint32_t v) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) v += (uint32_t)__shfl_xor((int)v, o, 64);
+  return v;
+}
+
+// max / sum over the four lanes of a query row (l, l ^ 16, l ^ 32, l ^ 48)
+FE2O3_DEVICE float row_max(float v) {
+  v = fmaxf(v, __shfl_xor(v, 16, 64));
+  return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+FE2O3_DEVICE float row_sum(float v) {
+  v += __shfl_xor(v, 16, 64);
+  return v + __shfl_xor(v, 32, 64);
+}
+
+FE2O3_DEVICE u32x4_t widen_codes8(uint32_t lo, uint32_t hi) {
+  u32x4_t x;
+  x[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+  x[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+  x[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+  x[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+  return x;
+}
+
+constexpr uint32_t wave_lds(int d) { return kKeys * (uint32_t)d * 4u; }  // K tile, V tile
+constexpr uint32_t scale_lds() { return 2u * kKeys * 4u; }               // per wave
+constexpr uint32_t stat_lds(int rt) { return 16u * rt * 8u; }            // per wave
+constexpr uint32_t query_lds(int d, int rt) { return rt == 1 ? 0u : 32u * rt * d; }
+template <int D, int RT>
+constexpr uint32_t smem_bytes() {
+  return kWaves * (wave_lds(D) + scale_lds() + stat_lds(RT)) + query_lds(D, RT);
+}
+
+// D: head_dim.  RT: query-row tiles of 16.  DEPTH: tiles in flight per wave.
+template <int D, bool E4M3, int RT, int DEPTH>
+struct Decode {
+  static constexpr uint32_t kRowBytes = E4M3 ? D : 2 * D;
+  static constexpr uint32_t kRowLanes = kRowBytes / 16u;      // lanes that load a row
+  static constexpr uint32_t kRowsPerLoad = 64u / kRowLanes;
+  static constexpr int kLoads = kKeys / kRowsPerLoad;         // of K, and of V
+  static constexpr int kDb = D / 16;                          // V^T row blocks
+
+  struct Stage {
+    u32x4_t k[kLoads], v[kLoads];
+    float scale;     // E4M3: lanes below 32 the K scale of key l, the others the V scale
+    uint32_t valid;  // bit per key
+  };
+
+  const Args& a;
+  uint8_t* smem;
+  const uint32_t lane, lr, g, wave;
+  uint8_t* own;
+  float* own_scales;
+
+  FE2O3_DEVICE Decode(const Args& args, uint8_t* lds)
+      : a(args), smem(lds), lane(threadIdx.x & 63u), lr(lane & 15u), g(lane >> 4),
+        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+    own = smem + wave * wave_lds(D);
+    own_scales = (float*)(smem + kWaves * wave_lds(D) + wave * scale_lds());
+  }
+  FE2O3_DEVICE float2* stat(uint32_t w) const {
+    return (float2*)(smem + kWaves * (wave_lds(D) + scale_lds()) + w * stat_lds(RT));
+  }
+
+  // Query rows stay in registers where they are one tile; more would take the
+  // registers of the sums, and lie in LDS for all waves: 16-byte chunk c of row
+  // r at c ^ swz_q(r), which the reads of 8 rows and 2 chunks do not conflict in.
+  static FE2O3_DEVICE uint32_t swz_q(uint32_t r) {
+    return D == 128 ? 2u * (r & 7u) : 2u * (r >> 1 & 3u);
+  }
+  FE2O3_DEVICE uint8_t* queries() const {
+    return smem + kWaves * (wave_lds(D) + scale_lds() + stat_lds(RT));
+  }
+
+  // Keys of tiles [tile, tile + n) of sequence `seq` for block `hb` of the KV
+  // heads' query rows.  whole: the span's every tile, so the output itself;
+  // otherwise the workspace's place `slot` of this workgroup.
+  FE2O3_DEVICE void run(uint32_t seq, uint32_t hb, const Span& sp, uint32_t tile, uint32_t n,
+                        uint32_t slot) {
+    const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
+    const uint32_t row0 = block * kBlockRows;             // of the group
+    const uint32_t rows = min(a.group - row0, (uint32_t)kBlockRows);
+    const uint32_t q_head = head * a.group + row0;
+    const uint32_t* table = a.table + (uint64_t)seq * a.table_cols;
+    const uint8_t* kb = a.cache.k + head * a.cache.head_stride * (E4M3 ? 1u : 2u);
+    const uint8_t* vb = a.cache.v + head * a.cache.head_stride * (E4M3 ? 1u : 2u);
+    const float* sb = (lane < 32u ? a.cache.k_scale : a.cache.v_scale);
+
+    const uint32_t end = sp.tile0 + tile + n;
+    uint32_t t = sp.tile0 + tile + wave;
+    auto inside = [&](uint32_t key) { return key >= sp.first && key < sp.end; };
+    // the table's entry for this lane's key of tile t; none past the run
+    auto entry = [&](uint32_t at) {
+      const uint32_t key = at * kKeys + (lane & 31u);
+      return at < end && inside(key) ? table[a.cache.page.div(key)] : 0xffffffffu;
+    };
+    auto issue = [&](Stage& st, uint32_t at, uint32_t page) {
+      const uint32_t key = at * kKeys + (lane & 31u);
+      const uint32_t place = key - a.cache.page.div(key) * a.cache.page.divisor;
+      const bool ok = page < a.cache.pages;
+      st.valid = (uint32_t)__ballot(ok);
+      // a key that is left out reads slot 0, which every cache has
+      uint64_t off = ok ? page * a.cache.page_stride + place * a.cache.token_stride : 0u;
+      if constexpr (E4M3) {
+        const uint64_t at_scale =
+            ((uint64_t)(ok ? page : 0u) * a.cache.kv_heads + head) * a.cache.page.divisor +
+            (ok ? place : 0u);
+        st.scale = sb[at_scale];
+      } else {
+        off *= 2u;
+      }
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint64_t row = shfl64(off, i * kRowsPerLoad + lane / kRowLanes);
+        st.k[i] = *reinterpret_cast<const u32x4_t*>(kb + row + (lane % kRowLanes) * 16u);
+        st.v[i] = *reinterpret_cast<const u32x4_t*>(vb + row + (lane % kRowLanes) * 16u);
+      }
+    };
+
+    Stage st[DEPTH];
+    uint32_t page[DEPTH];
+#pragma unroll
+    for (int s = 0; s < DEPTH; ++s) page[s] = entry(t + s * kWaves);
+
+    const uint16_t* q = a.q + seq * a.q_stride + (uint64_t)q_head * D;
+    bf16x8_t q_own[D / 32];
+    if constexpr (RT == 1) {
+#pragma unroll
+      for (int ds = 0; ds < D / 32; ++ds) {
+        u32x4_t x = *reinterpret_cast<const u32x4_t*>(q + (lr < rows ? lr : 0u) * D + ds * 32 + g * 8u);
+        if (lr >= rows) x = u32x4_t{0, 0, 0, 0};
+        q_own[ds] = __builtin_bit_cast(bf16x8_t, x);
+      }
+    } else {
+      for (uint32_t i = threadIdx.x; i < 16u * RT * (D / 8u); i += kThreads) {
+        const uint32_t r = i / (D / 8u), c = i % (D / 8u);
+        u32x4_t x = {0, 0, 0, 0};
+        if (r < rows) x = *reinterpret_cast<const u32x4_t*>(q + r * D + c * 8u);
+        *reinterpret_cast<u32x4_t*>(queries() + r * (2u * D) + ((c ^ swz_q(r)) << 4)) = x;
+      }
+      __syncthreads();
+    }
+    auto query = [&](int rt, int ds) {
+      if constexpr (RT == 1) return q_own[ds];
+      else
+        return *reinterpret_cast<const bf16x8_t*>(
+            queries() + (rt * 16u + lr) * (2u * D) + (((4u * ds + g) ^ swz_q(lr)) << 4));
+    };
+    f32x4_t acc[RT][kDb];
+    float m_ref[RT], l_run[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      // as in the prompt kernel: the lowest finite value, against which scores of
+      // -inf alone have exponentials of 0
+      m_ref[rt] = -__FLT_MAX__;
+      l_run[rt] = 0.0f;
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) acc[rt][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+#pragma unroll
+    for (int s = 0; s < DEPTH; ++s)
+      if (t + s * kWaves < end) {
+        issue(st[s], t + s * kWaves, page[s]);
+        page[s] = entry(t + (s + DEPTH) * kWaves);
+      }
+
+    // the stage's tile into the wave's LDS.  Keys that are left out have scores
+    // of -inf whatever K holds, but 0 times their V must be 0: V becomes +0.
+    auto put = [&](Stage& s) {
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        const uint32_t r = i * kRowsPerLoad + lane / kRowLanes, c = lane % kRowLanes;
+        if (s.valid != 0xffffffffu && (s.valid >> r & 1u) == 0u) s.v[i] = u32x4_t{0, 0, 0, 0};
+        uint8_t* at = own + r * (2u * D);
+        if constexpr (E4M3) {
+          const uint32_t c0 = (2u * c ^ swz<D>(r)) << 4, c1 = ((2u * c + 1u) ^ swz<D>(r)) << 4;
+          *reinterpret_cast<u32x4_t*>(at + c0) = widen_codes8(s.k[i][0], s.k[i][1]);
+          *reinterpret_cast<u32x4_t*>(at + c1) = widen_codes8(s.k[i][2], s.k[i][3]);
+          *reinterpret_cast<u32x4_t*>(at + kKeys * 2u * D + c0) = widen_codes8(s.v[i][0], s.v[i][1]);
+          *reinterpret_cast<u32x4_t*>(at + kKeys * 2u * D + c1) = widen_codes8(s.v[i][2], s.v[i][3]);
+        } else {
+          const uint32_t c0 = (c ^ swz<D>(r)) << 4;
+          *reinterpret_cast<u32x4_t*>(at + c0) = s.k[i];
+          *reinterpret_cast<u32x4_t*>(at + kKeys * 2u * D + c0) = s.v[i];
+        }
+      }
+      if constexpr (E4M3)
+        own_scales[lane] = (s.valid >> (lane & 31u) & 1u) != 0u ? s.scale : 0.0f;
+    };
+
+    auto compute = [&](uint32_t valid) {
+      f32x4_t sc[RT][2];
+#pragma unroll
+      for (int ds = 0; ds < D / 32; ++ds) {
+        bf16x8_t kf[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const uint32_t r = 8u * (lr >> 2) + 4u * b + (lr & 3u);
+          kf[b] = *reinterpret_cast<const bf16x8_t*>(own + r * (2u * D) +
+                                                     (((4u * ds + g) ^ swz<D>(r)) << 4));
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const bf16x8_t qf = query(rt, ds);
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            sc[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                kf[b], qf, ds == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[rt][b], 0, 0, 0);
+        }
+      }
+      // scores to the log2 domain; lane's key j (0..7) is 8 g + j
+      float ks[8], vs[8];
+      if constexpr (E4M3) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(own_scales + 8u * g + 4 * h);
+          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(own_scales + 32u + 8u * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            ks[4 * h + e] = x[e] * a.scale_log2;
+            vs[4 * h + e] = y[e];
+          }
+        }
+      }
+      bf16x8_t pf[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = sc[rt][j >> 2][j & 3] * (E4M3 ? ks[j] : a.scale_log2);
+          if (valid != 0xffffffffu && (valid >> (8u * g + j) & 1u) == 0u) x[j] = -INFINITY;
+        }
+        float p[8], psum;
+        auto probabilities = [&] {
+          psum = 0.0f;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            p[j] = __builtin_amdgcn_exp2f(x[j] - m_ref[rt]);
+            psum += p[j];
+          }
+        };
+        probabilities();
+        if (__any(!(psum <= kLazyBound))) {
+          float top = x[0];
+#pragma unroll
+          for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+          const float m_new = fmaxf(m_ref[rt], row_max(top));
+          const float alpha = __builtin_amdgcn_exp2f(m_ref[rt] - m_new);
+          m_ref[rt] = m_new;
+          l_run[rt] *= alpha;
+#pragma unroll
+          for (int db = 0; db < kDb; ++db)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[rt][db][e] *= alpha;
+          probabilities();
+        }
+        l_run[rt] += psum;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) pf[rt][j] = (__bf16)(E4M3 ? p[j] * vs[j] : p[j]);
+      }
+      // O^T += V^T P^T: lane i of group g receives d 16 db + i of keys 8 g .. + 7
+      const uint8_t* vt = own + kKeys * 2u * D;
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) {
+        const uint32_t d = 16u * db + 4u * (lr & 3u);
+        bf16x4_t half[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t r = 8u * g + 4u * h + (lr >> 2);
+          half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+              (lds_bf16x4_t*)(vt + r * (2u * D) + (((d >> 3) ^ swz<D>(r)) << 4) + (d & 7u) * 2u));
+        }
+        const bf16x8_t vf = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[rt], acc[rt][db], 0, 0, 0);
+      }
+    };
+
+    // A wave's LDS operations run in order, so a tile's reads see its writes and
+    // the next tile's writes wait for them; the fences keep the compiler from
+    // reordering them (it sees one lane's addresses).
+    while (t < end) {
+#pragma unroll
+      for (int s = 0; s < DEPTH; ++s) {
+        if (t >= end) break;
+        put(st[s]);
+        const uint32_t valid = st[s].valid;
+        asm volatile("" ::: "memory");
+        if (t + DEPTH * kWaves < end) {
+          issue(st[s], t + DEPTH * kWaves, page[s]);
+          page[s] = entry(t + 2 * DEPTH * kWaves);
+        }
+        compute(valid);
+        asm volatile("" ::: "memory");
+        t += kWaves;
+      }
+    }
+    finish(seq, q_head, rows, n == sp.tiles, slot, acc, m_ref, l_run);
+  }
+
+  // The waves' sums of a run added in wave order, 16 query rows at a time.
+  FE2O3_DEVICE void finish(uint32_t seq, uint32_t q_head, uint32_t rows, bool whole, uint32_t slot,
+                           const f32x4_t (&acc)[RT][kDb], const float (&m_ref)[RT],
+                           const float (&l_run)[RT]) {
+    constexpr uint32_t kStride = D + 4u;  // floats between rows in LDS
+    static_assert(16u * kStride * 4u <= wave_lds(D), "the sums reuse the tiles' LDS");
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const float l = row_sum(l_run[rt]);
+      if (g == 0u) stat(wave)[rt * 16u + lr] = float2{m_ref[rt], l};
+    }
+    const uint64_t part = ((uint64_t)blockIdx.x * 2u + slot) * a.rows;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (rt * 16u >= rows) break;
+      float* mine = (float*)own + lr * kStride + 4u * g;
+#pragma unroll
+      for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(mine + 16 * db) = acc[rt][db];
+      __syncthreads();
+      const uint32_t count = min(rows - rt * 16u, 16u) * (D / 4u);
+      for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+        const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u)), row = rt * 16u + r;
+        float2 s[kWaves];
+        float m = -__FLT_MAX__, l = 0.0f;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+          s[w] = stat(w)[row];
+          m = fmaxf(m, s[w].x);
+        }
+        f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) {
+          const float weight = __builtin_amdgcn_exp2f(s[w].x - m);
+          l += weight * s[w].y;
+          y += weight * *reinterpret_cast<const f32x4_t*>((const float*)(smem + w * wave_lds(D)) +
+                                                          r * kStride + d);
+        }
+        if (whole) {
+          const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: +0
+          const uint64_t out = (uint64_t)seq * a.q_heads + q_head + row;
+          *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
+              u32x2_t{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+          if (a.lse != nullptr && d == 0u)
+            a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+        } else {
+          *reinterpret_cast<f32x4_t*>(a.sums + (part + row) * D + d) = y;
+          if (d == 0u) *reinterpret_cast<float2*>(a.stats + (part + row) * 2u) = float2{m, l};
+        }
+      }
+      __syncthreads();
+    }
+  }
+};
+
+// One workgroup per sequence and block of query rows, for calls whose
+// sequences are too short to be worth a join.
+template <int D, bool E4M3, int RT, int DEPTH>
+__global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_whole_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
+  const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
+  if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
+  const Span sp = span_of(a, a.lengths[seq]);
+  Decode<D, E4M3, RT, DEPTH>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+}
+
+// The workgroup's run of the list of all tiles (sequence, then block of query
+// rows, then tile), which is a multiple of kWaves tiles long.
+template <int D, bool E4M3, int RT, int DEPTH>
+__global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_split_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t lane = threadIdx.x & 63u, blocks = a.cache.kv_heads * a.blocks_per_head;
+  uint32_t mine = 0;
+  for (uint32_t s = lane; s < a.seqs; s += 64u) mine += span_of(a, a.lengths[s]).tiles;
+  const uint32_t total = wave_sum_u32(mine) * blocks;
+  const uint32_t run = ((total - 1u) / gridDim.x / kWaves + 1u) * kWaves;
+  uint32_t at = blockIdx.x * run;  // below (total / grid + 4) * grid: the host keeps it in 32 bits
+  const uint32_t end = min(at + run, total);
+  uint4 record = {0u, 0u, 0u, 0u};
+  if (at < total) {
+    // the sequence that `at` falls into: tiles before it, `skipped`
+    uint32_t seq = 0, skipped = 0;
+    for (uint32_t base = 0;; base += 64u) {
+      const uint32_t s = base + lane;
+      uint32_t scan = s < a.seqs ? span_of(a, a.lengths[s]).tiles : 0u;
+#pragma unroll
+      for (uint32_t o = 1u; o < 64u; o <<= 1) {
+        const uint32_t below = (uint32_t)__shfl_up((int)scan, o, 64);
+        if (lane >= o) scan += below;
+      }
+      const uint32_t before = (uint32_t)__popcll(
+          __ballot(s < a.seqs && (skipped + scan) * blocks <= at));
+      if (before < 64u) {
+        if (before != 0u) skipped += (uint32_t)__shfl((int)scan, (int)before - 1, 64);
+        seq = base + before;
+        break;
+      }
+      skipped += (uint32_t)__shfl((int)scan, 63, 64);
+    }
+    seq = __builtin_amdgcn_readfirstlane(seq);
+    uint32_t rest = __builtin_amdgcn_readfirstlane(at - skipped * blocks);
+    Span sp = span_of(a, a.lengths[seq]);
+    uint32_t hb = rest / sp.tiles, tile = rest - hb * sp.tiles;
+    Decode<D, E4M3, RT, DEPTH> decode(a, smem);
+    while (true) {
+      const uint32_t n = min(sp.tiles - tile, end - at);
+      // begun before this run: place 0; begun in it and going on: place 1
+      decode.run(seq, hb, sp, tile, n, tile == 0u ? 1u : 0u);
+      at += n;
+      if (at >= end) {
+        const uint32_t left = sp.tiles - tile - n;
+        if (tile == 0u && left != 0u)  // as many runs as what is left reaches into
+          record = uint4{1u, (left - 1u) / run + 1u, seq, hb};
+        break;
+      }
+      tile = 0u;
+      if (++hb == blocks) {
+        hb = 0u;
+        sp = span_of(a, a.lengths[++seq]);
+      }
+    }
+  }
+  if (threadIdx.x == 0u) a.records[blockIdx.x] = record;
+}
+
+// Query row blockIdx.y of the head that run blockIdx.x began and did not
+// finish: place 1 of that run and place 0 of the runs that follow, in order.
+template <int D>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(Args a) {
+  __shared__ f32x4_t part_sum[kThreads];
+  const uint4 record = a.records[blockIdx.x];
+  if (record.x == 0u) return;
+  const uint32_t parts = record.y + 1u, seq = record.z, hb = record.w;
+  const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
+  const uint32_t row = blockIdx.y;
+  if (block * kBlockRows + row >= a.group) return;
+  auto at = [&](uint32_t i) {
+    return ((uint64_t)(blockIdx.x + i) * 2u + (i == 0u ? 1u : 0u)) * a.rows + row;
+  };
+  float m = -__FLT_MAX__;
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t i = lane; i < parts; i += 64u) m = fmaxf(m, a.stats[at(i) * 2u]);
+  m = wave_max(m);
+  // D / 4 threads cover a row; the others take every kWays-th part
+  constexpr uint32_t kQuads = D / 4u, kWays = kThreads / kQuads;
+  const uint32_t way = threadIdx.x / kQuads, d = 4u * (threadIdx.x % kQuads);
+  f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+  float l = 0.0f;
+#pragma unroll 4
+  for (uint32_t i = way; i < parts; i += kWays) {
+    const uint64_t p = at(i);
+    const float2 s = *reinterpret_cast<const float2*>(a.stats + p * 2u);
+    const float weight = __builtin_amdgcn_exp2f(s.x - m);
+    l += weight * s.y;
+    y += weight * *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d);
+  }
+  __shared__ float part_l[kWays];
+  part_sum[threadIdx.x] = y;
+  if (d == 0u) part_l[way] = l;
+  __syncthreads();
+  if (way != 0u) return;
+  l = 0.0f;
+  y = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (uint32_t w = 0; w < kWays; ++w) {
+    y += part_sum[w * kQuads + threadIdx.x];
+    l += part_l[w];
+  }
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const uint64_t out = (uint64_t)seq * a.q_heads + head * a.group + block * kBlockRows + row;
+  *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
+      u32x2_t{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+  if (a.lse != nullptr && d == 0u)
+    a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+}
+
+template <int D, bool E4M3, int RT>
+int32_t launch(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
+  constexpr int kDepth = 1;
+  constexpr uint32_t kSmem = smem_bytes<D, RT>();
+  const auto whole_fn = paged_whole_kernel<D, E4M3, RT, kDepth>;
+  const auto split_fn = paged_split_kernel<D, E4M3, RT, kDepth>;
+  static const int32_t lds_rc = fe2o3_host::set_dynamic_lds(
+      {(const void*)whole_fn, (const void*)split_fn}, (int)kSmem);
+  if (lds_rc != FE2O3_OK) return lds_rc;
+  if (whole) {
+    const dim3 grid(workgroups < kGridX ? workgroups : kGridX, (workgroups - 1u) / kGridX + 1u);
+    whole_fn<<<grid, kThreads, kSmem, s>>>(a);
+    return fe2o3_host::after_launch();
+  }
+  split_fn<<<workgroups, kThreads, kSmem, s>>>(a);
+  const int32_t rc = fe2o3_host::after_launch();
+  if (rc != FE2O3_OK) return rc;
+  paged_join_kernel<D><<<dim3(workgroups, a.rows), kThreads, 0, s>>>(a);
+  return fe2o3_host::after_launch();
+}
+
+template <int D, bool E4M3>
+int32_t launch_rows(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
+  if (a.rows <= 16u) return launch<D, E4M3, 1>(a, whole, workgroups, s);
+  if (a.rows <= 32u) return launch<D, E4M3, 2>(a, whole, workgroups, s);
+  return launch<D, E4M3, 4>(a, whole, workgroups, s);
+}
+
+#define FE2O3_PAGED(D, F, RT)                                                                  \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F "," #RT ">", (const void*)paged_whole_kernel<D, F, RT, 1>, kThreads, smem_bytes<D, RT>()}), \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_split_kernel<" #D "," #F "," #RT ">", (const void*)paged_split_kernel<D, F, RT, 1>, kThreads, smem_bytes<D, RT>()})
+const fe2o3_host::KernelRegistrar kRegistered[] = {
+    FE2O3_PAGED(64, false, 1), FE2O3_PAGED(64, false, 2), FE2O3_PAGED(64, false, 4),
+    FE2O3_PAGED(64, true, 1), FE2O3_PAGED(64, true, 2), FE2O3_PAGED(64, true, 4),
+    FE2O3_PAGED(128, false, 1), FE2O3_PAGED(128, false, 2), FE2O3_PAGED(128, false, 4),
+    FE2O3_PAGED(128, true, 1), FE2O3_PAGED(128, true, 2), FE2O3_PAGED(128, true, 4),
+    fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<64>", (const void*)paged_join_kernel<64>, kThreads, 0}),
+    fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<128>", (const void*)paged_join_kernel<128>, kThreads, 0})};
+#undef FE2O3_PAGED
+
+}  // namespace
+
+extern "C" int32_t fe2o3_paged_attention_decode(
+    const Fe2o3KvCacheV1* cache, const uint16_t* q, uint64_t q_len, const uint32_t* block_table,
+    uint64_t table_len, const uint32_t* lengths, uint64_t lengths_len, uint16_t* o, uint64_t o_len,
+    float* lse, uint64_t lse_len, void* workspace, uint64_t workspace_bytes, uint32_t seqs,
+    uint32_t q_heads, uint32_t table_cols, uint32_t max_length, uint64_t q_stride,
+    uint32_t window, float scale, void* stream) {
+  FE2O3_ENTRY("fe2o3_paged_attention_decode");
+  Args a;
+  int32_t rc = kv_cache::check(cache, &a.cache);
+  if (rc != FE2O3_OK) return rc;
+  const uint32_t d = cache->head_dim, kv_heads = cache->kv_heads;
+  if (d != 64u && d != 128u) return FE2O3_ERR_SHAPE;
+  if (q_heads == 0u || q_heads % kv_heads != 0u) return FE2O3_ERR_SHAPE;
+  if (max_length >= (1u << 31) || max_length > (uint64_t)table_cols * cache->page_size)
+    return FE2O3_ERR_SHAPE;
+  if (!(scale > 0.0f) || !__builtin_isfinite(scale)) return FE2O3_ERR_SHAPE;
+  const uint32_t group = q_heads / kv_heads;
+  const uint32_t blocks_per_head = (group - 1u) / kBlockRows + 1u;
+  const uint64_t row = (uint64_t)q_heads * d;
+  // every product below is of factors that keep it under 2^64
+  const uint64_t blocks = (uint64_t)kv_heads * blocks_per_head;  // at most q_heads
+  const uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys + 1u;  // a window may add one
+  if (blocks * tiles >= (UINT64_C(1) << 31) || seqs * (blocks * tiles) >= (UINT64_C(1) << 31))
+    return FE2O3_ERR_SHAPE;
+  if (seqs > 1u && q_stride < row) return FE2O3_ERR_STRIDE;
+  if (seqs == 0u) return FE2O3_OK;
+  uint64_t extent = row, bytes;
+  if (!kv_cache::reach(seqs, q_stride, &extent) || !kv_cache::mul_ok(extent, 2u, &bytes))
+    return FE2O3_ERR_OVERFLOW;
+  const uint64_t heads = (uint64_t)seqs * q_heads;
+  uint64_t o_need;
+  if (!kv_cache::mul_ok(heads, d, &o_need)) return FE2O3_ERR_OVERFLOW;
+  if (q_len < extent || table_len != (uint64_t)seqs * table_cols || lengths_len != seqs ||
+      o_len != o_need || (lse != nullptr && lse_len != heads))
+    return FE2O3_ERR_LENGTH;
+  if (!q || (table_len != 0u && !block_table) || !lengths || !o || !workspace)
+    return FE2O3_ERR_NULL;
+  if (!kv_cache::rows_aligned(a.cache, cache->format, 16u) ||
+      (((uintptr_t)q | (uintptr_t)o | (uintptr_t)workspace) & 15u) != 0u ||
+      (seqs > 1u && q_stride % 8u != 0u) || ((uintptr_t)lse & 3u) != 0u)
+    return FE2O3_ERR_ALIGNMENT;
+  if (workspace_bytes < FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES(q_heads, kv_heads, d))
+    return FE2O3_ERR_WORKSPACE;
+  tile_plan::Topology topo;
+  rc = fe2o3_host::device_topology(&topo);
+  if (rc != FE2O3_OK) return rc;
+  a.q = q;
+  a.table = block_table;
+  a.lengths = lengths;
+  a.o = o;
+  a.lse = lse;
+  a.rows = group < kBlockRows ? group : kBlockRows;
+  a.records = (uint4*)workspace;
+  a.sums = (float*)((uint8_t*)workspace + 16u * kMaxWorkgroups);
+  a.stats = a.sums + (uint64_t)kMaxWorkgroups * 2u * a.rows * d;
+  a.q_stride = q_stride;
+  a.seqs = seqs;
+  a.q_heads = q_heads;
+  a.group = group;
+  a.blocks_per_head = blocks_per_head;
+  a.table_cols = table_cols;
+  a.max_length = max_length;
+  a.window = window;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  const uint64_t units = seqs * blocks;
+  const bool whole = tiles <= 2u * kWaves;
+  uint32_t workgroups = (uint32_t)units;
+  if (!whole) {
+    const uint64_t most = units * ((tiles + kWaves - 1u) / kWaves);
+    const uint32_t slots = 2u * topo.cus < kMaxWorkgroups ? 2u * topo.cus : kMaxWorkgroups;
+    workgroups = (uint32_t)(most < slots ? most : slots);
+  }
+  hipStream_t s = (hipStream_t)stream;
+  const bool e4m3 = cache->format == FE2O3_KV_E4M3;
+  if (d == 64u)
+    return e4m3 ? launch_rows<64, true>(a, whole, workgroups, s)
+                : launch_rows<64, false>(a, whole, workgroups, s);
+  return e4m3 ? launch_rows<128, true>(a, whole, workgroups, s)
+              : launch_rows<128, false>(a, whole, workgroups, s);
+}

@@ -291,6 +291,213 @@ def moe_routing_check(routing: dict, tokens: int, experts: int, capacity: int,
           *_ps(record), stream=stream, sync=sync)
 
 
+# ---- paged key-value cache ---------------------------------------------------------------
+
+KV_BF16, KV_E4M3 = 0, 1
+KV_NO_SLOT = 0xFFFFFFFF
+PAGED_ATTENTION_MAX_WORKGROUPS = 1024
+
+# what an array of each kind may hold: numpy types of a DeviceBuffer and the
+# names of a tensor's
+_BF16, _CODES, _INDEX, _FLOAT, _BYTES = "bf16", "e4m3", "u32", "f32", "bytes"
+_HOLDS = {
+    _BF16: (("uint16",), ("torch.bfloat16",)),
+    _CODES: (("uint8",), ("torch.uint8", "torch.float8_e4m3fn")),
+    _INDEX: (("uint32",), ("torch.int32", "torch.uint32")),
+    _FLOAT: (("float32",), ("torch.float32",)),
+    _BYTES: (("uint8",), ("torch.uint8", "torch.int8")),
+}
+_kinds: dict = {}  # element type -> the kinds it may stand for
+
+
+def _kinds_of(dtype, column):
+    found = _kinds.get(dtype)
+    if found is None:
+        found = _kinds[dtype] = frozenset(k for k, v in _HOLDS.items() if str(dtype) in v[column])
+    return found
+
+
+def _array(x, kind, name, dense=True):
+    """(pointer, elements) of a DeviceBuffer or a device tensor that holds
+    `kind`.  A tensor's last dimension is contiguous; dense: all of them are,
+    otherwise the elements are the extent its strides span."""
+    if isinstance(x, DeviceBuffer):
+        if kind not in _kinds_of(x.dtype, 0):
+            raise TypeError(f"{name} must hold {kind}, not {x.dtype}")
+        return x.ptr, x.count
+    if not hasattr(x, "data_ptr"):
+        raise TypeError(f"{name} must be a DeviceBuffer or a device tensor")
+    if kind not in _kinds_of(x.dtype, 1):
+        raise TypeError(f"{name} must hold {kind}, not {x.dtype}")
+    if not x.is_cuda:
+        raise TypeError(f"{name} must be in device memory")
+    if x.is_contiguous():
+        return x.data_ptr(), x.numel()
+    if dense:
+        raise ValueError(f"{name} must be contiguous")
+    count = x.numel()
+    if count:
+        if x.shape[-1] > 1 and x.stride(-1) != 1:
+            raise ValueError(f"the last dimension of {name} must be contiguous")
+        count = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+    return x.data_ptr(), count
+
+
+def _device_of(x):
+    return x.ctx.device if isinstance(x, DeviceBuffer) else x.get_device()
+
+
+def _check_device(*arrays):
+    """Every array on the current device, where the launch goes."""
+    current = C.c_int32()
+    check(_lib.lib().fe2o3_rt_get_device(C.byref(current)), "get device")
+    for x in arrays:
+        if x is not None and _device_of(x) != current.value:
+            raise ValueError(f"array on device {_device_of(x)}, the current one is {current.value}")
+
+
+def _strides(x):
+    """A tensor's strides; 0 for a dimension of one, whose stride says nothing."""
+    return tuple(s if n > 1 else 0 for n, s in zip(x.shape, x.stride()))
+
+
+def _shape_of(x, dims, name):
+    shape = getattr(x, "shape", None)
+    if shape is not None and len(shape) != dims:
+        raise ValueError(f"{name} must have {dims} dimensions, not {len(shape)}")
+    return shape
+
+
+class KvCache:
+    """A paged key-value cache: K and V rows in slots page * page_size + place,
+    bf16, or e4m3 codes with scales [pages, kv_heads, page_size].
+
+    k and v are device tensors [pages, page_size, kv_heads, head_dim] of any
+    strides but the last (a cache laid out [pages, kv_heads, page_size,
+    head_dim] is passed as its transpose(1, 2)), or DeviceBuffers with `shape`
+    given that way and `strides` (page, token, head; dense by default) in
+    elements.  K and V have the same strides.  The record holds the arrays, not
+    copies of them.
+    """
+
+    def __init__(self, k, v, k_scale=None, v_scale=None, *, shape=None, strides=None):
+        k_shape = _shape_of(k, 4, "k")
+        if k_shape is not None:
+            strides = _strides(k)
+            if k_shape != v.shape or strides != _strides(v):
+                raise ValueError("k and v must have the same shape and strides")
+            shape, strides = k_shape, strides[:3]
+        elif shape is None:
+            raise ValueError("a cache of DeviceBuffers needs its shape")
+        pages, page_size, kv_heads, head_dim = (int(n) for n in shape)
+        if strides is None:
+            strides = (page_size * kv_heads * head_dim, kv_heads * head_dim, head_dim)
+        self.format = KV_BF16 if k_scale is None else KV_E4M3
+        if (k_scale is None) != (v_scale is None):
+            raise ValueError("k_scale and v_scale go together")
+        for scale in (k_scale, v_scale):
+            found = None if scale is None else _shape_of(scale, 3, "scales")
+            if found is not None and tuple(found) != (pages, kv_heads, page_size):
+                raise ValueError(f"scales of {tuple(found)}, not {(pages, kv_heads, page_size)}")
+        kind = _BF16 if k_scale is None else _CODES
+        scales = ((None, 0), (None, 0)) if k_scale is None else (
+            _array(k_scale, _FLOAT, "k_scale"), _array(v_scale, _FLOAT, "v_scale"))
+        self.arrays = (k, v, k_scale, v_scale)
+        self.shape = (pages, page_size, kv_heads, head_dim)
+        self.record = _lib.Fe2o3KvCacheV1(
+            *_array(k, kind, "k", dense=False), *_array(v, kind, "v", dense=False),
+            *scales[0], *scales[1], *strides, self.format, *self.shape, 0)
+
+
+def _rows(cache, k, v, strides):
+    """(token, head) strides of K and V rows, and their tokens where they say so."""
+    shape = _shape_of(k, 3, "k")
+    _, _, kv_heads, head_dim = cache.shape
+    if shape is None:
+        return strides or (kv_heads * head_dim, head_dim), None
+    found = _strides(k)
+    if shape != v.shape or found != _strides(v):
+        raise ValueError("k and v must have the same shape and strides")
+    if tuple(shape[1:]) != (kv_heads, head_dim):
+        raise ValueError(f"rows of {tuple(shape[1:])} for a cache of {(kv_heads, head_dim)}")
+    return found[:2], shape[0]
+
+
+def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sync=True) -> None:
+    """Writes rows k, v (bf16 [tokens, kv_heads, head_dim]; DeviceBuffers with
+    `strides` (token, head)) into slots[t] of the cache, quantised where it is
+    e4m3.  A slot out of range (KV_NO_SLOT) is skipped; each slot at most once
+    a call (fe2o3_kv_cache_write)."""
+    (token_stride, head_stride), rows = _rows(cache, k, v, strides)
+    _check_device(*cache.arrays, k, v, slots)
+    slots_ptr, tokens = _array(slots, _INDEX, "slots")
+    if rows is not None and rows != tokens:
+        raise ValueError(f"{rows} rows and {tokens} slots")
+    _call("fe2o3_kv_cache_write", C.byref(cache.record), *_array(k, _BF16, "k", dense=False),
+          *_array(v, _BF16, "v", dense=False), slots_ptr, tokens, tokens, token_stride,
+          head_stride, stream=stream, sync=sync)
+
+
+def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, tokens=None,
+                  stream=None, sync=True) -> None:
+    """Reads cached rows into k, v (bf16 [tokens, kv_heads, head_dim]): sequence
+    s, on pages block_table[s], to rows starts[s] .. starts[s + 1] - 1.  Rows in
+    no sequence keep their values (fe2o3_kv_cache_read).  DeviceBuffers take
+    `strides` (token, head) and `tokens`."""
+    (token_stride, head_stride), rows = _rows(cache, k, v, strides)
+    _check_device(*cache.arrays, block_table, starts, k, v)
+    starts_ptr, starts_len = _array(starts, _INDEX, "starts")
+    table_ptr, table_len = _array(block_table, _INDEX, "block_table")
+    seqs = starts_len - 1
+    if seqs < 0:
+        raise ValueError("starts must hold one value more than there are sequences")
+    if rows is None:
+        rows = k.count // (cache.shape[2] * cache.shape[3]) if tokens is None else tokens
+    _call("fe2o3_kv_cache_read", C.byref(cache.record), table_ptr, table_len, starts_ptr,
+          starts_len, *_array(k, _BF16, "k", dense=False), *_array(v, _BF16, "v", dense=False),
+          seqs, table_len // seqs if seqs else 0, rows, token_stride, head_stride,
+          stream=stream, sync=sync)
+
+
+def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int) -> int:
+    """FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES: scratch of one decode call."""
+    rows = min(q_heads // kv_heads, 64)
+    return PAGED_ATTENTION_MAX_WORKGROUPS * (16 + 8 * (head_dim + 2) * rows)
+
+
+def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, workspace, *,
+                           max_length: int, scale: float, window: int = 0, q_heads=None,
+                           q_stride=None, stream=None, sync=True) -> None:
+    """Attention of one new token per sequence over its cached keys: q and out
+    bf16 [seqs, q_heads, head_dim], lse f32 [seqs, q_heads] or None, block_table
+    [seqs, cols], lengths [seqs], at most max_length each; window > 0 keeps the
+    last `window` keys (fe2o3_paged_attention_decode).  workspace: device bytes,
+    paged_attention_workspace_bytes at least, of no use to another call that may
+    overlap.  DeviceBuffers take q_heads, and q_stride between sequences."""
+    _check_device(*cache.arrays, q, block_table, lengths, out, lse, workspace)
+    head_dim = cache.shape[3]
+    q_shape = _shape_of(q, 3, "q")
+    if q_shape is not None:
+        q_heads, q_stride = q_shape[1], q.stride(0)
+        if q_shape[2] != head_dim or _strides(q)[1] not in (0, head_dim):
+            raise ValueError("q must be [seqs, q_heads, head_dim] with a sequence's heads dense")
+    elif q_heads is None:
+        raise ValueError("q in a DeviceBuffer needs q_heads")
+    elif q_stride is None:
+        q_stride = q_heads * head_dim
+    lengths_ptr, seqs = _array(lengths, _INDEX, "lengths")
+    if q_shape is not None and q_shape[0] != seqs:
+        raise ValueError(f"{q_shape[0]} rows of q and {seqs} lengths")
+    table_ptr, table_len = _array(block_table, _INDEX, "block_table")
+    _call("fe2o3_paged_attention_decode", C.byref(cache.record),
+          *_array(q, _BF16, "q", dense=False), table_ptr, table_len, lengths_ptr, seqs,
+          *_array(out, _BF16, "out"),
+          *((None, 0) if lse is None else _array(lse, _FLOAT, "lse")),
+          *_array(workspace, _BYTES, "workspace"), seqs, q_heads,
+          table_len // seqs if seqs else 0, max_length, q_stride, window, scale,
+          stream=stream, sync=sync)
+
+
 def kernel_resources(entry: str) -> list[dict]:
     """Every kernel behind C-ABI entry point `entry` with its launch facts and
     the resources the runtime reports for the loaded code object

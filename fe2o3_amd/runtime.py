@@ -85,9 +85,14 @@ class Event:
 
 
 def stream_handle(stream) -> int | None:
+    """The HIP stream of a Stream or of a torch.cuda.Stream; None (the null
+    stream) of None."""
     if stream is None:
         return None
-    return stream.handle
+    if isinstance(stream, Stream):
+        return stream.handle
+    foreign = getattr(stream, "cuda_stream", None)
+    return stream.handle if foreign is None else foreign
 
 
 class DeviceBuffer:

@@ -319,6 +319,126 @@ int32_t fe2o3_flash_attention_fwd(const uint16_t *q, uint64_t q_len,
                                   uint32_t head_dim, int32_t causal,
                                   float scale, void *stream);
 
+/* ---- paged key-value cache -------------------------------------------------------------
+ * Not in the reference, whose attention example has no decoding step.  The
+ * cache holds pages of page_size tokens; a slot is page * page_size + the
+ * token's place in the page.  Row (page, place, head) of K and of V is
+ * head_dim contiguous elements at
+ *   page * page_stride + place * token_stride + head * head_stride
+ * (elements, the same strides for both arrays): [pages, page_size, kv_heads,
+ * head_dim], [pages, kv_heads, page_size, head_dim], and either with K and V
+ * beside each other in one allocation.
+ *
+ * FE2O3_KV_BF16 keeps the rows as they are.  FE2O3_KV_E4M3 keeps OCP E4M3FN
+ * codes and for each row a scale, in k_scale and v_scale [pages, kv_heads,
+ * page_size]: scale = max(max |x|, 2^-126) / 448, code = e4m3_rne(x / scale)
+ * (fe2o3_fp8_scale_from_amax and fe2o3_quantize_e4m3 on each row).  A NaN takes
+ * no part in the maximum and stays a NaN; a row with an infinity has an
+ * infinite scale and reads back as NaN.
+ *
+ * The record is checked in this order: NULL record FE2O3_ERR_NULL; another
+ * format, a size of 0, or 2^31 slots or more FE2O3_ERR_SHAPE; strides with
+ * which rows share elements FE2O3_ERR_STRIDE (FE2O3_ERR_OVERFLOW where an
+ * extent passes 64 bits); k_len or v_len short of the extent, or scale lengths
+ * other than pages * kv_heads * page_size (0 for bf16) FE2O3_ERR_LENGTH; NULL
+ * arrays FE2O3_ERR_NULL; bf16 at an odd address or scales off their 4 bytes
+ * FE2O3_ERR_ALIGNMENT.
+ *
+ * Slots, block tables, starts and lengths are device data that the host
+ * cannot validate.  No value in them leads an access outside the arrays; what
+ * each entry point does with one out of range stands with it.  They are u32:
+ * -1 of an int32 array is out of every range. */
+#define FE2O3_KV_BF16 0u
+#define FE2O3_KV_E4M3 1u
+#define FE2O3_KV_NO_SLOT 0xffffffffu
+
+typedef struct Fe2o3KvCacheV1 {
+  void *k; /* uint16_t bf16 bits or uint8_t codes */
+  uint64_t k_len;
+  void *v;
+  uint64_t v_len;
+  float *k_scale; /* NULL for bf16 */
+  uint64_t k_scale_len;
+  float *v_scale;
+  uint64_t v_scale_len;
+  uint64_t page_stride, token_stride, head_stride;
+  uint32_t format, pages, page_size, kv_heads, head_dim, reserved;
+} Fe2o3KvCacheV1;
+
+/* Writes rows K[t, h, :] and V[t, h, :] (bf16, both at t * token_stride + h *
+ * head_stride elements of their arrays: columns of a fused projection's
+ * output, or [heads, seq, head_dim]) into slot slots[t], t < tokens, for every
+ * h < kv_heads.  A slot out of range (FE2O3_KV_NO_SLOT: a padded row) is
+ * skipped.  Two tokens of a call that name one slot leave it unspecified.
+ * Everything else in the cache keeps its bytes.  k_len and v_len cover the
+ * rows' extent; slots_len = tokens.  Errors after the cache's: kv_heads *
+ * tokens of 2^31 or more FE2O3_ERR_SHAPE, FE2O3_ERR_STRIDE, FE2O3_ERR_OVERFLOW
+ * and FE2O3_ERR_LENGTH as for the cache, FE2O3_ERR_NULL.  Any alignment;
+ * 16-byte accesses where head_dim is a multiple of 8 and rows allow it. */
+int32_t fe2o3_kv_cache_write(const Fe2o3KvCacheV1 *cache, const uint16_t *k, uint64_t k_len,
+                             const uint16_t *v, uint64_t v_len, const uint32_t *slots,
+                             uint64_t slots_len, uint32_t tokens, uint64_t token_stride,
+                             uint64_t head_stride, void *stream);
+
+/* Reads cached rows back as bf16 (E4M3: the f32 product code * scale, RNE to
+ * bf16), several sequences packed one behind another: output row t with
+ * starts[s] <= t < starts[s + 1] is token t - starts[s] of sequence s, whose
+ * page p is block_table[s * table_cols + p].  Output row (t, h) lies at t *
+ * token_stride + h * head_stride of k and of v, t < tokens.  Rows in no
+ * sequence (before starts[0], from starts[seqs] on) keep their bytes; rows
+ * past a sequence's table_cols pages, or on a page out of range, are +0.
+ * starts: seqs + 1 values that do not fall (others give unspecified rows).
+ * table_len = seqs * table_cols, starts_len = seqs + 1.  Errors as for the
+ * write. */
+int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_table,
+                            uint64_t table_len, const uint32_t *starts, uint64_t starts_len,
+                            uint16_t *k, uint64_t k_len, uint16_t *v, uint64_t v_len,
+                            uint32_t seqs, uint32_t table_cols, uint32_t tokens,
+                            uint64_t token_stride, uint64_t head_stride, void *stream);
+
+/* Attention of one new token per sequence over its cached keys: with group =
+ * q_heads / kv_heads (whole), query head i of sequence s reads KV head i /
+ * group, and
+ *   o[s, i] = softmax(scale * q[s, i] . K^T) V,  lse[s, i] = its log-sum-exp
+ * over keys max(0, lengths[s] - window) <= j < lengths[s] (window 0: all of
+ * them), fp32 statistics and sums.  q [seqs, q_heads, head_dim] bf16, its
+ * sequences q_stride elements apart; o dense [seqs, q_heads, head_dim] bf16;
+ * lse [seqs, q_heads] f32 or NULL.  The new token's own key is in the cache
+ * already where lengths counts it.  Length 0, or no key on a valid page: o =
+ * +0, lse = -inf.  A length above max_length counts as max_length (at most
+ * table_cols * page_size, and below 2^31); a key on a page out of range is
+ * left out.
+ * What cached rows no sequence reaches hold (NaN included) has no effect.
+ *
+ * The keys of all sequences are dealt evenly to the workgroups, so the bits of
+ * a sequence's result depend on the batch; the same call gives the same bits.
+ * workspace: device scratch of FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES(q_heads,
+ * kv_heads, head_dim) bytes, 16-byte aligned, at any contents; calls that
+ * overlap need one each.
+ *
+ * head_dim is 64 or 128.  Errors after the cache's: head_dim, kv_heads = 0 or
+ * no divisor of q_heads, max_length out of its range, or 2^31 or more key
+ * tiles in all (seqs * kv_heads * max_length / 32, times group / 64)
+ * FE2O3_ERR_SHAPE; q_stride below q_heads * head_dim FE2O3_ERR_STRIDE; lengths
+ * FE2O3_ERR_LENGTH (q_len covers the extent); NULL FE2O3_ERR_NULL; cache rows,
+ * q rows or o off 16 bytes, lse or workspace off theirs FE2O3_ERR_ALIGNMENT;
+ * a scale that is not positive and finite FE2O3_ERR_SHAPE; a short workspace
+ * FE2O3_ERR_WORKSPACE. */
+#define FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS 1024u
+#define FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES(q_heads, kv_heads, head_dim)                  \
+  (UINT64_C(16) * FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS +                                    \
+   UINT64_C(8) * FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS * ((uint64_t)(head_dim) + 2u) *       \
+       ((q_heads) / (kv_heads) < 64u ? (q_heads) / (kv_heads) : 64u))
+int32_t fe2o3_paged_attention_decode(const Fe2o3KvCacheV1 *cache, const uint16_t *q,
+                                     uint64_t q_len, const uint32_t *block_table,
+                                     uint64_t table_len, const uint32_t *lengths,
+                                     uint64_t lengths_len, uint16_t *o, uint64_t o_len,
+                                     float *lse, uint64_t lse_len, void *workspace,
+                                     uint64_t workspace_bytes, uint32_t seqs, uint32_t q_heads,
+                                     uint32_t table_cols, uint32_t max_length,
+                                     uint64_t q_stride, uint32_t window, float scale,
+                                     void *stream);
+
 /* ---- top-2 MoE ------------------------------------------------------------------------ */
 
 #define FE2O3_DROP_ROUTE 0xffffffffu
