@@ -80,11 +80,21 @@ FE2O3_DEVICE Span span_of(const Args& a, uint32_t length) {
 // LDS rows of 2 D bytes, 16-byte chunk c of row r at c ^ swz(r).  K is read 8
 // rows at once, r % 4 and bit 3 apart, two chunks each; V as 4 rows of 2 chunks
 // for each of the lane groups, whose rows differ in bit 3 within half a wave:
-// either way 16 chunks in 16 different places of 256 bytes.
+// either way 16 chunks in 16 different places of 256 bytes.  The lowest bit
+// parts the rows that widened codes are written to at once, of which each lane
+// writes two chunks one after the other.
 template <int D>
-FE2O3_DEVICE uint32_t swz(uint32_t r) {
-  if constexpr (D == 128) return 2u * ((r & 3u) | (r >> 1 & 4u));
-  else return 2u * ((r >> 1 & 1u) | (r >> 2 & 2u));
+FE2O3_DEVICE constexpr uint32_t swz(uint32_t r) {
+  if constexpr (D == 128) return 2u * ((r & 3u) | (r >> 1 & 4u)) | ((r ^ r >> 1) & 1u);
+  else return 2u * ((r >> 1 & 1u) | (r >> 2 & 2u)) | (r >> 1 & 1u);
+}
+
+// The same of a sequence that the whole wave works on, in scalar registers, so
+// that what follows from it branches as a whole.
+FE2O3_DEVICE uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+FE2O3_DEVICE Span uniform_span_of(const Args& a, uint32_t seq) {
+  const Span s = span_of(a, a.lengths[seq]);
+  return Span{uniform(s.first), uniform(s.end), uniform(s.tile0), uniform(s.tiles)};
 }
 
 FE2O3_DEVICE uint64_t shfl64(uint64_t v, uint32_t lane) {
@@ -93,10 +103,20 @@ FE2O3_DEVICE uint64_t shfl64(uint64_t v, uint32_t lane) {
   return lo | (uint64_t)hi << 32;
 }
 
-FE2O3_DEVICE uint32_t wave_sum_u32(uint32_t v) {
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v += (uint32_t)__shfl_xor((int)v, o, 64);
+// Inclusive sums over the lanes of a wave, within rows of 16 by lane shifts, then
+// over the rows: DPP moves, which take no trip through LDS.
+FE2O3_DEVICE uint32_t wave_scan(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);  // row_shr:1
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+  // lane 15 of a row to the next one (rows 1 and 3), lane 31 to rows 2 and 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, false);
   return v;
+}
+FE2O3_DEVICE uint32_t at_lane(uint32_t v, uint32_t lane) {
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, (int)lane);
 }
 
 // max / sum over the four lanes of a query row (l, l ^ 16, l ^ 32, l ^ 48)
@@ -144,15 +164,22 @@ struct Decode {
 
   const Args& a;
   uint8_t* smem;
-  const uint32_t lane, lr, g, wave;
+  const uint32_t wave;
   uint8_t* own;
   float* own_scales;
 
   FE2O3_DEVICE Decode(const Args& args, uint8_t* lds)
-      : a(args), smem(lds), lane(threadIdx.x & 63u), lr(lane & 15u), g(lane >> 4),
-        wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+      : a(args), smem(lds), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
     own = smem + wave * wave_lds(D);
     own_scales = (float*)(smem + kWaves * wave_lds(D) + wave * scale_lds());
+  }
+  // The thread's number, as a value that the compiler cannot follow: what is
+  // derived from it is then made where it is used, not kept in registers over
+  // every run of a workgroup.
+  static FE2O3_DEVICE uint32_t thread() {
+    uint32_t t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
   }
   FE2O3_DEVICE float2* stat(uint32_t w) const {
     return (float2*)(smem + kWaves * (wave_lds(D) + scale_lds()) + w * stat_lds(RT));
@@ -173,6 +200,7 @@ struct Decode {
   // otherwise the workspace's place `slot` of this workgroup.
   FE2O3_DEVICE void run(uint32_t seq, uint32_t hb, const Span& sp, uint32_t tile, uint32_t n,
                         uint32_t slot) {
+    const uint32_t tid = thread(), lane = tid & 63u, lr = lane & 15u, g = lane >> 4;
     const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
     const uint32_t row0 = block * kBlockRows;             // of the group
     const uint32_t rows = min(a.group - row0, (uint32_t)kBlockRows);
@@ -194,7 +222,7 @@ struct Decode {
       const uint32_t key = at * kKeys + (lane & 31u);
       const uint32_t place = key - a.cache.page.div(key) * a.cache.page.divisor;
       const bool ok = page < a.cache.pages;
-      st.valid = (uint32_t)__ballot(ok);
+      st.valid = uniform((uint32_t)__ballot(ok));
       // a key that is left out reads slot 0, which every cache has
       uint64_t off = ok ? page * a.cache.page_stride + place * a.cache.token_stride : 0u;
       if constexpr (E4M3) {
@@ -208,8 +236,10 @@ struct Decode {
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         const uint64_t row = shfl64(off, i * kRowsPerLoad + lane / kRowLanes);
-        st.k[i] = *reinterpret_cast<const u32x4_t*>(kb + row + (lane % kRowLanes) * 16u);
-        st.v[i] = *reinterpret_cast<const u32x4_t*>(vb + row + (lane % kRowLanes) * 16u);
+        st.k[i] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4_t*>(kb + row + (lane % kRowLanes) * 16u));
+        st.v[i] = __builtin_nontemporal_load(
+            reinterpret_cast<const u32x4_t*>(vb + row + (lane % kRowLanes) * 16u));
       }
     };
 
@@ -228,7 +258,7 @@ struct Decode {
         q_own[ds] = __builtin_bit_cast(bf16x8_t, x);
       }
     } else {
-      for (uint32_t i = threadIdx.x; i < 16u * RT * (D / 8u); i += kThreads) {
+      for (uint32_t i = tid; i < 16u * RT * (D / 8u); i += kThreads) {
         const uint32_t r = i / (D / 8u), c = i % (D / 8u);
         u32x4_t x = {0, 0, 0, 0};
         if (r < rows) x = *reinterpret_cast<const u32x4_t*>(q + r * D + c * 8u);
@@ -261,40 +291,60 @@ struct Decode {
         page[s] = entry(t + (s + DEPTH) * kWaves);
       }
 
+    // LDS addresses.  own is aligned to a row of 256 bytes and the swizzle moves
+    // chunk bits alone, so another chunk (or 32-byte piece) of a row is an
+    // exclusive or, and another row with the same swizzle an offset.
+    const uint32_t pr = lane / kRowLanes, pc = lane % kRowLanes;  // as loaded: row, piece
+    const uint32_t own_at = wave * wave_lds(D);
+    uint32_t put_at = own_at + pr * (2u * D) + (((E4M3 ? 2u : 1u) * pc ^ swz<D>(pr)) << 4);
+    const uint32_t k_row = 8u * (lr >> 2) + (lr & 3u), v_row = 8u * g + (lr >> 2);
+    uint32_t k_at = own_at + k_row * (2u * D) + ((g ^ swz<D>(k_row)) << 4);
+    uint32_t v_at = own_at + kKeys * 2u * D + v_row * (2u * D) +
+                    ((((lr & 3u) >> 1) ^ swz<D>(v_row)) << 4) + (lr & 1u) * 8u;
+
     // the stage's tile into the wave's LDS.  Keys that are left out have scores
     // of -inf whatever K holds, but 0 times their V must be 0: V becomes +0.
     auto put = [&](Stage& s) {
+      asm volatile("" : "+v"(put_at));
+      if (s.valid != 0xffffffffu) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i)
+          if ((s.valid >> (i * kRowsPerLoad + pr) & 1u) == 0u) s.v[i] = u32x4_t{0, 0, 0, 0};
+        asm volatile("");  // a branch, not a select in every tile
+      }
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
-        const uint32_t r = i * kRowsPerLoad + lane / kRowLanes, c = lane % kRowLanes;
-        if (s.valid != 0xffffffffu && (s.valid >> r & 1u) == 0u) s.v[i] = u32x4_t{0, 0, 0, 0};
-        uint8_t* at = own + r * (2u * D);
+        // the swizzle of row i R + pr (R a power of two above pr) is that of both
+        const uint32_t at =
+            (put_at ^ swz<D>(i * kRowsPerLoad) << 4) + i * kRowsPerLoad * (2u * D);
         if constexpr (E4M3) {
-          const uint32_t c0 = (2u * c ^ swz<D>(r)) << 4, c1 = ((2u * c + 1u) ^ swz<D>(r)) << 4;
-          *reinterpret_cast<u32x4_t*>(at + c0) = widen_codes8(s.k[i][0], s.k[i][1]);
-          *reinterpret_cast<u32x4_t*>(at + c1) = widen_codes8(s.k[i][2], s.k[i][3]);
-          *reinterpret_cast<u32x4_t*>(at + kKeys * 2u * D + c0) = widen_codes8(s.v[i][0], s.v[i][1]);
-          *reinterpret_cast<u32x4_t*>(at + kKeys * 2u * D + c1) = widen_codes8(s.v[i][2], s.v[i][3]);
+          *reinterpret_cast<u32x4_t*>(smem + at) = widen_codes8(s.k[i][0], s.k[i][1]);
+          *reinterpret_cast<u32x4_t*>(smem + (at ^ 16u)) = widen_codes8(s.k[i][2], s.k[i][3]);
+          *reinterpret_cast<u32x4_t*>(smem + at + kKeys * 2u * D) = widen_codes8(s.v[i][0], s.v[i][1]);
+          *reinterpret_cast<u32x4_t*>(smem + (at ^ 16u) + kKeys * 2u * D) =
+              widen_codes8(s.v[i][2], s.v[i][3]);
         } else {
-          const uint32_t c0 = (c ^ swz<D>(r)) << 4;
-          *reinterpret_cast<u32x4_t*>(at + c0) = s.k[i];
-          *reinterpret_cast<u32x4_t*>(at + kKeys * 2u * D + c0) = s.v[i];
+          *reinterpret_cast<u32x4_t*>(smem + at) = s.k[i];
+          *reinterpret_cast<u32x4_t*>(smem + at + kKeys * 2u * D) = s.v[i];
         }
       }
       if constexpr (E4M3)
-        own_scales[lane] = (s.valid >> (lane & 31u) & 1u) != 0u ? s.scale : 0.0f;
+        own_scales[lane] = (s.valid >> (lane & 31u) & 1u) != 0u
+                               ? s.scale * (lane < 32u ? a.scale_log2 : 1.0f)
+                               : 0.0f;
     };
 
     auto compute = [&](uint32_t valid) {
+      // the addresses of the pieces are made here, tile by tile: kept over the
+      // loop they would take the registers of a stage
+      asm volatile("" : "+v"(k_at), "+v"(v_at));
       f32x4_t sc[RT][2];
 #pragma unroll
       for (int ds = 0; ds < D / 32; ++ds) {
         bf16x8_t kf[2];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const uint32_t r = 8u * (lr >> 2) + 4u * b + (lr & 3u);
-          kf[b] = *reinterpret_cast<const bf16x8_t*>(own + r * (2u * D) +
-                                                     (((4u * ds + g) ^ swz<D>(r)) << 4));
+          kf[b] = *reinterpret_cast<const bf16x8_t*>(smem + (k_at ^ (64u * ds)) + 8u * D * b);
         }
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
@@ -314,26 +364,30 @@ struct Decode {
           const f32x4_t y = *reinterpret_cast<const f32x4_t*>(own_scales + 32u + 8u * g + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            ks[4 * h + e] = x[e] * a.scale_log2;
+            ks[4 * h + e] = x[e];
             vs[4 * h + e] = y[e];
           }
         }
       }
-      bf16x8_t pf[RT];
+      bf16x8_t pf[RT], pl[RT];
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
-        float x[8];
+        float x[8];  // scores in the log2 domain, bf16 cache: before its scale
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = sc[rt][j >> 2][j & 3] * (E4M3 ? ks[j] : a.scale_log2);
-          if (valid != 0xffffffffu && (valid >> (8u * g + j) & 1u) == 0u) x[j] = -INFINITY;
+        for (int j = 0; j < 8; ++j) x[j] = sc[rt][j >> 2][j & 3] * (E4M3 ? ks[j] : 1.0f);
+        if (valid != 0xffffffffu) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if ((valid >> (8u * g + j) & 1u) == 0u) x[j] = -INFINITY;
+          asm volatile("");
         }
         float p[8], psum;
         auto probabilities = [&] {
           psum = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(x[j] - m_ref[rt]);
+            p[j] = __builtin_amdgcn_exp2f(
+                E4M3 ? x[j] - m_ref[rt] : __builtin_fmaf(x[j], a.scale_log2, -m_ref[rt]));
             psum += p[j];
           }
         };
@@ -342,6 +396,7 @@ struct Decode {
           float top = x[0];
 #pragma unroll
           for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+          if (!E4M3) top *= a.scale_log2;  // positive
           const float m_new = fmaxf(m_ref[rt], row_max(top));
           const float alpha = __builtin_amdgcn_exp2f(m_ref[rt] - m_new);
           m_ref[rt] = m_new;
@@ -354,24 +409,27 @@ struct Decode {
         }
         l_run[rt] += psum;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) pf[rt][j] = (__bf16)(E4M3 ? p[j] * vs[j] : p[j]);
+        for (int j = 0; j < 8; ++j) {
+          const float y = E4M3 ? p[j] * vs[j] : p[j];
+          pf[rt][j] = (__bf16)y;
+          pl[rt][j] = (__bf16)(y - (float)pf[rt][j]);
+        }
       }
       // O^T += V^T P^T: lane i of group g receives d 16 db + i of keys 8 g .. + 7
-      const uint8_t* vt = own + kKeys * 2u * D;
 #pragma unroll
       for (int db = 0; db < kDb; ++db) {
-        const uint32_t d = 16u * db + 4u * (lr & 3u);
         bf16x4_t half[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const uint32_t r = 8u * g + 4u * h + (lr >> 2);
+        for (int h = 0; h < 2; ++h)
           half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (lds_bf16x4_t*)(vt + r * (2u * D) + (((d >> 3) ^ swz<D>(r)) << 4) + (d & 7u) * 2u));
-        }
+              (lds_bf16x4_t*)(smem + (v_at ^ (32u * db)) + 8u * D * h));
         const bf16x8_t vf = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
+        {
           acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[rt], acc[rt][db], 0, 0, 0);
+          acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[rt], acc[rt][db], 0, 0, 0);
+        }
       }
     };
 
@@ -402,6 +460,7 @@ struct Decode {
                            const f32x4_t (&acc)[RT][kDb], const float (&m_ref)[RT],
                            const float (&l_run)[RT]) {
     constexpr uint32_t kStride = D + 4u;  // floats between rows in LDS
+    const uint32_t tid = thread(), lr = tid & 15u, g = tid >> 4 & 3u;
     static_assert(16u * kStride * 4u <= wave_lds(D), "the sums reuse the tiles' LDS");
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -417,7 +476,7 @@ struct Decode {
       for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(mine + 16 * db) = acc[rt][db];
       __syncthreads();
       const uint32_t count = min(rows - rt * 16u, 16u) * (D / 4u);
-      for (uint32_t i = threadIdx.x; i < count; i += kThreads) {
+      for (uint32_t i = tid; i < count; i += kThreads) {
         const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u)), row = rt * 16u + r;
         float2 s[kWaves];
         float m = -__FLT_MAX__, l = 0.0f;
@@ -459,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_whole_kernel(
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
-  const Span sp = span_of(a, a.lengths[seq]);
+  const Span sp = uniform_span_of(a, seq);
   Decode<D, E4M3, RT, DEPTH>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
@@ -469,37 +528,37 @@ template <int D, bool E4M3, int RT, int DEPTH>
 __global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_split_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 63u, blocks = a.cache.kv_heads * a.blocks_per_head;
-  uint32_t mine = 0;
-  for (uint32_t s = lane; s < a.seqs; s += 64u) mine += span_of(a, a.lengths[s]).tiles;
-  const uint32_t total = wave_sum_u32(mine) * blocks;
-  const uint32_t run = ((total - 1u) / gridDim.x / kWaves + 1u) * kWaves;
-  uint32_t at = blockIdx.x * run;  // below (total / grid + 4) * grid: the host keeps it in 32 bits
+  // tiles of all sequences; lane l scans sequence base + l, so that up to 64 of
+  // them are read once
+  auto tiles_of = [&](uint32_t s) { return s < a.seqs ? span_of(a, a.lengths[s]).tiles : 0u; };
+  uint32_t scan = wave_scan(tiles_of(lane)), tiles = at_lane(scan, 63u);
+  const uint32_t first_scan = scan;
+  for (uint32_t base = 64u; base < a.seqs; base += 64u)
+    tiles += at_lane(wave_scan(tiles_of(base + lane)), 63u);
+  const uint32_t total = tiles * blocks;
+  const uint32_t run = uniform((total - 1u) / gridDim.x / kWaves + 1u) * kWaves;
+  uint32_t at = blockIdx.x * run;  // below total + 4 grid: the host keeps it in 32 bits
   const uint32_t end = min(at + run, total);
   uint4 record = {0u, 0u, 0u, 0u};
   if (at < total) {
-    // the sequence that `at` falls into: tiles before it, `skipped`
+    // the sequence that `at` falls into, and the tiles before it
     uint32_t seq = 0, skipped = 0;
-    for (uint32_t base = 0;; base += 64u) {
-      const uint32_t s = base + lane;
-      uint32_t scan = s < a.seqs ? span_of(a, a.lengths[s]).tiles : 0u;
-#pragma unroll
-      for (uint32_t o = 1u; o < 64u; o <<= 1) {
-        const uint32_t below = (uint32_t)__shfl_up((int)scan, o, 64);
-        if (lane >= o) scan += below;
-      }
-      const uint32_t before = (uint32_t)__popcll(
-          __ballot(s < a.seqs && (skipped + scan) * blocks <= at));
+    scan = first_scan;
+    while (true) {
+      const uint32_t before =
+          (uint32_t)__popcll(__ballot(seq + lane < a.seqs && (skipped + scan) * blocks <= at));
       if (before < 64u) {
-        if (before != 0u) skipped += (uint32_t)__shfl((int)scan, (int)before - 1, 64);
-        seq = base + before;
+        if (before != 0u) skipped += at_lane(scan, before - 1u);
+        seq += before;
         break;
       }
-      skipped += (uint32_t)__shfl((int)scan, 63, 64);
+      skipped += at_lane(scan, 63u);
+      seq += 64u;
+      scan = wave_scan(tiles_of(seq + lane));
     }
-    seq = __builtin_amdgcn_readfirstlane(seq);
-    uint32_t rest = __builtin_amdgcn_readfirstlane(at - skipped * blocks);
-    Span sp = span_of(a, a.lengths[seq]);
-    uint32_t hb = rest / sp.tiles, tile = rest - hb * sp.tiles;
+    const uint32_t rest = at - skipped * blocks;
+    Span sp = uniform_span_of(a, seq);
+    uint32_t hb = uniform(rest / sp.tiles), tile = rest - hb * sp.tiles;
     Decode<D, E4M3, RT, DEPTH> decode(a, smem);
     while (true) {
       const uint32_t n = min(sp.tiles - tile, end - at);
@@ -515,56 +574,64 @@ __global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_split_kernel(
       tile = 0u;
       if (++hb == blocks) {
         hb = 0u;
-        sp = span_of(a, a.lengths[++seq]);
+        sp = uniform_span_of(a, ++seq);
       }
     }
   }
   if (threadIdx.x == 0u) a.records[blockIdx.x] = record;
 }
 
-// Query row blockIdx.y of the head that run blockIdx.x began and did not
-// finish: place 1 of that run and place 0 of the runs that follow, in order.
-template <int D>
+// Query rows blockIdx.y * ROWS .. of the head that run blockIdx.x began and did
+// not finish: place 1 of that run and place 0 of the runs that follow, in order.
+// D / 4 threads cover a row; the threads that ROWS rows leave over take every
+// kWays-th part of them.
+template <int D, int ROWS>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(Args a) {
-  __shared__ f32x4_t part_sum[kThreads];
   const uint4 record = a.records[blockIdx.x];
   if (record.x == 0u) return;
   const uint32_t parts = record.y + 1u, seq = record.z, hb = record.w;
   const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
-  const uint32_t row = blockIdx.y;
-  if (block * kBlockRows + row >= a.group) return;
+  constexpr uint32_t kQuads = D / 4u, kWays = kThreads / (kQuads * ROWS);
+  const uint32_t quad = threadIdx.x % kQuads, d = 4u * quad;
+  const uint32_t r = threadIdx.x / kQuads % ROWS, way = threadIdx.x / (kQuads * ROWS);
+  const uint32_t row = blockIdx.y * ROWS + r;
+  const bool has = row < a.rows && block * kBlockRows + row < a.group;
   auto at = [&](uint32_t i) {
-    return ((uint64_t)(blockIdx.x + i) * 2u + (i == 0u ? 1u : 0u)) * a.rows + row;
+    return ((uint64_t)(blockIdx.x + i) * 2u + (i == 0u ? 1u : 0u)) * a.rows + (has ? row : 0u);
   };
-  float m = -__FLT_MAX__;
-  const uint32_t lane = threadIdx.x & 63u;
-  for (uint32_t i = lane; i < parts; i += 64u) m = fmaxf(m, a.stats[at(i) * 2u]);
-  m = wave_max(m);
-  // D / 4 threads cover a row; the others take every kWays-th part
-  constexpr uint32_t kQuads = D / 4u, kWays = kThreads / kQuads;
-  const uint32_t way = threadIdx.x / kQuads, d = 4u * (threadIdx.x % kQuads);
+  // each way keeps a reference of its own
   f32x4_t y = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.0f;
+  float l = 0.0f, m = -__FLT_MAX__;
 #pragma unroll 4
   for (uint32_t i = way; i < parts; i += kWays) {
     const uint64_t p = at(i);
     const float2 s = *reinterpret_cast<const float2*>(a.stats + p * 2u);
-    const float weight = __builtin_amdgcn_exp2f(s.x - m);
-    l += weight * s.y;
-    y += weight * *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d);
+    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d);
+    const float top = fmaxf(m, s.x);
+    const float old = __builtin_amdgcn_exp2f(m - top), weight = __builtin_amdgcn_exp2f(s.x - top);
+    m = top;
+    l = l * old + weight * s.y;
+    y = y * old + weight * x;
   }
-  __shared__ float part_l[kWays];
-  part_sum[threadIdx.x] = y;
-  if (d == 0u) part_l[way] = l;
-  __syncthreads();
-  if (way != 0u) return;
-  l = 0.0f;
-  y = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  if constexpr (kWays > 1u) {
+    __shared__ f32x4_t part_sum[kThreads];
+    __shared__ float2 part_stat[kThreads];
+    part_sum[threadIdx.x] = y;
+    part_stat[threadIdx.x] = float2{m, l};
+    __syncthreads();
+    if (way != 0u) return;
 #pragma unroll
-  for (uint32_t w = 0; w < kWays; ++w) {
-    y += part_sum[w * kQuads + threadIdx.x];
-    l += part_l[w];
+    for (uint32_t w = 1; w < kWays; ++w) {
+      const uint32_t from = w * kQuads * ROWS + threadIdx.x;
+      const float2 s = part_stat[from];
+      const float top = fmaxf(m, s.x);
+      const float old = __builtin_amdgcn_exp2f(m - top), weight = __builtin_amdgcn_exp2f(s.x - top);
+      m = top;
+      l = l * old + weight * s.y;
+      y = y * old + weight * part_sum[from];
+    }
   }
+  if (!has) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
   const uint64_t out = (uint64_t)seq * a.q_heads + head * a.group + block * kBlockRows + row;
   *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
@@ -573,9 +640,14 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(Args a) {
     a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
+template <bool E4M3, int RT>
+constexpr int depth_of() {
+  return E4M3 && RT == 1 ? 2 : 1;
+}
+
 template <int D, bool E4M3, int RT>
 int32_t launch(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
-  constexpr int kDepth = 1;
+  constexpr int kDepth = depth_of<E4M3, RT>();
   constexpr uint32_t kSmem = smem_bytes<D, RT>();
   const auto whole_fn = paged_whole_kernel<D, E4M3, RT, kDepth>;
   const auto split_fn = paged_split_kernel<D, E4M3, RT, kDepth>;
@@ -590,7 +662,17 @@ int32_t launch(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
   split_fn<<<workgroups, kThreads, kSmem, s>>>(a);
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
-  paged_join_kernel<D><<<dim3(workgroups, a.rows), kThreads, 0, s>>>(a);
+  // Few heads have many parts each, which a row's threads share; many have few,
+  // and rows share the threads.
+  const uint64_t heads = (uint64_t)a.seqs * a.cache.kv_heads * a.blocks_per_head;
+  constexpr int kRows = (int)(kThreads / (D / 4));
+  if (a.rows >= (uint32_t)kRows && heads * 8u >= workgroups)
+    paged_join_kernel<D, kRows>
+        <<<dim3(workgroups, (a.rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a);
+  else if (a.rows >= 4u && heads * 16u >= workgroups)
+    paged_join_kernel<D, 4><<<dim3(workgroups, (a.rows - 1u) / 4u + 1u), kThreads, 0, s>>>(a);
+  else
+    paged_join_kernel<D, 1><<<dim3(workgroups, a.rows), kThreads, 0, s>>>(a);
   return fe2o3_host::after_launch();
 }
 
@@ -598,20 +680,26 @@ template <int D, bool E4M3>
 int32_t launch_rows(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
   if (a.rows <= 16u) return launch<D, E4M3, 1>(a, whole, workgroups, s);
   if (a.rows <= 32u) return launch<D, E4M3, 2>(a, whole, workgroups, s);
+  if (a.rows <= 48u) return launch<D, E4M3, 3>(a, whole, workgroups, s);
   return launch<D, E4M3, 4>(a, whole, workgroups, s);
 }
 
 #define FE2O3_PAGED(D, F, RT)                                                                  \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F "," #RT ">", (const void*)paged_whole_kernel<D, F, RT, 1>, kThreads, smem_bytes<D, RT>()}), \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_split_kernel<" #D "," #F "," #RT ">", (const void*)paged_split_kernel<D, F, RT, 1>, kThreads, smem_bytes<D, RT>()})
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F "," #RT ">", (const void*)paged_whole_kernel<D, F, RT, depth_of<F, RT>()>, kThreads, smem_bytes<D, RT>()}), \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_split_kernel<" #D "," #F "," #RT ">", (const void*)paged_split_kernel<D, F, RT, depth_of<F, RT>()>, kThreads, smem_bytes<D, RT>()})
+#define FE2O3_JOIN(D, ROWS)                                                                    \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #ROWS ">", (const void*)paged_join_kernel<D, ROWS>, kThreads, 0})
 const fe2o3_host::KernelRegistrar kRegistered[] = {
-    FE2O3_PAGED(64, false, 1), FE2O3_PAGED(64, false, 2), FE2O3_PAGED(64, false, 4),
-    FE2O3_PAGED(64, true, 1), FE2O3_PAGED(64, true, 2), FE2O3_PAGED(64, true, 4),
-    FE2O3_PAGED(128, false, 1), FE2O3_PAGED(128, false, 2), FE2O3_PAGED(128, false, 4),
-    FE2O3_PAGED(128, true, 1), FE2O3_PAGED(128, true, 2), FE2O3_PAGED(128, true, 4),
-    fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<64>", (const void*)paged_join_kernel<64>, kThreads, 0}),
-    fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<128>", (const void*)paged_join_kernel<128>, kThreads, 0})};
+    FE2O3_PAGED(64, false, 1), FE2O3_PAGED(64, false, 2), FE2O3_PAGED(64, false, 3),
+    FE2O3_PAGED(64, false, 4), FE2O3_PAGED(64, true, 1), FE2O3_PAGED(64, true, 2),
+    FE2O3_PAGED(64, true, 3), FE2O3_PAGED(64, true, 4), FE2O3_PAGED(128, false, 1),
+    FE2O3_PAGED(128, false, 2), FE2O3_PAGED(128, false, 3), FE2O3_PAGED(128, false, 4),
+    FE2O3_PAGED(128, true, 1), FE2O3_PAGED(128, true, 2), FE2O3_PAGED(128, true, 3),
+    FE2O3_PAGED(128, true, 4),
+    FE2O3_JOIN(64, 1), FE2O3_JOIN(64, 4), FE2O3_JOIN(64, 16),
+    FE2O3_JOIN(128, 1), FE2O3_JOIN(128, 4), FE2O3_JOIN(128, 8)};
 #undef FE2O3_PAGED
+#undef FE2O3_JOIN
 
 }  // namespace
 
@@ -684,7 +772,9 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   uint32_t workgroups = (uint32_t)units;
   if (!whole) {
     const uint64_t most = units * ((tiles + kWaves - 1u) / kWaves);
-    const uint32_t slots = 2u * topo.cus < kMaxWorkgroups ? 2u * topo.cus : kMaxWorkgroups;
+    // as many as are resident at once: two a CU of one tile of query rows, else one
+    const uint32_t resident = (a.rows <= 16u ? 2u : 1u) * topo.cus;
+    const uint32_t slots = resident < kMaxWorkgroups ? resident : kMaxWorkgroups;
     workgroups = (uint32_t)(most < slots ? most : slots);
   }
   hipStream_t s = (hipStream_t)stream;

@@ -297,75 +297,79 @@ KV_BF16, KV_E4M3 = 0, 1
 KV_NO_SLOT = 0xFFFFFFFF
 PAGED_ATTENTION_MAX_WORKGROUPS = 1024
 
-# what an array of each kind may hold: numpy types of a DeviceBuffer and the
-# names of a tensor's
+# what an array of each kind may hold: element types of a DeviceBuffer, and of
+# a tensor
 _BF16, _CODES, _INDEX, _FLOAT, _BYTES = "bf16", "e4m3", "u32", "f32", "bytes"
 _HOLDS = {
-    _BF16: (("uint16",), ("torch.bfloat16",)),
-    _CODES: (("uint8",), ("torch.uint8", "torch.float8_e4m3fn")),
-    _INDEX: (("uint32",), ("torch.int32", "torch.uint32")),
-    _FLOAT: (("float32",), ("torch.float32",)),
-    _BYTES: (("uint8",), ("torch.uint8", "torch.int8")),
+    _BF16: ("uint16", "torch.bfloat16"),
+    _CODES: ("uint8", "torch.uint8", "torch.float8_e4m3fn"),
+    _INDEX: ("uint32", "torch.int32", "torch.uint32"),
+    _FLOAT: ("float32", "torch.float32"),
+    _BYTES: ("uint8", "torch.uint8", "torch.int8"),
 }
 _kinds: dict = {}  # element type -> the kinds it may stand for
 
 
-def _kinds_of(dtype, column):
+def _kinds_of(dtype):
     found = _kinds.get(dtype)
     if found is None:
-        found = _kinds[dtype] = frozenset(k for k, v in _HOLDS.items() if str(dtype) in v[column])
+        found = _kinds[dtype] = frozenset(k for k, v in _HOLDS.items() if str(dtype) in v)
     return found
 
 
-def _array(x, kind, name, dense=True):
-    """(pointer, elements) of a DeviceBuffer or a device tensor that holds
-    `kind`.  A tensor's last dimension is contiguous; dense: all of them are,
-    otherwise the elements are the extent its strides span."""
+def _operand(x, kind, name, device, dense=True):
+    """(pointer, elements) of a DeviceBuffer or a tensor that holds `kind` on
+    `device`.  dense: the tensor is contiguous; otherwise its last dimension
+    is, and the elements are the extent that its strides span."""
     if isinstance(x, DeviceBuffer):
-        if kind not in _kinds_of(x.dtype, 0):
+        if kind not in _kinds_of(x.dtype):
             raise TypeError(f"{name} must hold {kind}, not {x.dtype}")
+        if x.ctx.device != device:
+            raise ValueError(f"{name} on device {x.ctx.device}, not {device}")
         return x.ptr, x.count
     if not hasattr(x, "data_ptr"):
         raise TypeError(f"{name} must be a DeviceBuffer or a device tensor")
-    if kind not in _kinds_of(x.dtype, 1):
+    if kind not in _kinds_of(x.dtype):
         raise TypeError(f"{name} must hold {kind}, not {x.dtype}")
-    if not x.is_cuda:
-        raise TypeError(f"{name} must be in device memory")
+    where = x.get_device()
+    if where != device:
+        if where < 0:
+            raise TypeError(f"{name} must be in device memory")
+        raise ValueError(f"{name} on device {where}, not {device}")
     if x.is_contiguous():
         return x.data_ptr(), x.numel()
     if dense:
         raise ValueError(f"{name} must be contiguous")
     count = x.numel()
     if count:
-        if x.shape[-1] > 1 and x.stride(-1) != 1:
+        shape, strides = x.shape, x.stride()
+        if shape[-1] > 1 and strides[-1] != 1:
             raise ValueError(f"the last dimension of {name} must be contiguous")
-        count = 1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))
+        count = 1
+        for n, stride in zip(shape, strides):
+            count += (n - 1) * stride
     return x.data_ptr(), count
 
 
-def _device_of(x):
-    return x.ctx.device if isinstance(x, DeviceBuffer) else x.get_device()
-
-
-def _check_device(*arrays):
-    """Every array on the current device, where the launch goes."""
-    current = C.c_int32()
-    check(_lib.lib().fe2o3_rt_get_device(C.byref(current)), "get device")
-    for x in arrays:
-        if x is not None and _device_of(x) != current.value:
-            raise ValueError(f"array on device {_device_of(x)}, the current one is {current.value}")
-
-
-def _strides(x):
-    """A tensor's strides; 0 for a dimension of one, whose stride says nothing."""
-    return tuple(s if n > 1 else 0 for n, s in zip(x.shape, x.stride()))
-
-
-def _shape_of(x, dims, name):
+def _layout(x, dims, name):
+    """(shape, strides) of a tensor, a stride of 0 for a dimension of one, whose
+    stride says nothing; (None, None) of a DeviceBuffer."""
+    if isinstance(x, DeviceBuffer):
+        return None, None
     shape = getattr(x, "shape", None)
-    if shape is not None and len(shape) != dims:
-        raise ValueError(f"{name} must have {dims} dimensions, not {len(shape)}")
-    return shape
+    if shape is None or len(shape) != dims:
+        raise ValueError(f"{name} must be a DeviceBuffer or a tensor of {dims} dimensions")
+    strides = x.stride()
+    if 1 in shape:
+        strides = tuple(s if n > 1 else 0 for n, s in zip(shape, strides))
+    return shape, strides
+
+
+def _pair_layout(k, v, dims):
+    shape, strides = _layout(k, dims, "k")
+    if _layout(v, dims, "v") != (shape, strides):
+        raise ValueError("k and v must have the same shape and strides")
+    return shape, strides
 
 
 class KvCache:
@@ -381,46 +385,61 @@ class KvCache:
     """
 
     def __init__(self, k, v, k_scale=None, v_scale=None, *, shape=None, strides=None):
-        k_shape = _shape_of(k, 4, "k")
-        if k_shape is not None:
-            strides = _strides(k)
-            if k_shape != v.shape or strides != _strides(v):
-                raise ValueError("k and v must have the same shape and strides")
-            shape, strides = k_shape, strides[:3]
-        elif shape is None:
+        found, found_strides = _pair_layout(k, v, 4)
+        if found is not None:
+            shape, strides = found, found_strides[:3]
+            self.device = k.get_device()
+            if self.device < 0:
+                raise TypeError("a cache lies in device memory")
+        else:
+            self.device = k.ctx.device
+        if shape is None:
             raise ValueError("a cache of DeviceBuffers needs its shape")
-        pages, page_size, kv_heads, head_dim = (int(n) for n in shape)
+        pages, page_size, kv_heads, head_dim = self.shape = shape
         if strides is None:
             strides = (page_size * kv_heads * head_dim, kv_heads * head_dim, head_dim)
-        self.format = KV_BF16 if k_scale is None else KV_E4M3
         if (k_scale is None) != (v_scale is None):
             raise ValueError("k_scale and v_scale go together")
-        for scale in (k_scale, v_scale):
-            found = None if scale is None else _shape_of(scale, 3, "scales")
-            if found is not None and tuple(found) != (pages, kv_heads, page_size):
-                raise ValueError(f"scales of {tuple(found)}, not {(pages, kv_heads, page_size)}")
-        kind = _BF16 if k_scale is None else _CODES
-        scales = ((None, 0), (None, 0)) if k_scale is None else (
-            _array(k_scale, _FLOAT, "k_scale"), _array(v_scale, _FLOAT, "v_scale"))
         self.arrays = (k, v, k_scale, v_scale)
-        self.shape = (pages, page_size, kv_heads, head_dim)
+        k_ptr = v_ptr = None
+        scales = 0
+        if k_scale is None:
+            self.format, kind = KV_BF16, _BF16
+        else:
+            self.format, kind = KV_E4M3, _CODES
+            for scale in (k_scale, v_scale):
+                found = _layout(scale, 3, "scales")[0]
+                if found is not None and tuple(found) != (pages, kv_heads, page_size):
+                    raise ValueError(f"scales of {tuple(found)}, "
+                                     f"not {(pages, kv_heads, page_size)}")
+            k_ptr, scales = _operand(k_scale, _FLOAT, "k_scale", self.device)
+            v_ptr, v_scales = _operand(v_scale, _FLOAT, "v_scale", self.device)
+            if scales != v_scales:
+                raise ValueError("k_scale and v_scale must have the same length")
         self.record = _lib.Fe2o3KvCacheV1(
-            *_array(k, kind, "k", dense=False), *_array(v, kind, "v", dense=False),
-            *scales[0], *scales[1], *strides, self.format, *self.shape, 0)
+            *_operand(k, kind, "k", self.device, False),
+            *_operand(v, kind, "v", self.device, False), k_ptr, scales, v_ptr, scales,
+            *strides, self.format, pages, page_size, kv_heads, head_dim, 0)
 
 
-def _rows(cache, k, v, strides):
-    """(token, head) strides of K and V rows, and their tokens where they say so."""
-    shape = _shape_of(k, 3, "k")
+def _on_current_device(cache):
+    """The cache's device, which has to be the current one: launches go there."""
+    current = C.c_int32()
+    check(_lib.lib().fe2o3_rt_get_device(C.byref(current)), "get device")
+    if current.value != cache.device:
+        raise ValueError(f"cache on device {cache.device}, the current one is {current.value}")
+    return cache.device
+
+
+def _row_layout(cache, k, v, strides):
+    """Tokens (None of DeviceBuffers) and (token, head) strides of K and V rows."""
     _, _, kv_heads, head_dim = cache.shape
+    shape, found = _pair_layout(k, v, 3)
     if shape is None:
-        return strides or (kv_heads * head_dim, head_dim), None
-    found = _strides(k)
-    if shape != v.shape or found != _strides(v):
-        raise ValueError("k and v must have the same shape and strides")
-    if tuple(shape[1:]) != (kv_heads, head_dim):
+        return None, strides or (kv_heads * head_dim, head_dim)
+    if shape[1] != kv_heads or shape[2] != head_dim:
         raise ValueError(f"rows of {tuple(shape[1:])} for a cache of {(kv_heads, head_dim)}")
-    return found[:2], shape[0]
+    return shape[0], found[:2]
 
 
 def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sync=True) -> None:
@@ -428,14 +447,14 @@ def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sy
     `strides` (token, head)) into slots[t] of the cache, quantised where it is
     e4m3.  A slot out of range (KV_NO_SLOT) is skipped; each slot at most once
     a call (fe2o3_kv_cache_write)."""
-    (token_stride, head_stride), rows = _rows(cache, k, v, strides)
-    _check_device(*cache.arrays, k, v, slots)
-    slots_ptr, tokens = _array(slots, _INDEX, "slots")
+    device = _on_current_device(cache)
+    rows, strides = _row_layout(cache, k, v, strides)
+    slots_ptr, tokens = _operand(slots, _INDEX, "slots", device)
     if rows is not None and rows != tokens:
         raise ValueError(f"{rows} rows and {tokens} slots")
-    _call("fe2o3_kv_cache_write", C.byref(cache.record), *_array(k, _BF16, "k", dense=False),
-          *_array(v, _BF16, "v", dense=False), slots_ptr, tokens, tokens, token_stride,
-          head_stride, stream=stream, sync=sync)
+    _call("fe2o3_kv_cache_write", C.byref(cache.record), *_operand(k, _BF16, "k", device, False),
+          *_operand(v, _BF16, "v", device, False), slots_ptr, tokens, tokens, *strides,
+          stream=stream, sync=sync)
 
 
 def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, tokens=None,
@@ -444,19 +463,19 @@ def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, to
     s, on pages block_table[s], to rows starts[s] .. starts[s + 1] - 1.  Rows in
     no sequence keep their values (fe2o3_kv_cache_read).  DeviceBuffers take
     `strides` (token, head) and `tokens`."""
-    (token_stride, head_stride), rows = _rows(cache, k, v, strides)
-    _check_device(*cache.arrays, block_table, starts, k, v)
-    starts_ptr, starts_len = _array(starts, _INDEX, "starts")
-    table_ptr, table_len = _array(block_table, _INDEX, "block_table")
+    device = _on_current_device(cache)
+    rows, strides = _row_layout(cache, k, v, strides)
+    starts_ptr, starts_len = _operand(starts, _INDEX, "starts", device)
+    table_ptr, table_len = _operand(block_table, _INDEX, "block_table", device)
     seqs = starts_len - 1
     if seqs < 0:
         raise ValueError("starts must hold one value more than there are sequences")
     if rows is None:
         rows = k.count // (cache.shape[2] * cache.shape[3]) if tokens is None else tokens
     _call("fe2o3_kv_cache_read", C.byref(cache.record), table_ptr, table_len, starts_ptr,
-          starts_len, *_array(k, _BF16, "k", dense=False), *_array(v, _BF16, "v", dense=False),
-          seqs, table_len // seqs if seqs else 0, rows, token_stride, head_stride,
-          stream=stream, sync=sync)
+          starts_len, *_operand(k, _BF16, "k", device, False),
+          *_operand(v, _BF16, "v", device, False), seqs, table_len // seqs if seqs else 0, rows,
+          *strides, stream=stream, sync=sync)
 
 
 def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int) -> int:
@@ -474,26 +493,26 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
     last `window` keys (fe2o3_paged_attention_decode).  workspace: device bytes,
     paged_attention_workspace_bytes at least, of no use to another call that may
     overlap.  DeviceBuffers take q_heads, and q_stride between sequences."""
-    _check_device(*cache.arrays, q, block_table, lengths, out, lse, workspace)
+    device = _on_current_device(cache)
     head_dim = cache.shape[3]
-    q_shape = _shape_of(q, 3, "q")
-    if q_shape is not None:
-        q_heads, q_stride = q_shape[1], q.stride(0)
-        if q_shape[2] != head_dim or _strides(q)[1] not in (0, head_dim):
+    lengths_ptr, seqs = _operand(lengths, _INDEX, "lengths", device)
+    shape, strides = _layout(q, 3, "q")
+    if shape is not None:
+        q_heads, q_stride = shape[1], strides[0]
+        if shape[0] != seqs:
+            raise ValueError(f"{shape[0]} rows of q and {seqs} lengths")
+        if shape[2] != head_dim or strides[1] not in (0, head_dim):
             raise ValueError("q must be [seqs, q_heads, head_dim] with a sequence's heads dense")
     elif q_heads is None:
         raise ValueError("q in a DeviceBuffer needs q_heads")
     elif q_stride is None:
         q_stride = q_heads * head_dim
-    lengths_ptr, seqs = _array(lengths, _INDEX, "lengths")
-    if q_shape is not None and q_shape[0] != seqs:
-        raise ValueError(f"{q_shape[0]} rows of q and {seqs} lengths")
-    table_ptr, table_len = _array(block_table, _INDEX, "block_table")
+    table_ptr, table_len = _operand(block_table, _INDEX, "block_table", device)
+    lse_ptr, lse_len = (None, 0) if lse is None else _operand(lse, _FLOAT, "lse", device)
     _call("fe2o3_paged_attention_decode", C.byref(cache.record),
-          *_array(q, _BF16, "q", dense=False), table_ptr, table_len, lengths_ptr, seqs,
-          *_array(out, _BF16, "out"),
-          *((None, 0) if lse is None else _array(lse, _FLOAT, "lse")),
-          *_array(workspace, _BYTES, "workspace"), seqs, q_heads,
+          *_operand(q, _BF16, "q", device, False), table_ptr, table_len, lengths_ptr, seqs,
+          *_operand(out, _BF16, "out", device), lse_ptr, lse_len,
+          *_operand(workspace, _BYTES, "workspace", device), seqs, q_heads,
           table_len // seqs if seqs else 0, max_length, q_stride, window, scale,
           stream=stream, sync=sync)
 

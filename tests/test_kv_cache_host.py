@@ -287,3 +287,6 @@ def test_arrays_on_another_device_are_refused(monkeypatch):
     monkeypatch.setattr(_lib, "lib", lambda: Lib())
     with pytest.raises(ValueError, match="device 1"):
         kernels.kv_cache_write(cache, here, there, slots)
+    far = kernels.KvCache(*(_Fake((4, 16, 2, 64), (2048, 128, 64, 1), device=1) for _ in "kv"))
+    with pytest.raises(ValueError, match="the current one is 0"):
+        kernels.kv_cache_write(far, there, there, slots)
