@@ -44,6 +44,11 @@ using kv_cache::View;
 
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr uint32_t kKeys = 32;              // keys per tile
+#ifdef XSETUP
+constexpr uint32_t kSetup = XSETUP;
+#else
+constexpr uint32_t kSetup = 1;              // rounds that a head's start counts for
+#endif
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
 constexpr uint32_t kGridX = 1u << 22;       // a grid holds fewer than 2^32 threads a dimension
@@ -75,18 +80,6 @@ FE2O3_DEVICE Span span_of(const Args& a, uint32_t length) {
   s.tile0 = s.first / kKeys;
   s.tiles = max((s.end + kKeys - 1u) / kKeys - s.tile0, 1u);
   return s;
-}
-
-// LDS rows of 2 D bytes, 16-byte chunk c of row r at c ^ swz(r).  K is read 8
-// rows at once, r % 4 and bit 3 apart, two chunks each; V as 4 rows of 2 chunks
-// for each of the lane groups, whose rows differ in bit 3 within half a wave:
-// either way 16 chunks in 16 different places of 256 bytes.  The lowest bit
-// parts the rows that widened codes are written to at once, of which each lane
-// writes two chunks one after the other.
-template <int D>
-FE2O3_DEVICE constexpr uint32_t swz(uint32_t r) {
-  if constexpr (D == 128) return 2u * ((r & 3u) | (r >> 1 & 4u)) | ((r ^ r >> 1) & 1u);
-  else return 2u * ((r >> 1 & 1u) | (r >> 2 & 2u)) | (r >> 1 & 1u);
 }
 
 // The same of a sequence that the whole wave works on, in scalar registers, so
@@ -138,41 +131,77 @@ FE2O3_DEVICE u32x4_t widen_codes8(uint32_t lo, uint32_t hi) {
   return x;
 }
 
-constexpr uint32_t wave_lds(int d) { return kKeys * (uint32_t)d * 4u; }  // K tile, V tile
-constexpr uint32_t scale_lds() { return 2u * kKeys * 4u; }               // per wave
-constexpr uint32_t stat_lds(int rt) { return 16u * rt * 8u; }            // per wave
-constexpr uint32_t query_lds(int d, int rt) { return rt == 1 ? 0u : 32u * rt * d; }
-template <int D, int RT>
-constexpr uint32_t smem_bytes() {
-  return kWaves * (wave_lds(D) + scale_lds() + stat_lds(RT)) + query_lds(D, RT);
+// A tile in a wave's LDS: the K rows, then the V rows, as the cache holds them.
+// 16-byte chunk c of row r lies at chunk c ^ swz(r), so that the lanes that are
+// served at once reach all banks:
+//   K, 8 rows (r % 4 and bit 3 apart) of two neighbouring chunks;
+//   V, half a wave's transposing read: bf16 4 rows of two chunks for each of two
+//   lane groups, whose rows differ in bit 3; e4m3 8 rows of one chunk for each.
+template <int D, bool E4M3>
+struct Tile {
+  static constexpr uint32_t kRowBytes = E4M3 ? D : 2 * D;
+  static constexpr uint32_t kRowLanes = kRowBytes / 16u;  // lanes that load a row
+  static constexpr uint32_t kRowsPerLoad = 64u / kRowLanes;
+  static constexpr int kLoads = kKeys / kRowsPerLoad;     // of K, and of V
+  static constexpr uint32_t kBytes = kKeys * kRowBytes;   // of K, and of V
+  static FE2O3_DEVICE constexpr uint32_t swz(uint32_t r) {
+    if constexpr (E4M3)
+      return D == 128 ? (r >> 2 & 1u) | (r & 2u) | (r >> 1 & 4u) : (r >> 2 & 1u) | (r >> 2 & 2u);
+    else
+      return D == 128 ? 2u * ((r & 3u) | (r >> 1 & 4u)) : 2u * ((r >> 1 & 1u) | (r >> 2 & 2u));
+  }
+  // the sums of 16 query rows take the tile's place at the end of a run
+  static constexpr uint32_t kSumStride = D + 4u;  // floats
+  static constexpr uint32_t kSumBytes = 16u * kSumStride * 4u;
+  static constexpr uint32_t kLds = 2u * kBytes > kSumBytes ? 2u * kBytes : kSumBytes;
+  static_assert(kLds % 256u == 0u, "chunks are chosen by exclusive or");
+};
+
+// LDS of a workgroup: the waves' tiles, their tiles' scales, their reference and
+// sum of each query row, and the queries where they are more than one tile.
+template <int D, bool E4M3, int RT>
+struct Lds {
+  static constexpr uint32_t kScales = kWaves * Tile<D, E4M3>::kLds;
+  static constexpr uint32_t kStats = kScales + kWaves * 2u * kKeys * 4u;
+  static constexpr uint32_t kQueries = kStats + kWaves * 16u * RT * 8u;
+  static constexpr uint32_t kQueryTile = D / 32 * 1024u;
+  static constexpr uint32_t kBytes = kQueries + (RT == 1 ? 0u : RT * kQueryTile);
+};
+
+// Workgroups per CU.
+template <int D, bool E4M3, int RT>
+constexpr int per_cu() {
+  if (RT > 1) return 1;
+#ifdef XPC
+  if (E4M3) return XPC;
+#endif
+  return D == 64 ? 3 : 2;
 }
 
-// D: head_dim.  RT: query-row tiles of 16.  DEPTH: tiles in flight per wave.
-template <int D, bool E4M3, int RT, int DEPTH>
+// D: head_dim.  RT: query-row tiles of 16.
+template <int D, bool E4M3, int RT>
 struct Decode {
-  static constexpr uint32_t kRowBytes = E4M3 ? D : 2 * D;
-  static constexpr uint32_t kRowLanes = kRowBytes / 16u;      // lanes that load a row
-  static constexpr uint32_t kRowsPerLoad = 64u / kRowLanes;
-  static constexpr int kLoads = kKeys / kRowsPerLoad;         // of K, and of V
-  static constexpr int kDb = D / 16;                          // V^T row blocks
+  using T = Tile<D, E4M3>;
+  using L = Lds<D, E4M3, RT>;
+  static constexpr int kDb = D / 16;     // V^T row blocks
+  static constexpr int kFrags = D / 32;  // 16-byte pieces of a query operand per lane
 
   struct Stage {
-    u32x4_t k[kLoads], v[kLoads];
+    u32x4_t k[T::kLoads], v[T::kLoads];
     float scale;     // E4M3: lanes below 32 the K scale of key l, the others the V scale
     uint32_t valid;  // bit per key
+  };
+  struct Query {
+    u32x4_t f[kFrags];
   };
 
   const Args& a;
   uint8_t* smem;
   const uint32_t wave;
-  uint8_t* own;
-  float* own_scales;
 
   FE2O3_DEVICE Decode(const Args& args, uint8_t* lds)
-      : a(args), smem(lds), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
-    own = smem + wave * wave_lds(D);
-    own_scales = (float*)(smem + kWaves * wave_lds(D) + wave * scale_lds());
-  }
+      : a(args), smem(lds), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+
   // The thread's number, as a value that the compiler cannot follow: what is
   // derived from it is then made where it is used, not kept in registers over
   // every run of a workgroup.
@@ -181,23 +210,33 @@ struct Decode {
     asm volatile("" : "+v"(t));
     return t;
   }
+  FE2O3_DEVICE float* scales(uint32_t w) const {
+    return (float*)(smem + L::kScales + w * (2u * kKeys * 4u));
+  }
   FE2O3_DEVICE float2* stat(uint32_t w) const {
-    return (float2*)(smem + kWaves * (wave_lds(D) + scale_lds()) + w * stat_lds(RT));
+    return (float2*)(smem + L::kStats + w * (16u * RT * 8u));
   }
 
-  // Query rows stay in registers where they are one tile; more would take the
-  // registers of the sums, and lie in LDS for all waves: 16-byte chunk c of row
-  // r at c ^ swz_q(r), which the reads of 8 rows and 2 chunks do not conflict in.
-  static FE2O3_DEVICE uint32_t swz_q(uint32_t r) {
-    return D == 128 ? 2u * (r & 7u) : 2u * (r >> 1 & 3u);
-  }
-  FE2O3_DEVICE uint8_t* queries() const {
-    return smem + kWaves * (wave_lds(D) + scale_lds() + stat_lds(RT));
+  // The query operand of lane (lr, g) for row `row` of `rows` (others 0): piece f
+  // has the d that the lane's piece of K has (compute): bf16 32 f + 8 g .. + 7;
+  // e4m3, where a lane reads 16 codes at once, halves of 16 g .. + 15 and, 128
+  // wide, of 64 more.
+  FE2O3_DEVICE Query query(const uint16_t* q, uint32_t row, uint32_t rows, uint32_t g) const {
+    Query r;
+    const bool has = row < rows;
+    const uint16_t* from = q + (has ? row : 0u) * D + g * (E4M3 ? 16u : 8u);
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f) {
+      r.f[f] = *reinterpret_cast<const u32x4_t*>(from + (E4M3 ? (f >> 1) * 64 + (f & 1) * 8
+                                                              : f * 32));
+      if (!has) r.f[f] = u32x4_t{0, 0, 0, 0};
+    }
+    return r;
   }
 
   // Keys of tiles [tile, tile + n) of sequence `seq` for block `hb` of the KV
-  // heads' query rows.  whole: the span's every tile, so the output itself;
-  // otherwise the workspace's place `slot` of this workgroup.
+  // heads' query rows.  Place `slot` of this workgroup's workspace takes the
+  // sums unless they are the span's every tile.
   FE2O3_DEVICE void run(uint32_t seq, uint32_t hb, const Span& sp, uint32_t tile, uint32_t n,
                         uint32_t slot) {
     const uint32_t tid = thread(), lane = tid & 63u, lr = lane & 15u, g = lane >> 4;
@@ -206,19 +245,22 @@ struct Decode {
     const uint32_t rows = min(a.group - row0, (uint32_t)kBlockRows);
     const uint32_t q_head = head * a.group + row0;
     const uint32_t* table = a.table + (uint64_t)seq * a.table_cols;
-    const uint8_t* kb = a.cache.k + head * a.cache.head_stride * (E4M3 ? 1u : 2u);
-    const uint8_t* vb = a.cache.v + head * a.cache.head_stride * (E4M3 ? 1u : 2u);
+    const uint64_t head_at = head * a.cache.head_stride * (E4M3 ? 1u : 2u);
+    const uint32_t pr = lane / T::kRowLanes, pc = lane % T::kRowLanes;  // as loaded: row, piece
+    const uint8_t* kb = a.cache.k + head_at + pc * 16u;
+    const uint8_t* vb = a.cache.v + head_at + pc * 16u;
     const float* sb = (lane < 32u ? a.cache.k_scale : a.cache.v_scale);
 
     const uint32_t end = sp.tile0 + tile + n;
     uint32_t t = sp.tile0 + tile + wave;
-    auto inside = [&](uint32_t key) { return key >= sp.first && key < sp.end; };
     // the table's entry for this lane's key of tile t; none past the run
     auto entry = [&](uint32_t at) {
       const uint32_t key = at * kKeys + (lane & 31u);
-      return at < end && inside(key) ? table[a.cache.page.div(key)] : 0xffffffffu;
+      return at < end && key >= sp.first && key < sp.end ? table[a.cache.page.div(key)]
+                                                         : 0xffffffffu;
     };
-    auto issue = [&](Stage& st, uint32_t at, uint32_t page) {
+    Stage st;
+    auto issue = [&](uint32_t at, uint32_t page) {
       const uint32_t key = at * kKeys + (lane & 31u);
       const uint32_t place = key - a.cache.page.div(key) * a.cache.page.divisor;
       const bool ok = page < a.cache.pages;
@@ -233,44 +275,35 @@ struct Decode {
       } else {
         off *= 2u;
       }
+      // nontemporal: 16384 tokens of 8 heads run at 6.4 TB/s, at 5.7 without
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        const uint64_t row = shfl64(off, i * kRowsPerLoad + lane / kRowLanes);
-        st.k[i] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4_t*>(kb + row + (lane % kRowLanes) * 16u));
-        st.v[i] = __builtin_nontemporal_load(
-            reinterpret_cast<const u32x4_t*>(vb + row + (lane % kRowLanes) * 16u));
+      for (int i = 0; i < T::kLoads; ++i) {
+        const uint64_t row = shfl64(off, i * T::kRowsPerLoad + pr);
+        st.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kb + row));
+        st.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vb + row));
       }
     };
 
-    Stage st[DEPTH];
-    uint32_t page[DEPTH];
-#pragma unroll
-    for (int s = 0; s < DEPTH; ++s) page[s] = entry(t + s * kWaves);
-
+    uint32_t page = entry(t);
     const uint16_t* q = a.q + seq * a.q_stride + (uint64_t)q_head * D;
-    bf16x8_t q_own[D / 32];
+    Query q_own;
+    auto query_at = [&](int rt) { return smem + L::kQueries + rt * L::kQueryTile; };
     if constexpr (RT == 1) {
-#pragma unroll
-      for (int ds = 0; ds < D / 32; ++ds) {
-        u32x4_t x = *reinterpret_cast<const u32x4_t*>(q + (lr < rows ? lr : 0u) * D + ds * 32 + g * 8u);
-        if (lr >= rows) x = u32x4_t{0, 0, 0, 0};
-        q_own[ds] = __builtin_bit_cast(bf16x8_t, x);
-      }
+      q_own = query(q, lr, rows, g);
     } else {
-      for (uint32_t i = tid; i < 16u * RT * (D / 8u); i += kThreads) {
-        const uint32_t r = i / (D / 8u), c = i % (D / 8u);
-        u32x4_t x = {0, 0, 0, 0};
-        if (r < rows) x = *reinterpret_cast<const u32x4_t*>(q + r * D + c * 8u);
-        *reinterpret_cast<u32x4_t*>(queries() + r * (2u * D) + ((c ^ swz_q(r)) << 4)) = x;
+      // more than one tile of query rows would take the registers of the sums:
+      // they lie in LDS for all waves, in the order of the lanes
+      for (uint32_t rt = wave; rt < (uint32_t)RT; rt += kWaves) {
+        const Query x = query(q, rt * 16u + lr, rows, g);
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+          *reinterpret_cast<u32x4_t*>(query_at(rt) + f * 1024 + lane * 16u) = x.f[f];
       }
       __syncthreads();
     }
-    auto query = [&](int rt, int ds) {
-      if constexpr (RT == 1) return q_own[ds];
-      else
-        return *reinterpret_cast<const bf16x8_t*>(
-            queries() + (rt * 16u + lr) * (2u * D) + (((4u * ds + g) ^ swz_q(lr)) << 4));
+    auto query_frag = [&](int rt, int f) {
+      if constexpr (RT == 1) return q_own.f[f];
+      else return *reinterpret_cast<const u32x4_t*>(query_at(rt) + f * 1024 + lane * 16u);
     };
     f32x4_t acc[RT][kDb];
     float m_ref[RT], l_run[RT];
@@ -284,54 +317,46 @@ struct Decode {
       for (int db = 0; db < kDb; ++db) acc[rt][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-#pragma unroll
-    for (int s = 0; s < DEPTH; ++s)
-      if (t + s * kWaves < end) {
-        issue(st[s], t + s * kWaves, page[s]);
-        page[s] = entry(t + (s + DEPTH) * kWaves);
-      }
+    if (t < end) {
+      issue(t, page);
+      page = entry(t + kWaves);
+    }
 
-    // LDS addresses.  own is aligned to a row of 256 bytes and the swizzle moves
-    // chunk bits alone, so another chunk (or 32-byte piece) of a row is an
-    // exclusive or, and another row with the same swizzle an offset.
-    const uint32_t pr = lane / kRowLanes, pc = lane % kRowLanes;  // as loaded: row, piece
-    const uint32_t own_at = wave * wave_lds(D);
-    uint32_t put_at = own_at + pr * (2u * D) + (((E4M3 ? 2u : 1u) * pc ^ swz<D>(pr)) << 4);
-    const uint32_t k_row = 8u * (lr >> 2) + (lr & 3u), v_row = 8u * g + (lr >> 2);
-    uint32_t k_at = own_at + k_row * (2u * D) + ((g ^ swz<D>(k_row)) << 4);
-    uint32_t v_at = own_at + kKeys * 2u * D + v_row * (2u * D) +
-                    ((((lr & 3u) >> 1) ^ swz<D>(v_row)) << 4) + (lr & 1u) * 8u;
+    // LDS addresses.  The wave's tile is aligned to 256 bytes and the swizzle
+    // moves chunk bits alone, so another chunk of a row is an exclusive or, and
+    // another row an offset and the exclusive or of its swizzle.  Row m of key
+    // block b is key 8 (m / 4) + 4 b + m % 4.
+    const uint32_t own_at = wave * T::kLds;
+    const uint32_t k_row = 8u * (lr >> 2) + (lr & 3u);
+    const uint32_t v_row = 8u * g + (E4M3 ? lr >> 1 : lr >> 2);
+    uint32_t put_at = own_at + pr * T::kRowBytes + ((pc ^ T::swz(pr)) << 4);
+    uint32_t k_at = own_at + k_row * T::kRowBytes +
+                    ((g ^ T::swz(k_row)) << 4);
+    uint32_t v_at = own_at + T::kBytes + v_row * T::kRowBytes +
+                    ((((E4M3 ? 0u : (lr & 3u) >> 1)) ^ T::swz(v_row)) << 4) + (lr & 1u) * 8u;
 
     // the stage's tile into the wave's LDS.  Keys that are left out have scores
     // of -inf whatever K holds, but 0 times their V must be 0: V becomes +0.
-    auto put = [&](Stage& s) {
+    auto put = [&] {
       asm volatile("" : "+v"(put_at));
-      if (s.valid != 0xffffffffu) {
+      if (st.valid != 0xffffffffu) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i)
-          if ((s.valid >> (i * kRowsPerLoad + pr) & 1u) == 0u) s.v[i] = u32x4_t{0, 0, 0, 0};
+        for (int i = 0; i < T::kLoads; ++i)
+          if ((st.valid >> (i * T::kRowsPerLoad + pr) & 1u) == 0u) st.v[i] = u32x4_t{0, 0, 0, 0};
         asm volatile("");  // a branch, not a select in every tile
       }
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
+      for (int i = 0; i < T::kLoads; ++i) {
         // the swizzle of row i R + pr (R a power of two above pr) is that of both
-        const uint32_t at =
-            (put_at ^ swz<D>(i * kRowsPerLoad) << 4) + i * kRowsPerLoad * (2u * D);
-        if constexpr (E4M3) {
-          *reinterpret_cast<u32x4_t*>(smem + at) = widen_codes8(s.k[i][0], s.k[i][1]);
-          *reinterpret_cast<u32x4_t*>(smem + (at ^ 16u)) = widen_codes8(s.k[i][2], s.k[i][3]);
-          *reinterpret_cast<u32x4_t*>(smem + at + kKeys * 2u * D) = widen_codes8(s.v[i][0], s.v[i][1]);
-          *reinterpret_cast<u32x4_t*>(smem + (at ^ 16u) + kKeys * 2u * D) =
-              widen_codes8(s.v[i][2], s.v[i][3]);
-        } else {
-          *reinterpret_cast<u32x4_t*>(smem + at) = s.k[i];
-          *reinterpret_cast<u32x4_t*>(smem + at + kKeys * 2u * D) = s.v[i];
-        }
+        const uint32_t at = (put_at ^ T::swz(i * T::kRowsPerLoad) << 4) +
+                            i * T::kRowsPerLoad * T::kRowBytes;
+        *reinterpret_cast<u32x4_t*>(smem + at) = st.k[i];
+        *reinterpret_cast<u32x4_t*>(smem + at + T::kBytes) = st.v[i];
       }
       if constexpr (E4M3)
-        own_scales[lane] = (s.valid >> (lane & 31u) & 1u) != 0u
-                               ? s.scale * (lane < 32u ? a.scale_log2 : 1.0f)
-                               : 0.0f;
+        scales(wave)[lane] = (st.valid >> (lane & 31u) & 1u) != 0u
+                                 ? st.scale * (lane < 32u ? a.scale_log2 : 1.0f)
+                                 : 0.0f;
     };
 
     auto compute = [&](uint32_t valid) {
@@ -339,29 +364,42 @@ struct Decode {
       // loop they would take the registers of a stage
       asm volatile("" : "+v"(k_at), "+v"(v_at));
       f32x4_t sc[RT][2];
+      // Codes are widened to bf16, exactly, where the MFMA takes them.  The fp8 MFMA
+      // would take them as they are (and a query as the sum of two e4m3), but
+      // drops what is 2^-15 of its largest product: lse was off by 6e-5.
 #pragma unroll
-      for (int ds = 0; ds < D / 32; ++ds) {
-        bf16x8_t kf[2];
+      for (int f = 0; f < kFrags; f += E4M3 ? 2 : 1) {
+        bf16x8_t kf[2][E4M3 ? 2 : 1];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          kf[b] = *reinterpret_cast<const bf16x8_t*>(smem + (k_at ^ (64u * ds)) + 8u * D * b);
+          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
+              smem + (k_at ^ (E4M3 ? 32u : 64u) * f ^ T::swz(4u * b) << 4) +
+              4u * T::kRowBytes * b);
+          if constexpr (E4M3) {
+            kf[b][0] = __builtin_bit_cast(bf16x8_t, widen_codes8(x[0], x[1]));
+            kf[b][1] = __builtin_bit_cast(bf16x8_t, widen_codes8(x[2], x[3]));
+          } else {
+            kf[b][0] = __builtin_bit_cast(bf16x8_t, x);
+          }
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          const bf16x8_t qf = query(rt, ds);
+        for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-          for (int b = 0; b < 2; ++b)
-            sc[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                kf[b], qf, ds == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[rt][b], 0, 0, 0);
-        }
+          for (int h = 0; h < (E4M3 ? 2 : 1); ++h) {
+            const bf16x8_t qf = __builtin_bit_cast(bf16x8_t, query_frag(rt, f + h));
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+              sc[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  kf[b][h], qf, f + h == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[rt][b], 0, 0, 0);
+          }
       }
-      // scores to the log2 domain; lane's key j (0..7) is 8 g + j
+      // lane's key j (0..7) is 8 g + j
       float ks[8], vs[8];
       if constexpr (E4M3) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(own_scales + 8u * g + 4 * h);
-          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(own_scales + 32u + 8u * g + 4 * h);
+          const f32x4_t x = *reinterpret_cast<const f32x4_t*>(scales(wave) + 8u * g + 4 * h);
+          const f32x4_t y = *reinterpret_cast<const f32x4_t*>(scales(wave) + 32u + 8u * g + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             ks[4 * h + e] = x[e];
@@ -408,6 +446,8 @@ struct Decode {
           probabilities();
         }
         l_run[rt] += psum;
+        // two bf16 parts: the second MFMA takes what the first one's rounding
+        // (half a step, 2^-8) leaves, for 1% more time
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const float y = E4M3 ? p[j] * vs[j] : p[j];
@@ -418,15 +458,21 @@ struct Decode {
       // O^T += V^T P^T: lane i of group g receives d 16 db + i of keys 8 g .. + 7
 #pragma unroll
       for (int db = 0; db < kDb; ++db) {
-        bf16x4_t half[2];
+        bf16x8_t vf;
+        if constexpr (E4M3) {
+          const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+              (lds_i32x2_t*)(smem + (v_at ^ (16u * db))));
+          vf = __builtin_bit_cast(bf16x8_t, widen_codes8((uint32_t)c[0], (uint32_t)c[1]));
+        } else {
+          bf16x4_t half[2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
-          half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-              (lds_bf16x4_t*)(smem + (v_at ^ (32u * db)) + 8u * D * h));
-        const bf16x8_t vf = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          for (int h = 0; h < 2; ++h)
+            half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                (lds_bf16x4_t*)(smem + (v_at ^ (32u * db)) + 4u * T::kRowBytes * h));
+          vf = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-        {
+        for (int rt = 0; rt < RT; ++rt) {
           acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[rt], acc[rt][db], 0, 0, 0);
           acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[rt], acc[rt][db], 0, 0, 0);
         }
@@ -435,22 +481,18 @@ struct Decode {
 
     // A wave's LDS operations run in order, so a tile's reads see its writes and
     // the next tile's writes wait for them; the fences keep the compiler from
-    // reordering them (it sees one lane's addresses).
-    while (t < end) {
-#pragma unroll
-      for (int s = 0; s < DEPTH; ++s) {
-        if (t >= end) break;
-        put(st[s]);
-        const uint32_t valid = st[s].valid;
-        asm volatile("" ::: "memory");
-        if (t + DEPTH * kWaves < end) {
-          issue(st[s], t + DEPTH * kWaves, page[s]);
-          page[s] = entry(t + 2 * DEPTH * kWaves);
-        }
-        compute(valid);
-        asm volatile("" ::: "memory");
-        t += kWaves;
+    // reordering them (it sees one lane's addresses).  One tile is in flight while
+    // another is computed: two were no faster (8 x 32 heads x 4096: 87, 97 us).
+    for (; t < end; t += kWaves) {
+      put();
+      const uint32_t valid = st.valid;
+      asm volatile("" ::: "memory");
+      if (t + kWaves < end) {
+        issue(t + kWaves, page);
+        page = entry(t + 2u * kWaves);
       }
+      compute(valid);
+      asm volatile("" ::: "memory");
     }
     finish(seq, q_head, rows, n == sp.tiles, slot, acc, m_ref, l_run);
   }
@@ -459,9 +501,7 @@ struct Decode {
   FE2O3_DEVICE void finish(uint32_t seq, uint32_t q_head, uint32_t rows, bool whole, uint32_t slot,
                            const f32x4_t (&acc)[RT][kDb], const float (&m_ref)[RT],
                            const float (&l_run)[RT]) {
-    constexpr uint32_t kStride = D + 4u;  // floats between rows in LDS
     const uint32_t tid = thread(), lr = tid & 15u, g = tid >> 4 & 3u;
-    static_assert(16u * kStride * 4u <= wave_lds(D), "the sums reuse the tiles' LDS");
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float l = row_sum(l_run[rt]);
@@ -471,7 +511,7 @@ struct Decode {
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (rt * 16u >= rows) break;
-      float* mine = (float*)own + lr * kStride + 4u * g;
+      float* mine = (float*)(smem + wave * T::kLds) + lr * T::kSumStride + 4u * g;
 #pragma unroll
       for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(mine + 16 * db) = acc[rt][db];
       __syncthreads();
@@ -490,8 +530,8 @@ struct Decode {
         for (uint32_t w = 0; w < kWaves; ++w) {
           const float weight = __builtin_amdgcn_exp2f(s[w].x - m);
           l += weight * s[w].y;
-          y += weight * *reinterpret_cast<const f32x4_t*>((const float*)(smem + w * wave_lds(D)) +
-                                                          r * kStride + d);
+          y += weight * *reinterpret_cast<const f32x4_t*>((const float*)(smem + w * T::kLds) +
+                                                          r * T::kSumStride + d);
         }
         if (whole) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: +0
@@ -512,36 +552,39 @@ struct Decode {
 
 // One workgroup per sequence and block of query rows, for calls whose
 // sequences are too short to be worth a join.
-template <int D, bool E4M3, int RT, int DEPTH>
-__global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_whole_kernel(Args a) {
+template <int D, bool E4M3, int RT>
+__global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of(a, seq);
-  Decode<D, E4M3, RT, DEPTH>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+  Decode<D, E4M3, RT>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
-// The workgroup's run of the list of all tiles (sequence, then block of query
-// rows, then tile), which is a multiple of kWaves tiles long.
-template <int D, bool E4M3, int RT, int DEPTH>
-__global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_split_kernel(Args a) {
+// The workgroup's run of the list of all work: sequence, then block of query
+// rows, then round, a round being a tile for each wave.  What starting on a head
+// costs (its pages, queries and first loads, and the sums at the end) counts as
+// kSetup rounds before its first.
+template <int D, bool E4M3, int RT>
+__global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t lane = threadIdx.x & 63u, blocks = a.cache.kv_heads * a.blocks_per_head;
-  // tiles of all sequences; lane l scans sequence base + l, so that up to 64 of
-  // them are read once
-  auto tiles_of = [&](uint32_t s) { return s < a.seqs ? span_of(a, a.lengths[s]).tiles : 0u; };
-  uint32_t scan = wave_scan(tiles_of(lane)), tiles = at_lane(scan, 63u);
+  // lane l scans sequence base + l, so that up to 64 of them are read once
+  auto rounds_of = [&](uint32_t s) {
+    return s < a.seqs ? (span_of(a, a.lengths[s]).tiles + kWaves - 1u) / kWaves + kSetup : 0u;
+  };
+  uint32_t scan = wave_scan(rounds_of(lane)), rounds = at_lane(scan, 63u);
   const uint32_t first_scan = scan;
   for (uint32_t base = 64u; base < a.seqs; base += 64u)
-    tiles += at_lane(wave_scan(tiles_of(base + lane)), 63u);
-  const uint32_t total = tiles * blocks;
-  const uint32_t run = uniform((total - 1u) / gridDim.x / kWaves + 1u) * kWaves;
-  uint32_t at = blockIdx.x * run;  // below total + 4 grid: the host keeps it in 32 bits
+    rounds += at_lane(wave_scan(rounds_of(base + lane)), 63u);
+  const uint32_t total = rounds * blocks;
+  const uint32_t run = uniform((total - 1u) / gridDim.x + 1u);
+  uint32_t at = blockIdx.x * run;  // below total + grid: the host keeps it in 32 bits
   const uint32_t end = min(at + run, total);
   uint4 record = {0u, 0u, 0u, 0u};
   if (at < total) {
-    // the sequence that `at` falls into, and the tiles before it
+    // the sequence that `at` falls into, and the rounds before it
     uint32_t seq = 0, skipped = 0;
     scan = first_scan;
     while (true) {
@@ -554,27 +597,31 @@ __global__ void __launch_bounds__(kThreads, RT == 1 ? 2 : 1) paged_split_kernel(
       }
       skipped += at_lane(scan, 63u);
       seq += 64u;
-      scan = wave_scan(tiles_of(seq + lane));
+      scan = wave_scan(rounds_of(seq + lane));
     }
     const uint32_t rest = at - skipped * blocks;
     Span sp = uniform_span_of(a, seq);
-    uint32_t hb = uniform(rest / sp.tiles), tile = rest - hb * sp.tiles;
-    Decode<D, E4M3, RT, DEPTH> decode(a, smem);
+    uint32_t length = (sp.tiles + kWaves - 1u) / kWaves + kSetup;  // of a head, in rounds
+    uint32_t hb = uniform(rest / length), pos = rest - hb * length;
+    Decode<D, E4M3, RT> decode(a, smem);
     while (true) {
-      const uint32_t n = min(sp.tiles - tile, end - at);
+      const uint32_t stop = min(length, pos + (end - at));
+      const uint32_t tile = kWaves * (max(pos, kSetup) - kSetup);
+      const uint32_t tile_end = min(sp.tiles, kWaves * (max(stop, kSetup) - kSetup));
       // begun before this run: place 0; begun in it and going on: place 1
-      decode.run(seq, hb, sp, tile, n, tile == 0u ? 1u : 0u);
-      at += n;
+      if (tile < tile_end)
+        decode.run(seq, hb, sp, tile, tile_end - tile, tile == 0u ? 1u : 0u);
+      at += stop - pos;
       if (at >= end) {
-        const uint32_t left = sp.tiles - tile - n;
-        if (tile == 0u && left != 0u)  // as many runs as what is left reaches into
-          record = uint4{1u, (left - 1u) / run + 1u, seq, hb};
+        if (tile == 0u && tile_end != 0u && stop < length)  // the runs that the rest reaches into
+          record = uint4{1u, (length - stop - 1u) / run + 1u, seq, hb};
         break;
       }
-      tile = 0u;
+      pos = 0u;
       if (++hb == blocks) {
         hb = 0u;
         sp = uniform_span_of(a, ++seq);
+        length = (sp.tiles + kWaves - 1u) / kWaves + kSetup;
       }
     }
   }
@@ -640,31 +687,30 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(Args a) {
     a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
-template <bool E4M3, int RT>
-constexpr int depth_of() {
-  return E4M3 && RT == 1 ? 2 : 1;
-}
-
 template <int D, bool E4M3, int RT>
-int32_t launch(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
-  constexpr int kDepth = depth_of<E4M3, RT>();
-  constexpr uint32_t kSmem = smem_bytes<D, RT>();
-  const auto whole_fn = paged_whole_kernel<D, E4M3, RT, kDepth>;
-  const auto split_fn = paged_split_kernel<D, E4M3, RT, kDepth>;
+int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
+  constexpr uint32_t kSmem = Lds<D, E4M3, RT>::kBytes;
+  const auto whole_fn = paged_whole_kernel<D, E4M3, RT>;
+  const auto split_fn = paged_split_kernel<D, E4M3, RT>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds(
       {(const void*)whole_fn, (const void*)split_fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
-  if (whole) {
-    const dim3 grid(workgroups < kGridX ? workgroups : kGridX, (workgroups - 1u) / kGridX + 1u);
+  const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
+  if (tiles <= (2u + kSetup) * kWaves) {
+    const dim3 grid(heads < kGridX ? heads : kGridX, (heads - 1u) / kGridX + 1u);
     whole_fn<<<grid, kThreads, kSmem, s>>>(a);
     return fe2o3_host::after_launch();
   }
+  // as many workgroups as are resident at once, and work for each wave
+  const uint64_t most = heads * ((tiles + kWaves - 1u) / kWaves);
+  uint32_t workgroups = per_cu<D, E4M3, RT>() * cus;
+  if (workgroups > kMaxWorkgroups) workgroups = kMaxWorkgroups;
+  if (workgroups > most) workgroups = (uint32_t)most;
   split_fn<<<workgroups, kThreads, kSmem, s>>>(a);
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
   // Few heads have many parts each, which a row's threads share; many have few,
   // and rows share the threads.
-  const uint64_t heads = (uint64_t)a.seqs * a.cache.kv_heads * a.blocks_per_head;
   constexpr int kRows = (int)(kThreads / (D / 4));
   if (a.rows >= (uint32_t)kRows && heads * 8u >= workgroups)
     paged_join_kernel<D, kRows>
@@ -677,16 +723,16 @@ int32_t launch(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
 }
 
 template <int D, bool E4M3>
-int32_t launch_rows(const Args& a, bool whole, uint32_t workgroups, hipStream_t s) {
-  if (a.rows <= 16u) return launch<D, E4M3, 1>(a, whole, workgroups, s);
-  if (a.rows <= 32u) return launch<D, E4M3, 2>(a, whole, workgroups, s);
-  if (a.rows <= 48u) return launch<D, E4M3, 3>(a, whole, workgroups, s);
-  return launch<D, E4M3, 4>(a, whole, workgroups, s);
+int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
+  if (a.rows <= 16u) return launch<D, E4M3, 1>(a, tiles, cus, s);
+  if (a.rows <= 32u) return launch<D, E4M3, 2>(a, tiles, cus, s);
+  if (a.rows <= 48u) return launch<D, E4M3, 3>(a, tiles, cus, s);
+  return launch<D, E4M3, 4>(a, tiles, cus, s);
 }
 
 #define FE2O3_PAGED(D, F, RT)                                                                  \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F "," #RT ">", (const void*)paged_whole_kernel<D, F, RT, depth_of<F, RT>()>, kThreads, smem_bytes<D, RT>()}), \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_split_kernel<" #D "," #F "," #RT ">", (const void*)paged_split_kernel<D, F, RT, depth_of<F, RT>()>, kThreads, smem_bytes<D, RT>()})
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F "," #RT ">", (const void*)paged_whole_kernel<D, F, RT>, kThreads, Lds<D, F, RT>::kBytes}), \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_split_kernel<" #D "," #F "," #RT ">", (const void*)paged_split_kernel<D, F, RT>, kThreads, Lds<D, F, RT>::kBytes})
 #define FE2O3_JOIN(D, ROWS)                                                                    \
   fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #ROWS ">", (const void*)paged_join_kernel<D, ROWS>, kThreads, 0})
 const fe2o3_host::KernelRegistrar kRegistered[] = {
@@ -724,7 +770,8 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   const uint64_t row = (uint64_t)q_heads * d;
   // every product below is of factors that keep it under 2^64
   const uint64_t blocks = (uint64_t)kv_heads * blocks_per_head;  // at most q_heads
-  const uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys + 1u;  // a window may add one
+  // a window may add a tile; what a head's start counts for is within these
+  const uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys + 1u + kWaves * kSetup;
   if (blocks * tiles >= (UINT64_C(1) << 31) || seqs * (blocks * tiles) >= (UINT64_C(1) << 31))
     return FE2O3_ERR_SHAPE;
   if (seqs > 1u && q_stride < row) return FE2O3_ERR_STRIDE;
@@ -767,21 +814,11 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.max_length = max_length;
   a.window = window;
   a.scale_log2 = scale * 1.4426950408889634f;
-  const uint64_t units = seqs * blocks;
-  const bool whole = tiles <= 2u * kWaves;
-  uint32_t workgroups = (uint32_t)units;
-  if (!whole) {
-    const uint64_t most = units * ((tiles + kWaves - 1u) / kWaves);
-    // as many as are resident at once: two a CU of one tile of query rows, else one
-    const uint32_t resident = (a.rows <= 16u ? 2u : 1u) * topo.cus;
-    const uint32_t slots = resident < kMaxWorkgroups ? resident : kMaxWorkgroups;
-    workgroups = (uint32_t)(most < slots ? most : slots);
-  }
   hipStream_t s = (hipStream_t)stream;
   const bool e4m3 = cache->format == FE2O3_KV_E4M3;
   if (d == 64u)
-    return e4m3 ? launch_rows<64, true>(a, whole, workgroups, s)
-                : launch_rows<64, false>(a, whole, workgroups, s);
-  return e4m3 ? launch_rows<128, true>(a, whole, workgroups, s)
-              : launch_rows<128, false>(a, whole, workgroups, s);
+    return e4m3 ? launch_rows<64, true>(a, tiles, topo.cus, s)
+                : launch_rows<64, false>(a, tiles, topo.cus, s);
+  return e4m3 ? launch_rows<128, true>(a, tiles, topo.cus, s)
+              : launch_rows<128, false>(a, tiles, topo.cus, s);
 }
