@@ -30,9 +30,9 @@
 // The tiles of all sequences and KV heads, one behind another, are dealt in
 // equal runs to as many workgroups as the device holds, so that one long
 // sequence fills it as well as many, and mixed lengths leave no tail.  Each
-// workgroup finds its run from the lengths.  A run that a sequence's head
-// does not fit into leaves its sums in the workspace; paged_join_kernel adds
-// those of each head in the order of the keys.
+// workgroup finds its run from the lengths.  A head that takes more than one run
+// has its sums in the workspace; paged_join_kernel adds them in the order of the
+// keys.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -44,11 +44,6 @@ using kv_cache::View;
 
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
 constexpr uint32_t kKeys = 32;              // keys per tile
-#ifdef XSETUP
-constexpr uint32_t kSetup = XSETUP;
-#else
-constexpr uint32_t kSetup = 1;              // rounds that a head's start counts for
-#endif
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
 constexpr uint32_t kGridX = 1u << 22;       // a grid holds fewer than 2^32 threads a dimension
@@ -60,12 +55,11 @@ struct Args {
   const uint32_t *table, *lengths;
   uint16_t* o;
   float* lse;
-  uint4* records;  // workspace: the head that each workgroup's run leaves unfinished,
-  float* stats;    // reference and sum, [workgroup][2][rows][2],
-  float* sums;     // and weighted V, [workgroup][2][rows][head_dim]
+  float* stats;  // workspace: reference and sum, [workgroup][2][rows][2],
+  float* sums;   // and weighted V, [workgroup][2][rows][head_dim]
   uint64_t q_stride;
   uint32_t seqs, q_heads, group, blocks_per_head, rows;  // rows: per block, at most kBlockRows
-  uint32_t table_cols, max_length, window;
+  uint32_t table_cols, max_length, window, workgroups;
   float scale_log2;
 };
 
@@ -178,11 +172,13 @@ constexpr int per_cu() {
   return D == 64 ? 3 : 2;
 }
 
-// D: head_dim.  RT: query-row tiles of 16.
-template <int D, bool E4M3, int RT>
+// D: head_dim.  RT: query-row tiles of 16.  WH: KV heads that a workgroup works on
+// at once, kWaves / WH waves on each.
+template <int D, bool E4M3, int RT, int WH>
 struct Decode {
   using T = Tile<D, E4M3>;
   using L = Lds<D, E4M3, RT>;
+  static constexpr uint32_t kStep = kWaves / WH;  // tiles of a head per round
   static constexpr int kDb = D / 16;     // V^T row blocks
   static constexpr int kFrags = D / 32;  // 16-byte pieces of a query operand per lane
 
@@ -234,14 +230,14 @@ struct Decode {
     return r;
   }
 
-  // Keys of tiles [tile, tile + n) of sequence `seq` for block `hb` of the KV
-  // heads' query rows.  Place `slot` of this workgroup's workspace takes the
-  // sums unless they are the span's every tile.
-  FE2O3_DEVICE void run(uint32_t seq, uint32_t hb, const Span& sp, uint32_t tile, uint32_t n,
+  // Keys of tiles [tile, tile + n) of sequence `seq` for blocks hb0 .. hb0 + WH - 1
+  // of the KV heads' query rows.  Place `slot` of this workgroup's workspace
+  // takes the sums unless they are the span's every tile.
+  FE2O3_DEVICE void run(uint32_t seq, uint32_t hb0, const Span& sp, uint32_t tile, uint32_t n,
                         uint32_t slot) {
     const uint32_t tid = thread(), lane = tid & 63u, lr = lane & 15u, g = lane >> 4;
-    const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
-    const uint32_t row0 = block * kBlockRows;             // of the group
+    const uint32_t head = WH > 1 ? hb0 + wave / kStep : hb0 / a.blocks_per_head;
+    const uint32_t row0 = WH > 1 ? 0u : (hb0 - head * a.blocks_per_head) * kBlockRows;
     const uint32_t rows = min(a.group - row0, (uint32_t)kBlockRows);
     const uint32_t q_head = head * a.group + row0;
     const uint32_t* table = a.table + (uint64_t)seq * a.table_cols;
@@ -252,7 +248,7 @@ struct Decode {
     const float* sb = (lane < 32u ? a.cache.k_scale : a.cache.v_scale);
 
     const uint32_t end = sp.tile0 + tile + n;
-    uint32_t t = sp.tile0 + tile + wave;
+    uint32_t t = sp.tile0 + tile + wave % kStep;
     // the table's entry for this lane's key of tile t; none past the run
     auto entry = [&](uint32_t at) {
       const uint32_t key = at * kKeys + (lane & 31u);
@@ -319,7 +315,7 @@ struct Decode {
 
     if (t < end) {
       issue(t, page);
-      page = entry(t + kWaves);
+      page = entry(t + kStep);
     }
 
     // LDS addresses.  The wave's tile is aligned to 256 bytes and the swizzle
@@ -483,21 +479,22 @@ struct Decode {
     // the next tile's writes wait for them; the fences keep the compiler from
     // reordering them (it sees one lane's addresses).  One tile is in flight while
     // another is computed: two were no faster (8 x 32 heads x 4096: 87, 97 us).
-    for (; t < end; t += kWaves) {
+    for (; t < end; t += kStep) {
       put();
       const uint32_t valid = st.valid;
       asm volatile("" ::: "memory");
-      if (t + kWaves < end) {
-        issue(t + kWaves, page);
-        page = entry(t + 2u * kWaves);
+      if (t + kStep < end) {
+        issue(t + kStep, page);
+        page = entry(t + 2u * kStep);
       }
       compute(valid);
       asm volatile("" ::: "memory");
     }
-    finish(seq, q_head, rows, n == sp.tiles, slot, acc, m_ref, l_run);
+    finish(seq, q_head - wave / kStep * a.group, rows, n == sp.tiles, slot, acc, m_ref, l_run);
   }
 
-  // The waves' sums of a run added in wave order, 16 query rows at a time.
+  // The sums of a run's waves added for each head in wave order, 16 query rows at a
+  // time.  q_head: the first head's first.
   FE2O3_DEVICE void finish(uint32_t seq, uint32_t q_head, uint32_t rows, bool whole, uint32_t slot,
                            const f32x4_t (&acc)[RT][kDb], const float (&m_ref)[RT],
                            const float (&l_run)[RT]) {
@@ -507,7 +504,7 @@ struct Decode {
       const float l = row_sum(l_run[rt]);
       if (g == 0u) stat(wave)[rt * 16u + lr] = float2{m_ref[rt], l};
     }
-    const uint64_t part = ((uint64_t)blockIdx.x * 2u + slot) * a.rows;
+    const uint64_t part = ((uint64_t)blockIdx.x * 2u + slot) * WH * a.rows;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (rt * 16u >= rows) break;
@@ -515,34 +512,38 @@ struct Decode {
 #pragma unroll
       for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(mine + 16 * db) = acc[rt][db];
       __syncthreads();
-      const uint32_t count = min(rows - rt * 16u, 16u) * (D / 4u);
+      const uint32_t count = WH * min(rows - rt * 16u, 16u) * (D / 4u);
       for (uint32_t i = tid; i < count; i += kThreads) {
-        const uint32_t r = i / (D / 4u), d = 4u * (i % (D / 4u)), row = rt * 16u + r;
-        float2 s[kWaves];
+        // rows of one head behind another's: RT > 1 has one head
+        const uint32_t at = i / (D / 4u), d = 4u * (i % (D / 4u));
+        const uint32_t wh = WH > 1 ? at / rows : 0u, r = at - wh * rows, row = rt * 16u + r;
+        float2 s[kStep];
         float m = -__FLT_MAX__, l = 0.0f;
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) {
-          s[w] = stat(w)[row];
-          m = fmaxf(m, s[w].x);
+        for (uint32_t x = 0; x < kStep; ++x) {
+          s[x] = stat(wh * kStep + x)[row];
+          m = fmaxf(m, s[x].x);
         }
         f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) {
-          const float weight = __builtin_amdgcn_exp2f(s[w].x - m);
-          l += weight * s[w].y;
-          y += weight * *reinterpret_cast<const f32x4_t*>((const float*)(smem + w * T::kLds) +
-                                                          r * T::kSumStride + d);
+        for (uint32_t x = 0; x < kStep; ++x) {
+          const float weight = __builtin_amdgcn_exp2f(s[x].x - m);
+          l += weight * s[x].y;
+          y += weight * *reinterpret_cast<const f32x4_t*>(
+                            (const float*)(smem + (wh * kStep + x) * T::kLds) +
+                            r * T::kSumStride + d);
         }
         if (whole) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: +0
-          const uint64_t out = (uint64_t)seq * a.q_heads + q_head + row;
+          const uint64_t out = (uint64_t)seq * a.q_heads + q_head + wh * a.group + row;
           *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
               u32x2_t{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
           if (a.lse != nullptr && d == 0u)
             a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
         } else {
-          *reinterpret_cast<f32x4_t*>(a.sums + (part + row) * D + d) = y;
-          if (d == 0u) *reinterpret_cast<float2*>(a.stats + (part + row) * 2u) = float2{m, l};
+          const uint64_t p = part + wh * a.rows + row;
+          *reinterpret_cast<f32x4_t*>(a.sums + p * D + d) = y;
+          if (d == 0u) *reinterpret_cast<float2*>(a.stats + p * 2u) = float2{m, l};
         }
       }
       __syncthreads();
@@ -559,166 +560,204 @@ __global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_whole
   const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of(a, seq);
-  Decode<D, E4M3, RT>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+  Decode<D, E4M3, RT, 1>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
-// The workgroup's run of the list of all work: sequence, then block of query
-// rows, then round, a round being a tile for each wave.  What starting on a head
-// costs (its pages, queries and first loads, and the sums at the end) counts as
-// kSetup rounds before its first.
-template <int D, bool E4M3, int RT>
-__global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split_kernel(Args a) {
-  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  const uint32_t lane = threadIdx.x & 63u, blocks = a.cache.kv_heads * a.blocks_per_head;
-  // lane l scans sequence base + l, so that up to 64 of them are read once
-  auto rounds_of = [&](uint32_t s) {
-    return s < a.seqs ? (span_of(a, a.lengths[s]).tiles + kWaves - 1u) / kWaves + kSetup : 0u;
-  };
-  uint32_t scan = wave_scan(rounds_of(lane)), rounds = at_lane(scan, 63u);
-  const uint32_t first_scan = scan;
-  for (uint32_t base = 64u; base < a.seqs; base += 64u)
-    rounds += at_lane(wave_scan(rounds_of(base + lane)), 63u);
-  const uint32_t total = rounds * blocks;
-  const uint32_t run = uniform((total - 1u) / gridDim.x + 1u);
-  uint32_t at = blockIdx.x * run;  // below total + grid: the host keeps it in 32 bits
-  const uint32_t end = min(at + run, total);
-  uint4 record = {0u, 0u, 0u, 0u};
-  if (at < total) {
-    // the sequence that `at` falls into, and the rounds before it
-    uint32_t seq = 0, skipped = 0;
-    scan = first_scan;
+// The list of all work: sequence, then block of query rows (or WH KV heads), then
+// round, a round being a tile for each wave.  What starting on a head costs (its
+// pages, queries and first loads, and the sums at the end) counts as kSetup
+// rounds before its first.  Workgroup i takes rounds i run .. + run - 1.
+template <int RT, int WH>
+struct Plan {
+  static constexpr uint32_t kStep = kWaves / WH, kSetup = RT == 1 ? 1u : 2u;
+  const Args& a;
+  uint32_t lane, blocks;
+  uint32_t first_scan;  // rounds of a block of sequences 0 .. lane
+  uint32_t total, run;
+
+  static FE2O3_DEVICE uint32_t rounds(const Span& sp) {
+    return (sp.tiles + kStep - 1u) / kStep + kSetup;
+  }
+  // of sequence base + lane and those from base on before it
+  FE2O3_DEVICE uint32_t scan(uint32_t base) const {
+    const uint32_t s = base + lane;
+    return wave_scan(s < a.seqs ? rounds(span_of(a, a.lengths[s])) : 0u);
+  }
+  FE2O3_DEVICE explicit Plan(const Args& args)
+      : a(args), lane(threadIdx.x & 63u), blocks(a.cache.kv_heads * a.blocks_per_head / WH) {
+    first_scan = scan(0u);
+    total = at_lane(first_scan, 63u);
+    for (uint32_t base = 64u; base < a.seqs; base += 64u) total += at_lane(scan(base), 63u);
+    total *= blocks;
+    run = uniform((total - 1u) / a.workgroups + 1u);
+  }
+  // the sequence that round `at` falls into, and the rounds of a block before it
+  FE2O3_DEVICE uint32_t find(uint32_t at, uint32_t* before) const {
+    uint32_t seq = 0, skipped = 0, sums = first_scan;
     while (true) {
-      const uint32_t before =
-          (uint32_t)__popcll(__ballot(seq + lane < a.seqs && (skipped + scan) * blocks <= at));
-      if (before < 64u) {
-        if (before != 0u) skipped += at_lane(scan, before - 1u);
-        seq += before;
-        break;
+      const uint32_t n =
+          (uint32_t)__popcll(__ballot(seq + lane < a.seqs && (skipped + sums) * blocks <= at));
+      if (n < 64u) {
+        *before = n != 0u ? skipped + at_lane(sums, n - 1u) : skipped;
+        return seq + n;
       }
-      skipped += at_lane(scan, 63u);
+      skipped += at_lane(sums, 63u);
       seq += 64u;
-      scan = wave_scan(rounds_of(seq + lane));
-    }
-    const uint32_t rest = at - skipped * blocks;
-    Span sp = uniform_span_of(a, seq);
-    uint32_t length = (sp.tiles + kWaves - 1u) / kWaves + kSetup;  // of a head, in rounds
-    uint32_t hb = uniform(rest / length), pos = rest - hb * length;
-    Decode<D, E4M3, RT> decode(a, smem);
-    while (true) {
-      const uint32_t stop = min(length, pos + (end - at));
-      const uint32_t tile = kWaves * (max(pos, kSetup) - kSetup);
-      const uint32_t tile_end = min(sp.tiles, kWaves * (max(stop, kSetup) - kSetup));
-      // begun before this run: place 0; begun in it and going on: place 1
-      if (tile < tile_end)
-        decode.run(seq, hb, sp, tile, tile_end - tile, tile == 0u ? 1u : 0u);
-      at += stop - pos;
-      if (at >= end) {
-        if (tile == 0u && tile_end != 0u && stop < length)  // the runs that the rest reaches into
-          record = uint4{1u, (length - stop - 1u) / run + 1u, seq, hb};
-        break;
-      }
-      pos = 0u;
-      if (++hb == blocks) {
-        hb = 0u;
-        sp = uniform_span_of(a, ++seq);
-        length = (sp.tiles + kWaves - 1u) / kWaves + kSetup;
-      }
+      sums = scan(seq);
     }
   }
-  if (threadIdx.x == 0u) a.records[blockIdx.x] = record;
+  // the rounds of a block before sequence seq
+  FE2O3_DEVICE uint32_t before(uint32_t seq) const {
+    uint32_t skipped = 0, sums = first_scan;
+    for (uint32_t base = 0; base + 64u <= seq; base += 64u) {
+      skipped += at_lane(sums, 63u);
+      sums = scan(base + 64u);
+    }
+    return seq % 64u != 0u ? skipped + at_lane(sums, seq % 64u - 1u) : skipped;
+  }
+};
+
+template <int D, bool E4M3, int RT, int WH>
+__global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split_kernel(Args a) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  using P = Plan<RT, WH>;
+  const P plan(a);
+  uint32_t at = blockIdx.x * plan.run;  // below total + grid: the host keeps it in 32 bits
+  const uint32_t end = min(at + plan.run, plan.total);
+  if (at >= plan.total) return;
+  uint32_t before;
+  uint32_t seq = plan.find(at, &before);
+  const uint32_t rest = at - before * plan.blocks;
+  Span sp = uniform_span_of(a, seq);
+  uint32_t length = P::rounds(sp);
+  uint32_t hb = uniform(rest / length), pos = rest - hb * length;
+  Decode<D, E4M3, RT, WH> decode(a, smem);
+  while (true) {
+    const uint32_t stop = min(length, pos + (end - at));
+    const uint32_t tile = P::kStep * (max(pos, P::kSetup) - P::kSetup);
+    const uint32_t tile_end = min(sp.tiles, P::kStep * (max(stop, P::kSetup) - P::kSetup));
+    // begun before this run: place 0; begun in it and going on: place 1
+    if (tile < tile_end)
+      decode.run(seq, hb * WH, sp, tile, tile_end - tile, tile == 0u ? 1u : 0u);
+    at += stop - pos;
+    if (at >= end) return;
+    pos = 0u;
+    if (++hb == plan.blocks) {
+      hb = 0u;
+      sp = uniform_span_of(a, ++seq);
+      length = P::rounds(sp);
+    }
+  }
 }
 
-// Query rows blockIdx.y * ROWS .. of the head that run blockIdx.x began and did
-// not finish: place 1 of that run and place 0 of the runs that follow, in order.
-// D / 4 threads cover a row; the threads that ROWS rows leave over take every
-// kWays-th part of them.
-template <int D, int ROWS>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(Args a) {
-  const uint4 record = a.records[blockIdx.x];
-  if (record.x == 0u) return;
-  const uint32_t parts = record.y + 1u, seq = record.z, hb = record.w;
-  const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
-  constexpr uint32_t kQuads = D / 4u, kWays = kThreads / (kQuads * ROWS);
+// Query rows blockIdx.y * ROWS .. of sequence and block (or WH heads) blockIdx.x:
+// the sums that the runs over it left, if it took more than one: place 1 of the
+// run that began it and place 0 of the runs that follow, in order.  D / 4 threads
+// cover a row; the threads that ROWS rows leave over take every kWays-th part.
+template <int D, int RT, int WH, int ROWS, int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a) {
+  using P = Plan<RT, WH>;
+  const P plan(a);
+  const uint32_t seq = uniform(blockIdx.x / plan.blocks), hb = blockIdx.x - seq * plan.blocks;
+  const Span sp = uniform_span_of(a, seq);
+  const uint32_t length = P::rounds(sp), start = plan.before(seq) * plan.blocks + hb * length;
+  const uint32_t first = uniform((start + P::kSetup) / plan.run);
+  const uint32_t parts = uniform((start + length - 1u) / plan.run) - first + 1u;
+  if (parts == 1u) return;
+  constexpr uint32_t kQuads = D / 4u, kWays = THREADS / (kQuads * ROWS);
   const uint32_t quad = threadIdx.x % kQuads, d = 4u * quad;
   const uint32_t r = threadIdx.x / kQuads % ROWS, way = threadIdx.x / (kQuads * ROWS);
-  const uint32_t row = blockIdx.y * ROWS + r;
-  const bool has = row < a.rows && block * kBlockRows + row < a.group;
-  auto at = [&](uint32_t i) {
-    return ((uint64_t)(blockIdx.x + i) * 2u + (i == 0u ? 1u : 0u)) * a.rows + (has ? row : 0u);
-  };
-  // each way keeps a reference of its own
+  const uint32_t row = blockIdx.y * ROWS + r;  // one head's behind another's
+  float m = -__FLT_MAX__, l = 0.0f;
   f32x4_t y = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.0f, m = -__FLT_MAX__;
-#pragma unroll 4
-  for (uint32_t i = way; i < parts; i += kWays) {
-    const uint64_t p = at(i);
-    const float2 s = *reinterpret_cast<const float2*>(a.stats + p * 2u);
-    const f32x4_t x = *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d);
+  auto add = [&](float2 s, f32x4_t x) {
     const float top = fmaxf(m, s.x);
     const float old = __builtin_amdgcn_exp2f(m - top), weight = __builtin_amdgcn_exp2f(s.x - top);
     m = top;
     l = l * old + weight * s.y;
     y = y * old + weight * x;
+  };
+#pragma unroll 4
+  for (uint32_t i = way; i < parts; i += kWays) {
+    const uint64_t p = ((uint64_t)(first + i) * 2u + (i == 0u ? 1u : 0u)) * WH * a.rows +
+                       min(row, WH * a.rows - 1u);
+    add(*reinterpret_cast<const float2*>(a.stats + p * 2u),
+        *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d));
   }
   if constexpr (kWays > 1u) {
-    __shared__ f32x4_t part_sum[kThreads];
-    __shared__ float2 part_stat[kThreads];
+    __shared__ f32x4_t part_sum[THREADS];
+    __shared__ float2 part_stat[THREADS];
     part_sum[threadIdx.x] = y;
     part_stat[threadIdx.x] = float2{m, l};
     __syncthreads();
     if (way != 0u) return;
-#pragma unroll
-    for (uint32_t w = 1; w < kWays; ++w) {
-      const uint32_t from = w * kQuads * ROWS + threadIdx.x;
-      const float2 s = part_stat[from];
-      const float top = fmaxf(m, s.x);
-      const float old = __builtin_amdgcn_exp2f(m - top), weight = __builtin_amdgcn_exp2f(s.x - top);
-      m = top;
-      l = l * old + weight * s.y;
-      y = y * old + weight * part_sum[from];
-    }
+#pragma unroll 8
+    for (uint32_t w = 1; w < kWays; ++w)
+      add(part_stat[w * kQuads * ROWS + threadIdx.x], part_sum[w * kQuads * ROWS + threadIdx.x]);
+  }
+  uint32_t q_head;
+  bool has = row < WH * a.rows;
+  if constexpr (WH > 1) {  // a.rows is the group
+    q_head = hb * WH * a.group + row;
+  } else {
+    const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
+    has = has && block * kBlockRows + row < a.group;
+    q_head = head * a.group + block * kBlockRows + row;
   }
   if (!has) return;
   const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-  const uint64_t out = (uint64_t)seq * a.q_heads + head * a.group + block * kBlockRows + row;
+  const uint64_t out = (uint64_t)seq * a.q_heads + q_head;
   *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
       u32x2_t{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
   if (a.lse != nullptr && d == 0u)
     a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
-template <int D, bool E4M3, int RT>
-int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
+template <int D, bool E4M3, int RT, int WH>
+int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   constexpr uint32_t kSmem = Lds<D, E4M3, RT>::kBytes;
-  const auto whole_fn = paged_whole_kernel<D, E4M3, RT>;
-  const auto split_fn = paged_split_kernel<D, E4M3, RT>;
-  static const int32_t lds_rc = fe2o3_host::set_dynamic_lds(
-      {(const void*)whole_fn, (const void*)split_fn}, (int)kSmem);
+  const auto fn = paged_split_kernel<D, E4M3, RT, WH>;
+  static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
-  const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
-  if (tiles <= (2u + kSetup) * kWaves) {
-    const dim3 grid(heads < kGridX ? heads : kGridX, (heads - 1u) / kGridX + 1u);
-    whole_fn<<<grid, kThreads, kSmem, s>>>(a);
-    return fe2o3_host::after_launch();
-  }
   // as many workgroups as are resident at once, and work for each wave
-  const uint64_t most = heads * ((tiles + kWaves - 1u) / kWaves);
+  const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head / WH;
+  const uint64_t most = heads * ((tiles + kWaves / WH - 1u) / (kWaves / WH));
   uint32_t workgroups = per_cu<D, E4M3, RT>() * cus;
   if (workgroups > kMaxWorkgroups) workgroups = kMaxWorkgroups;
   if (workgroups > most) workgroups = (uint32_t)most;
-  split_fn<<<workgroups, kThreads, kSmem, s>>>(a);
+  a.workgroups = workgroups;
+  fn<<<workgroups, kThreads, kSmem, s>>>(a);
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
-  // Few heads have many parts each, which a row's threads share; many have few,
-  // and rows share the threads.
-  constexpr int kRows = (int)(kThreads / (D / 4));
-  if (a.rows >= (uint32_t)kRows && heads * 8u >= workgroups)
-    paged_join_kernel<D, kRows>
-        <<<dim3(workgroups, (a.rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a);
-  else if (a.rows >= 4u && heads * 16u >= workgroups)
-    paged_join_kernel<D, 4><<<dim3(workgroups, (a.rows - 1u) / 4u + 1u), kThreads, 0, s>>>(a);
+  // Many heads have few parts each, and rows share the threads; few have many,
+  // which a row's threads share.
+  constexpr int kRows = kThreads / (D / 4);
+  const uint32_t rows = WH * a.rows;
+  if (heads * 4u >= workgroups)
+    paged_join_kernel<D, RT, WH, kRows, kThreads>
+        <<<dim3(heads, (rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a);
+  else if (heads * 32u >= workgroups)
+    paged_join_kernel<D, RT, WH, 1, kThreads><<<dim3(heads, rows), kThreads, 0, s>>>(a);
   else
-    paged_join_kernel<D, 1><<<dim3(workgroups, a.rows), kThreads, 0, s>>>(a);
+    paged_join_kernel<D, RT, WH, 1, 1024><<<dim3(heads, rows), 1024, 0, s>>>(a);
+  return fe2o3_host::after_launch();
+}
+
+template <int D, bool E4M3, int RT>
+int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
+  if (tiles > (2u + 2u) * kWaves) {
+    if constexpr (RT == 1)
+      if (a.cache.kv_heads % kWaves == 0u)
+        return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
+    return launch_split<D, E4M3, RT, 1>(a, tiles, cus, s);
+  }
+  constexpr uint32_t kSmem = Lds<D, E4M3, RT>::kBytes;
+  const auto fn = paged_whole_kernel<D, E4M3, RT>;
+  static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
+  if (lds_rc != FE2O3_OK) return lds_rc;
+  const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
+  const dim3 grid(heads < kGridX ? heads : kGridX, (heads - 1u) / kGridX + 1u);
+  fn<<<grid, kThreads, kSmem, s>>>(a);
   return fe2o3_host::after_launch();
 }
 
@@ -730,22 +769,34 @@ int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) 
   return launch<D, E4M3, 4>(a, tiles, cus, s);
 }
 
-#define FE2O3_PAGED(D, F, RT)                                                                  \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F "," #RT ">", (const void*)paged_whole_kernel<D, F, RT>, kThreads, Lds<D, F, RT>::kBytes}), \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_split_kernel<" #D "," #F "," #RT ">", (const void*)paged_split_kernel<D, F, RT>, kThreads, Lds<D, F, RT>::kBytes})
-#define FE2O3_JOIN(D, ROWS)                                                                    \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #ROWS ">", (const void*)paged_join_kernel<D, ROWS>, kThreads, 0})
+#define FE2O3_KERNEL(NAME, FN, LDS) \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", NAME, (const void*)FN, kThreads, LDS})
+#define FE2O3_SPLIT(D, F, RT, WH) \
+  FE2O3_KERNEL("paged_split_kernel<" #D "," #F "," #RT "," #WH ">", (paged_split_kernel<D, F, RT, WH>), (Lds<D, F, RT>::kBytes))
+#define FE2O3_PAGED(D, F, RT) \
+  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT ">", (paged_whole_kernel<D, F, RT>), (Lds<D, F, RT>::kBytes)), \
+  FE2O3_SPLIT(D, F, RT, 1)
+#define FE2O3_PAGED_ALL(D, F) \
+  FE2O3_PAGED(D, F, 1), FE2O3_PAGED(D, F, 2), FE2O3_PAGED(D, F, 3), FE2O3_PAGED(D, F, 4), \
+  FE2O3_SPLIT(D, F, 1, 4)
+#define FE2O3_JOIN_OF(D, RT, WH, ROWS, THREADS)                                                \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #RT "," #WH "," #ROWS ">", (const void*)paged_join_kernel<D, RT, WH, ROWS, THREADS>, THREADS, 0})
+#define FE2O3_JOIN(D, RT, WH, ROWS) \
+  FE2O3_JOIN_OF(D, RT, WH, ROWS, kThreads), FE2O3_JOIN_OF(D, RT, WH, 1, kThreads), \
+  FE2O3_JOIN_OF(D, RT, WH, 1, 1024)
+#define FE2O3_JOIN_ALL(D, ROWS) \
+  FE2O3_JOIN(D, 1, 1, ROWS), FE2O3_JOIN(D, 1, 4, ROWS), FE2O3_JOIN(D, 2, 1, ROWS), \
+  FE2O3_JOIN(D, 3, 1, ROWS), FE2O3_JOIN(D, 4, 1, ROWS)
 const fe2o3_host::KernelRegistrar kRegistered[] = {
-    FE2O3_PAGED(64, false, 1), FE2O3_PAGED(64, false, 2), FE2O3_PAGED(64, false, 3),
-    FE2O3_PAGED(64, false, 4), FE2O3_PAGED(64, true, 1), FE2O3_PAGED(64, true, 2),
-    FE2O3_PAGED(64, true, 3), FE2O3_PAGED(64, true, 4), FE2O3_PAGED(128, false, 1),
-    FE2O3_PAGED(128, false, 2), FE2O3_PAGED(128, false, 3), FE2O3_PAGED(128, false, 4),
-    FE2O3_PAGED(128, true, 1), FE2O3_PAGED(128, true, 2), FE2O3_PAGED(128, true, 3),
-    FE2O3_PAGED(128, true, 4),
-    FE2O3_JOIN(64, 1), FE2O3_JOIN(64, 4), FE2O3_JOIN(64, 16),
-    FE2O3_JOIN(128, 1), FE2O3_JOIN(128, 4), FE2O3_JOIN(128, 8)};
+    FE2O3_PAGED_ALL(64, false), FE2O3_PAGED_ALL(64, true), FE2O3_PAGED_ALL(128, false),
+    FE2O3_PAGED_ALL(128, true), FE2O3_JOIN_ALL(64, 16), FE2O3_JOIN_ALL(128, 8)};
+#undef FE2O3_KERNEL
+#undef FE2O3_SPLIT
+#undef FE2O3_PAGED_ALL
 #undef FE2O3_PAGED
 #undef FE2O3_JOIN
+#undef FE2O3_JOIN_OF
+#undef FE2O3_JOIN_ALL
 
 }  // namespace
 
@@ -771,7 +822,7 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   // every product below is of factors that keep it under 2^64
   const uint64_t blocks = (uint64_t)kv_heads * blocks_per_head;  // at most q_heads
   // a window may add a tile; what a head's start counts for is within these
-  const uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys + 1u + kWaves * kSetup;
+  const uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys + 1u + 2u * kWaves;
   if (blocks * tiles >= (UINT64_C(1) << 31) || seqs * (blocks * tiles) >= (UINT64_C(1) << 31))
     return FE2O3_ERR_SHAPE;
   if (seqs > 1u && q_stride < row) return FE2O3_ERR_STRIDE;
@@ -802,9 +853,9 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.o = o;
   a.lse = lse;
   a.rows = group < kBlockRows ? group : kBlockRows;
-  a.records = (uint4*)workspace;
-  a.sums = (float*)((uint8_t*)workspace + 16u * kMaxWorkgroups);
-  a.stats = a.sums + (uint64_t)kMaxWorkgroups * 2u * a.rows * d;
+  const uint32_t part_rows = FE2O3_PAGED_ATTENTION_PART_ROWS(q_heads, kv_heads);
+  a.sums = (float*)workspace;
+  a.stats = a.sums + (uint64_t)kMaxWorkgroups * 2u * part_rows * d;
   a.q_stride = q_stride;
   a.seqs = seqs;
   a.q_heads = q_heads;

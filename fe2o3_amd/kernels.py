@@ -295,7 +295,7 @@ def moe_routing_check(routing: dict, tokens: int, experts: int, capacity: int,
 
 KV_BF16, KV_E4M3 = 0, 1
 KV_NO_SLOT = 0xFFFFFFFF
-PAGED_ATTENTION_MAX_WORKGROUPS = 1024
+PAGED_ATTENTION_MAX_WORKGROUPS = 768
 
 # what an array of each kind may hold: element types of a DeviceBuffer, and of
 # a tensor
@@ -481,7 +481,9 @@ def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, to
 def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int) -> int:
     """FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES: scratch of one decode call."""
     rows = min(q_heads // kv_heads, 64)
-    return PAGED_ATTENTION_MAX_WORKGROUPS * (16 + 8 * (head_dim + 2) * rows)
+    if kv_heads % 4 == 0 and rows <= 16:  # four heads at once
+        rows *= 4
+    return PAGED_ATTENTION_MAX_WORKGROUPS * 8 * (head_dim + 2) * rows
 
 
 def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, workspace, *,

@@ -424,11 +424,16 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_t
  * q rows or o off 16 bytes, lse or workspace off theirs FE2O3_ERR_ALIGNMENT;
  * a scale that is not positive and finite FE2O3_ERR_SHAPE; a short workspace
  * FE2O3_ERR_WORKSPACE. */
-#define FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS 1024u
+#define FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS 768u
+/* query rows of one workgroup's sums: of one KV head, or of four at once */
+#define FE2O3_PAGED_ATTENTION_PART_ROWS(q_heads, kv_heads)                                  \
+  ((q_heads) / (kv_heads) >= 64u                             ? 64u                          \
+   : (kv_heads) % 4u == 0u && (q_heads) / (kv_heads) <= 16u ? (q_heads) / (kv_heads) * 4u   \
+                                                             : (q_heads) / (kv_heads))
 #define FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES(q_heads, kv_heads, head_dim)                  \
-  (UINT64_C(16) * FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS +                                    \
-   UINT64_C(8) * FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS * ((uint64_t)(head_dim) + 2u) *       \
-       ((q_heads) / (kv_heads) < 64u ? (q_heads) / (kv_heads) : 64u))
+  (FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS *                                                   \
+   UINT64_C(8) * ((uint64_t)(head_dim) + 2u) *                                              \
+   FE2O3_PAGED_ATTENTION_PART_ROWS(q_heads, kv_heads))
 int32_t fe2o3_paged_attention_decode(const Fe2o3KvCacheV1 *cache, const uint16_t *q,
                                      uint64_t q_len, const uint32_t *block_table,
                                      uint64_t table_len, const uint32_t *lengths,

@@ -71,7 +71,7 @@ def test_record_layout_matches_the_header(tmp_path):
     for field, _ in rec._fields_:
         lines.append(f'printf("%zu\\n", offsetof(Fe2o3KvCacheV1, {field}));')
         expect.append(str(getattr(rec, field).offset))
-    heads = [(8, 8, 64), (32, 8, 128), (128, 1, 128)]
+    heads = [(8, 8, 64), (32, 8, 128), (128, 1, 128), (6, 2, 64), (64, 4, 128), (68, 4, 64)]
     from fe2o3_amd import kernels
     for q, kv, d in heads:
         lines.append('printf("%llu\\n", (unsigned long long)'
