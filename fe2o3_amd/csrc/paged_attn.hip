@@ -42,10 +42,11 @@ namespace {
 using namespace fe2o3;
 using kv_cache::View;
 
-constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;
+constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;  // of a workgroup, if not said otherwise
 constexpr uint32_t kKeys = 32;              // keys per tile
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
+constexpr uint32_t kWholeTiles = 40;        // of a call without a join
 constexpr uint32_t kGridX = 1u << 22;       // a grid holds fewer than 2^32 threads a dimension
 constexpr uint32_t kBlockRows = 64;         // query heads that one pass over K and V serves
 
@@ -153,11 +154,11 @@ struct Tile {
 
 // LDS of a workgroup: the waves' tiles, their tiles' scales, their reference and
 // sum of each query row, and the queries where they are more than one tile.
-template <int D, bool E4M3, int RT>
+template <int D, bool E4M3, int RT, uint32_t W = kWaves>
 struct Lds {
-  static constexpr uint32_t kScales = kWaves * Tile<D, E4M3>::kLds;
-  static constexpr uint32_t kStats = kScales + kWaves * 2u * kKeys * 4u;
-  static constexpr uint32_t kQueries = kStats + kWaves * 16u * RT * 8u;
+  static constexpr uint32_t kScales = W * Tile<D, E4M3>::kLds;
+  static constexpr uint32_t kStats = kScales + W * 2u * kKeys * 4u;
+  static constexpr uint32_t kQueries = kStats + W * 16u * RT * 8u;
   static constexpr uint32_t kQueryTile = D / 32 * 1024u;
   static constexpr uint32_t kBytes = kQueries + (RT == 1 ? 0u : RT * kQueryTile);
 };
@@ -173,12 +174,12 @@ constexpr int per_cu() {
 }
 
 // D: head_dim.  RT: query-row tiles of 16.  WH: KV heads that a workgroup works on
-// at once, kWaves / WH waves on each.
-template <int D, bool E4M3, int RT, int WH>
+// at once, of its W waves W / WH on each.
+template <int D, bool E4M3, int RT, int WH, uint32_t W = kWaves>
 struct Decode {
   using T = Tile<D, E4M3>;
-  using L = Lds<D, E4M3, RT>;
-  static constexpr uint32_t kStep = kWaves / WH;  // tiles of a head per round
+  using L = Lds<D, E4M3, RT, W>;
+  static constexpr uint32_t kStep = W / WH;  // tiles of a head per round
   static constexpr int kDb = D / 16;     // V^T row blocks
   static constexpr int kFrags = D / 32;  // 16-byte pieces of a query operand per lane
 
@@ -289,7 +290,7 @@ struct Decode {
     } else {
       // more than one tile of query rows would take the registers of the sums:
       // they lie in LDS for all waves, in the order of the lanes
-      for (uint32_t rt = wave; rt < (uint32_t)RT; rt += kWaves) {
+      for (uint32_t rt = wave; rt < (uint32_t)RT; rt += W) {
         const Query x = query(q, rt * 16u + lr, rows, g);
 #pragma unroll
         for (int f = 0; f < kFrags; ++f)
@@ -513,7 +514,7 @@ struct Decode {
       for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(mine + 16 * db) = acc[rt][db];
       __syncthreads();
       const uint32_t count = WH * min(rows - rt * 16u, 16u) * (D / 4u);
-      for (uint32_t i = tid; i < count; i += kThreads) {
+      for (uint32_t i = tid; i < count; i += W * 64u) {
         // rows of one head behind another's: RT > 1 has one head
         const uint32_t at = i / (D / 4u), d = 4u * (i % (D / 4u));
         const uint32_t wh = WH > 1 ? at / rows : 0u, r = at - wh * rows, row = rt * 16u + r;
@@ -551,16 +552,16 @@ struct Decode {
   }
 };
 
-// One workgroup per sequence and block of query rows, for calls whose
+// One workgroup of W waves per sequence and block of query rows, for calls whose
 // sequences are too short to be worth a join.
-template <int D, bool E4M3, int RT>
-__global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_whole_kernel(Args a) {
+template <int D, bool E4M3, int RT, uint32_t W>
+__global__ void __launch_bounds__(W * 64, (W == kWaves ? per_cu<D, E4M3, RT>() : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of(a, seq);
-  Decode<D, E4M3, RT, 1>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+  Decode<D, E4M3, RT, 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
 // The list of all work: sequence, then block of query rows (or WH KV heads), then
@@ -572,7 +573,8 @@ struct Plan {
   static constexpr uint32_t kStep = kWaves / WH, kSetup = RT == 1 ? 1u : 2u;
   const Args& a;
   uint32_t lane, blocks;
-  uint32_t first_scan;  // rounds of a block of sequences 0 .. lane
+  uint32_t first_length;  // of sequence `lane`
+  uint32_t first_scan;    // rounds of a block of sequences 0 .. lane
   uint32_t total, run;
 
   static FE2O3_DEVICE uint32_t rounds(const Span& sp) {
@@ -585,11 +587,15 @@ struct Plan {
   }
   FE2O3_DEVICE explicit Plan(const Args& args)
       : a(args), lane(threadIdx.x & 63u), blocks(a.cache.kv_heads * a.blocks_per_head / WH) {
-    first_scan = scan(0u);
+    first_length = lane < a.seqs ? a.lengths[lane] : 0u;
+    first_scan = wave_scan(lane < a.seqs ? rounds(span_of(a, first_length)) : 0u);
     total = at_lane(first_scan, 63u);
     for (uint32_t base = 64u; base < a.seqs; base += 64u) total += at_lane(scan(base), 63u);
     total *= blocks;
     run = uniform((total - 1u) / a.workgroups + 1u);
+  }
+  FE2O3_DEVICE Span span(uint32_t seq) const {
+    return span_of(a, seq < 64u ? at_lane(first_length, seq) : uniform(a.lengths[seq]));
   }
   // the sequence that round `at` falls into, and the rounds of a block before it
   FE2O3_DEVICE uint32_t find(uint32_t at, uint32_t* before) const {
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split
   uint32_t before;
   uint32_t seq = plan.find(at, &before);
   const uint32_t rest = at - before * plan.blocks;
-  Span sp = uniform_span_of(a, seq);
+  Span sp = plan.span(seq);
   uint32_t length = P::rounds(sp);
   uint32_t hb = uniform(rest / length), pos = rest - hb * length;
   Decode<D, E4M3, RT, WH> decode(a, smem);
@@ -644,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split
     pos = 0u;
     if (++hb == plan.blocks) {
       hb = 0u;
-      sp = uniform_span_of(a, ++seq);
+      sp = plan.span(++seq);
       length = P::rounds(sp);
     }
   }
@@ -659,7 +665,7 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a) {
   using P = Plan<RT, WH>;
   const P plan(a);
   const uint32_t seq = uniform(blockIdx.x / plan.blocks), hb = blockIdx.x - seq * plan.blocks;
-  const Span sp = uniform_span_of(a, seq);
+  const Span sp = plan.span(seq);
   const uint32_t length = P::rounds(sp), start = plan.before(seq) * plan.blocks + hb * length;
   const uint32_t first = uniform((start + P::kSetup) / plan.run);
   const uint32_t parts = uniform((start + length - 1u) / plan.run) - first + 1u;
@@ -721,7 +727,7 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   if (lds_rc != FE2O3_OK) return lds_rc;
   // as many workgroups as are resident at once, and work for each wave
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head / WH;
-  const uint64_t most = heads * ((tiles + kWaves / WH - 1u) / (kWaves / WH));
+  const uint64_t most = heads * ((tiles + kWaves / WH - 1u) / (kWaves / WH) + Plan<RT, WH>::kSetup);
   uint32_t workgroups = per_cu<D, E4M3, RT>() * cus;
   if (workgroups > kMaxWorkgroups) workgroups = kMaxWorkgroups;
   if (workgroups > most) workgroups = (uint32_t)most;
@@ -736,29 +742,42 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   if (heads * 4u >= workgroups)
     paged_join_kernel<D, RT, WH, kRows, kThreads>
         <<<dim3(heads, (rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a);
-  else if (heads * 32u >= workgroups)
+  else if (heads * 64u >= workgroups)
     paged_join_kernel<D, RT, WH, 1, kThreads><<<dim3(heads, rows), kThreads, 0, s>>>(a);
   else
     paged_join_kernel<D, RT, WH, 1, 1024><<<dim3(heads, rows), 1024, 0, s>>>(a);
   return fe2o3_host::after_launch();
 }
 
-template <int D, bool E4M3, int RT>
-int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
-  if (tiles > (2u + 2u) * kWaves) {
-    if constexpr (RT == 1)
-      if (a.cache.kv_heads % kWaves == 0u)
-        return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
-    return launch_split<D, E4M3, RT, 1>(a, tiles, cus, s);
-  }
-  constexpr uint32_t kSmem = Lds<D, E4M3, RT>::kBytes;
-  const auto fn = paged_whole_kernel<D, E4M3, RT>;
+template <int D, bool E4M3, int RT, uint32_t W>
+int32_t launch_whole(const Args& a, hipStream_t s) {
+  constexpr uint32_t kSmem = Lds<D, E4M3, RT, W>::kBytes;
+  const auto fn = paged_whole_kernel<D, E4M3, RT, W>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
   const dim3 grid(heads < kGridX ? heads : kGridX, (heads - 1u) / kGridX + 1u);
-  fn<<<grid, kThreads, kSmem, s>>>(a);
+  fn<<<grid, W * 64u, kSmem, s>>>(a);
   return fe2o3_host::after_launch();
+}
+
+template <int D, bool E4M3, int RT>
+int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
+  const uint64_t heads = (uint64_t)a.seqs * a.cache.kv_heads * a.blocks_per_head;
+  // RT == 1: eight waves a CU, of one workgroup while there are no more
+  const uint32_t resident = (RT == 1 ? 2u : 1u) * cus;
+  const bool wide = RT == 1 && heads <= cus;
+  const uint64_t rounds_whole =
+      wide ? (tiles + 7u) / 8u : ((tiles + 3u) / 4u * heads + resident - 1u) / resident;
+  const uint64_t rounds_split = (heads * tiles + 4u * resident - 1u) / (4u * resident);
+  if (tiles <= kWholeTiles && rounds_whole <= rounds_split + 2u) {
+    if constexpr (RT == 1)
+      if (wide && tiles > kWaves) return launch_whole<D, E4M3, RT, 8>(a, s);
+    return launch_whole<D, E4M3, RT, kWaves>(a, s);
+  }
+  if constexpr (RT == 1)
+    if (a.cache.kv_heads % kWaves == 0u) return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
+  return launch_split<D, E4M3, RT, 1>(a, tiles, cus, s);
 }
 
 template <int D, bool E4M3>
@@ -774,11 +793,12 @@ int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) 
 #define FE2O3_SPLIT(D, F, RT, WH) \
   FE2O3_KERNEL("paged_split_kernel<" #D "," #F "," #RT "," #WH ">", (paged_split_kernel<D, F, RT, WH>), (Lds<D, F, RT>::kBytes))
 #define FE2O3_PAGED(D, F, RT) \
-  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT ">", (paged_whole_kernel<D, F, RT>), (Lds<D, F, RT>::kBytes)), \
+  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT ",4>", (paged_whole_kernel<D, F, RT, 4>), (Lds<D, F, RT>::kBytes)), \
   FE2O3_SPLIT(D, F, RT, 1)
 #define FE2O3_PAGED_ALL(D, F) \
   FE2O3_PAGED(D, F, 1), FE2O3_PAGED(D, F, 2), FE2O3_PAGED(D, F, 3), FE2O3_PAGED(D, F, 4), \
-  FE2O3_SPLIT(D, F, 1, 4)
+  FE2O3_SPLIT(D, F, 1, 4), \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F ",1,8>", (const void*)paged_whole_kernel<D, F, 1, 8>, 512, Lds<D, F, 1, 8>::kBytes})
 #define FE2O3_JOIN_OF(D, RT, WH, ROWS, THREADS)                                                \
   fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #RT "," #WH "," #ROWS ">", (const void*)paged_join_kernel<D, RT, WH, ROWS, THREADS>, THREADS, 0})
 #define FE2O3_JOIN(D, RT, WH, ROWS) \
@@ -821,10 +841,11 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   const uint64_t row = (uint64_t)q_heads * d;
   // every product below is of factors that keep it under 2^64
   const uint64_t blocks = (uint64_t)kv_heads * blocks_per_head;  // at most q_heads
-  // a window may add a tile; what a head's start counts for is within these
-  const uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys + 1u + 2u * kWaves;
-  if (blocks * tiles >= (UINT64_C(1) << 31) || seqs * (blocks * tiles) >= (UINT64_C(1) << 31))
-    return FE2O3_ERR_SHAPE;
+  uint64_t tiles = ((uint64_t)max_length + kKeys - 1u) / kKeys;
+  if (window != 0u && window < max_length) tiles = ((uint64_t)window + kKeys - 1u) / kKeys + 1u;
+  // rounds of the plan, a head's start among them, and what a grid adds
+  const uint64_t most = blocks * (tiles + 2u * kWaves);
+  if (most >= (UINT64_C(1) << 31) || seqs * most >= (UINT64_C(1) << 31)) return FE2O3_ERR_SHAPE;
   if (seqs > 1u && q_stride < row) return FE2O3_ERR_STRIDE;
   if (seqs == 0u) return FE2O3_OK;
   uint64_t extent = row, bytes;
