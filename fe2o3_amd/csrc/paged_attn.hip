@@ -404,33 +404,43 @@ struct Decode {
           }
         }
       }
-      bf16x8_t pf[RT], pl[RT];
+      // scores in the log2 domain (bf16 cache: before its scale), then probabilities
+      // of all query rows, so that one branch serves them
+      float x[RT][8], p[RT][8], psum[RT];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        float x[8];  // scores in the log2 domain, bf16 cache: before its scale
+      for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = sc[rt][j >> 2][j & 3] * (E4M3 ? ks[j] : 1.0f);
-        if (valid != 0xffffffffu) {
+        for (int j = 0; j < 8; ++j) x[rt][j] = sc[rt][j >> 2][j & 3] * (E4M3 ? ks[j] : 1.0f);
+      if (valid != 0xffffffffu) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if ((valid >> (8u * g + j) & 1u) == 0u) x[j] = -INFINITY;
-          asm volatile("");
+        for (int j = 0; j < 8; ++j) {
+          const bool keep = (valid >> (8u * g + j) & 1u) != 0u;
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) x[rt][j] = keep ? x[rt][j] : -INFINITY;
         }
-        float p[8], psum;
-        auto probabilities = [&] {
-          psum = 0.0f;
+        asm volatile("");
+      }
+      auto probabilities = [&] {
+        bool small = true;
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          psum[rt] = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            p[j] = __builtin_amdgcn_exp2f(
-                E4M3 ? x[j] - m_ref[rt] : __builtin_fmaf(x[j], a.scale_log2, -m_ref[rt]));
-            psum += p[j];
+            p[rt][j] = __builtin_amdgcn_exp2f(
+                E4M3 ? x[rt][j] - m_ref[rt] : __builtin_fmaf(x[rt][j], a.scale_log2, -m_ref[rt]));
+            psum[rt] += p[rt][j];
           }
-        };
-        probabilities();
-        if (__any(!(psum <= kLazyBound))) {
-          float top = x[0];
+          small = small && psum[rt] <= kLazyBound;
+        }
+        return small;
+      };
+      if (__any(!probabilities())) {
 #pragma unroll
-          for (int j = 1; j < 8; ++j) top = fmaxf(top, x[j]);
+        for (int rt = 0; rt < RT; ++rt) {
+          float top = x[rt][0];
+#pragma unroll
+          for (int j = 1; j < 8; ++j) top = fmaxf(top, x[rt][j]);
           if (!E4M3) top *= a.scale_log2;  // positive
           const float m_new = fmaxf(m_ref[rt], row_max(top));
           const float alpha = __builtin_amdgcn_exp2f(m_ref[rt] - m_new);
@@ -440,39 +450,51 @@ struct Decode {
           for (int db = 0; db < kDb; ++db)
 #pragma unroll
             for (int e = 0; e < 4; ++e) acc[rt][db][e] *= alpha;
-          probabilities();
         }
-        l_run[rt] += psum;
-        // two bf16 parts: the second MFMA takes what the first one's rounding
-        // (half a step, 2^-8) leaves, for 1% more time
+        (void)probabilities();
+      }
+      // two bf16 parts: the second MFMA takes what the first one's rounding (half
+      // a step, 2^-8) leaves, for 1% more time
+      bf16x8_t pf[RT], pl[RT];
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        l_run[rt] += psum[rt];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = E4M3 ? p[j] * vs[j] : p[j];
+          const float y = E4M3 ? p[rt][j] * vs[j] : p[rt][j];
           pf[rt][j] = (__bf16)y;
           pl[rt][j] = (__bf16)(y - (float)pf[rt][j]);
         }
       }
-      // O^T += V^T P^T: lane i of group g receives d 16 db + i of keys 8 g .. + 7
+      // O^T += V^T P^T: lane i of group g receives d 16 db + i of keys 8 g .. + 7.
+      // Two blocks of d at a time, so that no MFMA waits for the one before it.
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) {
-        bf16x8_t vf;
-        if constexpr (E4M3) {
-          const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-              (lds_i32x2_t*)(smem + (v_at ^ (16u * db))));
-          vf = __builtin_bit_cast(bf16x8_t, widen_codes8((uint32_t)c[0], (uint32_t)c[1]));
-        } else {
-          bf16x4_t half[2];
+      for (int d2 = 0; d2 < kDb; d2 += 2) {
+        bf16x8_t vf[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-                (lds_bf16x4_t*)(smem + (v_at ^ (32u * db)) + 4u * T::kRowBytes * h));
-          vf = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+        for (int i = 0; i < 2; ++i) {
+          const int db = d2 + i;
+          if constexpr (E4M3) {
+            const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+                (lds_i32x2_t*)(smem + (v_at ^ (16u * db))));
+            vf[i] = __builtin_bit_cast(bf16x8_t, widen_codes8((uint32_t)c[0], (uint32_t)c[1]));
+          } else {
+            bf16x4_t half[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                  (lds_bf16x4_t*)(smem + (v_at ^ (32u * db)) + 4u * T::kRowBytes * h));
+            vf[i] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          }
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-          acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pf[rt], acc[rt][db], 0, 0, 0);
-          acc[rt][db] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, pl[rt], acc[rt][db], 0, 0, 0);
-        }
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              acc[rt][d2 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  vf[i], part == 0 ? pf[rt] : pl[rt], acc[rt][d2 + i], 0, 0, 0);
       }
     };
 
