@@ -73,11 +73,45 @@ FE2O3_DEVICE float amax8(u32x4_t x, float m) {
   return m;
 }
 
-FE2O3_DEVICE u32x2_t quantize8(u32x4_t x, float scale) {
-  u32x2_t q = {0, 0};
+// A row's scale and what divides by it.  x / scale is x r with r the rounded
+// reciprocal, corrected once by its remainder: for the scales that a row of bf16
+// has (its largest of 128 significands, over 448) and every bf16 x up to that
+// largest, this is the correctly rounded quotient, checked over all of them
+// (tests/test_kv_cache_host.py); x r alone differs by a code for 140 of 385088.
+// Three operations instead of the division's ten: 32768 tokens of 8 heads 75 us
+// -> 47.  Scales below the smallest normal or infinite divide as they are.
+struct RowScale {
+  float scale, r;
+  bool usual;
+  explicit FE2O3_DEVICE RowScale(float amax) {
+    scale = fmaxf(amax, 1.17549435e-38f) / 448.0f;
+    r = 1.0f / scale;
+    usual = scale >= 1.17549435e-38f && scale <= __FLT_MAX__;
+  }
+  FE2O3_DEVICE float quotient(float x) const {
+    const float q = x * r;
+    return __builtin_fmaf(__builtin_fmaf(-q, scale, x), r, q);
+  }
+};
+
+FE2O3_DEVICE u32x2_t quantize8(u32x4_t x, const RowScale& s) {
+  u32x2_t q;
+  if (s.usual) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    q[i / 4] |= (uint32_t)e4m3_from_f32(bf16_of(x, i) / scale) << (8 * (i & 3));
+    for (int w = 0; w < 2; ++w) {
+      // the quotients are at most 448 in magnitude: nothing to saturate
+      int c = __builtin_amdgcn_cvt_pk_fp8_f32(s.quotient(bf16_of(x, 4 * w)),
+                                              s.quotient(bf16_of(x, 4 * w + 1)), 0, false);
+      c = __builtin_amdgcn_cvt_pk_fp8_f32(s.quotient(bf16_of(x, 4 * w + 2)),
+                                          s.quotient(bf16_of(x, 4 * w + 3)), c, true);
+      q[w] = (uint32_t)c;
+    }
+  } else {
+    q = u32x2_t{0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      q[i / 4] |= (uint32_t)e4m3_from_f32(bf16_of(x, i) / s.scale) << (8 * (i & 3));
+  }
   return q;
 }
 
@@ -154,13 +188,12 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
         km = fmaxf(km, __shfl_xor(km, o, 64));
         vm = fmaxf(vm, __shfl_xor(vm, o, 64));
       }
-      const float ks = fmaxf(km, 1.17549435e-38f) / 448.0f;
-      const float vs = fmaxf(vm, 1.17549435e-38f) / 448.0f;
+      const RowScale ks(km), vs(vm);
       if (c0 == 0u) {
         const uint64_t at =
             ((uint64_t)page * a.cache.kv_heads + head) * a.cache.page.divisor + place;
-        a.cache.k_scale[at] = ks;
-        a.cache.v_scale[at] = vs;
+        a.cache.k_scale[at] = ks.scale;
+        a.cache.v_scale[at] = vs.scale;
       }
       for (uint32_t c = c0; c < chunks; c += lanes) {
         const uint32_t n = chunk_left(a.cache.head_dim, c);
