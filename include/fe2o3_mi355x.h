@@ -389,7 +389,7 @@ int32_t fe2o3_kv_cache_write(const Fe2o3KvCacheV1 *cache, const uint16_t *k, uin
  * past a sequence's table_cols pages, or on a page out of range, are +0.
  * starts: seqs + 1 values that do not fall (others give unspecified rows).
  * table_len = seqs * table_cols, starts_len = seqs + 1.  Errors as for the
- * write. */
+ * write; seqs of 2^31 or more FE2O3_ERR_SHAPE. */
 int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_table,
                             uint64_t table_len, const uint32_t *starts, uint64_t starts_len,
                             uint16_t *k, uint64_t k_len, uint16_t *v, uint64_t v_len,
