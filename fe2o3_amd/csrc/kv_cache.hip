@@ -331,6 +331,8 @@ int32_t fe2o3_kv_cache_write(const Fe2o3KvCacheV1* cache, const uint16_t* k, uin
   if (rc != FE2O3_OK) return rc;
   if (k_len < extent || v_len < extent) return FE2O3_ERR_LENGTH;
   if (!k || !v || !slots) return FE2O3_ERR_NULL;
+  if ((((uintptr_t)k | (uintptr_t)v) & 1u) != 0u || ((uintptr_t)slots & 3u) != 0u)
+    return FE2O3_ERR_ALIGNMENT;
   a.k = k;
   a.v = v;
   a.slots = slots;
@@ -367,6 +369,9 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1* cache, const uint32_t* block_t
   if (rc != FE2O3_OK) return rc;
   if (k_len < extent || v_len < extent) return FE2O3_ERR_LENGTH;
   if (!k || !v || !starts || (table_len != 0u && !block_table)) return FE2O3_ERR_NULL;
+  if ((((uintptr_t)k | (uintptr_t)v) & 1u) != 0u ||
+      (((uintptr_t)starts | (uintptr_t)block_table) & 3u) != 0u)
+    return FE2O3_ERR_ALIGNMENT;
   a.table = block_table;
   a.starts = starts;
   a.k = k;

@@ -307,14 +307,17 @@ _HOLDS = {
     _FLOAT: ("float32", "torch.float32"),
     _BYTES: ("uint8", "torch.uint8", "torch.int8"),
 }
-_kinds: dict = {}  # element type -> the kinds it may stand for
 
 
-def _kinds_of(dtype):
-    found = _kinds.get(dtype)
-    if found is None:
-        found = _kinds[dtype] = frozenset(k for k, v in _HOLDS.items() if str(dtype) in v)
-    return found
+class _Kinds(dict):
+    """element type -> the kinds it may stand for"""
+
+    def __missing__(self, dtype):
+        found = self[dtype] = frozenset(k for k, v in _HOLDS.items() if str(dtype) in v)
+        return found
+
+
+_kinds = _Kinds()
 
 
 def _operand(x, kind, name, device, dense=True):
@@ -322,14 +325,14 @@ def _operand(x, kind, name, device, dense=True):
     `device`.  dense: the tensor is contiguous; otherwise its last dimension
     is, and the elements are the extent that its strides span."""
     if isinstance(x, DeviceBuffer):
-        if kind not in _kinds_of(x.dtype):
+        if kind not in _kinds[x.dtype]:
             raise TypeError(f"{name} must hold {kind}, not {x.dtype}")
         if x.ctx.device != device:
             raise ValueError(f"{name} on device {x.ctx.device}, not {device}")
         return x.ptr, x.count
     if not hasattr(x, "data_ptr"):
         raise TypeError(f"{name} must be a DeviceBuffer or a device tensor")
-    if kind not in _kinds_of(x.dtype):
+    if kind not in _kinds[x.dtype]:
         raise TypeError(f"{name} must hold {kind}, not {x.dtype}")
     where = x.get_device()
     if where != device:
@@ -340,15 +343,19 @@ def _operand(x, kind, name, device, dense=True):
         return x.data_ptr(), x.numel()
     if dense:
         raise ValueError(f"{name} must be contiguous")
-    count = x.numel()
-    if count:
-        shape, strides = x.shape, x.stride()
-        if shape[-1] > 1 and strides[-1] != 1:
-            raise ValueError(f"the last dimension of {name} must be contiguous")
-        count = 1
-        for n, stride in zip(shape, strides):
-            count += (n - 1) * stride
-    return x.data_ptr(), count
+    return x.data_ptr(), _extent(x.shape, x.stride(), name)
+
+
+def _extent(shape, strides, name):
+    """Elements that a tensor's strides span; its last dimension is contiguous."""
+    if 0 in shape:
+        return 0
+    if strides[-1] != 1 and shape[-1] > 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    count = 1
+    for n, stride in zip(shape, strides):
+        count += (n - 1) * stride
+    return count
 
 
 def _layout(x, dims, name):
@@ -365,11 +372,23 @@ def _layout(x, dims, name):
     return shape, strides
 
 
-def _pair_layout(k, v, dims):
+def _pair(k, v, dims, kind, device):
+    """Shape and strides of K and V (None of DeviceBuffers), which are the same for
+    both, and (pointer, elements) of each."""
     shape, strides = _layout(k, dims, "k")
-    if _layout(v, dims, "v") != (shape, strides):
+    if shape is None:
+        if not isinstance(v, DeviceBuffer):
+            raise ValueError("k and v must be of one kind")
+        return None, None, _operand(k, kind, "k", device) + _operand(v, kind, "v", device)
+    if k.get_device() != device or v.get_device() != device:
+        _operand(k, kind, "k", device, False)
+        _operand(v, kind, "v", device, False)
+    if kind not in _kinds[k.dtype] or kind not in _kinds[v.dtype]:
+        raise TypeError(f"k and v must hold {kind}, not {k.dtype}, {v.dtype}")
+    if (v.shape, v.stride()) != (shape, strides) and _layout(v, dims, "v") != (shape, strides):
         raise ValueError("k and v must have the same shape and strides")
-    return shape, strides
+    count = _extent(shape, strides, "k and v")
+    return shape, strides, (k.data_ptr(), count, v.data_ptr(), count)
 
 
 class KvCache:
@@ -385,41 +404,41 @@ class KvCache:
     """
 
     def __init__(self, k, v, k_scale=None, v_scale=None, *, shape=None, strides=None):
-        found, found_strides = _pair_layout(k, v, 4)
+        if (k_scale is None) != (v_scale is None):
+            raise ValueError("k_scale and v_scale go together")
+        self.device = device = _device_of(k)
+        self.format, kind = (KV_BF16, _BF16) if k_scale is None else (KV_E4M3, _CODES)
+        found, found_strides, arrays = _pair(k, v, 4, kind, device)
         if found is not None:
             shape, strides = found, found_strides[:3]
-            self.device = k.get_device()
-            if self.device < 0:
-                raise TypeError("a cache lies in device memory")
-        else:
-            self.device = k.ctx.device
-        if shape is None:
+        elif shape is None:
             raise ValueError("a cache of DeviceBuffers needs its shape")
         pages, page_size, kv_heads, head_dim = self.shape = shape
         if strides is None:
             strides = (page_size * kv_heads * head_dim, kv_heads * head_dim, head_dim)
-        if (k_scale is None) != (v_scale is None):
-            raise ValueError("k_scale and v_scale go together")
         self.arrays = (k, v, k_scale, v_scale)
-        k_ptr = v_ptr = None
-        scales = 0
-        if k_scale is None:
-            self.format, kind = KV_BF16, _BF16
-        else:
-            self.format, kind = KV_E4M3, _CODES
+        scales = (None, 0, None, 0)
+        if k_scale is not None:
             for scale in (k_scale, v_scale):
                 found = _layout(scale, 3, "scales")[0]
                 if found is not None and tuple(found) != (pages, kv_heads, page_size):
                     raise ValueError(f"scales of {tuple(found)}, "
                                      f"not {(pages, kv_heads, page_size)}")
-            k_ptr, scales = _operand(k_scale, _FLOAT, "k_scale", self.device)
-            v_ptr, v_scales = _operand(v_scale, _FLOAT, "v_scale", self.device)
-            if scales != v_scales:
-                raise ValueError("k_scale and v_scale must have the same length")
-        self.record = _lib.Fe2o3KvCacheV1(
-            *_operand(k, kind, "k", self.device, False),
-            *_operand(v, kind, "v", self.device, False), k_ptr, scales, v_ptr, scales,
-            *strides, self.format, pages, page_size, kv_heads, head_dim, 0)
+            scales = (_operand(k_scale, _FLOAT, "k_scale", device)
+                      + _operand(v_scale, _FLOAT, "v_scale", device))
+        self.record = _lib.Fe2o3KvCacheV1(*arrays, *scales, *strides, self.format, pages, page_size,
+                                          kv_heads, head_dim, 0)
+
+
+def _device_of(k):
+    if isinstance(k, DeviceBuffer):
+        return k.ctx.device
+    if not hasattr(k, "get_device"):
+        raise TypeError("k must be a DeviceBuffer or a device tensor")
+    device = k.get_device()
+    if device < 0:
+        raise TypeError("a cache lies in device memory")
+    return device
 
 
 def _on_current_device(cache):
@@ -431,15 +450,16 @@ def _on_current_device(cache):
     return cache.device
 
 
-def _row_layout(cache, k, v, strides):
-    """Tokens (None of DeviceBuffers) and (token, head) strides of K and V rows."""
+def _rows(cache, k, v, strides, device):
+    """K and V rows of a cache's heads: tokens (None of DeviceBuffers), (token, head)
+    strides, and (pointer, elements) of each."""
     _, _, kv_heads, head_dim = cache.shape
-    shape, found = _pair_layout(k, v, 3)
+    shape, found, arrays = _pair(k, v, 3, _BF16, device)
     if shape is None:
-        return None, strides or (kv_heads * head_dim, head_dim)
+        return None, strides or (kv_heads * head_dim, head_dim), arrays
     if shape[1] != kv_heads or shape[2] != head_dim:
         raise ValueError(f"rows of {tuple(shape[1:])} for a cache of {(kv_heads, head_dim)}")
-    return shape[0], found[:2]
+    return shape[0], found[:2], arrays
 
 
 def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sync=True) -> None:
@@ -448,13 +468,12 @@ def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sy
     e4m3.  A slot out of range (KV_NO_SLOT) is skipped; each slot at most once
     a call (fe2o3_kv_cache_write)."""
     device = _on_current_device(cache)
-    rows, strides = _row_layout(cache, k, v, strides)
+    rows, strides, arrays = _rows(cache, k, v, strides, device)
     slots_ptr, tokens = _operand(slots, _INDEX, "slots", device)
     if rows is not None and rows != tokens:
         raise ValueError(f"{rows} rows and {tokens} slots")
-    _call("fe2o3_kv_cache_write", C.byref(cache.record), *_operand(k, _BF16, "k", device, False),
-          *_operand(v, _BF16, "v", device, False), slots_ptr, tokens, tokens, *strides,
-          stream=stream, sync=sync)
+    _call("fe2o3_kv_cache_write", C.byref(cache.record), *arrays, slots_ptr, tokens, tokens,
+          *strides, stream=stream, sync=sync)
 
 
 def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, tokens=None,
@@ -464,7 +483,7 @@ def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, to
     no sequence keep their values (fe2o3_kv_cache_read).  DeviceBuffers take
     `strides` (token, head) and `tokens`."""
     device = _on_current_device(cache)
-    rows, strides = _row_layout(cache, k, v, strides)
+    rows, strides, arrays = _rows(cache, k, v, strides, device)
     starts_ptr, starts_len = _operand(starts, _INDEX, "starts", device)
     table_ptr, table_len = _operand(block_table, _INDEX, "block_table", device)
     seqs = starts_len - 1
@@ -473,9 +492,8 @@ def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, to
     if rows is None:
         rows = k.count // (cache.shape[2] * cache.shape[3]) if tokens is None else tokens
     _call("fe2o3_kv_cache_read", C.byref(cache.record), table_ptr, table_len, starts_ptr,
-          starts_len, *_operand(k, _BF16, "k", device, False),
-          *_operand(v, _BF16, "v", device, False), seqs, table_len // seqs if seqs else 0, rows,
-          *strides, stream=stream, sync=sync)
+          starts_len, *arrays, seqs, table_len // seqs if seqs else 0, rows, *strides,
+          stream=stream, sync=sync)
 
 
 def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int) -> int:

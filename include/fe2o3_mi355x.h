@@ -373,8 +373,8 @@ typedef struct Fe2o3KvCacheV1 {
  * Everything else in the cache keeps its bytes.  k_len and v_len cover the
  * rows' extent; slots_len = tokens.  Errors after the cache's: kv_heads *
  * tokens of 2^31 or more FE2O3_ERR_SHAPE, FE2O3_ERR_STRIDE, FE2O3_ERR_OVERFLOW
- * and FE2O3_ERR_LENGTH as for the cache, FE2O3_ERR_NULL.  Any alignment;
- * 16-byte accesses where head_dim is a multiple of 8 and rows allow it. */
+ * and FE2O3_ERR_LENGTH as for the cache, FE2O3_ERR_NULL, and for arrays off
+ * their elements' alignment FE2O3_ERR_ALIGNMENT; rows may start anywhere else. */
 int32_t fe2o3_kv_cache_write(const Fe2o3KvCacheV1 *cache, const uint16_t *k, uint64_t k_len,
                              const uint16_t *v, uint64_t v_len, const uint32_t *slots,
                              uint64_t slots_len, uint32_t tokens, uint64_t token_stride,
@@ -417,11 +417,11 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_t
  * overlap need one each.
  *
  * head_dim is 64 or 128.  Errors after the cache's: head_dim, kv_heads = 0 or
- * no divisor of q_heads, max_length out of its range, or 2^31 or more key
- * tiles in all (seqs * kv_heads * max_length / 32, times group / 64)
+ * no divisor of q_heads, max_length out of its range, or 2^31 or more tiles of
+ * 32 keys in all (seqs * kv_heads * (max_length / 32 + 8), times group / 64)
  * FE2O3_ERR_SHAPE; q_stride below q_heads * head_dim FE2O3_ERR_STRIDE; lengths
  * FE2O3_ERR_LENGTH (q_len covers the extent); NULL FE2O3_ERR_NULL; cache rows,
- * q rows or o off 16 bytes, lse or workspace off theirs FE2O3_ERR_ALIGNMENT;
+ * q rows, o or workspace off 16 bytes, the others off 4 FE2O3_ERR_ALIGNMENT;
  * a scale that is not positive and finite FE2O3_ERR_SHAPE; a short workspace
  * FE2O3_ERR_WORKSPACE. */
 #define FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS 768u

@@ -86,6 +86,32 @@ def test_record_layout_matches_the_header(tmp_path):
     assert got[:-1] == expect
 
 
+def test_e4m3_quotients_by_reciprocal():
+    """The cache write divides by a row's scale s through q = x r, r = RN(1 / s),
+    corrected once: q + (x - q s) r with fused multiply-adds.  For every scale that a
+    row of bf16 can have (s = RN(amax / 448), 128 significands) and every bf16 x up to
+    amax down to where its code is 0, that is the correctly rounded quotient; powers
+    of two change nothing while nothing is subnormal.  In 80-bit arithmetic, whose 64
+    bits hold x - q s exactly, and q + e r to more than twice fp32's."""
+    f, wide = np.float32, np.longdouble
+    if np.finfo(wide).nmant < 63:
+        pytest.skip("no 80-bit floating point")
+    sig = np.arange(128, 256).astype(f)
+    checked = 0
+    for amax in sig:
+        s = f(amax / f(448))
+        r = f(f(1) / s)
+        for k in range(-1, 24):
+            x = (sig * f(2.0 ** -k)).astype(f)
+            x = x[x <= amax]
+            q = (x * r).astype(f)
+            e = (x.astype(wide) - q.astype(wide) * wide(s)).astype(f)
+            got = (q.astype(wide) + e.astype(wide) * wide(r)).astype(f)
+            assert np.array_equal(got, (x / s).astype(f))
+            checked += x.size
+    assert checked > 350000
+
+
 def test_page_division(tmp_path):
     exe = tmp_path / "fast_div_check"
     subprocess.run(["g++", "-O2", "-std=c++17", "-o", str(exe),
@@ -142,6 +168,8 @@ def test_write_refusals(L):
     assert _write(L, rec, v_len=3 * 128 - 1) == LENGTH
     for name in ("k", "v", "slots"):
         assert _write(L, rec, **{name: None}) == NULL
+    for name, off in (("k", 1), ("v", 3), ("slots", 2)):
+        assert _write(L, rec, **{name: P + off}) == ALIGNMENT
     # no tokens: nothing is launched and no array is looked at
     assert _write(L, rec, tokens=0, slots_len=0, k=None, k_len=0, v=None, v_len=0,
                   slots=None) == 0
@@ -157,6 +185,8 @@ def test_read_refusals(L):
     assert _read(L, rec, k_len=3 * 128 - 1) == LENGTH
     for name in ("k", "v", "starts", "table"):
         assert _read(L, rec, **{name: None}) == NULL
+    for name, off in (("k", 1), ("v", 3), ("starts", 2), ("table", 1)):
+        assert _read(L, rec, **{name: P + off}) == ALIGNMENT
     assert _read(L, rec, tokens=0, k=None, k_len=0, v=None, v_len=0) == 0
     assert _read(L, rec, seqs=0, table_len=0, starts_len=1) == 0
 
@@ -186,7 +216,8 @@ def test_decode_refusals(L):
         assert _decode(L, rec, **{name: None}) == NULL
     for name in ("q", "o", "workspace"):
         assert _decode(L, rec, **{name: P + 8}) == ALIGNMENT
-    assert _decode(L, rec, lse=P + 2) == ALIGNMENT
+    for name in ("lse", "table", "lengths"):
+        assert _decode(L, rec, **{name: P + 2}) == ALIGNMENT
     assert _decode(L, rec, q_stride=516, q_len=1 << 20) == ALIGNMENT
     # rows of the cache off 16 bytes
     assert _decode(L, _cache(k=P + 2)) == ALIGNMENT
