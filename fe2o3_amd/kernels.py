@@ -160,7 +160,9 @@ moe_expert_combine_f32_t8_k2_o16_v1_gpu = _typed(
 
 def _call(entry: str, *args, stream: Stream | None = None, sync: bool = True) -> None:
     fn = getattr(_lib.lib(), entry)
-    check(fn(*args, stream_handle(stream)), entry)
+    status = fn(*args, None if stream is None else stream_handle(stream))
+    if status != 0:
+        check(status, entry)
     if sync:
         if stream is None:
             check(_lib.lib().fe2o3_rt_device_synchronize(), "device synchronize")
@@ -350,7 +352,7 @@ def _extent(shape, strides, name):
     """Elements that a tensor's strides span; its last dimension is contiguous."""
     if 0 in shape:
         return 0
-    if strides[-1] != 1 and shape[-1] > 1:
+    if strides[-1] != 1 and shape[-1] != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
     count = 1
     for n, stride in zip(shape, strides):
@@ -358,36 +360,36 @@ def _extent(shape, strides, name):
     return count
 
 
-def _layout(x, dims, name):
-    """(shape, strides) of a tensor, a stride of 0 for a dimension of one, whose
-    stride says nothing; (None, None) of a DeviceBuffer."""
+def _dimensions(x, dims, name):
+    """Shape of a tensor of `dims` dimensions; None of a DeviceBuffer."""
     if isinstance(x, DeviceBuffer):
-        return None, None
+        return None
     shape = getattr(x, "shape", None)
     if shape is None or len(shape) != dims:
         raise ValueError(f"{name} must be a DeviceBuffer or a tensor of {dims} dimensions")
-    strides = x.stride()
-    if 1 in shape:
-        strides = tuple(s if n > 1 else 0 for n, s in zip(shape, strides))
-    return shape, strides
+    return shape
+
+
+def _same_strides(x, y):
+    """Whether two tensors of one shape have the same strides, but for dimensions of
+    one, whose stride says nothing."""
+    return all(n == 1 or s == t for n, s, t in zip(x.shape, x.stride(), y.stride()))
 
 
 def _pair(k, v, dims, kind, device):
     """Shape and strides of K and V (None of DeviceBuffers), which are the same for
     both, and (pointer, elements) of each."""
-    shape, strides = _layout(k, dims, "k")
-    if shape is None:
-        if not isinstance(v, DeviceBuffer):
-            raise ValueError("k and v must be of one kind")
+    shape = _dimensions(k, dims, "k")
+    if shape is None or isinstance(v, DeviceBuffer):
         return None, None, _operand(k, kind, "k", device) + _operand(v, kind, "v", device)
-    if k.get_device() != device or v.get_device() != device:
+    strides = k.stride()
+    if v.shape != shape or (v.stride() != strides and not _same_strides(k, v)):
+        raise ValueError("k and v must have the same shape and strides")
+    if (k.get_device() != device or v.get_device() != device or kind not in _kinds[k.dtype]
+            or kind not in _kinds[v.dtype]):  # which says what is wrong
         _operand(k, kind, "k", device, False)
         _operand(v, kind, "v", device, False)
-    if kind not in _kinds[k.dtype] or kind not in _kinds[v.dtype]:
-        raise TypeError(f"k and v must hold {kind}, not {k.dtype}, {v.dtype}")
-    if (v.shape, v.stride()) != (shape, strides) and _layout(v, dims, "v") != (shape, strides):
-        raise ValueError("k and v must have the same shape and strides")
-    count = _extent(shape, strides, "k and v")
+    count = k.numel() if k.is_contiguous() else _extent(shape, strides, "k and v")
     return shape, strides, (k.data_ptr(), count, v.data_ptr(), count)
 
 
@@ -420,7 +422,7 @@ class KvCache:
         scales = (None, 0, None, 0)
         if k_scale is not None:
             for scale in (k_scale, v_scale):
-                found = _layout(scale, 3, "scales")[0]
+                found = _dimensions(scale, 3, "scales")
                 if found is not None and tuple(found) != (pages, kv_heads, page_size):
                     raise ValueError(f"scales of {tuple(found)}, "
                                      f"not {(pages, kv_heads, page_size)}")
@@ -516,12 +518,13 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
     device = _on_current_device(cache)
     head_dim = cache.shape[3]
     lengths_ptr, seqs = _operand(lengths, _INDEX, "lengths", device)
-    shape, strides = _layout(q, 3, "q")
+    shape = _dimensions(q, 3, "q")
     if shape is not None:
-        q_heads, q_stride = shape[1], strides[0]
-        if shape[0] != seqs:
-            raise ValueError(f"{shape[0]} rows of q and {seqs} lengths")
-        if shape[2] != head_dim or strides[1] not in (0, head_dim):
+        rows, q_heads, width = shape
+        q_stride, head_stride, _ = q.stride()
+        if rows != seqs:
+            raise ValueError(f"{rows} rows of q and {seqs} lengths")
+        if width != head_dim or (head_stride != width and q_heads != 1):
             raise ValueError("q must be [seqs, q_heads, head_dim] with a sequence's heads dense")
     elif q_heads is None:
         raise ValueError("q in a DeviceBuffer needs q_heads")
