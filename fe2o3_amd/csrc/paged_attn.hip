@@ -9,13 +9,12 @@
 // unused rows cost nothing.
 //
 // A wave works on tiles of 32 keys of its own, with no barrier among waves:
-//   * K and V rows come to registers with 16-byte loads, adjacent lanes on
-//     adjacent pieces of a row, a tile (bf16, 128 wide) or more ahead of their
-//     use.  Lane l looks up the page of key l % 32; its offset reaches the
-//     lanes that load the row by a lane permutation, so pages of any size and
-//     place cost the same.
-//   * They pass through LDS of the wave's own as bf16 (codes are widened on the
-//     way, exactly), chunks XOR-permuted per row, into the MFMAs' layouts.
+//   * K and V rows come to registers with 16-byte nontemporal loads, adjacent
+//     lanes on adjacent pieces of a row, one tile ahead of their use.  Lane l
+//     looks up the page of key l % 32; its offset reaches the lanes that load the
+//     row by a lane permutation, so pages of any size and place cost the same.
+//   * They pass through LDS of the wave's own, chunks XOR-permuted per row, into
+//     the MFMAs' layouts; e4m3 codes are widened to bf16, exactly, on the way out.
 //   * S^T = K Q^T with v_mfma_f32_16x16x32_bf16: row m of key block b is key
 //     8 (m / 4) + 4 b + m % 4, so that lane l holds query row l % 16 and the
 //     eight keys 8 (l / 16) .. + 7, and the probabilities are the second
@@ -23,16 +22,25 @@
 //     reads.  The softmax is the prompt kernel's: exponentials against a
 //     running reference that is raised only when a tile exceeds it by 2^8.
 //   * An e4m3 cache's K scales multiply the scores, its V scales the
-//     probabilities before they are rounded to bf16 for the MFMA.
-// A workgroup's waves take every fourth tile of a run of tiles and add their
-// sums in LDS when the run or the sequence ends.
+//     probabilities before these are rounded for the MFMA.
+// With a multiple of four KV heads (and group <= 16) a workgroup's four waves
+// have a head each: they read neighbouring rows, and nothing is added in LDS.
+// Otherwise they take every fourth tile of one head and add their sums.
 //
-// The tiles of all sequences and KV heads, one behind another, are dealt in
-// equal runs to as many workgroups as the device holds, so that one long
-// sequence fills it as well as many, and mixed lengths leave no tail.  Each
+// The tiles of all sequences and heads, one behind another, are dealt in equal
+// runs to as many workgroups as the device holds, so that one long sequence
+// fills it as well as many, and mixed lengths leave no tail (Plan).  Each
 // workgroup finds its run from the lengths.  A head that takes more than one run
 // has its sums in the workspace; paged_join_kernel adds them in the order of the
-// keys.
+// keys.  Short calls run one workgroup a head instead (launch).
+//
+// Measured, of a repeated call, bytes of K and V read once (a kernel that only
+// reads them: 6.4-6.9 TB/s): 8 sequences of 4096 keys, 32 heads, bf16: 82 us =
+// 6.6 TB/s, and 4.6 of the join; 130001 keys of one sequence, 8 heads: 82 us and
+// 7; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 89 us = 6.2 TB/s, 4.7; 500
+// keys of one: 7.7 us.  48 query heads on one KV head, 48 sequences of 100 to 6000
+// keys: 25 us and 5.5, bound by one wave a SIMD and its chain of products,
+// exponentials and LDS reads.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -163,7 +171,8 @@ struct Lds {
   static constexpr uint32_t kBytes = kQueries + (RT == 1 ? 0u : RT * kQueryTile);
 };
 
-// Workgroups per CU.
+// Workgroups per CU: as many as registers and LDS allow, but two of the widest
+// (three of them, e4m3, 64 sequences of 4096 keys: 98.5 -> 105.5 us).
 template <int D, bool E4M3, int RT>
 constexpr int per_cu() {
   if (RT == 1) return D == 64 ? 3 : 2;
@@ -764,7 +773,8 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
   // Many heads have few parts each, and rows share the threads; few have many,
-  // which a row's threads share.
+  // which a row's threads share (one head's 256 parts: 16 us on 256 threads, 7 on
+  // 1024; 64 heads' 8 parts: 4.6 on either).
   constexpr int kRows = kThreads / (D / 4);
   const uint32_t rows = WH * a.rows, grid = heads < (1u << 20) ? heads : 1u << 20;
   if (heads >= workgroups / 4u)
@@ -792,7 +802,16 @@ int32_t launch_whole(const Args& a, hipStream_t s) {
 template <int D, bool E4M3, int RT>
 int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   const uint64_t heads = (uint64_t)a.seqs * a.cache.kv_heads * a.blocks_per_head;
-  // RT == 1: eight waves a CU, of one workgroup while there are no more
+  // Whether one workgroup a head is enough, without a plan and a join: rounds of
+  // tiles on the busiest wave, against an even share of them plus two rounds for
+  // the join, for heads of few tiles (us, even shares against one a head; 8 KV
+  // heads of 128, bf16):
+  //   1 x 500  9.4,  7.7    16 x 500  16.0, 10.8    30 x 500  18.9, 13.4
+  //   64 x 500 29.6, 23.5   200 x 500 75.7, 68.6    64 x 1..1000 28.8 (one a head)
+  //   1 x 1000 9.7, 14.8    4 x 1000  12.1, 15.7    16 x 1000 20.8, 17.7
+  //   64 x 1..2000 48.1, 55.2   30 x 1..2000 27.4, 30.1   40 windows of 1024
+  //   (64 wide, e4m3) 16.8, 13.0
+  // Few heads take eight waves each.
   const uint32_t resident = (per_cu<D, E4M3, RT>() == 1 ? 1u : 2u) * cus;
   const bool wide = RT == 1 && heads <= cus;
   const uint64_t rounds_whole =

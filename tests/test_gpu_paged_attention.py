@@ -232,12 +232,29 @@ def test_windows(gpu, fmt, window):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("q_heads,kv_heads", [(4, 2), (8, 4), (20, 1)])
+@pytest.mark.parametrize("window", [1500, 2047, 2048, 2049])
+def test_windows_over_many_runs(gpu, fmt, q_heads, kv_heads, window):
+    _check(gpu, fmt, [5000, 0, 1999, 2100, 7000], q_heads, kv_heads, 64, 16, window=window)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("lengths,q_heads,kv_heads,head_dim,page_size", [
     ([40001], 2, 1, 128, 16),           # one head of one sequence in as many runs as there are
     ([5000, 1, 0, 0, 9000, 33], 8, 2, 64, 16),
     ([2500] * 40, 4, 2, 128, 32),       # runs that end anywhere in a sequence
     ([int(x) for x in np.linspace(0, 700, 150)], 2, 1, 64, 8),  # more than a wave's lanes of sequences
     ([300] * 3 + [0] * 200 + [4000], 2, 2, 64, 64),
+    # a multiple of four KV heads: a wave each
+    ([40001], 8, 4, 128, 16),
+    ([5000, 1, 0, 0, 9000, 33], 16, 8, 64, 16),
+    ([1500, 1501, 1499, 31] * 6, 64, 4, 128, 32),
+    ([int(x) for x in np.linspace(0, 1400, 70)], 4, 4, 64, 8),
+    # more than one tile of query rows, more than one block of 64
+    ([5000, 1, 0, 4000, 33], 20, 1, 128, 16),
+    ([2500] * 9, 48, 1, 64, 16),
+    ([3000, 2999, 40], 64, 1, 128, 16),
+    ([3000, 0, 1700], 150, 1, 64, 16),
 ])
 def test_many_runs(gpu, fmt, lengths, q_heads, kv_heads, head_dim, page_size):
     _check(gpu, fmt, lengths, q_heads, kv_heads, head_dim, page_size)
@@ -249,6 +266,8 @@ def test_peaked_and_flat_scores(gpu, fmt, peak):
     """Scores up to several hundred, where one key has almost all of the weight
     and the running reference rises often, and scores of nearly 0."""
     _check(gpu, fmt, [900, 64, 3000], 8, 2, 128, 16, peak=peak)
+    _check(gpu, fmt, [900, 64, 3000], 8, 4, 64, 16, peak=peak)
+    _check(gpu, fmt, [900, 64, 3000], 36, 1, 128, 16, peak=peak)
 
 
 def test_rising_scores(gpu):
@@ -294,17 +313,19 @@ def test_pages_out_of_range_are_left_out(gpu, fmt):
     b.compare(b.run(), b.reference(drop=drop))
 
 
-def test_without_lse_and_repeated(gpu):
-    b = Batch(gpu, "bf16", [4000, 17, 900], 8, 2, 128, 16)
+@pytest.mark.parametrize("kv_heads", [2, 4])
+def test_without_lse_and_repeated(gpu, kv_heads):
+    b = Batch(gpu, "bf16", [4000, 17, 900], 8, kv_heads, 128, 16)
     b.compare(b.run(lse=False), b.reference(), lse=False)
     first, second = b.run(), b.run()
     assert_same(first[0].download(), second[0].download())
     assert_same(first[1].download(), second[1].download())
 
 
-def test_nonfinite_values_of_kept_keys(gpu):
+@pytest.mark.parametrize("length", [300, 3000])
+def test_nonfinite_values_of_kept_keys(gpu, length):
     """A NaN key or value shows in its own sequence and KV head only."""
-    b = Batch(gpu, "bf16", [300, 300], 4, 2, 64, 16)
+    b = Batch(gpu, "bf16", [length, length], 4, 2, 64, 16)
     want = b.reference()
     flat = b.arrays[0].download()
     rows = np.lib.stride_tricks.as_strided(flat, b.shape, [2 * s for s in b.strides] + [2])
