@@ -39,7 +39,7 @@
 // 6.6 TB/s, and 4.6 of the join; 130001 keys of one sequence, 8 heads: 82 us and
 // 7; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 89 us = 6.2 TB/s, 4.7; 500
 // keys of one: 7.7 us.  48 query heads on one KV head, 48 sequences of 100 to 6000
-// keys: 25 us and 5.5, bound by one wave a SIMD and its chain of products,
+// keys: 25 us and 4.1, bound by one wave a SIMD and its chain of products,
 // exponentials and LDS reads.
 #include "common.hpp"
 #include "internal.hpp"
@@ -56,6 +56,7 @@ constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
 constexpr uint32_t kWholeTiles = 40;        // of a call without a join
 constexpr uint32_t kGridX = 1u << 22;       // a grid holds fewer than 2^32 threads a dimension
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 constexpr uint32_t kBlockRows = 64;         // query heads that one pass over K and V serves
 
 struct Args {
@@ -596,58 +597,82 @@ __global__ void __launch_bounds__(W * 64, (W == kWaves ? per_cu<D, E4M3, RT>() :
 // round, a round being a tile for each wave.  What starting on a head costs (its
 // pages, queries and first loads, and the sums at the end) counts as kSetup
 // rounds before its first.  Workgroup i takes rounds i run .. + run - 1.
+//
+// Every wave counts the list by itself: lane l the sequences chunk l .. + chunk - 1,
+// four lengths a load, then one scan over the lanes; a place is found among the
+// lanes, then in a chunk.  4096 sequences of 1 to 300 keys, 2 heads: 127 us so, 134
+// by single lengths, 154 with a scan for every 64 sequences.
 template <int RT, int WH>
 struct Plan {
   static constexpr uint32_t kStep = kWaves / WH, kSetup = RT == 1 ? 1u : 2u;
   const Args& a;
-  uint32_t lane, blocks;
-  uint32_t first_length;  // of sequence `lane`
-  uint32_t first_scan;    // rounds of a block of sequences 0 .. lane
+  uint32_t lane, blocks, chunk;
+  uint32_t first_length;  // of sequence `lane`, if a chunk is one
+  uint32_t chunk_scan;    // rounds of a block of lanes 0 .. lane's chunks
   uint32_t total, run;
 
   static FE2O3_DEVICE uint32_t rounds(const Span& sp) {
     return (sp.tiles + kStep - 1u) / kStep + kSetup;
   }
-  // of sequence base + lane and those from base on before it
-  FE2O3_DEVICE uint32_t scan(uint32_t base) const {
-    const uint32_t s = base + lane;
-    return wave_scan(s < a.seqs ? rounds(span_of(a, a.lengths[s])) : 0u);
-  }
   FE2O3_DEVICE explicit Plan(const Args& args)
-      : a(args), lane(threadIdx.x & 63u), blocks(a.cache.kv_heads * a.blocks_per_head / WH) {
-    first_length = lane < a.seqs ? a.lengths[lane] : 0u;
-    first_scan = wave_scan(lane < a.seqs ? rounds(span_of(a, first_length)) : 0u);
-    total = at_lane(first_scan, 63u);
-    for (uint32_t base = 64u; base < a.seqs; base += 64u) total += at_lane(scan(base), 63u);
-    total *= blocks;
+      : a(args), lane(threadIdx.x & 63u), blocks(a.cache.kv_heads * a.blocks_per_head / WH),
+        chunk(a.seqs <= 64u ? 1u : ((a.seqs - 1u) / 256u + 1u) * 4u), first_length(0u) {
+    uint32_t sum = 0;
+    if (chunk == 1u) {
+      first_length = lane < a.seqs ? a.lengths[lane] : 0u;
+      sum = lane < a.seqs ? rounds(span_of(a, first_length)) : 0u;
+    } else {
+#pragma unroll 4
+      for (uint32_t i = 0; i < chunk; i += 4u) {
+        const uint32_t s = lane * chunk + i, from = min(s, a.seqs - 4u);
+        const u32x4_any_t x = *reinterpret_cast<const u32x4_any_t*>(a.lengths + from);
+#pragma unroll
+        for (uint32_t e = 0; e < 4u; ++e) sum += from + e >= s ? rounds(span_of(a, x[e])) : 0u;
+      }
+    }
+    chunk_scan = wave_scan(sum);
+    total = at_lane(chunk_scan, 63u) * blocks;
     run = uniform((total - 1u) / a.workgroups + 1u);
   }
-  FE2O3_DEVICE Span span(uint32_t seq) const {
-    return span_of(a, seq < 64u ? at_lane(first_length, seq) : uniform(a.lengths[seq]));
+  // rounds of a block of sequences base .. base + lane, those below limit
+  FE2O3_DEVICE uint32_t scan(uint32_t base, uint32_t limit) const {
+    const uint32_t s = base + lane;
+    return wave_scan(s < limit ? rounds(span_of(a, a.lengths[s])) : 0u);
   }
-  // the sequence that round `at` falls into, and the rounds of a block before it
+  FE2O3_DEVICE Span span(uint32_t seq) const {
+    return span_of(a, chunk == 1u ? at_lane(first_length, seq) : uniform(a.lengths[seq]));
+  }
+  // the sequence that round `at` (below total) falls into, and the rounds of a
+  // block before it
   FE2O3_DEVICE uint32_t find(uint32_t at, uint32_t* before) const {
-    uint32_t seq = 0, skipped = 0, sums = first_scan;
-    while (true) {
-      const uint32_t n =
-          (uint32_t)__popcll(__ballot(seq + lane < a.seqs && (skipped + sums) * blocks <= at));
-      if (n < 64u) {
-        *before = n != 0u ? skipped + at_lane(sums, n - 1u) : skipped;
-        return seq + n;
+    const uint32_t c = (uint32_t)__popcll(__ballot(chunk_scan * blocks <= at));
+    uint32_t skipped = c != 0u ? at_lane(chunk_scan, c - 1u) : 0u, seq = c * chunk;
+    if (chunk != 1u) {
+      const uint32_t limit = min(seq + chunk, a.seqs);
+      while (true) {
+        const uint32_t sums = scan(seq, limit);
+        const uint32_t n = (uint32_t)__popcll(
+            __ballot(seq + lane < limit && (skipped + sums) * blocks <= at));
+        if (n < 64u) {
+          if (n != 0u) skipped += at_lane(sums, n - 1u);
+          seq += n;
+          break;
+        }
+        skipped += at_lane(sums, 63u);
+        seq += 64u;
       }
-      skipped += at_lane(sums, 63u);
-      seq += 64u;
-      sums = scan(seq);
     }
+    *before = skipped;
+    return seq;
   }
   // the rounds of a block before sequence seq
   FE2O3_DEVICE uint32_t before(uint32_t seq) const {
-    uint32_t skipped = 0, sums = first_scan;
-    for (uint32_t base = 0; base + 64u <= seq; base += 64u) {
-      skipped += at_lane(sums, 63u);
-      sums = scan(base + 64u);
-    }
-    return seq % 64u != 0u ? skipped + at_lane(sums, seq % 64u - 1u) : skipped;
+    const uint32_t c = chunk == 1u ? seq : uniform(seq / chunk);
+    uint32_t skipped = c != 0u ? at_lane(chunk_scan, c - 1u) : 0u;
+    if (chunk != 1u)
+      for (uint32_t base = c * chunk; base < seq; base += 64u)
+        skipped += at_lane(scan(base, seq), 63u);
+    return skipped;
   }
 };
 
@@ -687,12 +712,13 @@ __global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split
 // Query rows blockIdx.y * ROWS .. of a sequence and block (or WH heads): the sums
 // that the runs over it left, if it took more than one: place 1 of the run that
 // began it and place 0 of the runs that follow, in order.  D / 4 threads cover a
-// row; the threads that ROWS rows leave over take every kWays-th part.  A
-// workgroup takes every gridDim.x-th of the `heads` there are.  Bound by latency:
-// the lengths, then the parts (4.6 us after 64 sequences, 7 us for the 256 parts of
-// one).
+// row; the threads that ROWS rows leave over take every kWays-th part.  blockIdx.x
+// is the head, or with by_runs the run that began it: of more heads than runs,
+// most lie within one (4096 sequences of 1 to 200 keys, 8 heads: 12 us; 213 over
+// the heads, counted 64 by 64).  Bound by latency: the lengths, then the parts (4.6 us after 64
+// sequences, 7 us for the 256 parts of one).
 template <int D, int RT, int WH, int ROWS, int THREADS>
-__global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, uint32_t heads) {
+__global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_runs) {
   using P = Plan<RT, WH>;
   constexpr uint32_t kQuads = D / 4u, kWays = THREADS / (kQuads * ROWS);
   __shared__ f32x4_t part_sum[kWays > 1u ? THREADS : 1];
@@ -701,59 +727,63 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, uint32_t he
   const uint32_t quad = threadIdx.x % kQuads, d = 4u * quad;
   const uint32_t r = threadIdx.x / kQuads % ROWS, way = threadIdx.x / (kQuads * ROWS);
   const uint32_t row = blockIdx.y * ROWS + r;  // one head's behind another's
-  for (uint32_t id = blockIdx.x; id < heads; id += gridDim.x) {
-    const uint32_t seq = uniform(id / plan.blocks), hb = id - seq * plan.blocks;
-    const Span sp = plan.span(seq);
-    const uint32_t length = P::rounds(sp), start = plan.before(seq) * plan.blocks + hb * length;
-    const uint32_t first = uniform((start + P::kSetup) / plan.run);
-    const uint32_t parts = uniform((start + length - 1u) / plan.run) - first + 1u;
-    if (parts == 1u) continue;
-    float m = -__FLT_MAX__, l = 0.0f;
-    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
-    auto add = [&](float2 s, f32x4_t x) {
-      const float top = fmaxf(m, s.x);
-      const float old = __builtin_amdgcn_exp2f(m - top);
-      const float weight = __builtin_amdgcn_exp2f(s.x - top);
-      m = top;
-      l = l * old + weight * s.y;
-      y = y * old + weight * x;
-    };
+  // by_runs: the head that the next run starts in
+  const uint32_t next = (blockIdx.x + 1u) * plan.run;
+  if (by_runs && next >= plan.total) return;
+  uint32_t before, seq;
+  if (by_runs) seq = plan.find(next, &before);
+  else before = plan.before(seq = uniform(blockIdx.x / plan.blocks));
+  const uint32_t length = P::rounds(plan.span(seq));
+  const uint32_t hb = by_runs ? uniform((next - before * plan.blocks) / length)
+                              : blockIdx.x - seq * plan.blocks;
+  const uint32_t start = before * plan.blocks + hb * length;
+  const uint32_t first = uniform((start + P::kSetup) / plan.run);
+  const uint32_t parts = uniform((start + length - 1u) / plan.run) - first + 1u;
+  if (parts == 1u || (by_runs && first != blockIdx.x)) return;
+  float m = -__FLT_MAX__, l = 0.0f;
+  f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](float2 s, f32x4_t x) {
+    const float top = fmaxf(m, s.x);
+    const float old = __builtin_amdgcn_exp2f(m - top);
+    const float weight = __builtin_amdgcn_exp2f(s.x - top);
+    m = top;
+    l = l * old + weight * s.y;
+    y = y * old + weight * x;
+  };
 #pragma unroll 4
-    for (uint32_t i = way; i < parts; i += kWays) {
-      const uint64_t p = ((uint64_t)(first + i) * 2u + (i == 0u ? 1u : 0u)) * WH * a.rows +
-                         min(row, WH * a.rows - 1u);
-      add(*reinterpret_cast<const float2*>(a.stats + p * 2u),
-          *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d));
-    }
-    if constexpr (kWays > 1u) {
-      part_sum[threadIdx.x] = y;
-      part_stat[threadIdx.x] = float2{m, l};
-      __syncthreads();
-      if (way == 0u) {
-#pragma unroll 8
-        for (uint32_t w = 1; w < kWays; ++w)
-          add(part_stat[w * kQuads * ROWS + threadIdx.x],
-              part_sum[w * kQuads * ROWS + threadIdx.x]);
-      }
-      __syncthreads();
-    }
-    uint32_t q_head;
-    bool has = way == 0u && row < WH * a.rows;
-    if constexpr (WH > 1) {  // a.rows is the group
-      q_head = hb * WH * a.group + row;
-    } else {
-      const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
-      has = has && block * kBlockRows + row < a.group;
-      q_head = head * a.group + block * kBlockRows + row;
-    }
-    if (!has) continue;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const uint64_t out = (uint64_t)seq * a.q_heads + q_head;
-    *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
-        u32x2_t{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
-    if (a.lse != nullptr && d == 0u)
-      a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
+  for (uint32_t i = way; i < parts; i += kWays) {
+    const uint64_t p = ((uint64_t)(first + i) * 2u + (i == 0u ? 1u : 0u)) * WH * a.rows +
+                       min(row, WH * a.rows - 1u);
+    add(*reinterpret_cast<const float2*>(a.stats + p * 2u),
+        *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d));
   }
+  if constexpr (kWays > 1u) {
+    part_sum[threadIdx.x] = y;
+    part_stat[threadIdx.x] = float2{m, l};
+    __syncthreads();
+    if (way == 0u) {
+#pragma unroll 8
+      for (uint32_t w = 1; w < kWays; ++w)
+        add(part_stat[w * kQuads * ROWS + threadIdx.x],
+            part_sum[w * kQuads * ROWS + threadIdx.x]);
+    }
+  }
+  uint32_t q_head;
+  bool has = way == 0u && row < WH * a.rows;
+  if constexpr (WH > 1) {  // a.rows is the group
+    q_head = hb * WH * a.group + row;
+  } else {
+    const uint32_t head = hb / a.blocks_per_head, block = hb - head * a.blocks_per_head;
+    has = has && block * kBlockRows + row < a.group;
+    q_head = head * a.group + block * kBlockRows + row;
+  }
+  if (!has) return;
+  const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+  const uint64_t out = (uint64_t)seq * a.q_heads + q_head;
+  *reinterpret_cast<u32x2_t*>(a.o + out * D + d) =
+      u32x2_t{pack_bf16x2(y[0] * inv, y[1] * inv), pack_bf16x2(y[2] * inv, y[3] * inv)};
+  if (a.lse != nullptr && d == 0u)
+    a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
 template <int D, bool E4M3, int RT, int WH>
@@ -774,16 +804,19 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   if (rc != FE2O3_OK) return rc;
   // Many heads have few parts each, and rows share the threads; few have many,
   // which a row's threads share (one head's 256 parts: 16 us on 256 threads, 7 on
-  // 1024; 64 heads' 8 parts: 4.6 on either).
+  // 1024; 8 parts of 64 heads of 16 rows: 4.6 either way, of 33 heads of 64 rows 5.6
+  // and, rows sharing, 4.3).
   constexpr int kRows = kThreads / (D / 4);
-  const uint32_t rows = WH * a.rows, grid = heads < (1u << 20) ? heads : 1u << 20;
-  if (heads >= workgroups / 4u)
+  const uint32_t rows = WH * a.rows;
+  const bool by_runs = heads > workgroups;
+  const uint32_t grid = by_runs ? workgroups : heads;
+  if (heads >= workgroups / 8u)
     paged_join_kernel<D, RT, WH, kRows, kThreads>
-        <<<dim3(grid, (rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a, heads);
+        <<<dim3(grid, (rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a, by_runs);
   else if (heads >= workgroups / 64u)
-    paged_join_kernel<D, RT, WH, 1, kThreads><<<dim3(grid, rows), kThreads, 0, s>>>(a, heads);
+    paged_join_kernel<D, RT, WH, 1, kThreads><<<dim3(grid, rows), kThreads, 0, s>>>(a, by_runs);
   else
-    paged_join_kernel<D, RT, WH, 1, 1024><<<dim3(grid, rows), 1024, 0, s>>>(a, heads);
+    paged_join_kernel<D, RT, WH, 1, 1024><<<dim3(grid, rows), 1024, 0, s>>>(a, by_runs);
   return fe2o3_host::after_launch();
 }
 

@@ -261,6 +261,18 @@ def test_many_runs(gpu, fmt, lengths, q_heads, kv_heads, head_dim, page_size):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("seqs", [65, 129, 700, 4300])  # to several chunks of a wave's lanes
+@pytest.mark.parametrize("q_heads,kv_heads", [(2, 1), (4, 4)])
+def test_many_sequences(gpu, fmt, seqs, q_heads, kv_heads):
+    """More heads than runs, so that most lie within one, and a long sequence
+    among them that takes several; the last ones are empty."""
+    lengths = [37 * i % 151 for i in range(seqs - 2)] + [0, 0]
+    lengths[seqs // 3] = 2000
+    lengths[seqs // 2] = 1300
+    _check(gpu, fmt, lengths, q_heads, kv_heads, 64, 16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("peak", [30.0, 1e-3])
 def test_peaked_and_flat_scores(gpu, fmt, peak):
     """Scores up to several hundred, where one key has almost all of the weight
