@@ -77,7 +77,7 @@ inline int32_t check(const Fe2o3KvCacheV1* c, View* out) {
   if (c->pages == 0u || c->page_size == 0u || c->kv_heads == 0u || c->head_dim == 0u)
     return FE2O3_ERR_SHAPE;
   const uint64_t slots = (uint64_t)c->pages * c->page_size;
-  if (slots >= (UINT64_C(1) << 31)) return FE2O3_ERR_SHAPE;
+  if (slots >= (UINT64_C(1) << 31) || c->head_dim >= (UINT32_C(1) << 31)) return FE2O3_ERR_SHAPE;
   uint64_t extent;
   const int32_t rc = rows_extent(c->page_size, c->kv_heads, c->head_dim, c->token_stride,
                                  c->head_stride, &extent);

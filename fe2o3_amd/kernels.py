@@ -294,6 +294,10 @@ def moe_routing_check(routing: dict, tokens: int, experts: int, capacity: int,
 
 
 # ---- paged key-value cache ---------------------------------------------------------------
+#
+# Calls go to `stream`, the null stream if None, whatever stream is torch's current
+# one: order them behind what writes their tensors, and without sync keep the
+# tensors until the stream is through.
 
 KV_BF16, KV_E4M3 = 0, 1
 KV_NO_SLOT = 0xFFFFFFFF
@@ -358,6 +362,15 @@ def _extent(shape, strides, name):
     for n, stride in zip(shape, strides):
         count += (n - 1) * stride
     return count
+
+
+def _table(block_table, seqs, device):
+    """(pointer, elements, columns) of a block table, flat or [seqs, columns]."""
+    ptr, count = _operand(block_table, _INDEX, "block_table", device)
+    shape = getattr(block_table, "shape", None)
+    if shape is not None and len(shape) != 1 and shape[0] != seqs:
+        raise ValueError(f"a block table of {tuple(shape)} for {seqs} sequences")
+    return ptr, count, count // seqs if seqs else 0
 
 
 def _dimensions(x, dims, name):
@@ -487,15 +500,14 @@ def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, to
     device = _on_current_device(cache)
     rows, strides, arrays = _rows(cache, k, v, strides, device)
     starts_ptr, starts_len = _operand(starts, _INDEX, "starts", device)
-    table_ptr, table_len = _operand(block_table, _INDEX, "block_table", device)
     seqs = starts_len - 1
     if seqs < 0:
         raise ValueError("starts must hold one value more than there are sequences")
+    table_ptr, table_len, cols = _table(block_table, seqs, device)
     if rows is None:
-        rows = k.count // (cache.shape[2] * cache.shape[3]) if tokens is None else tokens
+        rows = arrays[1] // (cache.shape[2] * cache.shape[3]) if tokens is None else tokens
     _call("fe2o3_kv_cache_read", C.byref(cache.record), table_ptr, table_len, starts_ptr,
-          starts_len, *arrays, seqs, table_len // seqs if seqs else 0, rows, *strides,
-          stream=stream, sync=sync)
+          starts_len, *arrays, seqs, cols, rows, *strides, stream=stream, sync=sync)
 
 
 def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int) -> int:
@@ -526,18 +538,19 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
             raise ValueError(f"{rows} rows of q and {seqs} lengths")
         if width != head_dim or (head_stride != width and q_heads != 1):
             raise ValueError("q must be [seqs, q_heads, head_dim] with a sequence's heads dense")
+        if getattr(out, "shape", shape) != shape:
+            raise ValueError(f"out of {tuple(out.shape)} for q of {tuple(shape)}")
     elif q_heads is None:
         raise ValueError("q in a DeviceBuffer needs q_heads")
     elif q_stride is None:
         q_stride = q_heads * head_dim
-    table_ptr, table_len = _operand(block_table, _INDEX, "block_table", device)
+    table_ptr, table_len, cols = _table(block_table, seqs, device)
     lse_ptr, lse_len = (None, 0) if lse is None else _operand(lse, _FLOAT, "lse", device)
     _call("fe2o3_paged_attention_decode", C.byref(cache.record),
           *_operand(q, _BF16, "q", device, False), table_ptr, table_len, lengths_ptr, seqs,
           *_operand(out, _BF16, "out", device), lse_ptr, lse_len,
-          *_operand(workspace, _BYTES, "workspace", device), seqs, q_heads,
-          table_len // seqs if seqs else 0, max_length, q_stride, window, scale,
-          stream=stream, sync=sync)
+          *_operand(workspace, _BYTES, "workspace", device), seqs, q_heads, cols, max_length,
+          q_stride, window, scale, stream=stream, sync=sync)
 
 
 def kernel_resources(entry: str) -> list[dict]:

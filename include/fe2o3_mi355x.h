@@ -337,17 +337,18 @@ int32_t fe2o3_flash_attention_fwd(const uint16_t *q, uint64_t q_len,
  * infinite scale and reads back as NaN.
  *
  * The record is checked in this order: NULL record FE2O3_ERR_NULL; another
- * format, a size of 0, or 2^31 slots or more FE2O3_ERR_SHAPE; strides with
- * which rows share elements FE2O3_ERR_STRIDE (FE2O3_ERR_OVERFLOW where an
- * extent passes 64 bits); k_len or v_len short of the extent, or scale lengths
- * other than pages * kv_heads * page_size (0 for bf16) FE2O3_ERR_LENGTH; NULL
- * arrays FE2O3_ERR_NULL; bf16 at an odd address or scales off their 4 bytes
- * FE2O3_ERR_ALIGNMENT.
+ * format, a size of 0, or slots or head_dim of 2^31 or more FE2O3_ERR_SHAPE;
+ * strides with which rows share elements FE2O3_ERR_STRIDE (FE2O3_ERR_OVERFLOW
+ * where an extent passes 64 bits); k_len or v_len short of the extent, or scale
+ * lengths other than pages * kv_heads * page_size (0 for bf16)
+ * FE2O3_ERR_LENGTH; NULL arrays FE2O3_ERR_NULL; bf16 at an odd address or
+ * scales off their 4 bytes FE2O3_ERR_ALIGNMENT.
  *
  * Slots, block tables, starts and lengths are device data that the host
  * cannot validate.  No value in them leads an access outside the arrays; what
  * each entry point does with one out of range stands with it.  They are u32:
- * -1 of an int32 array is out of every range. */
+ * -1 of an int32 array is past every page, slot and length.  No element that a
+ * call writes belongs to another of its arrays. */
 #define FE2O3_KV_BF16 0u
 #define FE2O3_KV_E4M3 1u
 #define FE2O3_KV_NO_SLOT 0xffffffffu

@@ -124,6 +124,7 @@ CACHE_REFUSALS = [
     (dict(format=2), SHAPE), (dict(pages=0), SHAPE), (dict(page_size=0), SHAPE),
     (dict(kv_heads=0), SHAPE), (dict(head_dim=0), SHAPE),
     (dict(pages=1 << 20, page_size=1 << 11), SHAPE),  # 2^31 slots
+    (dict(head_dim=1 << 31), SHAPE), (dict(head_dim=(1 << 32) - 3), SHAPE),
     (dict(head_stride=63), STRIDE), (dict(token_stride=63), STRIDE),
     (dict(token_stride=127), STRIDE),  # heads of one token reach into the next
     (dict(page_stride=16 * 128 - 1), STRIDE),
@@ -321,3 +322,33 @@ def test_arrays_on_another_device_are_refused(monkeypatch):
     far = kernels.KvCache(*(_Fake((4, 16, 2, 64), (2048, 128, 64, 1), device=1) for _ in "kv"))
     with pytest.raises(ValueError, match="the current one is 0"):
         kernels.kv_cache_write(far, there, there, slots)
+
+
+def test_shapes_that_do_not_fit_are_refused(monkeypatch):
+    """A block table or an output of as many elements in another shape."""
+    from fe2o3_amd import _lib, kernels
+
+    class Lib:
+        @staticmethod
+        def fe2o3_rt_get_device(out):
+            out._obj.value = 0
+            return 0
+
+        def __getattr__(self, name):
+            raise AssertionError(name)
+
+    monkeypatch.setattr(_lib, "lib", lambda: Lib())
+    cache = kernels.KvCache(*(_Fake((4, 16, 2, 64), (2048, 128, 64, 1)) for _ in "kv"))
+    q, lengths = _Fake((3, 4, 64), (256, 64, 1)), _Fake((3,), (1,), "torch.int32")
+    table, turned = (_Fake(s, (s[1], 1), "torch.int32") for s in ((3, 2), (2, 3)))
+    other = _Fake((4, 3, 64), (192, 64, 1))
+    ws = _Fake((1 << 20,), (1,), "torch.uint8")
+    with pytest.raises(ValueError, match="block table"):
+        kernels.paged_attention_decode(cache, q, turned, lengths, q, None, ws, max_length=32,
+                                       scale=1.0)
+    with pytest.raises(ValueError, match="out of"):
+        kernels.paged_attention_decode(cache, q, table, lengths, other, None, ws, max_length=32,
+                                       scale=1.0)
+    rows, starts = _Fake((9, 2, 64), (128, 64, 1)), _Fake((4,), (1,), "torch.int32")
+    with pytest.raises(ValueError, match="block table"):
+        kernels.kv_cache_read(cache, turned, starts, rows, rows)
