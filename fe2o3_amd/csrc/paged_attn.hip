@@ -25,7 +25,8 @@
 //     probabilities before these are rounded for the MFMA.
 // With a multiple of four KV heads (and group <= 16) a workgroup's four waves
 // have a head each: they read neighbouring rows, and nothing is added in LDS.
-// Otherwise they take every fourth tile of one head and add their sums.
+// Otherwise they take every fourth tile of one head and add their sums; of a group
+// above 32 four teams of three or four waves, a wave for every 16 query rows, do so.
 //
 // The tiles of all sequences and heads, one behind another, are dealt in equal
 // runs to as many workgroups as the device holds, so that one long sequence
@@ -37,10 +38,9 @@
 // Measured, of a repeated call, bytes of K and V read once (a kernel that only
 // reads them: 6.4-6.9 TB/s): 8 sequences of 4096 keys, 32 heads, bf16: 82 us =
 // 6.6 TB/s, and 4.6 of the join; 130001 keys of one sequence, 8 heads: 82 us and
-// 7; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 89 us = 6.2 TB/s, 4.7; 500
+// 7; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 88 us = 6.3 TB/s, 4.8; 500
 // keys of one: 7.7 us.  48 query heads on one KV head, 48 sequences of 100 to 6000
-// keys: 25 us and 4.1, bound by one wave a SIMD and its chain of products,
-// exponentials and LDS reads.
+// keys: 21 us and 4.0, half of it starting, adding and ending.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -157,43 +157,63 @@ struct Tile {
   // the sums of 16 query rows take the tile's place at the end of a run
   static constexpr uint32_t kSumStride = D + 4u;  // floats
   static constexpr uint32_t kSumBytes = 16u * kSumStride * 4u;
-  static constexpr uint32_t kLds = 2u * kBytes > kSumBytes ? 2u * kBytes : kSumBytes;
-  static_assert(kLds % 256u == 0u, "chunks are chosen by exclusive or");
 };
 
-// LDS of a workgroup: the waves' tiles, their tiles' scales, their reference and
-// sum of each query row, and the queries where they are more than one tile.
-template <int D, bool E4M3, int RT, uint32_t W = kWaves>
+// How RT tiles of 16 query rows are dealt: row_tiles to a wave, so that sharers waves
+// share each tile of keys; and the waves of a workgroup.  One wave's chain of products
+// and exponentials over three or four tiles of rows is longer than the loads of the
+// next keys, so they have a wave each (a KV head's 64 rows, 48 sequences of 24000 keys:
+// 118 us in one wave, 96 shared; 48 sequences of 100 to 6000 with 48 rows: 25 us, 21).
+// Two keep up, and a wave of their own reads LDS and widens codes once for both (32
+// rows, e4m3: 55 us, shared 73).
+constexpr int row_tiles(int rt) { return rt == 2 ? 2 : 1; }
+constexpr uint32_t sharers(int rt) { return (uint32_t)(rt / row_tiles(rt)); }
+constexpr uint32_t waves(int rt) { return kWaves * sharers(rt); }
+
+// LDS of a workgroup of W waves: their tiles, or two places for tiles that S waves
+// share, which the sums of 16 query rows of each wave take at the end of a run; their
+// tiles' scales; their reference and sum of each query row.
+template <int D, bool E4M3, uint32_t S, uint32_t W>
 struct Lds {
-  static constexpr uint32_t kScales = W * Tile<D, E4M3>::kLds;
-  static constexpr uint32_t kStats = kScales + W * 2u * kKeys * 4u;
-  static constexpr uint32_t kQueries = kStats + W * 16u * RT * 8u;
-  static constexpr uint32_t kQueryTile = D / 32 * 1024u;
-  static constexpr uint32_t kBytes = kQueries + (RT == 1 ? 0u : RT * kQueryTile);
+  using T = Tile<D, E4M3 && S == 1>;
+  static constexpr uint32_t kTiles = (S == 1 ? 2u : 4u) * T::kBytes;  // of S waves
+  static constexpr uint32_t kSums = S == 1 && kTiles > T::kSumBytes ? kTiles : T::kSumBytes;
+  static constexpr uint32_t kOwn = S == 1 ? kSums : kTiles;  // from S waves' to the next
+  static constexpr uint32_t kScales = W / S * kOwn > W * kSums ? W / S * kOwn : W * kSums;
+  static constexpr uint32_t kStats = kScales + (E4M3 ? W * 2u * kKeys * 4u : 0u);
+  static constexpr uint32_t kBytes = kStats + W * 16u * 8u;
+  static_assert(kOwn % 256u == 0u, "chunks are chosen by exclusive or");
 };
 
-// Workgroups per CU: as many as registers and LDS allow, but two of the widest
-// (three of them, e4m3, 64 sequences of 4096 keys: 98.5 -> 105.5 us).
+// Workgroups per CU: as many as registers and LDS allow, but two of the widest of one
+// row tile (three of them, e4m3, 64 sequences of 4096 keys: 98.5 -> 105.5 us).
 template <int D, bool E4M3, int RT>
 constexpr int per_cu() {
   if (RT == 1) return D == 64 ? 3 : 2;
-  return RT == 2 && (D == 64 || E4M3) ? 2 : RT == 3 && D == 64 ? 2 : 1;
+  return RT == 2 && (D == 64 || E4M3) ? 2 : 1;
 }
 
-// D: head_dim.  RT: query-row tiles of 16.  WH: KV heads that a workgroup works on
-// at once, of its W waves W / WH on each.
-template <int D, bool E4M3, int RT, int WH, uint32_t W = kWaves>
+// D: head_dim.  RW: tiles of 16 query rows of a wave.  S waves, a team, share a tile of
+// keys, or each has its own (1).  WH: KV heads that a workgroup works on at once, of its
+// W waves W / WH on each.
+template <int D, bool E4M3, int RW, uint32_t S, int WH, uint32_t W>
 struct Decode {
-  using T = Tile<D, E4M3>;
-  using L = Lds<D, E4M3, RT, W>;
-  static constexpr uint32_t kStep = W / WH;  // tiles of a head per round
+  // Codes lie in LDS as they are and are widened on the way out, but waves that share
+  // a tile would all widen it: they do on the way in, a part each.
+  static constexpr bool kCodes = E4M3 && S == 1;
+  using R = Tile<D, E4M3>;    // as loaded
+  using T = Tile<D, kCodes>;  // in LDS
+  using L = Lds<D, E4M3, S, W>;
+  static_assert(S == 1 || WH == 1, "waves share a tile of one head");
+  static constexpr uint32_t kStep = W / S / WH;  // tiles of a head per round
   static constexpr int kDb = D / 16;     // V^T row blocks
   static constexpr int kFrags = D / 32;  // 16-byte pieces of a query operand per lane
+  static constexpr uint32_t kMine = (2u * R::kLoads + S - 1u) / S;  // a wave's loads of a tile
 
   struct Stage {
-    u32x4_t k[T::kLoads], v[T::kLoads];
-    float scale;     // E4M3: lanes below 32 the K scale of key l, the others the V scale
-    uint32_t valid;  // bit per key
+    u32x4_t x[kMine];  // the wave's loads i (mine) of a tile: below kLoads K, then V
+    float scale;       // E4M3: lanes below 32 the K scale of key l, the others the V scale
+    uint32_t valid;    // bit per key
   };
   struct Query {
     u32x4_t f[kFrags];
@@ -201,10 +221,12 @@ struct Decode {
 
   const Args& a;
   uint8_t* smem;
-  const uint32_t wave;
+  const uint32_t wave, team, member;
+  uint32_t buffer;  // S > 1: where the next tile goes, 0 or the offset of the second place
 
   FE2O3_DEVICE Decode(const Args& args, uint8_t* lds)
-      : a(args), smem(lds), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+      : a(args), smem(lds), wave(uniform(threadIdx.x >> 6)), team(wave / S),
+        member(wave % S), buffer(0u) {}
 
   // The thread's number, as a value that the compiler cannot follow: what is
   // derived from it is then made where it is used, not kept in registers over
@@ -218,7 +240,12 @@ struct Decode {
     return (float*)(smem + L::kScales + w * (2u * kKeys * 4u));
   }
   FE2O3_DEVICE float2* stat(uint32_t w) const {
-    return (float2*)(smem + L::kStats + w * (16u * RT * 8u));
+    return (float2*)(smem + L::kStats + w * (16u * 8u));
+  }
+
+  // number j of the wave's loads of a tile
+  FE2O3_DEVICE uint32_t mine(uint32_t j) const {
+    return S == 1 ? j / 2u + j % 2u * R::kLoads : j * S + member;
   }
 
   // The query operand of lane (lr, g) for row `row` of `rows` (others 0): piece f
@@ -228,11 +255,11 @@ struct Decode {
   FE2O3_DEVICE Query query(const uint16_t* q, uint32_t row, uint32_t rows, uint32_t g) const {
     Query r;
     const bool has = row < rows;
-    const uint16_t* from = q + (has ? row : 0u) * D + g * (E4M3 ? 16u : 8u);
+    const uint16_t* from = q + (has ? row : 0u) * D + g * (kCodes ? 16u : 8u);
 #pragma unroll
     for (int f = 0; f < kFrags; ++f) {
-      r.f[f] = *reinterpret_cast<const u32x4_t*>(from + (E4M3 ? (f >> 1) * 64 + (f & 1) * 8
-                                                              : f * 32));
+      r.f[f] = *reinterpret_cast<const u32x4_t*>(from + (kCodes ? (f >> 1) * 64 + (f & 1) * 8
+                                                                : f * 32));
       if (!has) r.f[f] = u32x4_t{0, 0, 0, 0};
     }
     return r;
@@ -244,19 +271,19 @@ struct Decode {
   FE2O3_DEVICE void run(uint32_t seq, uint32_t hb0, const Span& sp, uint32_t tile, uint32_t n,
                         uint32_t slot) {
     const uint32_t tid = thread(), lane = tid & 63u, lr = lane & 15u, g = lane >> 4;
-    const uint32_t head = WH > 1 ? hb0 + wave / kStep : hb0 / a.blocks_per_head;
+    const uint32_t head = WH > 1 ? hb0 + team / kStep : hb0 / a.blocks_per_head;
     const uint32_t row0 = WH > 1 ? 0u : (hb0 - head * a.blocks_per_head) * kBlockRows;
     const uint32_t rows = min(a.group - row0, (uint32_t)kBlockRows);
     const uint32_t q_head = head * a.group + row0;
     const uint32_t* table = a.table + (uint64_t)seq * a.table_cols;
     const uint64_t head_at = head * a.cache.head_stride * (E4M3 ? 1u : 2u);
-    const uint32_t pr = lane / T::kRowLanes, pc = lane % T::kRowLanes;  // as loaded: row, piece
+    const uint32_t pr = lane / R::kRowLanes, pc = lane % R::kRowLanes;  // as loaded: row, piece
     const uint8_t* kb = a.cache.k + head_at + pc * 16u;
     const uint8_t* vb = a.cache.v + head_at + pc * 16u;
     const float* sb = (lane < 32u ? a.cache.k_scale : a.cache.v_scale);
 
     const uint32_t end = sp.tile0 + tile + n;
-    uint32_t t = sp.tile0 + tile + wave % kStep;
+    uint32_t t = sp.tile0 + tile + team % kStep;
     // the table's entry for this lane's key of tile t; none past the run
     auto entry = [&](uint32_t at) {
       const uint32_t key = at * kKeys + (lane & 31u);
@@ -281,40 +308,29 @@ struct Decode {
       }
       // nontemporal: 16384 tokens of 8 heads run at 6.4 TB/s, at 5.7 without
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) {
-        const uint64_t row = shfl64(off, i * T::kRowsPerLoad + pr);
-        st.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kb + row));
-        st.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vb + row));
+      for (uint32_t i = 0; i < R::kLoads; ++i) {
+        if constexpr (S == 1) {
+          const uint64_t row = shfl64(off, i * R::kRowsPerLoad + pr);
+          st.x[2u * i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kb + row));
+          st.x[2u * i + 1u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vb + row));
+        } else if (i < kMine && mine(i) < 2u * R::kLoads) {
+          const uint64_t row = shfl64(off, mine(i) % R::kLoads * R::kRowsPerLoad + pr);
+          st.x[i] = __builtin_nontemporal_load(
+              reinterpret_cast<const u32x4_t*>((mine(i) < R::kLoads ? kb : vb) + row));
+        }
       }
     };
 
     uint32_t page = entry(t);
     const uint16_t* q = a.q + seq * a.q_stride + (uint64_t)q_head * D;
-    Query q_own;
-    auto query_at = [&](int rt) { return smem + L::kQueries + rt * L::kQueryTile; };
-    if constexpr (RT == 1) {
-      q_own = query(q, lr, rows, g);
-    } else {
-      // more than one tile of query rows would take the registers of the sums:
-      // they lie in LDS for all waves, in the order of the lanes
-      for (uint32_t rt = wave; rt < (uint32_t)RT; rt += W) {
-        const Query x = query(q, rt * 16u + lr, rows, g);
+    Query qf[RW];
+    f32x4_t acc[RW][kDb];
+    // as in the prompt kernel: the lowest finite value, against which scores of -inf
+    // alone have exponentials of 0
+    float m_ref[RW], l_run[RW];
 #pragma unroll
-        for (int f = 0; f < kFrags; ++f)
-          *reinterpret_cast<u32x4_t*>(query_at(rt) + f * 1024 + lane * 16u) = x.f[f];
-      }
-      __syncthreads();
-    }
-    auto query_frag = [&](int rt, int f) {
-      if constexpr (RT == 1) return q_own.f[f];
-      else return *reinterpret_cast<const u32x4_t*>(query_at(rt) + f * 1024 + lane * 16u);
-    };
-    f32x4_t acc[RT][kDb];
-    float m_ref[RT], l_run[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      // as in the prompt kernel: the lowest finite value, against which scores of
-      // -inf alone have exponentials of 0
+    for (int rt = 0; rt < RW; ++rt) {
+      qf[rt] = query(q, (member * RW + rt) * 16u + lr, rows, g);
       m_ref[rt] = -__FLT_MAX__;
       l_run[rt] = 0.0f;
 #pragma unroll
@@ -330,14 +346,14 @@ struct Decode {
     // moves chunk bits alone, so another chunk of a row is an exclusive or, and
     // another row an offset and the exclusive or of its swizzle.  Row m of key
     // block b is key 8 (m / 4) + 4 b + m % 4.
-    const uint32_t own_at = wave * T::kLds;
+    const uint32_t own_at = team * L::kOwn;
     const uint32_t k_row = 8u * (lr >> 2) + (lr & 3u);
-    const uint32_t v_row = 8u * g + (E4M3 ? lr >> 1 : lr >> 2);
-    uint32_t put_at = own_at + pr * T::kRowBytes + ((pc ^ T::swz(pr)) << 4);
+    const uint32_t v_row = 8u * g + (kCodes ? lr >> 1 : lr >> 2);
+    uint32_t put_at = own_at + pr * T::kRowBytes + (((kCodes == E4M3 ? pc : 2u * pc) ^ T::swz(pr)) << 4);
     uint32_t k_at = own_at + k_row * T::kRowBytes +
                     ((g ^ T::swz(k_row)) << 4);
     uint32_t v_at = own_at + T::kBytes + v_row * T::kRowBytes +
-                    ((((E4M3 ? 0u : (lr & 3u) >> 1)) ^ T::swz(v_row)) << 4) + (lr & 1u) * 8u;
+                    ((((kCodes ? 0u : (lr & 3u) >> 1)) ^ T::swz(v_row)) << 4) + (lr & 1u) * 8u;
 
     // the stage's tile into the wave's LDS.  Keys that are left out have scores
     // of -inf whatever K holds, but 0 times their V must be 0: V becomes +0.
@@ -345,17 +361,26 @@ struct Decode {
       asm volatile("" : "+v"(put_at));
       if (st.valid != 0xffffffffu) {
 #pragma unroll
-        for (int i = 0; i < T::kLoads; ++i)
-          if ((st.valid >> (i * T::kRowsPerLoad + pr) & 1u) == 0u) st.v[i] = u32x4_t{0, 0, 0, 0};
+        for (uint32_t j = 0; j < kMine; ++j) {
+          const uint32_t i = mine(j), r = i % R::kLoads * R::kRowsPerLoad;
+          if (i >= R::kLoads && (st.valid >> (r + pr) & 1u) == 0u) st.x[j] = u32x4_t{0, 0, 0, 0};
+        }
         asm volatile("");  // a branch, not a select in every tile
       }
 #pragma unroll
-      for (int i = 0; i < T::kLoads; ++i) {
-        // the swizzle of row i R + pr (R a power of two above pr) is that of both
-        const uint32_t at = (put_at ^ T::swz(i * T::kRowsPerLoad) << 4) +
-                            i * T::kRowsPerLoad * T::kRowBytes;
-        *reinterpret_cast<u32x4_t*>(smem + at) = st.k[i];
-        *reinterpret_cast<u32x4_t*>(smem + at + T::kBytes) = st.v[i];
+      for (uint32_t j = 0; j < kMine; ++j) {
+        const uint32_t i = mine(j), r = i % R::kLoads * R::kRowsPerLoad;
+        if (S > 1 && i >= 2u * R::kLoads) break;
+        // the swizzle of row r + pr (r a multiple of a power of two above pr) is that
+        // of both
+        const uint32_t at = ((put_at + buffer) ^ T::swz(r) << 4) + r * T::kRowBytes +
+                            (i < R::kLoads ? 0u : T::kBytes);
+        if constexpr (kCodes == E4M3) {
+          *reinterpret_cast<u32x4_t*>(smem + at) = st.x[j];
+        } else {  // swizzles of bf16 rows are even: the two chunks stay together
+          *reinterpret_cast<u32x4_t*>(smem + at) = widen_codes8(st.x[j][0], st.x[j][1]);
+          *reinterpret_cast<u32x4_t*>(smem + at + 16u) = widen_codes8(st.x[j][2], st.x[j][3]);
+        }
       }
       if constexpr (E4M3)
         scales(wave)[lane] = (st.valid >> (lane & 31u) & 1u) != 0u
@@ -367,19 +392,20 @@ struct Decode {
       // the addresses of the pieces are made here, tile by tile: kept over the
       // loop they would take the registers of a stage
       asm volatile("" : "+v"(k_at), "+v"(v_at));
-      f32x4_t sc[RT][2];
+      const uint32_t k_from = k_at + buffer, v_from = v_at + buffer;
+      f32x4_t sc[RW][2];
       // Codes are widened to bf16, exactly, where the MFMA takes them.  The fp8 MFMA
       // would take them as they are (and a query as the sum of two e4m3), but
       // drops what is 2^-15 of its largest product: lse was off by 6e-5.
 #pragma unroll
-      for (int f = 0; f < kFrags; f += E4M3 ? 2 : 1) {
-        bf16x8_t kf[2][E4M3 ? 2 : 1];
+      for (int f = 0; f < kFrags; f += kCodes ? 2 : 1) {
+        bf16x8_t kf[2][kCodes ? 2 : 1];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const u32x4_t x = *reinterpret_cast<const u32x4_t*>(
-              smem + (k_at ^ (E4M3 ? 32u : 64u) * f ^ T::swz(4u * b) << 4) +
+              smem + (k_from ^ (kCodes ? 32u : 64u) * f ^ T::swz(4u * b) << 4) +
               4u * T::kRowBytes * b);
-          if constexpr (E4M3) {
+          if constexpr (kCodes) {
             kf[b][0] = __builtin_bit_cast(bf16x8_t, widen_codes8(x[0], x[1]));
             kf[b][1] = __builtin_bit_cast(bf16x8_t, widen_codes8(x[2], x[3]));
           } else {
@@ -387,15 +413,14 @@ struct Decode {
           }
         }
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
+        for (int rt = 0; rt < RW; ++rt)
 #pragma unroll
-          for (int h = 0; h < (E4M3 ? 2 : 1); ++h) {
-            const bf16x8_t qf = __builtin_bit_cast(bf16x8_t, query_frag(rt, f + h));
+          for (int h = 0; h < (kCodes ? 2 : 1); ++h)
 #pragma unroll
             for (int b = 0; b < 2; ++b)
               sc[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                  kf[b][h], qf, f + h == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[rt][b], 0, 0, 0);
-          }
+                  kf[b][h], __builtin_bit_cast(bf16x8_t, qf[rt].f[f + h]),
+                  f + h == 0 ? f32x4_t{0.f, 0.f, 0.f, 0.f} : sc[rt][b], 0, 0, 0);
       }
       // lane's key j (0..7) is 8 g + j
       float ks[8], vs[8];
@@ -413,9 +438,9 @@ struct Decode {
       }
       // scores in the log2 domain (bf16 cache: before its scale), then probabilities
       // of all query rows, so that one branch serves them
-      float x[RT][8], p[RT][8], psum[RT];
+      float x[RW][8], p[RW][8], psum[RW];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int rt = 0; rt < RW; ++rt)
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[rt][j] = sc[rt][j >> 2][j & 3] * (E4M3 ? ks[j] : 1.0f);
       if (valid != 0xffffffffu) {
@@ -423,14 +448,14 @@ struct Decode {
         for (int j = 0; j < 8; ++j) {
           const bool keep = (valid >> (8u * g + j) & 1u) != 0u;
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt) x[rt][j] = keep ? x[rt][j] : -INFINITY;
+          for (int rt = 0; rt < RW; ++rt) x[rt][j] = keep ? x[rt][j] : -INFINITY;
         }
         asm volatile("");
       }
       auto probabilities = [&] {
         bool small = true;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int rt = 0; rt < RW; ++rt) {
           psum[rt] = 0.0f;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -444,7 +469,7 @@ struct Decode {
       };
       if (__any(!probabilities())) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
+        for (int rt = 0; rt < RW; ++rt) {
           float top = x[rt][0];
 #pragma unroll
           for (int j = 1; j < 8; ++j) top = fmaxf(top, x[rt][j]);
@@ -462,9 +487,9 @@ struct Decode {
       }
       // two bf16 parts: the second MFMA takes what the first one's rounding (half
       // a step, 2^-8) leaves, for 1% more time
-      bf16x8_t pf[RT], pl[RT];
+      bf16x8_t pf[RW], pl[RW];
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
+      for (int rt = 0; rt < RW; ++rt) {
         l_run[rt] += psum[rt];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -481,23 +506,23 @@ struct Decode {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const int db = d2 + i;
-          if constexpr (E4M3) {
+          if constexpr (kCodes) {
             const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
-                (lds_i32x2_t*)(smem + (v_at ^ (16u * db))));
+                (lds_i32x2_t*)(smem + (v_from ^ (16u * db))));
             vf[i] = __builtin_bit_cast(bf16x8_t, widen_codes8((uint32_t)c[0], (uint32_t)c[1]));
           } else {
             bf16x4_t half[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h)
               half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
-                  (lds_bf16x4_t*)(smem + (v_at ^ (32u * db)) + 4u * T::kRowBytes * h));
+                  (lds_bf16x4_t*)(smem + (v_from ^ (32u * db)) + 4u * T::kRowBytes * h));
             vf[i] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
           }
         }
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
+          for (int rt = 0; rt < RW; ++rt)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
               acc[rt][d2 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
@@ -509,49 +534,67 @@ struct Decode {
     // the next tile's writes wait for them; the fences keep the compiler from
     // reordering them (it sees one lane's addresses).  One tile is in flight while
     // another is computed: two were no faster (8 x 32 heads x 4096: 87, 97 us).
-    for (; t < end; t += kStep) {
-      put();
-      const uint32_t valid = st.valid;
-      asm volatile("" ::: "memory");
-      if (t + kStep < end) {
-        issue(t + kStep, page);
-        page = entry(t + 2u * kStep);
+    // A tile that waves share goes to the other place than the one before it, which
+    // a wave that is behind may still read; the barrier leaves none two behind.
+    if constexpr (S == 1) {
+      for (; t < end; t += kStep) {
+        put();
+        const uint32_t valid = st.valid;
+        asm volatile("" ::: "memory");
+        if (t + kStep < end) {
+          issue(t + kStep, page);
+          page = entry(t + 2u * kStep);
+        }
+        compute(valid);
+        asm volatile("" ::: "memory");
       }
-      compute(valid);
-      asm volatile("" ::: "memory");
+    } else {
+      for (uint32_t round = sp.tile0 + tile; round < end; round += kStep, t += kStep) {
+        if (t < end) put();
+        const uint32_t valid = st.valid;
+        __syncthreads();
+        if (t + kStep < end) {
+          issue(t + kStep, page);
+          page = entry(t + 2u * kStep);
+        }
+        if (t < end) compute(valid);
+        buffer ^= 2u * T::kBytes;
+      }
+      __syncthreads();
     }
-    finish(seq, q_head - wave / kStep * a.group, rows, n == sp.tiles, slot, acc, m_ref, l_run);
+    finish(seq, WH > 1 ? q_head - team / kStep * a.group : q_head, rows, n == sp.tiles, slot, acc,
+           m_ref, l_run);
   }
 
-  // The sums of a run's waves added for each head in wave order, 16 query rows at a
-  // time.  q_head: the first head's first.
+  // The sums of a run's waves added for each head in wave order, 16 query rows of each
+  // wave at a time.  q_head: the first head's first.
   FE2O3_DEVICE void finish(uint32_t seq, uint32_t q_head, uint32_t rows, bool whole, uint32_t slot,
-                           const f32x4_t (&acc)[RT][kDb], const float (&m_ref)[RT],
-                           const float (&l_run)[RT]) {
+                           const f32x4_t (&acc)[RW][kDb], const float (&m_ref)[RW],
+                           const float (&l_run)[RW]) {
     const uint32_t tid = thread(), lr = tid & 15u, g = tid >> 4 & 3u;
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float l = row_sum(l_run[rt]);
-      if (g == 0u) stat(wave)[rt * 16u + lr] = float2{m_ref[rt], l};
-    }
     const uint64_t part = ((uint64_t)blockIdx.x * 2u + slot) * WH * a.rows;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
+    for (int rt = 0; rt < RW; ++rt) {
       if (rt * 16u >= rows) break;
-      float* mine = (float*)(smem + wave * T::kLds) + lr * T::kSumStride + 4u * g;
+      const float sum = row_sum(l_run[rt]);
+      if (g == 0u) stat(wave)[lr] = float2{m_ref[rt], sum};
+      float* own = (float*)(smem + wave * L::kSums) + lr * T::kSumStride + 4u * g;
 #pragma unroll
-      for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(mine + 16 * db) = acc[rt][db];
+      for (int db = 0; db < kDb; ++db) *reinterpret_cast<f32x4_t*>(own + 16 * db) = acc[rt][db];
       __syncthreads();
-      const uint32_t count = WH * min(rows - rt * 16u, 16u) * (D / 4u);
-      for (uint32_t i = tid; i < count; i += W * 64u) {
-        // rows of one head behind another's: RT > 1 has one head
+      // this turn's rows: of one head behind another's, or of every sharer
+      const uint32_t turn_rows = S > 1 ? 16u * S : min(rows - rt * 16u, 16u);
+      for (uint32_t i = tid; i < WH * turn_rows * (D / 4u); i += W * 64u) {
         const uint32_t at = i / (D / 4u), d = 4u * (i % (D / 4u));
-        const uint32_t wh = WH > 1 ? at / rows : 0u, r = at - wh * rows, row = rt * 16u + r;
+        const uint32_t wh = WH > 1 ? at / turn_rows : 0u, r = at - wh * turn_rows;
+        const uint32_t first = S == 1 ? wh * kStep : r / 16u, tile_row = r % 16u;
+        const uint32_t row = S == 1 ? rt * 16u + r : (first * RW + rt) * 16u + tile_row;
+        if (S > 1 && row >= rows) continue;
         float2 s[kStep];
         float m = -__FLT_MAX__, l = 0.0f;
 #pragma unroll
         for (uint32_t x = 0; x < kStep; ++x) {
-          s[x] = stat(wh * kStep + x)[row];
+          s[x] = stat(first + x * S)[tile_row];
           m = fmaxf(m, s[x].x);
         }
         f32x4_t y = {0.f, 0.f, 0.f, 0.f};
@@ -560,8 +603,8 @@ struct Decode {
           const float weight = __builtin_amdgcn_exp2f(s[x].x - m);
           l += weight * s[x].y;
           y += weight * *reinterpret_cast<const f32x4_t*>(
-                            (const float*)(smem + (wh * kStep + x) * T::kLds) +
-                            r * T::kSumStride + d);
+                            (const float*)(smem + (first + x * S) * L::kSums) +
+                            tile_row * T::kSumStride + d);
         }
         if (whole) {
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // no key: +0
@@ -584,13 +627,13 @@ struct Decode {
 // One workgroup of W waves per sequence and block of query rows, for calls whose
 // sequences are too short to be worth a join.
 template <int D, bool E4M3, int RT, uint32_t W>
-__global__ void __launch_bounds__(W * 64, (W == kWaves ? per_cu<D, E4M3, RT>() : 2)) paged_whole_kernel(Args a) {
+__global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, E4M3, RT>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of(a, seq);
-  Decode<D, E4M3, RT, 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+  Decode<D, E4M3, row_tiles(RT), sharers(RT), 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
 // The list of all work: sequence, then block of query rows (or WH KV heads), then
@@ -677,7 +720,7 @@ struct Plan {
 };
 
 template <int D, bool E4M3, int RT, int WH>
-__global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split_kernel(Args a) {
+__global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, E4M3, RT>() * sharers(RT))) paged_split_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   using P = Plan<RT, WH>;
   const P plan(a);
@@ -690,7 +733,7 @@ __global__ void __launch_bounds__(kThreads, (per_cu<D, E4M3, RT>())) paged_split
   Span sp = plan.span(seq);
   uint32_t length = P::rounds(sp);
   uint32_t hb = uniform(rest / length), pos = rest - hb * length;
-  Decode<D, E4M3, RT, WH> decode(a, smem);
+  Decode<D, E4M3, row_tiles(RT), sharers(RT), WH, waves(RT)> decode(a, smem);
   while (true) {
     const uint32_t stop = min(length, pos + (end - at));
     const uint32_t tile = P::kStep * (max(pos, P::kSetup) - P::kSetup);
@@ -788,18 +831,19 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_run
 
 template <int D, bool E4M3, int RT, int WH>
 int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
-  constexpr uint32_t kSmem = Lds<D, E4M3, RT>::kBytes;
+  constexpr uint32_t kSmem = Lds<D, E4M3, sharers(RT), waves(RT)>::kBytes;
+  using P = Plan<RT, WH>;
   const auto fn = paged_split_kernel<D, E4M3, RT, WH>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   // as many workgroups as are resident at once, and work for each wave
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head / WH;
-  const uint64_t most = heads * ((tiles + kWaves / WH - 1u) / (kWaves / WH) + Plan<RT, WH>::kSetup);
+  const uint64_t most = heads * ((tiles + P::kStep - 1u) / P::kStep + P::kSetup);
   uint32_t workgroups = per_cu<D, E4M3, RT>() * cus;
   if (workgroups > kMaxWorkgroups) workgroups = kMaxWorkgroups;
   if (workgroups > most) workgroups = (uint32_t)most;
   a.workgroups = workgroups;
-  fn<<<workgroups, kThreads, kSmem, s>>>(a);
+  fn<<<workgroups, waves(RT) * 64u, kSmem, s>>>(a);
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
   // Many heads have few parts each, and rows share the threads; few have many,
@@ -822,7 +866,7 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
 
 template <int D, bool E4M3, int RT, uint32_t W>
 int32_t launch_whole(const Args& a, hipStream_t s) {
-  constexpr uint32_t kSmem = Lds<D, E4M3, RT, W>::kBytes;
+  constexpr uint32_t kSmem = Lds<D, E4M3, sharers(RT), W>::kBytes;
   const auto fn = paged_whole_kernel<D, E4M3, RT, W>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
@@ -844,16 +888,21 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   //   1 x 1000 9.7, 14.8    4 x 1000  12.1, 15.7    16 x 1000 20.8, 17.7
   //   64 x 1..2000 48.1, 55.2   30 x 1..2000 27.4, 30.1   40 windows of 1024
   //   (64 wide, e4m3) 16.8, 13.0
-  // Few heads take eight waves each.
+  // Few heads take eight waves each.  More than one tile of query rows has more to
+  // join, and a head its own rounds at least (48 rows, one KV head):
+  //   48 x 170 14.0, 9.5    48 x 1000 16.4, 21.9    8 x 500   13.6, 13.1
+  //   64 x 500 16.0, 14.2   200 x 500 24.6, 15.9    300 x 500 32.5, 29.0
   const uint32_t resident = (per_cu<D, E4M3, RT>() == 1 ? 1u : 2u) * cus;
   const bool wide = RT == 1 && heads <= cus;
   const uint64_t rounds_whole =
       wide ? (tiles + 7u) / 8u : ((tiles + 3u) / 4u * heads + resident - 1u) / resident;
   const uint64_t rounds_split = (heads * tiles + 4u * resident - 1u) / (4u * resident);
-  if (tiles <= kWholeTiles && rounds_whole <= rounds_split + 2u) {
+  const uint64_t least = RT == 1 ? 0u : (tiles + 3u) / 4u;  // of one head
+  if (tiles <= kWholeTiles && (rounds_whole > least ? rounds_whole : least) <=
+                                  rounds_split + (RT == 1 ? 2u : 4u)) {
     if constexpr (RT == 1)
       if (wide && tiles > kWaves) return launch_whole<D, E4M3, RT, 8>(a, s);
-    return launch_whole<D, E4M3, RT, kWaves>(a, s);
+    return launch_whole<D, E4M3, RT, waves(RT)>(a, s);
   }
   if constexpr (RT == 1)
     if (a.cache.kv_heads % kWaves == 0u) return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
@@ -868,17 +917,17 @@ int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) 
   return launch<D, E4M3, 4>(a, tiles, cus, s);
 }
 
-#define FE2O3_KERNEL(NAME, FN, LDS) \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", NAME, (const void*)FN, kThreads, LDS})
+#define FE2O3_KERNEL(NAME, FN, THREADS, LDS) \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", NAME, (const void*)FN, THREADS, LDS})
 #define FE2O3_SPLIT(D, F, RT, WH) \
-  FE2O3_KERNEL("paged_split_kernel<" #D "," #F "," #RT "," #WH ">", (paged_split_kernel<D, F, RT, WH>), (Lds<D, F, RT>::kBytes))
-#define FE2O3_PAGED(D, F, RT) \
-  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT ",4>", (paged_whole_kernel<D, F, RT, 4>), (Lds<D, F, RT>::kBytes)), \
-  FE2O3_SPLIT(D, F, RT, 1)
-#define FE2O3_PAGED_ALL(D, F) \
-  FE2O3_PAGED(D, F, 1), FE2O3_PAGED(D, F, 2), FE2O3_PAGED(D, F, 3), FE2O3_PAGED(D, F, 4), \
-  FE2O3_SPLIT(D, F, 1, 4), \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_whole_kernel<" #D "," #F ",1,8>", (const void*)paged_whole_kernel<D, F, 1, 8>, 512, Lds<D, F, 1, 8>::kBytes})
+  FE2O3_KERNEL("paged_split_kernel<" #D "," #F "," #RT "," #WH ">", (paged_split_kernel<D, F, RT, WH>), waves(RT) * 64u, (Lds<D, F, sharers(RT), waves(RT)>::kBytes))
+#define FE2O3_WHOLE(D, F, RT) \
+  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT ">", (paged_whole_kernel<D, F, RT, waves(RT)>), waves(RT) * 64u, (Lds<D, F, sharers(RT), waves(RT)>::kBytes))
+#define FE2O3_PAGED_ALL(D, F)                                                                   \
+  FE2O3_SPLIT(D, F, 1, 1), FE2O3_SPLIT(D, F, 1, 4), FE2O3_SPLIT(D, F, 2, 1),                    \
+  FE2O3_SPLIT(D, F, 3, 1), FE2O3_SPLIT(D, F, 4, 1), FE2O3_WHOLE(D, F, 1),                       \
+  FE2O3_WHOLE(D, F, 2), FE2O3_WHOLE(D, F, 3), FE2O3_WHOLE(D, F, 4),                             \
+  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F ",1,8>", (paged_whole_kernel<D, F, 1, 8>), 512, (Lds<D, F, 1, 8>::kBytes))
 #define FE2O3_JOIN_OF(D, RT, WH, ROWS, THREADS)                                                \
   fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #RT "," #WH "," #ROWS ">", (const void*)paged_join_kernel<D, RT, WH, ROWS, THREADS>, THREADS, 0})
 #define FE2O3_JOIN(D, RT, WH, ROWS) \
@@ -893,7 +942,7 @@ const fe2o3_host::KernelRegistrar kRegistered[] = {
 #undef FE2O3_KERNEL
 #undef FE2O3_SPLIT
 #undef FE2O3_PAGED_ALL
-#undef FE2O3_PAGED
+#undef FE2O3_WHOLE
 #undef FE2O3_JOIN
 #undef FE2O3_JOIN_OF
 #undef FE2O3_JOIN_ALL

@@ -273,6 +273,18 @@ def test_many_sequences(gpu, fmt, seqs, q_heads, kv_heads):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("q_heads,kv_heads", [(33, 1), (48, 1), (98, 2), (64, 1)])
+@pytest.mark.parametrize("window", [0, 33, 700])
+def test_waves_that_share_tiles(gpu, fmt, head_dim, q_heads, kv_heads, window):
+    """More than 32 query heads a KV head: runs of every number of tiles that leaves some
+    of the four teams without one, pages that end inside tiles, rows that end inside a
+    wave's, and calls of one workgroup a head as well as many."""
+    _check(gpu, fmt, [1, 31, 33, 95, 130, 0, 257], q_heads, kv_heads, head_dim, 24, window=window)
+    _check(gpu, fmt, [2500, 0, 33, 1300], q_heads, kv_heads, head_dim, 40, window=window)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("peak", [30.0, 1e-3])
 def test_peaked_and_flat_scores(gpu, fmt, peak):
     """Scores up to several hundred, where one key has almost all of the weight
