@@ -273,6 +273,15 @@ def test_many_sequences(gpu, fmt, seqs, q_heads, kv_heads):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("q_heads", [20, 48, 70])  # 70: two blocks of query rows
+def test_many_sequences_of_many_query_heads(gpu, fmt, q_heads):
+    lengths = [41 * i % 97 for i in range(300)]
+    lengths[7] = 1500
+    lengths[298] = 1400
+    _check(gpu, fmt, lengths, q_heads, 1, 64, 16)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("head_dim", [64, 128])
 @pytest.mark.parametrize("q_heads,kv_heads", [(33, 1), (48, 1), (98, 2), (64, 1)])
 @pytest.mark.parametrize("window", [0, 33, 700])
