@@ -24,7 +24,8 @@
 //   * An e4m3 cache's K scales multiply the scores, its V scales the
 //     probabilities before these are rounded for the MFMA.
 // With a multiple of four KV heads (and group <= 16) a workgroup's four waves
-// have a head each: they read neighbouring rows, and nothing is added in LDS.
+// have a head each in large calls: they read neighbouring rows, and nothing is added
+// in LDS.
 // Otherwise they take every fourth tile of one head and add their sums; of a group
 // above 32 four teams of three or four waves, a wave for every 16 query rows, do so.
 //
@@ -904,8 +905,13 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
       if (wide && tiles > kWaves) return launch_whole<D, E4M3, RT, 8>(a, s);
     return launch_whole<D, E4M3, RT, waves(RT)>(a, s);
   }
+  // Four heads a workgroup read neighbouring rows, but every part that the join adds
+  // has the rows of four: worth it where a workgroup has six rounds at least (1 x 130001
+  // 91.8, 88.7 with four; 4 x 16000 49.6, 47.7; 1 x 40000 34.5, 35.4; 8 x 1200..2400,
+  // group 7: 17.7, 20.0; 1 x 17313 of 4 KV heads, group 16, e4m3: 15.5, 19.4).
   if constexpr (RT == 1)
-    if (a.cache.kv_heads % kWaves == 0u) return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
+    if (a.cache.kv_heads % kWaves == 0u && heads / kWaves * tiles >= 6u * resident)
+      return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
   return launch_split<D, E4M3, RT, 1>(a, tiles, cus, s);
 }
 

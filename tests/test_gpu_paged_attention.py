@@ -273,6 +273,19 @@ def test_many_sequences(gpu, fmt, seqs, q_heads, kv_heads):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("lengths,q_heads,kv_heads,head_dim", [
+    ([40001], 8, 4, 128), ([5000, 1, 0, 0, 9000, 33], 16, 8, 64),
+    ([1500, 1501, 1499, 31] * 6, 64, 4, 128), ([37 * i % 151 for i in range(700)], 4, 4, 64),
+])
+def test_four_heads_a_workgroup(gpu, fmt, lengths, q_heads, kv_heads, head_dim):
+    """A table with room for much longer sequences, for which four KV heads share a
+    workgroup whatever the lengths are."""
+    b = Batch(gpu, fmt, lengths, q_heads, kv_heads, head_dim, 64, cols=1700)
+    b.compare(b.run(max_length=1700 * 64), b.reference())
+    assert b.inputs_unchanged()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("q_heads", [20, 48, 70])  # 70: two blocks of query rows
 def test_many_sequences_of_many_query_heads(gpu, fmt, q_heads):
     lengths = [41 * i % 97 for i in range(300)]
