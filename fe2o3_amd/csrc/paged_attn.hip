@@ -37,9 +37,9 @@
 // keys.  Short calls run one workgroup a head instead (launch).
 //
 // Measured, of a repeated call, bytes of K and V read once (a kernel that only
-// reads them: 6.4-6.9 TB/s): 8 sequences of 4096 keys, 32 heads, bf16: 82 us =
+// reads them: 6.4-6.9 TB/s): 8 sequences of 4096 keys, 32 heads, bf16: 80-82 us =
 // 6.6 TB/s, and 4.6 of the join; 130001 keys of one sequence, 8 heads: 82 us and
-// 7; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 88 us = 6.3 TB/s, 4.8; 500
+// 6; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 88 us = 6.3 TB/s, 4.8; 500
 // keys of one: 7.7 us.  48 query heads on one KV head, 48 sequences of 100 to 6000
 // keys: 21 us and 4.0, half of it starting, adding and ending.
 #include "common.hpp"
@@ -760,13 +760,14 @@ __global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, E4M3, RT>() * share
 // is the head, or with by_runs the run that began it: of more heads than runs,
 // most lie within one (4096 sequences of 1 to 200 keys, 8 heads: 12 us; 213 over
 // the heads, counted 64 by 64).  Bound by latency: the lengths, then the parts (4.6 us after 64
-// sequences, 7 us for the 256 parts of one).
+// sequences, 6 us for the 256 parts of one).
 template <int D, int RT, int WH, int ROWS, int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_runs) {
   using P = Plan<RT, WH>;
   constexpr uint32_t kQuads = D / 4u, kWays = THREADS / (kQuads * ROWS);
-  __shared__ f32x4_t part_sum[kWays > 1u ? THREADS : 1];
-  __shared__ float2 part_stat[kWays > 1u ? THREADS : 1];
+  constexpr uint32_t kShared = kWays > 1u ? THREADS / 64u * kQuads * ROWS : 1u;
+  __shared__ f32x4_t part_sum[kShared];
+  __shared__ float2 part_stat[kShared];
   const P plan(a);
   const uint32_t quad = threadIdx.x % kQuads, d = 4u * quad;
   const uint32_t r = threadIdx.x / kQuads % ROWS, way = threadIdx.x / (kQuads * ROWS);
@@ -802,14 +803,35 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_run
         *reinterpret_cast<const f32x4_t*>(a.sums + p * D + d));
   }
   if constexpr (kWays > 1u) {
-    part_sum[threadIdx.x] = y;
-    part_stat[threadIdx.x] = float2{m, l};
+    // a wave's ways by lane exchanges, then the waves' sums: largest first, so that
+    // no addition waits for another's exponential
+    constexpr uint32_t kRowLanes = kQuads * ROWS, kAll = THREADS / 64;
+#pragma unroll
+    for (uint32_t o = kRowLanes; o < 64u; o <<= 1) {
+      const float2 s = {__shfl_xor(m, o, 64), __shfl_xor(l, o, 64)};
+      f32x4_t x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __shfl_xor(y[e], o, 64);
+      add(s, x);
+    }
+    const uint32_t lane = threadIdx.x & 63u;
+    if (lane < kRowLanes) {
+      part_sum[threadIdx.x / 64u * kRowLanes + lane] = y;
+      part_stat[threadIdx.x / 64u * kRowLanes + lane] = float2{m, l};
+    }
     __syncthreads();
     if (way == 0u) {
-#pragma unroll 8
-      for (uint32_t w = 1; w < kWays; ++w)
-        add(part_stat[w * kQuads * ROWS + threadIdx.x],
-            part_sum[w * kQuads * ROWS + threadIdx.x]);
+#pragma unroll
+      for (uint32_t w = 1; w < kAll; ++w) m = fmaxf(m, part_stat[w * kRowLanes + lane].x);
+      l = 0.0f;
+      y = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (uint32_t w = 0; w < kAll; ++w) {
+        const float2 s = part_stat[w * kRowLanes + lane];
+        const float weight = __builtin_amdgcn_exp2f(s.x - m);
+        l += weight * s.y;
+        y += weight * part_sum[w * kRowLanes + lane];
+      }
     }
   }
   uint32_t q_head;
@@ -848,7 +870,7 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
   // Many heads have few parts each, and rows share the threads; few have many,
-  // which a row's threads share (one head's 256 parts: 16 us on 256 threads, 7 on
+  // which a row's threads share (one head's 256 parts: 7.1 us on 256 threads, 6 on
   // 1024; 8 parts of 64 heads of 16 rows: 4.6 either way, of 33 heads of 64 rows 5.6
   // and, rows sharing, 4.3).
   constexpr int kRows = kThreads / (D / 4);
