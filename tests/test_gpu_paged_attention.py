@@ -580,6 +580,36 @@ def test_captured_and_replayed(gpu, fmt):
     assert workspace.guards_intact()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_two_calls_at_once(gpu, fmt):
+    """Steps on two streams, each with its own cache and workspace, side by side: the
+    bits of the same calls alone."""
+    batches = [Batch(gpu, fmt, [9000, 0, 33, 2000], 8, 2, 128, 16, seed=1),
+               Batch(gpu, fmt, [700 + 5 * i for i in range(90)], 48, 1, 64, 24, seed=2)]
+    alone = [b.run() for b in batches]
+    for b, got in zip(batches, alone):
+        b.compare(got, b.reference())
+    streams = [gpu.stream() for _ in batches]
+    kern = _k()
+    spaces = [Guarded(gpu, np.full(kern.paged_attention_workspace_bytes(
+        b.q_heads, b.kv_heads, b.head_dim), 0xFF, np.uint8)) for b in batches]
+    outs = [[b.outputs() for _ in range(4)] for b in batches]
+    gpu.synchronize()
+    for turn in range(4):
+        for b, stream, space, out in zip(batches, streams, spaces, outs):
+            kern.paged_attention_decode(
+                b.cache, b.dev_q.body, b.dev_table.body, b.dev_lengths.body, out[turn][0].body,
+                out[turn][1].body, space.body, max_length=max(b.lengths), scale=b.scale,
+                q_heads=b.q_heads, stream=stream, sync=False)
+    gpu.synchronize()
+    for b, want, out in zip(batches, alone, outs):
+        for o, stat in out:
+            assert_same(o.download(), want[0].download())
+            assert_same(stat.download(), want[1].download())
+            assert o.guards_intact() and stat.guards_intact()
+    assert all(space.guards_intact() for space in spaces)
+
+
 def test_tensors_and_streams(gpu):
     """The same calls on torch tensors, on a stream of torch's own, with K and V in
     one allocation and the rows columns of a fused projection."""
