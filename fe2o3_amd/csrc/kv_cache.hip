@@ -17,6 +17,7 @@ namespace {
 
 using namespace fe2o3;
 using kv_cache::FastDiv;
+using kv_cache::RowScale;
 using kv_cache::View;
 
 constexpr int kThreads = 256;
@@ -72,28 +73,6 @@ FE2O3_DEVICE float amax8(u32x4_t x, float m) {
   for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(bf16_of(x, i)));
   return m;
 }
-
-// A row's scale and what divides by it.  x / scale is x r with r the rounded
-// reciprocal, corrected once by its remainder: for the scales that a row of bf16
-// has (its largest of 128 significands, over 448) and every bf16 x up to that
-// largest, this is the correctly rounded quotient, checked over all of them
-// (tests/test_kv_cache_host.py); x r alone differs by a code for 140 of 385088.
-// Three operations instead of the division's ten, with the hardware's packing of
-// codes: 32768 tokens of 8 heads 79 us -> 44 (42 with nontemporal stores).  Scales
-// below the smallest normal or infinite divide as they are.
-struct RowScale {
-  float scale, r;
-  bool usual;
-  explicit FE2O3_DEVICE RowScale(float amax) {
-    scale = fmaxf(amax, 1.17549435e-38f) / 448.0f;
-    r = 1.0f / scale;
-    usual = scale >= 1.17549435e-38f && scale <= __FLT_MAX__;
-  }
-  FE2O3_DEVICE float quotient(float x) const {
-    const float q = x * r;
-    return __builtin_fmaf(__builtin_fmaf(-q, scale, x), r, q);
-  }
-};
 
 FE2O3_DEVICE u32x2_t quantize8(u32x4_t x, const RowScale& s) {
   u32x2_t q;

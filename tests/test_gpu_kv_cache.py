@@ -174,6 +174,31 @@ def test_write_zero_rows_and_ties(gpu):
     _write_case(gpu, "e4m3", 40, 2, 128, 16, values=values)
 
 
+def test_write_zeros_of_both_signs(gpu):
+    """Every row, of ordinary magnitude, holds zeros of both signs: the codes keep
+    the sign, as the encoder does."""
+    def values(rng, shape, part):
+        x = _bf16_bits(rng.standard_normal(shape).astype(np.float32))
+        x[..., 3::7] = 0x8000
+        x[..., 5::7] = 0
+        return x
+    for head_dim in (64, 100):
+        _write_case(gpu, "e4m3", 41, 2, head_dim, 16, values=values)
+
+
+def test_write_small_rows(gpu):
+    """Rows whose largest value lies anywhere from the smallest normal to far above
+    the scales that divide as they are, x of any significand and sign down to 2^-20
+    of it: the division's codes."""
+    def values(rng, shape, part):
+        top = 1 + np.arange(shape[0])[:, None, None] % 70
+        exponent = np.maximum(top - rng.integers(0, 20, shape), 0)
+        exponent[..., 0] = top[..., 0]
+        return (exponent << 7 | rng.integers(0, 128, shape)
+                | rng.integers(0, 2, shape) << 15).astype(np.uint16)
+    _write_case(gpu, "e4m3", 700, 2, 256, 16, values=values)
+
+
 def test_write_nonfinite_rows(gpu):
     """A NaN stays a NaN and leaves the rest of its row as it would be; a row with
     an infinity has an infinite scale."""

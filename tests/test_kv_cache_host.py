@@ -112,6 +112,16 @@ def test_e4m3_quotients_by_reciprocal():
     assert checked > 350000
 
 
+def test_e4m3_write_codes_are_the_divisions(tmp_path):
+    """The write's own quotients (kv_cache.hpp, RowScale) for every bf16 row maximum and
+    x of both signs, zeros among them: the codes of the division."""
+    exe = tmp_path / "row_scale_check"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-fopenmp", "-ffp-contract=off", "-o", str(exe),
+                    os.path.join(ROOT, "tests", "row_scale_check.cpp")], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "bad 0" in r.stdout, r.stdout
+
+
 def test_page_division(tmp_path):
     exe = tmp_path / "fast_div_check"
     subprocess.run(["g++", "-O2", "-std=c++17", "-o", str(exe),
