@@ -377,6 +377,19 @@ class LibraryMissing(ImportError):
     pass
 
 
+def _share_runtime():
+    """Gives the loaded HIP and HSA runtimes the names without a version by which
+    torch's libraries ask for them: torch imported later would otherwise map the
+    copies that it brings, and two runtimes in one process leave torch without a
+    device.  Loads nothing; where the loader does not find these names, torch has to
+    be imported first."""
+    for name in ("libamdhip64.so", "libhsa-runtime64.so"):
+        try:
+            C.CDLL(name, mode=os.RTLD_NOLOAD | os.RTLD_NOW)
+        except OSError:
+            pass
+
+
 def lib():
     """The loaded library with every signature declared.  Raises
     LibraryMissing when the .so has not been built."""
@@ -387,6 +400,7 @@ def lib():
                 f"{LIB_PATH} is not built; run __graft_entry__.build() "
                 "(no CPU fallback exists)")
         L = C.CDLL(LIB_PATH)
+        _share_runtime()
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(L, name, None)
             if fn is None:  # reported by tests/test_abi.py; calling it raises AttributeError
