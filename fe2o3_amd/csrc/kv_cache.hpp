@@ -34,6 +34,17 @@ struct FastDiv {
   }
 };
 
+// A list of workgroups as a grid of rows of kGridWidth: number blockIdx.y * kGridWidth +
+// blockIdx.x, those from n on in the last row with nothing to do.  A dimension of a grid
+// holds fewer than 2^32 threads, and a workgroup has up to 1024.
+constexpr uint32_t kGridWidth = 1u << 21;
+struct Grid {
+  uint32_t x, y;
+  static inline Grid of(uint32_t n) {  // 1 <= n < 2^31
+    return n < kGridWidth ? Grid{n, 1u} : Grid{kGridWidth, (n - 1u) / kGridWidth + 1u};
+  }
+};
+
 // A row's scale and what divides by it.  x / scale is q = RN(x r) with r the rounded
 // reciprocal, corrected once by its remainder: the correctly rounded quotient while
 // the remainder is exact (r is at most half an ulp off, q less than one).  The remainder's

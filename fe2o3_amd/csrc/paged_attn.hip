@@ -56,7 +56,6 @@ constexpr uint32_t kKeys = 32;              // keys per tile
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
 constexpr uint32_t kWholeTiles = 40;        // of a call without a join
-constexpr uint32_t kGridX = 1u << 22;       // a grid holds fewer than 2^32 threads a dimension
 typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
 constexpr uint32_t kBlockRows = 64;         // query heads that one pass over K and V serves
 
@@ -631,7 +630,7 @@ template <int D, bool E4M3, int RT, uint32_t W>
 __global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, E4M3, RT>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
-  const uint32_t id = blockIdx.y * kGridX + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
+  const uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of(a, seq);
   Decode<D, E4M3, row_tiles(RT), sharers(RT), 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
@@ -894,8 +893,8 @@ int32_t launch_whole(const Args& a, hipStream_t s) {
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
-  const dim3 grid(heads < kGridX ? heads : kGridX, (heads - 1u) / kGridX + 1u);
-  fn<<<grid, W * 64u, kSmem, s>>>(a);
+  const kv_cache::Grid grid = kv_cache::Grid::of(heads);
+  fn<<<dim3(grid.x, grid.y), W * 64u, kSmem, s>>>(a);
   return fe2o3_host::after_launch();
 }
 

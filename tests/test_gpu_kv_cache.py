@@ -357,3 +357,47 @@ def test_offsets_past_32_bits(gpu):
         for row, slot in enumerate(slots):
             if slot >= 8:
                 assert_same(got[slot - 8], a[row])
+
+
+def test_more_workgroups_than_a_grid_row(gpu):
+    """A write of more rows than one turn of the largest grid, and a read of more
+    tokens than a grid's first row, back from the written cache."""
+    torch = pytest.importorskip("torch")
+    kern = _k()
+    tokens, heads, page_size = (1 << 22) + 9, 64, 1024
+    pages = tokens // page_size + 2
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def bits(*shape):
+        return torch.randint(-32768, 32768, shape, dtype=torch.int16, device="cuda", generator=g)
+
+    held = [bits(pages, page_size, heads, 1) for _ in "kv"]
+    rows = [bits(tokens, heads, 1) for _ in "kv"]
+    slots = torch.randperm(pages * page_size, device="cuda", generator=g)[:tokens]
+    slots[5::7] = -1
+    want = [x.clone().view(-1, heads, 1) for x in held]
+    kept = slots >= 0
+    for w, x in zip(want, rows):
+        w[slots[kept]] = x[kept]
+    bf16 = torch.bfloat16
+    cache = kern.KvCache(*(x.view(bf16) for x in held))
+    kern.kv_cache_write(cache, *(x.view(bf16) for x in rows), slots.to(torch.int32))
+    for x, w in zip(held, want):
+        assert torch.equal(x.view(-1, heads, 1), w)
+
+    # one head of the cache: tokens past the first row of workgroups
+    narrow = [x[:, :, :1] for x in held]
+    starts = torch.tensor([3, 11, 11, tokens - 2], dtype=torch.int32, device="cuda")
+    cols = -(-tokens // page_size)
+    table = torch.randint(0, pages, (3, cols), dtype=torch.int32, device="cuda", generator=g)
+    out = [bits(tokens, 1, 1) for _ in "kv"]
+    expect = [x.clone() for x in out]
+    kern.kv_cache_read(kern.KvCache(*(x.view(bf16) for x in narrow)), table, starts,
+                       *(x.view(bf16) for x in out))
+    for s, (start, end) in enumerate([(3, 11), (11, 11), (11, tokens - 2)]):
+        at = torch.arange(end - start, device="cuda")
+        page = table[s, at // page_size].long()
+        for w, x in zip(expect, narrow):
+            w[start:end] = x[page, at % page_size]
+    for x, w in zip(out, expect):
+        assert torch.equal(x, w)

@@ -417,6 +417,46 @@ def test_offsets_past_32_bits(gpu):
     v.free()
 
 
+def test_more_heads_than_a_grid_row(gpu):
+    """2^21 sequences and some of up to four keys, a workgroup each, with the bound of
+    the other tests (scores of at most 64 in magnitude)."""
+    torch = pytest.importorskip("torch")
+    kern = _k()
+    seqs, d, page_size, pages = (1 << 21) + 5, 64, 4, 50
+    g = torch.Generator(device="cuda").manual_seed(2)
+    k, v = (torch.randn(pages, page_size, 1, d, device="cuda", generator=g).bfloat16()
+            for _ in "kv")
+    q = torch.randn(seqs, 1, d, device="cuda", generator=g).bfloat16()
+    lengths = torch.randint(0, 5, (seqs,), device="cuda", generator=g)
+    lengths[-5:] = torch.tensor([4, 0, 1, 3, 4], device="cuda")
+    table = torch.randint(0, pages, (seqs, 1), dtype=torch.int32, device="cuda", generator=g)
+    out = torch.full_like(q, 3.0)
+    lse = torch.full((seqs, 1), 7.0, device="cuda")
+    ws = torch.empty(kern.paged_attention_workspace_bytes(1, 1, d), dtype=torch.uint8,
+                     device="cuda")
+    kern.paged_attention_decode(kern.KvCache(k, v), q, table, lengths.to(torch.int32), out, lse,
+                                ws, max_length=4, scale=0.125)
+    step = 1 << 19
+    for at in range(0, seqs, step):
+        part = slice(at, min(at + step, seqs))
+        keys, values = (x[table[part, 0].long(), :, 0].double() for x in (k, v))
+        x = (keys * q[part].double()).sum(-1) * 0.125
+        x = x.masked_fill(torch.arange(4, device="cuda") >= lengths[part, None], -np.inf)
+        assert x.max() <= 64.0
+        empty = lengths[part] == 0
+        p = torch.softmax(torch.where(empty[:, None], 0.0, x), -1) * ~empty[:, None]
+        want = (p[..., None] * values).sum(1)
+        mean = (p[..., None] * values.abs()).sum(1)
+        tol = mean * (2.0 ** -8 * (1 + 2.0 ** -7) + 2 * 68 * 2.0 ** -18 + 2.0 ** -20) \
+            + want.abs() * 2.0 ** -8 * (1 + 2.0 ** -7)
+        assert torch.all((out[part, 0].double() - want).abs() <= tol), at
+        assert not torch.any(out[part, 0][empty].view(torch.int16))
+        full = torch.logsumexp(x, -1)
+        off = torch.where(empty, 0.0, (lse[part, 0].double() - full).abs())
+        assert torch.all(off <= 68 * 2.0 ** -18 + 2.0 ** -20 + 64 * 2.0 ** -22)
+        assert torch.equal(torch.isneginf(lse[part, 0]), empty)
+
+
 # ---- together, as a program uses them -----------------------------------------------------
 
 @pytest.mark.parametrize("fmt", FORMATS)

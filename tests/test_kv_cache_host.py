@@ -130,6 +130,38 @@ def test_page_division(tmp_path):
     assert r.returncode == 0 and "bad 0" in r.stdout, r.stdout
 
 
+def test_grids_stay_within_a_launch(tmp_path):
+    """Every number of workgroups has a grid of fewer than 2^32 threads a dimension,
+    of 1024 threads a workgroup, that holds it with less than a row to spare."""
+    src = tmp_path / "grid.cpp"
+    src.write_text('#include <stdio.h>\n'
+                   f'#include "{ROOT}/fe2o3_amd/csrc/kv_cache.hpp"\n' + """
+int main() {
+  using kv_cache::Grid;
+  unsigned long long bad = 0, tried = 0;
+  auto one = [&](uint64_t n) {
+    if (n < 1u || n >= UINT64_C(1) << 31) return;
+    const Grid g = Grid::of((uint32_t)n);
+    const uint64_t held = (uint64_t)g.x * g.y;
+    const bool row = g.y == 1u || g.x == kv_cache::kGridWidth;
+    if (UINT64_C(1024) * g.x >> 32 != 0u || g.y > 65535u || held < n || held - n >= g.x || !row)
+      ++bad;
+    ++tried;
+  };
+  for (uint64_t n = 1; n < 5000u; ++n) one(n);
+  for (int b = 10; b <= 31; ++b)
+    for (uint64_t e = 0; e < 9; ++e)
+      for (uint64_t m = 1; m < 8; ++m) one((UINT64_C(1) << b) * m + e - 4u);
+  printf("tried %llu bad %llu\\n", tried, bad);
+  return bad == 0 ? 0 : 1;
+}
+""")
+    exe = tmp_path / "grid"
+    subprocess.run(["g++", "-O2", "-std=c++17", "-o", str(exe), str(src)], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True)
+    assert r.returncode == 0 and "bad 0" in r.stdout, r.stdout
+
+
 CACHE_REFUSALS = [
     (dict(format=2), SHAPE), (dict(pages=0), SHAPE), (dict(page_size=0), SHAPE),
     (dict(kv_heads=0), SHAPE), (dict(head_dim=0), SHAPE),
