@@ -526,7 +526,8 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
     [seqs, cols], lengths [seqs], at most max_length each; window > 0 keeps the
     last `window` keys (fe2o3_paged_attention_decode).  workspace: device bytes,
     paged_attention_workspace_bytes at least, of no use to another call that may
-    overlap.  DeviceBuffers take q_heads, and q_stride between sequences."""
+    overlap.  out and lse may be flat.  DeviceBuffers take q_heads, and q_stride
+    between sequences."""
     device = _on_current_device(cache)
     head_dim = cache.shape[3]
     lengths_ptr, seqs = _operand(lengths, _INDEX, "lengths", device)
@@ -538,12 +539,14 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
             raise ValueError(f"{rows} rows of q and {seqs} lengths")
         if width != head_dim or (head_stride != width and q_heads != 1):
             raise ValueError("q must be [seqs, q_heads, head_dim] with a sequence's heads dense")
-        if getattr(out, "shape", shape) != shape:
-            raise ValueError(f"out of {tuple(out.shape)} for q of {tuple(shape)}")
     elif q_heads is None:
         raise ValueError("q in a DeviceBuffer needs q_heads")
     elif q_stride is None:
         q_stride = q_heads * head_dim
+    for name, x, want in (("out", out, (seqs, q_heads, head_dim)), ("lse", lse, (seqs, q_heads))):
+        found = getattr(x, "shape", want)
+        if found != want and len(found) != 1:
+            raise ValueError(f"{name} of {tuple(found)}, not {want}")
     table_ptr, table_len, cols = _table(block_table, seqs, device)
     lse_ptr, lse_len = (None, 0) if lse is None else _operand(lse, _FLOAT, "lse", device)
     _call("fe2o3_paged_attention_decode", C.byref(cache.record),

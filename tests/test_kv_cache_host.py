@@ -394,3 +394,44 @@ def test_shapes_that_do_not_fit_are_refused(monkeypatch):
     rows, starts = _Fake((9, 2, 64), (128, 64, 1)), _Fake((4,), (1,), "torch.int32")
     with pytest.raises(ValueError, match="block table"):
         kernels.kv_cache_read(cache, turned, starts, rows, rows)
+
+
+def test_statistics_and_outputs_of_another_shape_are_refused(monkeypatch):
+    """lse of [q_heads, seqs], and out of another shape where q is a DeviceBuffer."""
+    from fe2o3_amd import _lib, kernels, runtime
+
+    class Lib:
+        @staticmethod
+        def fe2o3_rt_get_device(out):
+            out._obj.value = 0
+            return 0
+
+        @staticmethod
+        def fe2o3_paged_attention_decode(*args):
+            raise OverflowError  # the checks are through
+
+        def __getattr__(self, name):
+            raise AssertionError(name)
+
+    monkeypatch.setattr(_lib, "lib", lambda: Lib())
+    cache = kernels.KvCache(*(_Fake((4, 16, 2, 64), (2048, 128, 64, 1)) for _ in "kv"))
+    lengths, table = _Fake((3,), (1,), "torch.int32"), _Fake((3, 2), (2, 1), "torch.int32")
+    ws = _Fake((1 << 20,), (1,), "torch.uint8")
+    held = runtime.DeviceBuffer.__new__(runtime._View)
+    held.ctx = type("Context", (), {"device": 0})()
+    held.dtype, held.count, held.ptr = np.dtype(np.uint16), 3 * 4 * 64, P
+    fits = _Fake((3, 4, 64), (256, 64, 1))
+    other = _Fake((4, 3, 64), (192, 64, 1))
+    stats, turned = (_Fake(s, (s[1], 1), "torch.float32") for s in ((3, 4), (4, 3)))
+    for q, more in ((fits, {}), (held, dict(q_heads=4))):
+        def call(out, lse):
+            kernels.paged_attention_decode(cache, q, table, lengths, out, lse, ws, max_length=32,
+                                           scale=1.0, **more)
+        with pytest.raises(ValueError, match="out of"):
+            call(other, None)
+        with pytest.raises(ValueError, match="lse of"):
+            call(fits, turned)
+        flat = _Fake((3 * 4 * 64,), (1,)), _Fake((12,), (1,), "torch.float32")
+        for out, lse in ((fits, stats), (fits, None), (held, stats), flat):
+            with pytest.raises(OverflowError):
+                call(out, lse)
