@@ -365,12 +365,15 @@ def _extent(shape, strides, name):
 
 
 def _table(block_table, seqs, device):
-    """(pointer, elements, columns) of a block table, flat or [seqs, columns]."""
+    """(pointer, elements, columns) of a block table, flat or [seqs, columns].  A flat
+    one of no sequences may have any number of columns: the most."""
     ptr, count = _operand(block_table, _INDEX, "block_table", device)
     shape = getattr(block_table, "shape", None)
     if shape is not None and len(shape) != 1 and shape[0] != seqs:
         raise ValueError(f"a block table of {tuple(shape)} for {seqs} sequences")
-    return ptr, count, count // seqs if seqs else 0
+    if seqs == 0:
+        return ptr, count, shape[1] if shape is not None and len(shape) == 2 else 0xFFFFFFFF
+    return ptr, count, count // seqs
 
 
 def _dimensions(x, dims, name):

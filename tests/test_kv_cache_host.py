@@ -435,3 +435,29 @@ def test_statistics_and_outputs_of_another_shape_are_refused(monkeypatch):
         for out, lse in ((fits, stats), (fits, None), (held, stats), flat):
             with pytest.raises(OverflowError):
                 call(out, lse)
+
+
+@pytest.mark.parametrize("table", [(0, 5), (0,)])
+def test_empty_batch(L, monkeypatch, table):
+    """A step of no sequences, with a max_length that its tables have pages for, and a
+    read of none: nothing to do, and no error."""
+    from fe2o3_amd import _lib, kernels
+
+    class Lib:
+        @staticmethod
+        def fe2o3_rt_get_device(out):
+            out._obj.value = 0
+            return 0
+
+        def __getattr__(self, name):
+            return getattr(L, name)  # returns before any HIP call
+
+    monkeypatch.setattr(_lib, "lib", lambda: Lib())
+    cache = kernels.KvCache(*(_Fake((4, 16, 2, 64), (2048, 128, 64, 1)) for _ in "kv"))
+    q, lse = _Fake((0, 4, 64), (256, 64, 1)), _Fake((0, 4), (4, 1), "torch.float32")
+    table = _Fake(table, (5, 1)[-len(table):], "torch.int32")
+    kernels.paged_attention_decode(cache, q, table, _Fake((0,), (1,), "torch.int32"), q, lse,
+                                   _Fake((1 << 20,), (1,), "torch.uint8"), max_length=80,
+                                   scale=0.125, sync=False)
+    rows = _Fake((3, 2, 64), (128, 64, 1))
+    kernels.kv_cache_read(cache, table, _Fake((1,), (1,), "torch.int32"), rows, rows, sync=False)
