@@ -991,7 +991,8 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   if (q_heads == 0u || q_heads % kv_heads != 0u) return FE2O3_ERR_SHAPE;
   if (max_length >= (1u << 31) || max_length > (uint64_t)table_cols * cache->page_size)
     return FE2O3_ERR_SHAPE;
-  if (!(scale > 0.0f) || !__builtin_isfinite(scale)) return FE2O3_ERR_SHAPE;
+  const float scale_log2 = scale * 1.4426950408889634f;
+  if (!(scale > 0.0f) || !__builtin_isfinite(scale_log2)) return FE2O3_ERR_SHAPE;
   const uint32_t group = q_heads / kv_heads;
   const uint32_t blocks_per_head = (group - 1u) / kBlockRows + 1u;
   const uint64_t row = (uint64_t)q_heads * d;
@@ -1042,7 +1043,7 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.table_cols = table_cols;
   a.max_length = max_length;
   a.window = window;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale_log2;
   hipStream_t s = (hipStream_t)stream;
   const bool e4m3 = cache->format == FE2O3_KV_E4M3;
   if (d == 64u)

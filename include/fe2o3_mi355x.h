@@ -423,8 +423,8 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_t
  * FE2O3_ERR_SHAPE; q_stride below q_heads * head_dim FE2O3_ERR_STRIDE; lengths
  * FE2O3_ERR_LENGTH (q_len covers the extent); NULL FE2O3_ERR_NULL; cache rows,
  * q rows, o or workspace off 16 bytes, the others off 4 FE2O3_ERR_ALIGNMENT;
- * a scale that is not positive and finite FE2O3_ERR_SHAPE; a short workspace
- * FE2O3_ERR_WORKSPACE. */
+ * a scale that is not positive, or not finite times log2 e, FE2O3_ERR_SHAPE; a
+ * short workspace FE2O3_ERR_WORKSPACE. */
 #define FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS 768u
 /* query rows of one workgroup's sums: of one KV head, or of four at once */
 #define FE2O3_PAGED_ATTENTION_PART_ROWS(q_heads, kv_heads)                                  \

@@ -461,3 +461,14 @@ def test_empty_batch(L, monkeypatch, table):
                                    scale=0.125, sync=False)
     rows = _Fake((3, 2, 64), (128, 64, 1))
     kernels.kv_cache_read(cache, table, _Fake((1,), (1,), "torch.int32"), rows, rows, sync=False)
+
+
+def test_decode_scale_within_its_range(L):
+    """Scores are taken in powers of two: a scale of which log2 e makes an infinity is
+    refused, the largest below it goes on to the check that this call fails."""
+    most = float(np.nextafter(np.finfo(np.float32).max / np.float32(1.4426950408889634),
+                              np.float32(0)))
+    assert _decode(L, _cache(), scale=3e38, workspace_bytes=0) == SHAPE
+    assert _decode(L, _cache(), scale=2.4e38, workspace_bytes=0) == SHAPE
+    assert _decode(L, _cache(), scale=most, workspace_bytes=0) == WORKSPACE
+    assert _decode(L, _cache(), scale=1e-45, workspace_bytes=0) == WORKSPACE
