@@ -485,18 +485,30 @@ struct Decode {
         }
         (void)probabilities();
       }
-      // two bf16 parts: the second MFMA takes what the first one's rounding (half
-      // a step, 2^-8) leaves, for 1% more time
+      // Two bf16 parts: the second MFMA takes what the first one leaves, to half a step
+      // of its own rounding, 2^-16 of the probability, for 1% more time.  The first part of a
+      // probability is the next bf16 below it, so that both are positive and an infinite
+      // V row's products do not cancel (rounded to nearest, the second may be 0 or
+      // negative).  Codes hold no infinity, and a V scale may have any sign.
       bf16x8_t pf[RW], pl[RW];
 #pragma unroll
       for (int rt = 0; rt < RW; ++rt) {
         l_run[rt] += psum[rt];
+        u32x4_t below;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = E4M3 ? p[rt][j] * vs[j] : p[rt][j];
-          pf[rt][j] = (__bf16)y;
-          pl[rt][j] = (__bf16)(y - (float)pf[rt][j]);
+          if constexpr (E4M3) {
+            const float y = p[rt][j] * vs[j];
+            pf[rt][j] = (__bf16)y;
+            pl[rt][j] = (__bf16)(y - (float)pf[rt][j]);
+          } else {  // +0 stays +0
+            const uint32_t part =
+                __builtin_elementwise_sub_sat(__float_as_uint(p[rt][j]), 1u) & 0xffff0000u;
+            below[j / 2] = j % 2 == 0 ? part >> 16 : below[j / 2] | part;
+            pl[rt][j] = (__bf16)(p[rt][j] - __uint_as_float(part));
+          }
         }
+        if constexpr (!E4M3) pf[rt] = __builtin_bit_cast(bf16x8_t, below);
       }
       // O^T += V^T P^T: lane i of group g receives d 16 db + i of keys 8 g .. + 7.
       // Two blocks of d at a time, so that no MFMA waits for the one before it.

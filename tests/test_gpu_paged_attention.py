@@ -386,6 +386,34 @@ def test_nonfinite_values_of_kept_keys(gpu, length):
     assert np.all(np.abs(clean - want[0]) <= want[2])
 
 
+@pytest.mark.parametrize("length", [1, 300, 3000])
+@pytest.mark.parametrize("q_heads,kv_heads", [(4, 2), (16, 4), (40, 2), (49, 1)])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_infinite_values_of_kept_keys(gpu, length, q_heads, kv_heads, head_dim):
+    """An infinite element of a kept V row is that element's result, whatever
+    rounding its key's probability has, the largest (1, exactly) among them; the
+    other elements are as they would be."""
+    b = Batch(gpu, "bf16", [length, length], q_heads, kv_heads, head_dim, 16)
+    want = b.reference()
+    flat = b.arrays[1].download()
+    rows = np.lib.stride_tricks.as_strided(flat, b.shape, [2 * s for s in b.strides] + [2])
+    first = (kv_heads - 1) * (q_heads // kv_heads)
+    p = b.k[1][:, -1] @ b.q[1, first] * b.scale
+    keys = [int(np.argmax(p)), length // 2, length - 1]
+    elements = [7, 20, 33]
+    for key, element in zip(keys, elements):
+        rows[b.table[1, key // 16], key % 16, -1, element] = 0xFF80 if element == 20 else 0x7F80
+    b.arrays[1].body.upload(flat)
+    o, stat = b.run()
+    x = bf16_to_f32(o.download()).reshape(2, q_heads, head_dim)
+    for element in elements:
+        assert np.all(x[1, first:, element] == (-np.inf if element == 20 else np.inf))
+    x[1, first:, elements] = want[0][1, first:, elements]
+    assert not np.any(np.isnan(x)) and np.all(np.abs(x - want[0]) <= want[2])
+    off = np.abs(stat.download().reshape(want[1].shape) - want[1])
+    assert np.all(off <= want[3])
+
+
 def test_shared_pages(gpu):
     """Two sequences with a common prefix on the same pages."""
     b = Batch(gpu, "e4m3", [640, 640], 8, 2, 128, 16)
