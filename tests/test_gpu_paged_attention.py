@@ -316,6 +316,100 @@ def test_peaked_and_flat_scores(gpu, fmt, peak):
     _check(gpu, fmt, [900, 64, 3000], 36, 1, 128, 16, peak=peak)
 
 
+def _split(y, parts):
+    """f32 values as the sum of one or two bf16 parts, by rounding to nearest."""
+    first = bf16_to_f32(_bf16_bits(y)).astype(np.float32)
+    if parts == 1:
+        return first.astype(np.float64)
+    return first.astype(np.float64) + bf16_to_f32(_bf16_bits(y - first)).astype(np.float64)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("q_heads,kv_heads", [(8, 2), (16, 4), (20, 1), (40, 1), (64, 1)])
+def test_probabilities_keep_sixteen_bits(gpu, fmt, head_dim, q_heads, kv_heads):
+    """Keys of two scores by turns whose weighted values cancel: with probabilities
+    (times the V scale) in one bf16 part the result would be off by some 2^-10 of the
+    mean magnitude A that it sums, which the one-part result below shows; two leave
+    2^-16.  The other errors: a score is one product here, exact, so its scalings,
+    exp2 and the products with scales move a probability by less than 2^-21; sums of
+    fp32 that cancel pair by pair, 2^-21 of A; the sum of the probabilities moves o
+    in proportion alone, by 2^-16 of it at most, and the output's rounding by 2^-8."""
+    lengths = [96, 2500, 640]
+    b = Batch(gpu, fmt, lengths, q_heads, kv_heads, head_dim, 16)
+    q = np.zeros_like(b.q)
+    q[..., 0] = 1.0
+    b.q = q
+    b.dev_q = Guarded(gpu, _bf16_bits(q))
+    rng = np.random.default_rng(head_dim)
+    sign = np.where(np.arange(head_dim) % 2, -1.0, 1.0)
+
+    def error(y):  # of one part
+        return _split(y, 1) - y
+    if fmt == "bf16":
+        # the score of the second kind: the probability that one part rounds most
+        c = -bf16_to_f32(np.arange(0x3F80, 0x40A0, dtype=np.uint16)).astype(np.float64)
+        p = np.exp(c * b.scale).astype(np.float32)
+        at = np.argmax(np.abs(error(p)) / p)
+        score, weight = c[at], [1.0, float(p[at])]
+        v = bf16_to_f32(_bf16_bits(rng.uniform(0.5, 1.0, head_dim))).astype(np.float64) * sign
+        w = -bf16_to_f32(_bf16_bits(v / weight[1])).astype(np.float64)
+        k_rows = [0, int(_bf16_bits(np.float32(score)))]
+        v_rows, v_scales = [_bf16_bits(v), _bf16_bits(w)], None
+        values = [v, w]
+    else:
+        # codes 1 and -1.5, with V scales that make them cancel: t, and t / 1.5 over p
+        t = np.linspace(1.0, 2.0, 4097, dtype=np.float32)[:-1]
+        t = t[np.argmax(np.abs(error(t) - 1.5 * error(t / np.float32(1.5))))]
+        k_scale = np.float32(3.0)
+        score = -3.0
+        p = np.float32(np.exp(score * b.scale))
+        v_scales = [np.float32(t), np.float32(np.float64(t) / 1.5 / np.float64(p))]
+        weight = [float(t), float(np.float32(p * v_scales[1]))]
+        k_rows = [0, 0xB8]
+        v_rows = [np.where(sign > 0, 0x38, 0xB8), np.where(sign > 0, 0xBC, 0x3C)]
+        values = [sign, -1.5 * sign]
+    size = 2 if fmt == "bf16" else 1
+    flats = [a.download() for a in b.arrays]
+    rows = [np.lib.stride_tricks.as_strided(x, b.shape, [size * s for s in b.strides] + [size])
+            for x in flats]
+    if fmt == "e4m3":
+        scale_flats = [a.download() for a in b.scales]
+        scales = [x.reshape(b.shape[0], kv_heads, 16) for x in scale_flats]
+    for s, count in enumerate(lengths):
+        for kind in range(2):
+            key = np.arange(kind, count, 2)
+            page, place = b.table[s, key // 16], key % 16
+            rows[0][page, place] = 0
+            rows[0][page, place, :, 0] = k_rows[kind]
+            rows[1][page, place] = v_rows[kind]
+            if fmt == "e4m3":
+                scales[0][page, :, place] = k_scale
+                scales[1][page, :, place] = v_scales[kind]
+    for a, x in zip(b.arrays, flats):
+        a.body.upload(x)
+    if fmt == "e4m3":
+        for a, x in zip(b.scales, scale_flats):
+            a.body.upload(x)
+    # every sequence has as many of each kind: o of one pair
+    total = 1.0 + float(np.exp(np.float64(score) * b.scale))
+    exact_weight = ([1.0, total - 1.0] if fmt == "bf16" else
+                    [float(v_scales[0]), (total - 1.0) * float(v_scales[1])])
+    want = sum(w * v for w, v in zip(exact_weight, values)) / total
+    mean = sum(w * np.abs(v) for w, v in zip(exact_weight, values)) / total
+    tol = mean * (2.0 ** -16 + 2.0 ** -20) + np.abs(want) * (2.0 ** -8 * (1 + 2.0 ** -6))
+
+    def emulated(parts):
+        x = sum(_split(np.float32(w), parts) * v for w, v in zip(weight, values)) / total
+        return bf16_to_f32(_bf16_bits(x.astype(np.float32))).astype(np.float64)
+    assert np.all(np.abs(emulated(2) - want) <= tol)
+    assert np.all(np.abs(emulated(1) - want) > 4 * tol)
+    o, _ = b.run()
+    x = bf16_to_f32(o.download()).reshape(len(lengths), q_heads, head_dim).astype(np.float64)
+    off = np.abs(x - want)
+    assert np.all(off <= tol), (off / tol).max()
+
+
 def test_rising_scores(gpu):
     """Keys in rising order of score raise the reference in every tile."""
     b = Batch(gpu, "bf16", [2000], 4, 1, 128, 16)
