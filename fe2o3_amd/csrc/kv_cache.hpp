@@ -15,7 +15,8 @@
 
 namespace kv_cache {
 
-// n / d and n % d of n < 2^31 by a multiplication and a shift: with 2^l the
+// n / d and n % d of n < 2^31 by a multiplication and a shift (Granlund and
+// Montgomery's division by an invariant integer): with 2^l the
 // least power of two >= d and m = ceil(2^(31+l) / d), n m / 2^(31+l) exceeds
 // n / d by n e / (d 2^(31+l)) with e < d <= 2^l, which is less than 1 / d for
 // n < 2^31, so the floors agree.  m fits 32 bits, since d > 2^(l-1) (for d = 1

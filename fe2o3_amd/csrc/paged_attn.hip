@@ -17,12 +17,12 @@
 //     the MFMAs' layouts; e4m3 codes are widened to bf16, exactly, on the way out.
 //   * S^T = K Q^T with v_mfma_f32_16x16x32_bf16: row m of key block b is key
 //     8 (m / 4) + 4 b + m % 4, so that lane l holds query row l % 16 and the
-//     eight keys 8 (l / 16) .. + 7, and the probabilities are the second
-//     operand of O^T += V^T P^T as they stand; V^T comes by transposing LDS
+//     eight keys 8 (l / 16) .. + 7, and the probabilities, in two bf16 parts, are the
+//     second operand of O^T += V^T P^T where they stand; V^T comes by transposing LDS
 //     reads.  The softmax is the prompt kernel's: exponentials against a
 //     running reference that is raised only when a tile exceeds it by 2^8.
 //   * An e4m3 cache's K scales multiply the scores, its V scales the
-//     probabilities before these are rounded for the MFMA.
+//     probabilities before these are split for the MFMA.
 // With a multiple of four KV heads (and group <= 16) a workgroup's four waves
 // have a head each in large calls: they read neighbouring rows, and nothing is added
 // in LDS.
@@ -164,8 +164,9 @@ struct Tile {
 // and exponentials over three or four tiles of rows is longer than the loads of the
 // next keys, so they have a wave each (a KV head's 64 rows, 48 sequences of 24000 keys:
 // 118 us in one wave, 96 shared; 48 sequences of 100 to 6000 with 48 rows: 25 us, 21).
-// Two keep up, and a wave of their own reads LDS and widens codes once for both (32
-// rows, e4m3: 55 us, shared 73).
+// Two keep up, and a wave of their own reads LDS and widens codes once for both (48
+// sequences of 24000 keys, e4m3: 32 rows 61 us, shared 107; 20 rows 59, 103; bf16: 32 rows
+// 101 either way, 20 rows 98, 100).
 constexpr int row_tiles(int rt) { return rt == 2 ? 2 : 1; }
 constexpr uint32_t sharers(int rt) { return (uint32_t)(rt / row_tiles(rt)); }
 constexpr uint32_t waves(int rt) { return kWaves * sharers(rt); }
@@ -545,7 +546,8 @@ struct Decode {
     // A wave's LDS operations run in order, so a tile's reads see its writes and
     // the next tile's writes wait for them; the fences keep the compiler from
     // reordering them (it sees one lane's addresses).  One tile is in flight while
-    // another is computed: two were no faster (8 x 32 heads x 4096: 87, 97 us).
+    // another is computed: two were no faster where a CU's waves have 128 KiB in flight
+    // so (8 x 32 heads x 4096: 87, 97 us).
     // A tile that waves share goes to the other place than the one before it, which
     // a wave that is behind may still read; the barrier leaves none two behind.
     if constexpr (S == 1) {
@@ -881,9 +883,11 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   const int32_t rc = fe2o3_host::after_launch();
   if (rc != FE2O3_OK) return rc;
   // Many heads have few parts each, and rows share the threads; few have many,
-  // which a row's threads share (one head's 256 parts: 7.1 us on 256 threads, 6 on
-  // 1024; 8 parts of 64 heads of 16 rows: 4.6 either way, of 33 heads of 64 rows 5.6
-  // and, rows sharing, 4.3).
+  // which a row's threads share.  us of the join with 512 workgroups; rows share from
+  // 64 heads on, 1024 threads take a row below 8 (rows sharing, 256, 1024 threads a row):
+  //   2 heads, 16 rows 28, 6.0, 5.8     2 x 64 rows 31, 7.2, 6.2    6 x 16 12, 4.6, 4.6
+  //   8 x 16            9.0, 4.6, 4.5   16 x 64      7.0, 5.7, 8.6  32 x 64 4.9, 5.4, 13
+  //   60 x 64           5.2, 7.7, 21    128 x 16     4.5, 6.2, 17   256 x 16 4.5, 9.8, 31
   constexpr int kRows = kThreads / (D / 4);
   const uint32_t rows = WH * a.rows;
   const bool by_runs = heads > workgroups;
@@ -922,6 +926,10 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   //   1 x 1000 9.7, 14.8    4 x 1000  12.1, 15.7    16 x 1000 20.8, 17.7
   //   64 x 1..2000 48.1, 55.2   30 x 1..2000 27.4, 30.1   40 windows of 1024
   //   (64 wide, e4m3) 16.8, 13.0
+  // Past 40 tiles one a head would be up to 7% faster for equal lengths, but up to 20%
+  // slower where they differ, which max_length does not tell:
+  //   64 x 1300 59.4, 55.8    64 x 1600 72.0, 67.0    16 x 1300 22.4, 22.6
+  //   64 x 1..1300 34.9, 37.0   64 x 1..2000 47.8, 55.0   64 x 1..3000 68.5, 81.3
   // Few heads take eight waves each.  More than one tile of query rows has more to
   // join, and a head its own rounds at least (48 rows, one KV head):
   //   48 x 170 14.0, 9.5    48 x 1000 16.4, 21.9    8 x 500   13.6, 13.1

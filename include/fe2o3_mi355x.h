@@ -333,8 +333,8 @@ int32_t fe2o3_flash_attention_fwd(const uint16_t *q, uint64_t q_len,
  * codes and for each row a scale, in k_scale and v_scale [pages, kv_heads,
  * page_size]: scale = max(max |x|, 2^-126) / 448, code = e4m3_rne(x / scale)
  * (fe2o3_fp8_scale_from_amax and fe2o3_quantize_e4m3 on each row).  A NaN takes
- * no part in the maximum and stays a NaN; a row with an infinity has an
- * infinite scale and reads back as NaN.
+ * no part in the maximum and stays a NaN, of either sign; a row with an infinity
+ * has an infinite scale and reads back as NaN.
  *
  * The record is checked in this order: NULL record FE2O3_ERR_NULL; another
  * format, a size of 0, or slots or head_dim of 2^31 or more FE2O3_ERR_SHAPE;
@@ -409,7 +409,9 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_t
  * +0, lse = -inf.  A length above max_length counts as max_length (at most
  * table_cols * page_size, and below 2^31); a key on a page out of range is
  * left out.
- * What cached rows no sequence reaches hold (NaN included) has no effect.
+ * What cached rows no sequence reaches hold (NaN included) has no effect.  A
+ * row's sums are relative to a score that a later one may exceed by 2^8 in weight:
+ * values stay finite where |V| times the number of keys is below 2^119.
  *
  * The keys of all sequences are dealt evenly to the workgroups, so the bits of
  * a sequence's result depend on the batch; the same call gives the same bits.
