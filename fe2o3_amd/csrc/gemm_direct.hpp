@@ -31,6 +31,7 @@
 #include "common.hpp"
 #include "gemm_pipe.hpp"
 #include "internal.hpp"
+#include "mxfp4.hpp"
 
 namespace gemm_direct {
 
@@ -52,7 +53,7 @@ typedef u32x8_t Frag;
 
 struct Bf16 {
   static constexpr uint32_t kBytes = 2;  // per element
-  static constexpr bool kScaled = false;
+  static constexpr bool kScaled = false, kBlocks = false;
   static constexpr int kDeep = 3;  // units in flight of the widest forms
   static FE2O3_DEVICE uint32_t tile_piece(uint32_t g, uint32_t h) { return 4u * h + g; }
   static FE2O3_DEVICE void mma(const Frag& b, const Frag& a, f32x4_t& acc) {
@@ -69,13 +70,38 @@ struct Bf16 {
 // OCP e4m3: the unscaled 16x16x128 MFMA, as in gemm_pipe::Fp8Mma16
 struct Fp8 {
   static constexpr uint32_t kBytes = 1;
-  static constexpr bool kScaled = true;
+  static constexpr bool kScaled = true, kBlocks = false;
   static constexpr int kDeep = 2;
   static FE2O3_DEVICE uint32_t tile_piece(uint32_t g, uint32_t h) { return 2u * g + h; }
   static FE2O3_DEVICE void mma(const Frag& b, const Frag& a, f32x4_t& acc) {
     acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
         __builtin_bit_cast(i32x8_t, b), __builtin_bit_cast(i32x8_t, a), acc, 0, 0, 0, 0, 0, 0);
   }
+};
+
+// Microscaled e2m1 (mxfp4.hpp): a unit is a panel of 256 k, whose halves are an MFMA
+// each.  sb, sa: the lane's scale bytes of both halves.
+struct Mxfp4 {
+  static constexpr uint32_t kBytes = 1;  // k counts bytes of codes, whole panels
+  static constexpr bool kScaled = false, kBlocks = true;
+  static constexpr int kDeep = 2;
+  static FE2O3_DEVICE uint32_t tile_piece(uint32_t g, uint32_t h) { return 4u * h + g; }
+  static FE2O3_DEVICE i32x8_t half(const Frag& f, int h) {  // the upper four are not read
+    return h == 0 ? __builtin_bit_cast(i32x8_t, __builtin_shufflevector(f, f, 0, 1, 2, 3, -1, -1, -1, -1))
+                  : __builtin_bit_cast(i32x8_t, __builtin_shufflevector(f, f, 4, 5, 6, 7, -1, -1, -1, -1));
+  }
+  static FE2O3_DEVICE void mma(const Frag& b, const Frag& a, uint32_t sb, uint32_t sa,
+                               f32x4_t& acc) {
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(half(b, 0), half(a, 0), acc, 4, 4, 0,
+                                                           (int)sb, 0, (int)sa);
+    acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(half(b, 1), half(a, 1), acc, 4, 4, 1,
+                                                           (int)sb, 1, (int)sa);
+  }
+};
+// The scales of both operands: 8 bytes a row of a unit, a_rows (b_rows) rows a unit.
+struct BlockScales {
+  const uint8_t *a, *b;
+  uint64_t a_rows, b_rows;
 };
 
 FE2O3_DEVICE u32x4_t load16(const uint8_t* p) {
@@ -93,6 +119,11 @@ struct ScalarBase {
     typedef __attribute__((address_space(1))) const uint8_t* Global;
     typedef __attribute__((address_space(1))) const u32x4_any_t* Global16;
     return *(Global16)((Global)p + off);
+  }
+  FE2O3_DEVICE u32x2_t load8(uint32_t off) const {  // aligned
+    typedef __attribute__((address_space(1))) const uint8_t* Global;
+    typedef __attribute__((address_space(1))) const u32x2_t* Global8;
+    return *(Global8)((Global)p + off);
   }
 };
 
@@ -162,7 +193,7 @@ FE2O3_DEVICE void block_of(uint32_t id, uint32_t tiles_m, uint32_t tiles_n, uint
 template <class T, int MB, int NB, int D, class Off = uint32_t, bool IN_ORDER = false>
 FE2O3_DEVICE void block(const uint8_t* __restrict__ a, const uint8_t* __restrict__ b,
                         uint16_t* __restrict__ c, uint32_t m, uint32_t n, uint32_t k, float scale,
-                        uint32_t xcds, uint8_t* smem) {
+                        uint32_t xcds, uint8_t* smem, const BlockScales& scales = {}) {
   const uint32_t lane = threadIdx.x & 63u, lr = lane & 15u, g = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t tiles_m = (m - 1u) / (16u * MB) + 1u, tiles_n = (n - 1u) / (16u * NB) + 1u;
@@ -200,6 +231,17 @@ FE2O3_DEVICE void block(const uint8_t* __restrict__ a, const uint8_t* __restrict
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   u32x4_t af[D][2 * MB], bf[D][2 * NB];
+  // T::kBlocks: the scales of row l % 16 of each block, and the byte pair of group l / 16;
+  // rows past the end repeat the last
+  u32x2_t as[D][MB], bs[D][NB];
+  uint32_t aso[MB], bso[NB];
+  const uint32_t pick = 0x0c0c0400u + g * 0x0101u;
+  if constexpr (T::kBlocks) {
+#pragma unroll
+    for (int i = 0; i < MB; ++i) aso[i] = min(16u * i + lr, m - 1u - row0) * 8u;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) bso[j] = min(16u * j + lr, n - 1u - col0) * 8u;
+  }
   constexpr uint32_t kStride = IN_ORDER ? 1u : kWaves;  // units between the wave's own
   const uint32_t first_unit = IN_ORDER ? 0u : wave;
   // the wave's unit u into set s
@@ -211,6 +253,15 @@ FE2O3_DEVICE void block(const uint8_t* __restrict__ a, const uint8_t* __restrict
     for (int j = 0; j < 2 * NB; ++j) bf[s][j] = pb.load16(bo[j]);
 #pragma unroll
     for (int i = 0; i < 2 * MB; ++i) af[s][i] = pa.load16(ao[i]);
+    if constexpr (T::kBlocks) {
+      const uint64_t unit = (uint64_t)u * kStride + first_unit;
+      const ScalarBase sa(scales.a + (unit * scales.a_rows + row0) * 8u);
+      const ScalarBase sb(scales.b + (unit * scales.b_rows + col0) * 8u);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) bs[s][j] = sb.load8(bso[j]);
+#pragma unroll
+      for (int i = 0; i < MB; ++i) as[s][i] = sa.load8(aso[i]);
+    }
   };
   auto put = [&](uint32_t blk, u32x4_t lo, u32x4_t hi) {
     *reinterpret_cast<u32x4_t*>(own + blk * 2048u + wr0) = lo;
@@ -238,7 +289,13 @@ FE2O3_DEVICE void block(const uint8_t* __restrict__ a, const uint8_t* __restrict
     for (int i = 0; i < MB; ++i) {
       const Frag fa = get(i);
 #pragma unroll
-      for (int j = 0; j < NB; ++j) T::mma(fb[j], fa, acc[i][j]);
+      for (int j = 0; j < NB; ++j) {
+        if constexpr (T::kBlocks)
+          T::mma(fb[j], fa, __builtin_amdgcn_perm(bs[s][j][1], bs[s][j][0], pick),
+                 __builtin_amdgcn_perm(as[s][i][1], as[s][i][0], pick), acc[i][j]);
+        else
+          T::mma(fb[j], fa, acc[i][j]);
+      }
     }
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
@@ -277,7 +334,7 @@ FE2O3_DEVICE void block(const uint8_t* __restrict__ a, const uint8_t* __restrict
     for (int s = 0; s < D; ++s)
       if ((uint32_t)s < mine) mma(s);
   }
-  if (kbytes % kUnit != 0u && units % kStride == first_unit) {  // the partial last unit
+  if (!T::kBlocks && kbytes % kUnit != 0u && units % kStride == first_unit) {  // the partial last unit
     const Off at = (Off)units * kUnit + 16u * pc;
     if (kbytes >= 16u) {
       // a piece that the row's end cuts (or that lies past it) is read 16
@@ -513,8 +570,10 @@ FE2O3_DEVICE void fill(uint16_t* __restrict__ c, uint64_t n) {
 // past it).
 template <class T, bool WIDE>
 FE2O3_DEVICE void run_form(int form, const uint8_t* a, const uint8_t* b, uint16_t* c, uint32_t m,
-                           uint32_t n, uint32_t k, float scale, uint32_t xcds, uint8_t* smem) {
-#define FE2O3_DIRECT(MB, NB, D) return block<T, MB, NB, D>(a, b, c, m, n, k, scale, xcds, smem)
+                           uint32_t n, uint32_t k, float scale, uint32_t xcds, uint8_t* smem,
+                           const BlockScales& scales = {}) {
+#define FE2O3_DIRECT(MB, NB, D) \
+  return block<T, MB, NB, D>(a, b, c, m, n, k, scale, xcds, smem, scales)
   if constexpr (!WIDE) {
     switch (form) {
       case 0: FE2O3_DIRECT(1, 1, 4);
@@ -528,10 +587,15 @@ FE2O3_DEVICE void run_form(int form, const uint8_t* a, const uint8_t* b, uint16_
       case 5: FE2O3_DIRECT(4, 1, 3);
       case 6: FE2O3_DIRECT(2, 4, T::kDeep);
       case 7: FE2O3_DIRECT(4, 2, T::kDeep);
-      case kInOrder:
-        return block<T, 2, 2, 2, uint32_t, true>(a, b, c, m, n, k, scale, xcds, smem);
+      case kInOrder:  // this and the last for operands at any alignment, of any K
+        if constexpr (!T::kBlocks)
+          block<T, 2, 2, 2, uint32_t, true>(a, b, c, m, n, k, scale, xcds, smem);
+        return;
       case kFill: return fill(c, (uint64_t)m * n);
-      default: return block<T, 1, 4, 1, uint64_t>(a, b, c, m, n, k, scale, xcds, smem);
+      default:
+        if constexpr (!T::kBlocks)
+          block<T, 1, 4, 1, uint64_t>(a, b, c, m, n, k, scale, xcds, smem);
+        return;
     }
   }
 #undef FE2O3_DIRECT

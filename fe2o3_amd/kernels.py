@@ -461,11 +461,16 @@ def _device_of(k):
 
 def _on_current_device(cache):
     """The cache's device, which has to be the current one: launches go there."""
+    current = _current_device()
+    if current != cache.device:
+        raise ValueError(f"cache on device {cache.device}, the current one is {current}")
+    return cache.device
+
+
+def _current_device():
     current = C.c_int32()
     check(_lib.lib().fe2o3_rt_get_device(C.byref(current)), "get device")
-    if current.value != cache.device:
-        raise ValueError(f"cache on device {cache.device}, the current one is {current.value}")
-    return cache.device
+    return current.value
 
 
 def _rows(cache, k, v, strides, device):
@@ -557,6 +562,100 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
           *_operand(out, _BF16, "out", device), lse_ptr, lse_len,
           *_operand(workspace, _BYTES, "workspace", device), seqs, q_heads, cols, max_length,
           q_stride, window, scale, stream=stream, sync=sync)
+
+
+# ---- microscaled 4-bit matrices ----------------------------------------------------------
+#
+# Arrays are DeviceBuffers or device tensors, on the current device; streams as for the
+# paged cache.
+
+MXFP4_BLOCK, MXFP4_PANEL = 32, 256
+
+
+def mxfp4_shapes(rows: int, cols: int) -> tuple[tuple, tuple]:
+    """Shapes of a packed matrix's codes and scales, both bytes."""
+    panels = -(-cols // MXFP4_PANEL)
+    return (rows, panels * 128), (panels, -(-rows // 16) * 16, 8)
+
+
+def _packed(codes, scales, names, device):
+    """(pointer, bytes) of codes and of scales, and their shapes where they are tensors."""
+    shapes = _dimensions(codes, 2, names[0]), _dimensions(scales, 3, names[1])
+    return (_operand(codes, _BYTES, names[0], device)
+            + _operand(scales, _BYTES, names[1], device)), shapes
+
+
+def _dense(x, name, device, rows, cols, stride):
+    """(pointer, elements, dtype code, rows, columns, row stride) of a matrix of f32 or
+    bf16: a tensor's own, a DeviceBuffer's as given."""
+    kind = _FLOAT if _FLOAT in _kinds[x.dtype] else _BF16
+    shape = _dimensions(x, 2, name)
+    if shape is not None:
+        if (rows, cols, stride) != (None, None, None):
+            raise ValueError(f"{name} has its own rows, cols and stride")
+        rows, cols = shape
+        stride = x.stride()[0]
+    elif rows is None or cols is None:
+        raise ValueError(f"{name} in a DeviceBuffer needs rows and cols")
+    elif stride is None:
+        stride = cols
+    return _operand(x, kind, name, device, False) + (kind == _BF16, rows, cols, stride)
+
+
+def quantize_mxfp4(x, codes, scales, *, rows=None, cols=None, stride=None, stream=None,
+                   sync=True) -> None:
+    """Packs x, f32 or bf16 [rows, cols] with the last dimension contiguous, into codes and
+    scales of mxfp4_shapes(rows, cols) (fe2o3_quantize_mxfp4).  A DeviceBuffer x takes
+    rows, cols and the elements between rows."""
+    device = _current_device()
+    ptr, count, dtype, rows, cols, stride = _dense(x, "x", device, rows, cols, stride)
+    packed = _checked_packed(codes, scales, rows, cols, device)
+    _call("fe2o3_quantize_mxfp4", ptr, count, dtype, *packed, rows, cols, stride, stream=stream,
+          sync=sync)
+
+
+def dequantize_mxfp4(codes, scales, x, *, rows=None, cols=None, stride=None, stream=None,
+                     sync=True) -> None:
+    """The packed matrix's values into x, f32 or bf16 [rows, cols]
+    (fe2o3_dequantize_mxfp4)."""
+    device = _current_device()
+    ptr, count, dtype, rows, cols, stride = _dense(x, "x", device, rows, cols, stride)
+    packed = _checked_packed(codes, scales, rows, cols, device)
+    _call("fe2o3_dequantize_mxfp4", *packed, ptr, count, dtype, rows, cols, stride,
+          stream=stream, sync=sync)
+
+
+def _checked_packed(codes, scales, rows, cols, device):
+    arrays, shapes = _packed(codes, scales, ("codes", "scales"), device)
+    for name, found, want in zip(("codes", "scales"), shapes, mxfp4_shapes(rows, cols)):
+        if found is not None and found != want:
+            raise ValueError(f"{name} of {tuple(found)} for a matrix of {(rows, cols)}, not {want}")
+    return arrays
+
+
+def gemm_mxfp4_nt(a, a_scales, b, b_scales, c, m=None, n=None, k=None, *, stream=None,
+                  sync=True) -> None:
+    """c (bf16 [m, n]) = A B^T of packed A [m, k] and B [n, k] (fe2o3_gemm_mxfp4_nt).  Sizes
+    come from tensors (k in whole panels); DeviceBuffers take m, n, k."""
+    device = _current_device()
+    left, (ca, sa) = _packed(a, a_scales, ("a", "a_scales"), device)
+    right, (cb, sb) = _packed(b, b_scales, ("b", "b_scales"), device)
+    shape = _dimensions(c, 2, "c")
+    if ca is not None:
+        found = (ca[0], cb[0] if cb is not None else n, 2 * ca[1])
+        given = (m, n, k if k is None else -(-k // MXFP4_PANEL) * MXFP4_PANEL)
+        if any(g is not None and g != f for g, f in zip(given, found)):
+            raise ValueError(f"m, n, k of {(m, n, k)} for operands of {found}")
+        m, n, k = found
+    if m is None or n is None or k is None:
+        raise ValueError("operands in DeviceBuffers need m, n and k")
+    for name, found, want in (("a", ca, mxfp4_shapes(m, k)[0]), ("b", cb, mxfp4_shapes(n, k)[0]),
+                              ("a_scales", sa, mxfp4_shapes(m, k)[1]),
+                              ("b_scales", sb, mxfp4_shapes(n, k)[1]), ("c", shape, (m, n))):
+        if found is not None and found != want:
+            raise ValueError(f"{name} of {tuple(found)}, not {want}")
+    _call("fe2o3_gemm_mxfp4_nt", *left, *right, *_operand(c, _BF16, "c", device), m, n, k,
+          stream=stream, sync=sync)
 
 
 def kernel_resources(entry: str) -> list[dict]:

@@ -628,6 +628,55 @@ int32_t fe2o3_gemm_fp8_nt(const uint8_t *a, uint64_t a_len, const uint8_t *b,
                           const float *scale_b, uint16_t *c, uint64_t c_len,
                           uint32_t m, uint32_t n, uint32_t k, void *stream);
 
+/* ---- microscaled 4-bit matrices (OCP Microscaling Formats 1.0, MXFP4) ---------------------
+ * Not in the reference, which has no 4-bit type.  Blocks of 32 columns of a row hold e2m1
+ * codes (0, 0.5, 1, 1.5, 2, 3, 4, 6, and a sign) on one scale byte e = 2^(e - 127), 255 a
+ * NaN.  A packed matrix of [rows, cols] is cut into panels of 256 columns, the last one
+ * filled up with zeros:
+ *   codes  [rows][panels * 128]            two to a byte, the even column in the low half
+ *   scales [panels][rows rounded up to 16][8]   a row's eight blocks of the panel
+ * FE2O3_MXFP4_PANELS, FE2O3_MXFP4_CODE_BYTES and FE2O3_MXFP4_SCALE_BYTES are these sizes.
+ * Scales in rows, [rows, cols / 32], become panels by a copy: [rows, panels, 8] with the
+ * first two dimensions changed over.  Scale bytes of rows past the last are neither
+ * written nor of effect; those of blocks past the last column multiply zeros, and must
+ * not be 255. */
+#define FE2O3_MXFP4_PANELS(cols) (((uint64_t)(cols) + 255u) / 256u)
+#define FE2O3_MXFP4_CODE_BYTES(rows, cols) \
+  ((uint64_t)(rows) * FE2O3_MXFP4_PANELS(cols) * 128u)
+#define FE2O3_MXFP4_SCALE_BYTES(rows, cols) \
+  (((uint64_t)(rows) + 15u) / 16u * 16u * FE2O3_MXFP4_PANELS(cols) * 8u)
+
+/* Packs x (dtype 0 = f32, 1 = bf16 bits), rows row_stride elements apart.  A block's scale
+ * is 2^(floor(log2 max |x|) - 2), at least 2^-127; each code is x / scale rounded to the
+ * nearest, ties to even, at most 6 (the largest values of a block may be a quarter off:
+ * the format's own rule), with x's sign, a zero's too.  A block with a NaN or an infinity
+ * has the scale 255.  x_len covers the rows' extent, q_len and scales_len are the sizes
+ * above.  Errors in this order: another dtype, more than 65535 panels, or 2^31 groups of
+ * 8 rows and a panel FE2O3_ERR_SHAPE; row_stride < cols (of more than one row)
+ * FE2O3_ERR_STRIDE; FE2O3_ERR_OVERFLOW; FE2O3_ERR_LENGTH; FE2O3_ERR_NULL; x off its
+ * elements' alignment, q or scales off 16 bytes FE2O3_ERR_ALIGNMENT. */
+int32_t fe2o3_quantize_mxfp4(const void *x, uint64_t x_len, uint32_t dtype, uint8_t *q,
+                             uint64_t q_len, uint8_t *scales, uint64_t scales_len,
+                             uint32_t rows, uint32_t cols, uint64_t row_stride, void *stream);
+
+/* x = code * scale of a packed matrix, exact in both types but for the largest scales
+ * (2 and more times 2^127, and 4 and 6 times 2^126, are infinities); elements between
+ * the rows of x keep their bytes.  Errors as for the packing. */
+int32_t fe2o3_dequantize_mxfp4(const uint8_t *q, uint64_t q_len, const uint8_t *scales,
+                               uint64_t scales_len, void *x, uint64_t x_len, uint32_t dtype,
+                               uint32_t rows, uint32_t cols, uint64_t row_stride, void *stream);
+
+/* C[m, n] bf16 = A B^T of packed A [m, k] and B [n, k], fp32 accumulation, each product
+ * code * scale * code * scale exact; a NaN scale makes NaN of its row's (column's)
+ * outputs.  Any m, n, k; k = 0 writes +0.  Few output tiles split k over a workgroup's
+ * waves, as in fe2o3_gemm_bf16_nt.  Errors: more than 65535 panels, or a grid of 2^31
+ * workgroups FE2O3_ERR_SHAPE; lengths other than the sizes above FE2O3_ERR_LENGTH;
+ * FE2O3_ERR_NULL; codes or scales off 16 bytes FE2O3_ERR_ALIGNMENT. */
+int32_t fe2o3_gemm_mxfp4_nt(const uint8_t *a, uint64_t a_len, const uint8_t *a_scales,
+                            uint64_t a_scales_len, const uint8_t *b, uint64_t b_len,
+                            const uint8_t *b_scales, uint64_t b_scales_len, uint16_t *c,
+                            uint64_t c_len, uint32_t m, uint32_t n, uint32_t k, void *stream);
+
 /* crates/fe2o3-host/src/moe_routing_expert_bridge_v1.rs:220-389
  * (check_host_observed_moe_routing_output_v1) with the compact pack plan of
  * crates/fe2o3-host/src/generated_moe_expert_v1.rs:159-190, on the device
