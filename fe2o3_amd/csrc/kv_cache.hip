@@ -1,6 +1,6 @@
 // kv_cache.hip -- a paged key-value cache on gfx950: new rows written into
-// their slots, copied or quantised to e4m3 with a scale per token and head,
-// and cached rows of several sequences read back as packed bf16.
+// their slots, copied, quantised to e4m3 with a scale per token and head, or to
+// microscaled 4-bit blocks of 32 (mxfp4.hpp), and cached rows of several sequences read back as packed bf16.
 //
 // Both are one pass over the rows, bound by memory: 32768 tokens of 8 heads, 128
 // wide, bf16 51 us = 5.2 TB/s, e4m3 41 us = 5.0; 16 sequences of 1 to 4097 read
@@ -14,6 +14,7 @@
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
+#include "mxfp4.hpp"
 
 namespace {
 
@@ -22,11 +23,15 @@ using kv_cache::FastDiv;
 using kv_cache::RowScale;
 using kv_cache::View;
 
+// a cache's format, FE2O3_KV_*
+constexpr uint32_t kBf16 = FE2O3_KV_BF16, kE4m3 = FE2O3_KV_E4M3, kMxfp4 = FE2O3_KV_MXFP4;
+
 constexpr int kThreads = 256;
 constexpr uint32_t kMaxGrid = 1u << 20;  // workgroups
 
 typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t u32x2_any_t __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t u32_any_t __attribute__((aligned(1)));
 
 // 8 bf16 values, the first `n` of them in memory (the others +0)
 FE2O3_DEVICE u32x4_t load_bf16x8(const uint16_t* p, uint32_t n) {
@@ -126,7 +131,7 @@ struct WriteArgs {
 
 // Rows of a group one after another, a whole grid's groups apart: a grid holds
 // at most kMaxGrid workgroups, and only the largest calls take a second turn.
-template <bool E4M3>
+template <uint32_t F>
 __global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
   const uint32_t lanes = 1u << a.lanes_log2, c0 = threadIdx.x & (lanes - 1u);
   const uint32_t chunks = (a.cache.head_dim + 7u) / 8u;
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
     const uint32_t page = a.cache.page.div(slot), place = slot - page * a.cache.page.divisor;
     const uint64_t to = page * a.cache.page_stride + place * a.cache.token_stride +
                         head * a.cache.head_stride;
-    if constexpr (!E4M3) {
+    if constexpr (F == kBf16) {
       uint16_t *ko = (uint16_t*)a.cache.k + to, *vo = (uint16_t*)a.cache.v + to;
       for (uint32_t c = c0; c < chunks; c += lanes) {
         const uint32_t n = chunk_left(a.cache.head_dim, c);
@@ -158,6 +163,26 @@ __global__ void __launch_bounds__(kThreads) kv_write_kernel(WriteArgs a) {
         }
         store_bf16x8(ko + 8u * c, kx, n);
         store_bf16x8(vo + 8u * c, vx, n);
+      }
+    } else if constexpr (F == kMxfp4) {
+      // four lanes a block; a head_dim of whole blocks has whole chunks
+      const uint64_t at = ((((uint64_t)page * a.cache.kv_heads + head) * a.cache.page.divisor) +
+                           place) * (chunks / 4u);
+      for (uint32_t c = c0; c < chunks; c += lanes) {
+        if (c != c0) {
+          kx = load_bf16x8(k + 8u * c, 8u);
+          vx = load_bf16x8(v + 8u * c, 8u);
+        }
+        const uint32_t ks = mxfp4::scale_byte(mxfp4::quad_max(mxfp4::top8(kx)));
+        const uint32_t vs = mxfp4::scale_byte(mxfp4::quad_max(mxfp4::top8(vx)));
+        *reinterpret_cast<u32_any_t*>(a.cache.k + to + 4u * c) =
+            mxfp4::encode8(kx, mxfp4::scale_float(ks));
+        *reinterpret_cast<u32_any_t*>(a.cache.v + to + 4u * c) =
+            mxfp4::encode8(vx, mxfp4::scale_float(vs));
+        if (c % 4u == 0u) {
+          a.cache.k_blocks()[at + c / 4u] = (uint8_t)ks;
+          a.cache.v_blocks()[at + c / 4u] = (uint8_t)vs;
+        }
       }
     } else {
       float km = amax8(kx, 0.0f), vm = amax8(vx, 0.0f);
@@ -206,7 +231,7 @@ struct ReadArgs {
 
 enum : uint32_t { kRowKept = 0u, kRowZero = 1u, kRowRead = 2u };
 
-template <bool E4M3>
+template <uint32_t F>
 __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
   __shared__ uint32_t staged[kStagedStarts];
   __shared__ uint32_t kind[kReadTokens], page_of[kReadTokens], place_of[kReadTokens];
@@ -254,7 +279,7 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
                           head * a.cache.head_stride;
     const uint64_t to = (uint64_t)(first + i) * a.token_stride + head * a.head_stride;
     float ks = 0.0f, vs = 0.0f;
-    if (E4M3 && read) {
+    if (F == kE4m3 && read) {
       const uint64_t at =
           ((uint64_t)page_of[i] * a.cache.kv_heads + head) * a.cache.page.divisor + place_of[i];
       ks = a.cache.k_scale[at];
@@ -264,7 +289,14 @@ __global__ void __launch_bounds__(kThreads) kv_read_kernel(ReadArgs a) {
       const uint32_t n = chunk_left(a.cache.head_dim, c);
       u32x4_t kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
       if (read) {
-        if constexpr (E4M3) {
+        if constexpr (F == kMxfp4) {
+          const uint64_t at = (((uint64_t)page_of[i] * a.cache.kv_heads + head) *
+                                   a.cache.page.divisor + place_of[i]) * (chunks / 4u) + c / 4u;
+          kx = mxfp4::decode8_bf16(*reinterpret_cast<const u32_any_t*>(a.cache.k + from + 4u * c),
+                                   mxfp4::scale_float(a.cache.k_blocks()[at]));
+          vx = mxfp4::decode8_bf16(*reinterpret_cast<const u32_any_t*>(a.cache.v + from + 4u * c),
+                                   mxfp4::scale_float(a.cache.v_blocks()[at]));
+        } else if constexpr (F == kE4m3) {
           kx = widen8(load_codes8(a.cache.k + from + 8u * c, n), ks);
           vx = widen8(load_codes8(a.cache.v + from + 8u * c, n), vs);
         } else {
@@ -285,11 +317,13 @@ uint32_t row_lanes_log2(uint32_t head_dim) {
   return log2;
 }
 
-const fe2o3_host::KernelRegistrar kRegistered[] = {
-    fe2o3_host::KernelRegistrar({"fe2o3_kv_cache_write", "kv_write_kernel<bf16>", (const void*)kv_write_kernel<false>, kThreads, 0}),
-    fe2o3_host::KernelRegistrar({"fe2o3_kv_cache_write", "kv_write_kernel<e4m3>", (const void*)kv_write_kernel<true>, kThreads, 0}),
-    fe2o3_host::KernelRegistrar({"fe2o3_kv_cache_read", "kv_read_kernel<bf16>", (const void*)kv_read_kernel<false>, kThreads, 0}),
-    fe2o3_host::KernelRegistrar({"fe2o3_kv_cache_read", "kv_read_kernel<e4m3>", (const void*)kv_read_kernel<true>, kThreads, 0})};
+#define FE2O3_KV_KERNELS(F, NAME) \
+  fe2o3_host::KernelRegistrar({"fe2o3_kv_cache_write", "kv_write_kernel<" NAME ">", (const void*)kv_write_kernel<F>, kThreads, 0}), \
+  fe2o3_host::KernelRegistrar({"fe2o3_kv_cache_read", "kv_read_kernel<" NAME ">", (const void*)kv_read_kernel<F>, kThreads, 0})
+const fe2o3_host::KernelRegistrar kRegistered[] = {FE2O3_KV_KERNELS(kBf16, "bf16"),
+                                                   FE2O3_KV_KERNELS(kE4m3, "e4m3"),
+                                                   FE2O3_KV_KERNELS(kMxfp4, "mxfp4")};
+#undef FE2O3_KV_KERNELS
 
 }  // namespace
 
@@ -326,8 +360,9 @@ int32_t fe2o3_kv_cache_write(const Fe2o3KvCacheV1* cache, const uint16_t* k, uin
   const uint64_t wgs = ((rows << a.lanes_log2) + kThreads - 1u) / kThreads;
   const uint32_t grid = (uint32_t)(wgs < kMaxGrid ? wgs : kMaxGrid);
   hipStream_t s = (hipStream_t)stream;
-  if (cache->format == FE2O3_KV_E4M3) kv_write_kernel<true><<<grid, kThreads, 0, s>>>(a);
-  else kv_write_kernel<false><<<grid, kThreads, 0, s>>>(a);
+  if (cache->format == kE4m3) kv_write_kernel<kE4m3><<<grid, kThreads, 0, s>>>(a);
+  else if (cache->format == kMxfp4) kv_write_kernel<kMxfp4><<<grid, kThreads, 0, s>>>(a);
+  else kv_write_kernel<kBf16><<<grid, kThreads, 0, s>>>(a);
   return fe2o3_host::after_launch();
 }
 
@@ -368,8 +403,9 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1* cache, const uint32_t* block_t
   const uint32_t wgs = (tokens - 1u) / kReadTokens + 1u;
   const dim3 grid(wgs < kMaxGrid ? wgs : kMaxGrid, (wgs - 1u) / kMaxGrid + 1u);
   hipStream_t s = (hipStream_t)stream;
-  if (cache->format == FE2O3_KV_E4M3) kv_read_kernel<true><<<grid, kThreads, 0, s>>>(a);
-  else kv_read_kernel<false><<<grid, kThreads, 0, s>>>(a);
+  if (cache->format == kE4m3) kv_read_kernel<kE4m3><<<grid, kThreads, 0, s>>>(a);
+  else if (cache->format == kMxfp4) kv_read_kernel<kMxfp4><<<grid, kThreads, 0, s>>>(a);
+  else kv_read_kernel<kBf16><<<grid, kThreads, 0, s>>>(a);
   return fe2o3_host::after_launch();
 }
 

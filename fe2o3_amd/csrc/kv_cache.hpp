@@ -70,10 +70,13 @@ struct RowScale {
   }
 };
 
-// A cache's arrays and strides, in elements of its format.
+// A cache's arrays and strides, in elements of its format (MXFP4: bytes).
 struct View {
   uint8_t *k, *v;
   float *k_scale, *v_scale;  // E4M3: [pages, kv_heads, page_size]
+  // MXFP4: bytes, [pages, kv_heads, page_size, head_dim / 32]
+  FE2O3_KV_HD uint8_t* k_blocks() const { return (uint8_t*)k_scale; }
+  FE2O3_KV_HD uint8_t* v_blocks() const { return (uint8_t*)v_scale; }
   uint64_t page_stride, token_stride, head_stride;
   FastDiv page;  // of the slots in a page
   uint32_t pages, kv_heads, head_dim;
@@ -109,23 +112,28 @@ inline int32_t rows_extent(uint64_t tokens, uint64_t heads, uint64_t head_dim,
 // The caller's record checked, in the order the header states.
 inline int32_t check(const Fe2o3KvCacheV1* c, View* out) {
   if (c == nullptr) return FE2O3_ERR_NULL;
-  if (c->format != FE2O3_KV_BF16 && c->format != FE2O3_KV_E4M3) return FE2O3_ERR_SHAPE;
+  if (c->format != FE2O3_KV_BF16 && c->format != FE2O3_KV_E4M3 && c->format != FE2O3_KV_MXFP4)
+    return FE2O3_ERR_SHAPE;
   if (c->pages == 0u || c->page_size == 0u || c->kv_heads == 0u || c->head_dim == 0u)
     return FE2O3_ERR_SHAPE;
   const uint64_t slots = (uint64_t)c->pages * c->page_size;
   if (slots >= (UINT64_C(1) << 31) || c->head_dim >= (UINT32_C(1) << 31)) return FE2O3_ERR_SHAPE;
+  const bool blocks = c->format == FE2O3_KV_MXFP4;
+  if (blocks && c->head_dim % 32u != 0u) return FE2O3_ERR_SHAPE;
   uint64_t extent;
-  const int32_t rc = rows_extent(c->page_size, c->kv_heads, c->head_dim, c->token_stride,
-                                 c->head_stride, &extent);
+  const int32_t rc = rows_extent(c->page_size, c->kv_heads, blocks ? c->head_dim / 2u : c->head_dim,
+                                 c->token_stride, c->head_stride, &extent);
   if (rc != FE2O3_OK) return rc;
   if (c->pages > 1u && c->page_stride < extent) return FE2O3_ERR_STRIDE;
   uint64_t bytes;
   if (!reach(c->pages, c->page_stride, &extent) || !mul_ok(extent, 2u, &bytes))
     return FE2O3_ERR_OVERFLOW;
   if (c->k_len < extent || c->v_len < extent) return FE2O3_ERR_LENGTH;
-  const bool scaled = c->format == FE2O3_KV_E4M3;
+  const bool scaled = c->format != FE2O3_KV_BF16;
   uint64_t scales = 0;
-  if (scaled && !mul_ok(slots, c->kv_heads, &scales)) return FE2O3_ERR_OVERFLOW;
+  if (scaled && (!mul_ok(slots, c->kv_heads, &scales) ||
+                 (blocks && !mul_ok(scales, c->head_dim / 32u, &scales))))
+    return FE2O3_ERR_OVERFLOW;
   if (c->k_scale_len != scales || c->v_scale_len != scales) return FE2O3_ERR_LENGTH;
   if (!c->k || !c->v || (scaled && (!c->k_scale || !c->v_scale))) return FE2O3_ERR_NULL;
   if (!scaled && (((uintptr_t)c->k | (uintptr_t)c->v) & 1u) != 0u) return FE2O3_ERR_ALIGNMENT;

@@ -45,12 +45,15 @@
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
+#include "mxfp4.hpp"
 
 namespace {
 
 using namespace fe2o3;
 using kv_cache::View;
 
+// a cache's format, FE2O3_KV_*
+constexpr uint32_t kBf16 = FE2O3_KV_BF16, kE4m3 = FE2O3_KV_E4M3, kMxfp4 = FE2O3_KV_MXFP4;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;  // of a workgroup, if not said otherwise
 constexpr uint32_t kKeys = 32;              // keys per tile
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
@@ -141,15 +144,15 @@ FE2O3_DEVICE u32x4_t widen_codes8(uint32_t lo, uint32_t hi) {
 //   K, 8 rows (r % 4 and bit 3 apart) of two neighbouring chunks;
 //   V, half a wave's transposing read: bf16 4 rows of two chunks for each of two
 //   lane groups, whose rows differ in bit 3; e4m3 8 rows of one chunk for each.
-template <int D, bool E4M3>
+template <int D, uint32_t F>
 struct Tile {
-  static constexpr uint32_t kRowBytes = E4M3 ? D : 2 * D;
+  static constexpr uint32_t kRowBytes = F == kBf16 ? 2 * D : F == kE4m3 ? D : D / 2;
   static constexpr uint32_t kRowLanes = kRowBytes / 16u;  // lanes that load a row
   static constexpr uint32_t kRowsPerLoad = 64u / kRowLanes;
   static constexpr int kLoads = kKeys / kRowsPerLoad;     // of K, and of V
   static constexpr uint32_t kBytes = kKeys * kRowBytes;   // of K, and of V
   static FE2O3_DEVICE constexpr uint32_t swz(uint32_t r) {
-    if constexpr (E4M3)
+    if constexpr (F == kE4m3)
       return D == 128 ? (r >> 2 & 1u) | (r & 2u) | (r >> 1 & 4u) : (r >> 2 & 1u) | (r >> 2 & 2u);
     else
       return D == 128 ? 2u * ((r & 3u) | (r >> 1 & 4u)) : 2u * ((r >> 1 & 1u) | (r >> 2 & 2u));
@@ -174,37 +177,40 @@ constexpr uint32_t waves(int rt) { return kWaves * sharers(rt); }
 // LDS of a workgroup of W waves: their tiles, or two places for tiles that S waves
 // share, which the sums of 16 query rows of each wave take at the end of a run; their
 // tiles' scales; their reference and sum of each query row.
-template <int D, bool E4M3, uint32_t S, uint32_t W>
+template <int D, uint32_t F, uint32_t S, uint32_t W>
 struct Lds {
-  using T = Tile<D, E4M3 && S == 1>;
+  using T = Tile<D, F == kE4m3 && S == 1 ? kE4m3 : kBf16>;
   static constexpr uint32_t kTiles = (S == 1 ? 2u : 4u) * T::kBytes;  // of S waves
   static constexpr uint32_t kSums = S == 1 && kTiles > T::kSumBytes ? kTiles : T::kSumBytes;
   static constexpr uint32_t kOwn = S == 1 ? kSums : kTiles;  // from S waves' to the next
   static constexpr uint32_t kScales = W / S * kOwn > W * kSums ? W / S * kOwn : W * kSums;
-  static constexpr uint32_t kStats = kScales + (E4M3 ? W * 2u * kKeys * 4u : 0u);
+  static constexpr uint32_t kStats = kScales + (F == kE4m3 ? W * 2u * kKeys * 4u : 0u);
   static constexpr uint32_t kBytes = kStats + W * 16u * 8u;
   static_assert(kOwn % 256u == 0u, "chunks are chosen by exclusive or");
 };
 
 // Workgroups per CU: as many as registers and LDS allow, but two of the widest of one
 // row tile (three of them, e4m3, 64 sequences of 4096 keys: 98.5 -> 105.5 us).
-template <int D, bool E4M3, int RT>
+template <int D, uint32_t F, int RT>
 constexpr int per_cu() {
   if (RT == 1) return D == 64 ? 3 : 2;
-  return RT == 2 && (D == 64 || E4M3) ? 2 : 1;
+  return RT == 2 && (D == 64 || F != kBf16) ? 2 : 1;
 }
 
 // D: head_dim.  RW: tiles of 16 query rows of a wave.  S waves, a team, share a tile of
 // keys, or each has its own (1).  WH: KV heads that a workgroup works on at once, of its
 // W waves W / WH on each.
-template <int D, bool E4M3, int RW, uint32_t S, int WH, uint32_t W>
+template <int D, uint32_t F, int RW, uint32_t S, int WH, uint32_t W>
 struct Decode {
   // Codes lie in LDS as they are and are widened on the way out, but waves that share
   // a tile would all widen it: they do on the way in, a part each.
-  static constexpr bool kCodes = E4M3 && S == 1;
-  using R = Tile<D, E4M3>;    // as loaded
-  using T = Tile<D, kCodes>;  // in LDS
-  using L = Lds<D, E4M3, S, W>;
+  // 4-bit codes are widened on the way in too, with their scales, so that what follows
+  // is a bf16 cache's.
+  static constexpr bool E4M3 = F == kE4m3, kCodes = E4M3 && S == 1;
+  using R = Tile<D, F>;                       // as loaded
+  using T = Tile<D, kCodes ? kE4m3 : kBf16>;  // in LDS
+  using L = Lds<D, F, S, W>;
+  static constexpr uint32_t kWiden = T::kRowBytes / R::kRowBytes;  // chunks from one loaded
   static_assert(S == 1 || WH == 1, "waves share a tile of one head");
   static constexpr uint32_t kStep = W / S / WH;  // tiles of a head per round
   static constexpr int kDb = D / 16;     // V^T row blocks
@@ -214,6 +220,7 @@ struct Decode {
   struct Stage {
     u32x4_t x[kMine];  // the wave's loads i (mine) of a tile: below kLoads K, then V
     float scale;       // E4M3: lanes below 32 the K scale of key l, the others the V scale
+    uint32_t blocks;   // MXFP4: the same of a row's scale bytes
     uint32_t valid;    // bit per key
   };
   struct Query {
@@ -277,7 +284,7 @@ struct Decode {
     const uint32_t rows = min(a.group - row0, (uint32_t)kBlockRows);
     const uint32_t q_head = head * a.group + row0;
     const uint32_t* table = a.table + (uint64_t)seq * a.table_cols;
-    const uint64_t head_at = head * a.cache.head_stride * (E4M3 ? 1u : 2u);
+    const uint64_t head_at = head * a.cache.head_stride * (F == kBf16 ? 2u : 1u);
     const uint32_t pr = lane / R::kRowLanes, pc = lane % R::kRowLanes;  // as loaded: row, piece
     const uint8_t* kb = a.cache.k + head_at + pc * 16u;
     const uint8_t* vb = a.cache.v + head_at + pc * 16u;
@@ -304,6 +311,13 @@ struct Decode {
             ((uint64_t)(ok ? page : 0u) * a.cache.kv_heads + head) * a.cache.page.divisor +
             (ok ? place : 0u);
         st.scale = sb[at_scale];
+      } else if constexpr (F == kMxfp4) {
+        const uint64_t row =
+            ((uint64_t)(ok ? page : 0u) * a.cache.kv_heads + head) * a.cache.page.divisor +
+            (ok ? place : 0u);
+        // a key that is left out: a scale that is no NaN, for its V of +0
+        if constexpr (D == 128) st.blocks = ok ? ((const uint32_t*)sb)[row] : 0u;
+        else st.blocks = ok ? (uint32_t)((const uint16_t*)sb)[row] : 0u;
       } else {
         off *= 2u;
       }
@@ -350,7 +364,7 @@ struct Decode {
     const uint32_t own_at = team * L::kOwn;
     const uint32_t k_row = 8u * (lr >> 2) + (lr & 3u);
     const uint32_t v_row = 8u * g + (kCodes ? lr >> 1 : lr >> 2);
-    uint32_t put_at = own_at + pr * T::kRowBytes + (((kCodes == E4M3 ? pc : 2u * pc) ^ T::swz(pr)) << 4);
+    uint32_t put_at = own_at + pr * T::kRowBytes + ((kWiden * pc ^ T::swz(pr)) << 4);
     uint32_t k_at = own_at + k_row * T::kRowBytes +
                     ((g ^ T::swz(k_row)) << 4);
     uint32_t v_at = own_at + T::kBytes + v_row * T::kRowBytes +
@@ -376,8 +390,16 @@ struct Decode {
         // of both
         const uint32_t at = ((put_at + buffer) ^ T::swz(r) << 4) + r * T::kRowBytes +
                             (i < R::kLoads ? 0u : T::kBytes);
-        if constexpr (kCodes == E4M3) {
+        if constexpr (kWiden == 1u) {
           *reinterpret_cast<u32x4_t*>(smem + at) = st.x[j];
+        } else if constexpr (F == kMxfp4) {
+          const uint32_t bytes =
+              (uint32_t)__shfl((int)st.blocks, (int)(r + pr + (i < R::kLoads ? 0u : 32u)), 64);
+          const float scale = mxfp4::scale_float(bytes >> (8u * pc) & 255u);
+#pragma unroll
+          for (uint32_t c = 0; c < 4u; ++c)
+            *reinterpret_cast<u32x4_t*>(smem + (at ^ c << 4)) =
+                mxfp4::decode8_bf16(st.x[j][c], scale);
         } else {  // swizzles of bf16 rows are even: the two chunks stay together
           *reinterpret_cast<u32x4_t*>(smem + at) = widen_codes8(st.x[j][0], st.x[j][1]);
           *reinterpret_cast<u32x4_t*>(smem + at + 16u) = widen_codes8(st.x[j][2], st.x[j][3]);
@@ -640,14 +662,14 @@ struct Decode {
 
 // One workgroup of W waves per sequence and block of query rows, for calls whose
 // sequences are too short to be worth a join.
-template <int D, bool E4M3, int RT, uint32_t W>
-__global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, E4M3, RT>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
+template <int D, uint32_t F, int RT, uint32_t W>
+__global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of(a, seq);
-  Decode<D, E4M3, row_tiles(RT), sharers(RT), 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+  Decode<D, F, row_tiles(RT), sharers(RT), 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
 // The list of all work: sequence, then block of query rows (or WH KV heads), then
@@ -733,8 +755,8 @@ struct Plan {
   }
 };
 
-template <int D, bool E4M3, int RT, int WH>
-__global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, E4M3, RT>() * sharers(RT))) paged_split_kernel(Args a) {
+template <int D, uint32_t F, int RT, int WH>
+__global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, F, RT>() * sharers(RT))) paged_split_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   using P = Plan<RT, WH>;
   const P plan(a);
@@ -747,7 +769,7 @@ __global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, E4M3, RT>() * share
   Span sp = plan.span(seq);
   uint32_t length = P::rounds(sp);
   uint32_t hb = uniform(rest / length), pos = rest - hb * length;
-  Decode<D, E4M3, row_tiles(RT), sharers(RT), WH, waves(RT)> decode(a, smem);
+  Decode<D, F, row_tiles(RT), sharers(RT), WH, waves(RT)> decode(a, smem);
   while (true) {
     const uint32_t stop = min(length, pos + (end - at));
     const uint32_t tile = P::kStep * (max(pos, P::kSetup) - P::kSetup);
@@ -865,17 +887,17 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_run
     a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
-template <int D, bool E4M3, int RT, int WH>
+template <int D, uint32_t F, int RT, int WH>
 int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
-  constexpr uint32_t kSmem = Lds<D, E4M3, sharers(RT), waves(RT)>::kBytes;
+  constexpr uint32_t kSmem = Lds<D, F, sharers(RT), waves(RT)>::kBytes;
   using P = Plan<RT, WH>;
-  const auto fn = paged_split_kernel<D, E4M3, RT, WH>;
+  const auto fn = paged_split_kernel<D, F, RT, WH>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   // as many workgroups as are resident at once, and work for each wave
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head / WH;
   const uint64_t most = heads * ((tiles + P::kStep - 1u) / P::kStep + P::kSetup);
-  uint32_t workgroups = per_cu<D, E4M3, RT>() * cus;
+  uint32_t workgroups = per_cu<D, F, RT>() * cus;
   if (workgroups > kMaxWorkgroups) workgroups = kMaxWorkgroups;
   if (workgroups > most) workgroups = (uint32_t)most;
   a.workgroups = workgroups;
@@ -902,10 +924,10 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   return fe2o3_host::after_launch();
 }
 
-template <int D, bool E4M3, int RT, uint32_t W>
+template <int D, uint32_t F, int RT, uint32_t W>
 int32_t launch_whole(const Args& a, hipStream_t s) {
-  constexpr uint32_t kSmem = Lds<D, E4M3, sharers(RT), W>::kBytes;
-  const auto fn = paged_whole_kernel<D, E4M3, RT, W>;
+  constexpr uint32_t kSmem = Lds<D, F, sharers(RT), W>::kBytes;
+  const auto fn = paged_whole_kernel<D, F, RT, W>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
@@ -914,7 +936,7 @@ int32_t launch_whole(const Args& a, hipStream_t s) {
   return fe2o3_host::after_launch();
 }
 
-template <int D, bool E4M3, int RT>
+template <int D, uint32_t F, int RT>
 int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   const uint64_t heads = (uint64_t)a.seqs * a.cache.kv_heads * a.blocks_per_head;
   // Whether one workgroup a head is enough, without a plan and a join: rounds of
@@ -934,7 +956,7 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   // join, and a head its own rounds at least (48 rows, one KV head):
   //   48 x 170 14.0, 9.5    48 x 1000 16.4, 21.9    8 x 500   13.6, 13.1
   //   64 x 500 16.0, 14.2   200 x 500 24.6, 15.9    300 x 500 32.5, 29.0
-  const uint32_t resident = (per_cu<D, E4M3, RT>() == 1 ? 1u : 2u) * cus;
+  const uint32_t resident = (per_cu<D, F, RT>() == 1 ? 1u : 2u) * cus;
   const bool wide = RT == 1 && heads <= cus;
   const uint64_t rounds_whole =
       wide ? (tiles + 7u) / 8u : ((tiles + 3u) / 4u * heads + resident - 1u) / resident;
@@ -943,8 +965,8 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   if (tiles <= kWholeTiles && (rounds_whole > least ? rounds_whole : least) <=
                                   rounds_split + (RT == 1 ? 2u : 4u)) {
     if constexpr (RT == 1)
-      if (wide && tiles > kWaves) return launch_whole<D, E4M3, RT, 8>(a, s);
-    return launch_whole<D, E4M3, RT, waves(RT)>(a, s);
+      if (wide && tiles > kWaves) return launch_whole<D, F, RT, 8>(a, s);
+    return launch_whole<D, F, RT, waves(RT)>(a, s);
   }
   // Four heads a workgroup read neighbouring rows, but every part that the join adds
   // has the rows of four: worth it where a workgroup has six rounds at least (1 x 130001
@@ -952,16 +974,16 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   // group 7: 17.7, 20.0; 1 x 17313 of 4 KV heads, group 16, e4m3: 15.5, 19.4).
   if constexpr (RT == 1)
     if (a.cache.kv_heads % kWaves == 0u && heads / kWaves * tiles >= 6u * resident)
-      return launch_split<D, E4M3, RT, kWaves>(a, tiles, cus, s);
-  return launch_split<D, E4M3, RT, 1>(a, tiles, cus, s);
+      return launch_split<D, F, RT, kWaves>(a, tiles, cus, s);
+  return launch_split<D, F, RT, 1>(a, tiles, cus, s);
 }
 
-template <int D, bool E4M3>
+template <int D, uint32_t F>
 int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
-  if (a.rows <= 16u) return launch<D, E4M3, 1>(a, tiles, cus, s);
-  if (a.rows <= 32u) return launch<D, E4M3, 2>(a, tiles, cus, s);
-  if (a.rows <= 48u) return launch<D, E4M3, 3>(a, tiles, cus, s);
-  return launch<D, E4M3, 4>(a, tiles, cus, s);
+  if (a.rows <= 16u) return launch<D, F, 1>(a, tiles, cus, s);
+  if (a.rows <= 32u) return launch<D, F, 2>(a, tiles, cus, s);
+  if (a.rows <= 48u) return launch<D, F, 3>(a, tiles, cus, s);
+  return launch<D, F, 4>(a, tiles, cus, s);
 }
 
 #define FE2O3_KERNEL(NAME, FN, THREADS, LDS) \
@@ -984,8 +1006,9 @@ int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) 
   FE2O3_JOIN(D, 1, 1, ROWS), FE2O3_JOIN(D, 1, 4, ROWS), FE2O3_JOIN(D, 2, 1, ROWS), \
   FE2O3_JOIN(D, 3, 1, ROWS), FE2O3_JOIN(D, 4, 1, ROWS)
 const fe2o3_host::KernelRegistrar kRegistered[] = {
-    FE2O3_PAGED_ALL(64, false), FE2O3_PAGED_ALL(64, true), FE2O3_PAGED_ALL(128, false),
-    FE2O3_PAGED_ALL(128, true), FE2O3_JOIN_ALL(64, 16), FE2O3_JOIN_ALL(128, 8)};
+    FE2O3_PAGED_ALL(64, kBf16),   FE2O3_PAGED_ALL(64, kE4m3),  FE2O3_PAGED_ALL(64, kMxfp4),
+    FE2O3_PAGED_ALL(128, kBf16),  FE2O3_PAGED_ALL(128, kE4m3), FE2O3_PAGED_ALL(128, kMxfp4),
+    FE2O3_JOIN_ALL(64, 16), FE2O3_JOIN_ALL(128, 8)};
 #undef FE2O3_KERNEL
 #undef FE2O3_SPLIT
 #undef FE2O3_PAGED_ALL
@@ -1065,10 +1088,15 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.window = window;
   a.scale_log2 = scale_log2;
   hipStream_t s = (hipStream_t)stream;
-  const bool e4m3 = cache->format == FE2O3_KV_E4M3;
-  if (d == 64u)
-    return e4m3 ? launch_rows<64, true>(a, tiles, topo.cus, s)
-                : launch_rows<64, false>(a, tiles, topo.cus, s);
-  return e4m3 ? launch_rows<128, true>(a, tiles, topo.cus, s)
-              : launch_rows<128, false>(a, tiles, topo.cus, s);
+  switch (cache->format) {
+    case kE4m3:
+      return d == 64u ? launch_rows<64, kE4m3>(a, tiles, topo.cus, s)
+                      : launch_rows<128, kE4m3>(a, tiles, topo.cus, s);
+    case kMxfp4:
+      return d == 64u ? launch_rows<64, kMxfp4>(a, tiles, topo.cus, s)
+                      : launch_rows<128, kMxfp4>(a, tiles, topo.cus, s);
+    default:
+      return d == 64u ? launch_rows<64, kBf16>(a, tiles, topo.cus, s)
+                      : launch_rows<128, kBf16>(a, tiles, topo.cus, s);
+  }
 }

@@ -299,7 +299,7 @@ def moe_routing_check(routing: dict, tokens: int, experts: int, capacity: int,
 # one: order them behind what writes their tensors, and without sync keep the
 # tensors until the stream is through.
 
-KV_BF16, KV_E4M3 = 0, 1
+KV_BF16, KV_E4M3, KV_MXFP4 = 0, 1, 4
 KV_NO_SLOT = 0xFFFFFFFF
 PAGED_ATTENTION_MAX_WORKGROUPS = 768
 
@@ -410,40 +410,54 @@ def _pair(k, v, dims, kind, device):
 
 
 class KvCache:
-    """A paged key-value cache: K and V rows in slots page * page_size + place,
-    bf16, or e4m3 codes with scales [pages, kv_heads, page_size].
+    """A paged key-value cache: K and V rows in slots page * page_size + place: bf16;
+    e4m3 codes with f32 scales [pages, kv_heads, page_size]; or microscaled 4-bit
+    codes, two to a byte, with scale bytes [pages, kv_heads, page_size, head_dim / 32].
 
-    k and v are device tensors [pages, page_size, kv_heads, head_dim] of any
-    strides but the last (a cache laid out [pages, kv_heads, page_size,
-    head_dim] is passed as its transpose(1, 2)), or DeviceBuffers with `shape`
-    given that way and `strides` (page, token, head; dense by default) in
-    elements.  K and V have the same strides.  The record holds the arrays, not
-    copies of them.
+    k and v are device tensors [pages, page_size, kv_heads, head_dim] (4-bit:
+    head_dim / 2 bytes) of any strides but the last (a cache laid out [pages,
+    kv_heads, page_size, head_dim] is passed as its transpose(1, 2)), or
+    DeviceBuffers with `shape` given that way and `strides` (page, token, head;
+    dense by default) in elements (4-bit: the shape with head_dim, the strides in
+    bytes).  K and V have the same strides; scales of bytes make the cache a 4-bit
+    one.  The record holds the arrays, not copies of them.
     """
 
     def __init__(self, k, v, k_scale=None, v_scale=None, *, shape=None, strides=None):
         if (k_scale is None) != (v_scale is None):
             raise ValueError("k_scale and v_scale go together")
         self.device = device = _device_of(k)
-        self.format, kind = (KV_BF16, _BF16) if k_scale is None else (KV_E4M3, _CODES)
+        packed = 1  # elements in one of the array's
+        if k_scale is None:
+            self.format, kind = KV_BF16, _BF16
+        elif _BYTES in _kinds[k_scale.dtype]:
+            self.format, kind, packed = KV_MXFP4, _BYTES, 2
+        else:
+            self.format, kind = KV_E4M3, _CODES
         found, found_strides, arrays = _pair(k, v, 4, kind, device)
         if found is not None:
-            shape, strides = found, found_strides[:3]
+            pages, page_size, kv_heads, width = found
+            strides, head_dim = found_strides[:3], packed * width
         elif shape is None:
             raise ValueError("a cache of DeviceBuffers needs its shape")
-        pages, page_size, kv_heads, head_dim = self.shape = shape
+        else:
+            pages, page_size, kv_heads, head_dim = shape
+        self.shape = (pages, page_size, kv_heads, head_dim)
         if strides is None:
-            strides = (page_size * kv_heads * head_dim, kv_heads * head_dim, head_dim)
+            row = head_dim // packed
+            strides = (page_size * kv_heads * row, kv_heads * row, row)
         self.arrays = (k, v, k_scale, v_scale)
         scales = (None, 0, None, 0)
         if k_scale is not None:
+            want, scale_kind = (pages, kv_heads, page_size), _FLOAT
+            if packed == 2:
+                want, scale_kind = want + (head_dim // MXFP4_BLOCK,), _BYTES
             for scale in (k_scale, v_scale):
-                found = _dimensions(scale, 3, "scales")
-                if found is not None and tuple(found) != (pages, kv_heads, page_size):
-                    raise ValueError(f"scales of {tuple(found)}, "
-                                     f"not {(pages, kv_heads, page_size)}")
-            scales = (_operand(k_scale, _FLOAT, "k_scale", device)
-                      + _operand(v_scale, _FLOAT, "v_scale", device))
+                found = _dimensions(scale, len(want), "scales")
+                if found is not None and found != want:
+                    raise ValueError(f"scales of {tuple(found)}, not {want}")
+            scales = (_operand(k_scale, scale_kind, "k_scale", device)
+                      + _operand(v_scale, scale_kind, "v_scale", device))
         self.record = _lib.Fe2o3KvCacheV1(*arrays, *scales, *strides, self.format, pages, page_size,
                                           kv_heads, head_dim, 0)
 
@@ -488,7 +502,7 @@ def _rows(cache, k, v, strides, device):
 def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sync=True) -> None:
     """Writes rows k, v (bf16 [tokens, kv_heads, head_dim]; DeviceBuffers with
     `strides` (token, head)) into slots[t] of the cache, quantised where it is
-    e4m3.  A slot out of range (KV_NO_SLOT) is skipped; each slot at most once
+    e4m3 or 4-bit.  A slot out of range (KV_NO_SLOT) is skipped; each slot at most once
     a call (fe2o3_kv_cache_write)."""
     device = _on_current_device(cache)
     rows, strides, arrays = _rows(cache, k, v, strides, device)

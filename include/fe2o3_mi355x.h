@@ -336,12 +336,20 @@ int32_t fe2o3_flash_attention_fwd(const uint16_t *q, uint64_t q_len,
  * no part in the maximum and stays a NaN, of either sign; a row with an infinity
  * has an infinite scale and reads back as NaN.
  *
+ * FE2O3_KV_MXFP4 keeps the microscaled 4-bit blocks of fe2o3_quantize_mxfp4: a row
+ * is head_dim / 2 bytes of codes and head_dim / 32 scale bytes, in k_scale and
+ * v_scale [pages, kv_heads, page_size, head_dim / 32] (uint8_t arrays, their
+ * pointers cast).  k_len, v_len and the strides count bytes of codes, the scale
+ * lengths bytes; head_dim is a multiple of 32.  A block with a NaN or an infinity
+ * reads back as NaN.
+ *
  * The record is checked in this order: NULL record FE2O3_ERR_NULL; another
- * format, a size of 0, or slots or head_dim of 2^31 or more FE2O3_ERR_SHAPE;
+ * format, a size of 0, slots or head_dim of 2^31 or more, or a head_dim that the
+ * format does not take FE2O3_ERR_SHAPE;
  * strides with which rows share elements FE2O3_ERR_STRIDE (FE2O3_ERR_OVERFLOW
  * where an extent passes 64 bits); k_len or v_len short of the extent, or scale
- * lengths other than pages * kv_heads * page_size (0 for bf16)
- * FE2O3_ERR_LENGTH; NULL arrays FE2O3_ERR_NULL; bf16 at an odd address or
+ * lengths other than pages * kv_heads * page_size (times head_dim / 32 for
+ * MXFP4; 0 for bf16) FE2O3_ERR_LENGTH; NULL arrays FE2O3_ERR_NULL; bf16 at an odd address or
  * scales off their 4 bytes FE2O3_ERR_ALIGNMENT.
  *
  * Slots, block tables, starts and lengths are device data that the host
@@ -351,10 +359,11 @@ int32_t fe2o3_flash_attention_fwd(const uint16_t *q, uint64_t q_len,
  * call writes belongs to another of its arrays. */
 #define FE2O3_KV_BF16 0u
 #define FE2O3_KV_E4M3 1u
+#define FE2O3_KV_MXFP4 4u
 #define FE2O3_KV_NO_SLOT 0xffffffffu
 
 typedef struct Fe2o3KvCacheV1 {
-  void *k; /* uint16_t bf16 bits or uint8_t codes */
+  void *k; /* uint16_t bf16 bits or uint8_t codes (MXFP4: two to a byte) */
   uint64_t k_len;
   void *v;
   uint64_t v_len;
@@ -382,7 +391,7 @@ int32_t fe2o3_kv_cache_write(const Fe2o3KvCacheV1 *cache, const uint16_t *k, uin
                              uint64_t head_stride, void *stream);
 
 /* Reads cached rows back as bf16 (E4M3: the f32 product code * scale, RNE to
- * bf16), several sequences packed one behind another: output row t with
+ * bf16; MXFP4: the value, exact), several sequences packed one behind another: output row t with
  * starts[s] <= t < starts[s + 1] is token t - starts[s] of sequence s, whose
  * page p is block_table[s * table_cols + p].  Output row (t, h) lies at t *
  * token_stride + h * head_stride of k and of v, t < tokens.  Rows in no

@@ -46,7 +46,8 @@ def two_to_a_byte(code):
 
 
 def one_a_byte(packed):
-    return np.stack((packed & 15, packed >> 4), -1).reshape(*packed.shape[:-1], -1)
+    return np.stack((packed & 15, packed >> 4), -1).reshape(*packed.shape[:-1],
+                                                             2 * packed.shape[-1])
 
 
 def pack(x):
