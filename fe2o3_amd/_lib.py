@@ -63,6 +63,15 @@ class Fe2o3KvCacheV1(C.Structure):
                 ("reserved", C.c_uint32)]
 
 
+class Fe2o3RotaryRowsV1(C.Structure):
+    """Rows of Q or of K and where they go (72 bytes)."""
+
+    _fields_ = [("x", C.c_void_p), ("x_len", C.c_uint64), ("out", C.c_void_p),
+                ("out_len", C.c_uint64), ("token_stride", C.c_uint64),
+                ("head_stride", C.c_uint64), ("out_token_stride", C.c_uint64),
+                ("out_head_stride", C.c_uint64), ("heads", C.c_uint32), ("reserved", C.c_uint32)]
+
+
 # ---- exact LDS GEMM lifecycle records (fe2o3_lds_gemm_slice1_*) ----------------------
 
 u8, c_char = C.c_uint8, C.c_char
@@ -308,6 +317,9 @@ SIGNATURES = {
     "fe2o3_paged_attention_decode": (
         i32, [C.POINTER(Fe2o3KvCacheV1), vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64,
               u32, u32, u32, u32, u64, u32, f32, vp]),
+    "fe2o3_rotary": (
+        i32, [C.POINTER(Fe2o3RotaryRowsV1), C.POINTER(Fe2o3RotaryRowsV1), vp, u64, vp, u64, u32,
+              u32, u32, u32, u32, f32, vp]),
     "fe2o3_moe_top2_route_f32_t8_e4_k2_c4_v1": (
         i32, [vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp]),
     "fe2o3_moe_top2_route": (

@@ -1,0 +1,274 @@
+// rotary.hip -- rotary positions of Q and K, and their gradient, for gfx950.
+//
+//   (a, b) -> m (a cos t - b sin t, b cos t + a sin t),  t = position * freq_i
+//
+// for the pairs i of a head's first rotary_dim elements: (i, i + rotary_dim / 2), or
+// (2 i, 2 i + 1) interleaved; the rest of the head is copied.  The inverse turns by -t:
+// with the same m it is the transposed map, which takes a gradient back.
+//
+// An angle reaches 10^6 radians, where 32 bits are off by 0.06, so it is taken in turns:
+// position * (freq / 2 pi) in 64 bits, less its nearest whole number, is exact to 2^-30
+// of a turn at the largest position; sine and cosine of what is left are f32.
+//
+// Bound by memory: x is read once and written once.  A workgroup takes a few tokens, each
+// pair's sine and cosine is computed once for all heads and kept in LDS, and a lane turns
+// eight pairs, 16 bytes of bf16 on each side.
+#include "common.hpp"
+#include "internal.hpp"
+#include "kv_cache.hpp"
+
+namespace {
+
+using namespace fe2o3;
+using kv_cache::FastDiv;
+
+constexpr int kThreads = 256;
+constexpr uint32_t kMaxPairs = 2048;
+constexpr uint32_t kTable = 2048;  // sines and cosines in LDS, 8 bytes each
+typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
+typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+
+// Rows of one of the two arrays, strides in elements.
+struct Rows {
+  const void* x;
+  void* out;
+  uint64_t token_stride, head_stride, out_token_stride, out_head_stride;
+  uint32_t heads;
+};
+
+struct Args {
+  Rows rows[2];
+  const uint32_t* positions;
+  const double* freq;
+  FastDiv heads;   // of both arrays
+  FastDiv chunks;  // of a head: eight pairs each, then 16 copied elements each
+  FastDiv pairs;
+  uint32_t tokens, per_wg, head_dim, turned;  // turned: chunks of pairs
+  float cos_scale, sin_scale;  // the inverse has another sign of the sine
+};
+
+template <class T>
+struct Eight;
+template <>
+struct Eight<uint16_t> {
+  // the bits, those of a NaN too
+  static FE2O3_DEVICE void copy(const uint16_t* p, uint32_t n, uint16_t* out) {
+    if (n >= 8u) {
+      *reinterpret_cast<u32x4_any_t*>(out) = *reinterpret_cast<const u32x4_any_t*>(p);
+      return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 7u; ++i)
+      if (i < n) out[i] = p[i];
+  }
+  static FE2O3_DEVICE void load(const uint16_t* p, uint32_t n, float (&v)[8]) {
+    if (n >= 8u) {
+      const u32x4_t w = *reinterpret_cast<const u32x4_any_t*>(p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+      return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? f32_from_bf16_bits(p[i]) : 0.0f;
+  }
+  static FE2O3_DEVICE void store(uint16_t* p, uint32_t n, const float (&v)[8]) {
+    if (n >= 8u) {
+      *reinterpret_cast<u32x4_any_t*>(p) =
+          u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                  pack_bf16x2(v[6], v[7])};
+      return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 7u; ++i)
+      if (i < n) p[i] = bf16_bits_from_f32(v[i]);
+  }
+};
+template <>
+struct Eight<float> {
+  static FE2O3_DEVICE void copy(const float* p, uint32_t n, float* out) {
+    float v[8];
+    load(p, n, v);
+    store(out, n, v);
+  }
+  static FE2O3_DEVICE void load(const float* p, uint32_t n, float (&v)[8]) {
+    if (n >= 8u) {
+      const f32x4_t a = *reinterpret_cast<const f32x4_any_t*>(p);
+      const f32x4_t b = *reinterpret_cast<const f32x4_any_t*>(p + 4);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+      return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? p[i] : 0.0f;
+  }
+  static FE2O3_DEVICE void store(float* p, uint32_t n, const float (&v)[8]) {
+    if (n >= 8u) {
+      *reinterpret_cast<f32x4_any_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<f32x4_any_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+      return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 7u; ++i)
+      if (i < n) p[i] = v[i];
+  }
+};
+
+template <class T, bool INTERLEAVED>
+__global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
+  __shared__ __attribute__((aligned(16))) float2 table[kTable];
+  __shared__ uint32_t skipped[kThreads];
+  const uint32_t first = (blockIdx.y * kv_cache::kGridWidth + blockIdx.x) * a.per_wg;
+  if (first >= a.tokens) return;  // the last row of a grid of two dimensions
+  const uint32_t count = min(a.per_wg, a.tokens - first);
+  const uint32_t pairs = a.pairs.divisor;
+  for (uint32_t i = threadIdx.x; i < count * pairs; i += kThreads) {
+    const uint32_t t = a.pairs.div(i), pair = i - t * pairs;
+    const uint32_t position = a.positions[first + t];
+    const double turns = (double)position * (a.freq[pair] * 0.15915494309189533577);
+    const float rest = (float)(turns - __builtin_rint(turns));
+    float s, c;
+    sincospif(2.0f * rest, &s, &c);
+    table[i] = float2{c * a.cos_scale, s * a.sin_scale};
+    if (pair == 0u) skipped[t] = position == FE2O3_KV_NO_SLOT;
+  }
+  __syncthreads();
+  const uint32_t heads = a.heads.divisor, chunks = a.chunks.divisor;
+  const uint32_t tasks = count * heads * chunks;
+  for (uint32_t i = threadIdx.x; i < tasks; i += kThreads) {
+    const uint32_t row = a.chunks.div(i), chunk = i - row * chunks;
+    const uint32_t t = a.heads.div(row), h = row - t * heads;
+    if (skipped[t]) continue;
+    const bool second = h >= a.rows[0].heads;
+    const Rows& r = a.rows[second ? 1 : 0];
+    const uint32_t head = second ? h - a.rows[0].heads : h;
+    const T* x = (const T*)r.x + (first + t) * r.token_stride + head * r.head_stride;
+    T* out = (T*)r.out + (first + t) * r.out_token_stride + head * r.out_head_stride;
+    float u[8], v[8];
+    if (chunk < a.turned) {
+      const uint32_t p0 = 8u * chunk, n = min(pairs - p0, 8u);
+      // interleaved: elements 2 p0 .. + 15; halves: eight of each
+      const uint32_t at = INTERLEAVED ? 2u * p0 : p0, bt = INTERLEAVED ? at + 8u : pairs + p0;
+      const uint32_t na = INTERLEAVED ? min(2u * n, 8u) : n, nb = INTERLEAVED ? 2u * n - na : n;
+      Eight<T>::load(x + at, na, u);
+      Eight<T>::load(x + bt, nb, v);
+      float uo[8], vo[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float2 cs = table[t * pairs + min(p0 + j, pairs - 1u)];
+        if constexpr (INTERLEAVED) {
+          const float p = j < 4 ? u[2 * j & 7] : v[2 * j & 7];
+          const float q = j < 4 ? u[2 * j + 1 & 7] : v[2 * j + 1 & 7];
+          const float po = p * cs.x - q * cs.y, qo = q * cs.x + p * cs.y;
+          if (j < 4) {
+            uo[2 * j & 7] = po;
+            uo[2 * j + 1 & 7] = qo;
+          } else {
+            vo[2 * j & 7] = po;
+            vo[2 * j + 1 & 7] = qo;
+          }
+        } else {
+          uo[j] = u[j] * cs.x - v[j] * cs.y;
+          vo[j] = v[j] * cs.x + u[j] * cs.y;
+        }
+      }
+      Eight<T>::store(out + at, na, uo);
+      Eight<T>::store(out + bt, nb, vo);
+    } else if (x != out) {
+      const uint32_t at = 2u * pairs + 16u * (chunk - a.turned), n = min(a.head_dim - at, 16u);
+      const uint32_t na = min(n, 8u), nb = n - na;
+      Eight<T>::copy(x + at, na, out + at);
+      Eight<T>::copy(x + at + 8u, nb, out + at + 8u);
+    }
+  }
+}
+
+const fe2o3_host::KernelRegistrar kRegistered[] = {
+    fe2o3_host::KernelRegistrar({"fe2o3_rotary", "rotary_kernel<bf16>", (const void*)rotary_kernel<uint16_t, false>, kThreads, 0}),
+    fe2o3_host::KernelRegistrar({"fe2o3_rotary", "rotary_kernel<bf16,interleaved>", (const void*)rotary_kernel<uint16_t, true>, kThreads, 0}),
+    fe2o3_host::KernelRegistrar({"fe2o3_rotary", "rotary_kernel<f32>", (const void*)rotary_kernel<float, false>, kThreads, 0}),
+    fe2o3_host::KernelRegistrar({"fe2o3_rotary", "rotary_kernel<f32,interleaved>", (const void*)rotary_kernel<float, true>, kThreads, 0})};
+
+// The caller's record, its strides and lengths, for `tokens` rows.
+int32_t check_rows(const Fe2o3RotaryRowsV1* r, uint32_t tokens, uint32_t head_dim, Rows* out) {
+  uint64_t extent, out_extent, bytes;
+  int32_t rc = kv_cache::rows_extent(tokens, r->heads, head_dim, r->token_stride, r->head_stride,
+                                     &extent);
+  if (rc == FE2O3_OK)
+    rc = kv_cache::rows_extent(tokens, r->heads, head_dim, r->out_token_stride, r->out_head_stride,
+                               &out_extent);
+  if (rc != FE2O3_OK) return rc;
+  if (!kv_cache::mul_ok(extent, 4u, &bytes) || !kv_cache::mul_ok(out_extent, 4u, &bytes))
+    return FE2O3_ERR_OVERFLOW;
+  if (r->x_len < extent || r->out_len < out_extent) return FE2O3_ERR_LENGTH;
+  *out = Rows{r->x, r->out, r->token_stride, r->head_stride, r->out_token_stride,
+              r->out_head_stride, r->heads};
+  return FE2O3_OK;
+}
+
+}  // namespace
+
+extern "C" int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1* q, const Fe2o3RotaryRowsV1* k,
+                                const uint32_t* positions, uint64_t positions_len,
+                                const double* freq, uint64_t freq_len, uint32_t dtype,
+                                uint32_t tokens, uint32_t head_dim, uint32_t rotary_dim,
+                                uint32_t flags, float scale, void* stream) {
+  FE2O3_ENTRY("fe2o3_rotary");
+  if (q == nullptr) return FE2O3_ERR_NULL;
+  const uint64_t heads = (uint64_t)q->heads + (k ? k->heads : 0u);
+  const uint32_t pairs = rotary_dim / 2u;
+  if (dtype > 1u || flags > 3u || rotary_dim == 0u || rotary_dim % 2u != 0u ||
+      rotary_dim > head_dim || pairs > kMaxPairs || !__builtin_isfinite(scale))
+    return FE2O3_ERR_SHAPE;
+  if (q->heads == 0u || (k && k->heads == 0u)) return FE2O3_ERR_SHAPE;
+  const uint32_t turned = (pairs + 7u) / 8u;
+  const uint64_t chunks = turned + ((uint64_t)(head_dim - rotary_dim) + 15u) / 16u;
+  uint64_t tasks;  // of one token
+  if (!kv_cache::mul_ok(heads, chunks, &tasks) || tasks >= (UINT64_C(1) << 22) ||
+      tokens >= (1u << 31))
+    return FE2O3_ERR_SHAPE;
+  if (positions_len != tokens || freq_len != pairs) return FE2O3_ERR_LENGTH;
+  if (tokens == 0u) return FE2O3_OK;
+  Args a{};
+  int32_t rc = check_rows(q, tokens, head_dim, &a.rows[0]);
+  if (rc == FE2O3_OK && k) rc = check_rows(k, tokens, head_dim, &a.rows[1]);
+  if (rc != FE2O3_OK) return rc;
+  if (!q->x || !q->out || (k && (!k->x || !k->out)) || !positions || !freq) return FE2O3_ERR_NULL;
+  uintptr_t any = (uintptr_t)q->x | (uintptr_t)q->out;
+  if (k) any |= (uintptr_t)k->x | (uintptr_t)k->out;
+  if ((any & (dtype == 0u ? 3u : 1u)) != 0u || ((uintptr_t)positions & 3u) != 0u ||
+      ((uintptr_t)freq & 7u) != 0u)
+    return FE2O3_ERR_ALIGNMENT;
+  a.positions = positions;
+  a.freq = freq;
+  a.heads = FastDiv::of((uint32_t)heads);
+  a.chunks = FastDiv::of((uint32_t)chunks);
+  a.pairs = FastDiv::of(pairs);
+  a.tokens = tokens;
+  a.head_dim = head_dim;
+  a.turned = turned;
+  a.cos_scale = scale;
+  a.sin_scale = (flags & FE2O3_ROTARY_INVERSE) != 0u ? -scale : scale;
+  // a pair for every thread where the tokens still fill the device twice
+  tile_plan::Topology topo;
+  rc = fe2o3_host::device_topology(&topo);
+  if (rc != FE2O3_OK) return rc;
+  uint32_t per_wg = pairs < kThreads ? kThreads / pairs : 1u;
+  const uint32_t most = tokens / (2u * topo.cus);
+  if (per_wg > most) per_wg = most > 1u ? most : 1u;
+  a.per_wg = per_wg;
+  const kv_cache::Grid g = kv_cache::Grid::of((tokens - 1u) / per_wg + 1u);
+  const dim3 grid(g.x, g.y);
+  hipStream_t s = (hipStream_t)stream;
+  if ((flags & FE2O3_ROTARY_INTERLEAVED) != 0u) {
+    if (dtype == 0u) rotary_kernel<float, true><<<grid, kThreads, 0, s>>>(a);
+    else rotary_kernel<uint16_t, true><<<grid, kThreads, 0, s>>>(a);
+  } else {
+    if (dtype == 0u) rotary_kernel<float, false><<<grid, kThreads, 0, s>>>(a);
+    else rotary_kernel<uint16_t, false><<<grid, kThreads, 0, s>>>(a);
+  }
+  return fe2o3_host::after_launch();
+}

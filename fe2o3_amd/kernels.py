@@ -305,13 +305,15 @@ PAGED_ATTENTION_MAX_WORKGROUPS = 768
 
 # what an array of each kind may hold: element types of a DeviceBuffer, and of
 # a tensor
-_BF16, _CODES, _INDEX, _FLOAT, _BYTES = "bf16", "e4m3", "u32", "f32", "bytes"
+_BF16, _CODES, _INDEX, _FLOAT, _BYTES, _DOUBLE = (
+    "bf16", "e4m3", "u32", "f32", "bytes", "f64")
 _HOLDS = {
     _BF16: ("uint16", "torch.bfloat16"),
     _CODES: ("uint8", "torch.uint8", "torch.float8_e4m3fn"),
     _INDEX: ("uint32", "torch.int32", "torch.uint32"),
     _FLOAT: ("float32", "torch.float32"),
     _BYTES: ("uint8", "torch.uint8", "torch.int8"),
+    _DOUBLE: ("float64", "torch.float64"),
 }
 
 
@@ -576,6 +578,98 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
           *_operand(out, _BF16, "out", device), lse_ptr, lse_len,
           *_operand(workspace, _BYTES, "workspace", device), seqs, q_heads, cols, max_length,
           q_stride, window, scale, stream=stream, sync=sync)
+
+
+# ---- rotary positions ----------------------------------------------------------------------
+
+ROTARY_INTERLEAVED, ROTARY_INVERSE = 1, 2
+
+
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, factor: float = 1.0,
+                       schedule: str = "linear", original_length: int = 4096,
+                       slow_turns: float = 1.0, fast_turns: float = 32.0):
+    """(radians a position for each pair, in 64 bits, numpy; the scale of rotary()) for a
+    context `factor` times as long as the model's own original_length:
+
+      "linear"    every pair factor times slower
+      "base"      base stretched, so that the slowest pair is factor times slower and the
+                  fastest keeps its speed
+      "by_turns"  pairs of fast_turns and more over original_length keep their speed,
+                  those of slow_turns and fewer are factor times slower, a straight line
+                  between; the scale is 0.1 ln(factor) + 1
+    """
+    if rotary_dim <= 0 or rotary_dim % 2:
+        raise ValueError("rotary_dim must be positive and even")
+    if base <= 0 or factor <= 0 or original_length <= 0 or not 0 <= slow_turns < fast_turns:
+        raise ValueError("base, factor and original_length must be positive, "
+                         "and slow_turns below fast_turns")
+    if schedule not in ("linear", "base", "by_turns"):
+        raise ValueError(f"no schedule {schedule!r}")
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    if schedule == "base":
+        if rotary_dim > 2:
+            base = base * factor ** (rotary_dim / (rotary_dim - 2))
+        return base ** (-2.0 * i / rotary_dim), 1.0
+    freq = base ** (-2.0 * i / rotary_dim)
+    if schedule == "linear":
+        return freq / factor, 1.0
+    turns = original_length * freq / (2.0 * np.pi)
+    keep = np.clip((turns - slow_turns) / (fast_turns - slow_turns), 0.0, 1.0)
+    return freq * (keep + (1.0 - keep) / factor), 0.1 * float(np.log(max(factor, 1.0))) + 1.0
+
+
+def _rotary_rows(x, out, name, kind, device, tokens, shape, strides):
+    """The record of an array's rows, (tokens, heads, head_dim)."""
+    found = _dimensions(x, 3, name)
+    if found is None:
+        if shape is None:
+            raise ValueError(f"{name} in a DeviceBuffer needs its heads and head_dim")
+        found = (tokens, *shape)
+        given = strides or (shape[0] * shape[1], shape[1])
+    else:
+        given = x.stride()[:2]
+    if out is None or out is x:
+        out, out_strides = x, given
+    else:
+        out_shape = _dimensions(out, 3, name + "_out")
+        if out_shape is not None and tuple(out_shape) != tuple(found):
+            raise ValueError(f"{name}_out of {tuple(out_shape)}, not {tuple(found)}")
+        out_strides = (out.stride()[:2] if out_shape is not None
+                       else (found[1] * found[2], found[2]))
+    ptr, count = _operand(x, kind, name, device, False)
+    out_ptr, out_count = (ptr, count) if out is x else _operand(out, kind, name + "_out", device,
+                                                                False)
+    return _lib.Fe2o3RotaryRowsV1(ptr, count, out_ptr, out_count, *given, *out_strides, found[1],
+                                  0), found
+
+
+def rotary(q, k, positions, freq, *, q_out=None, k_out=None, interleaved=False, inverse=False,
+           scale=1.0, q_shape=None, k_shape=None, q_strides=None, k_strides=None, stream=None,
+           sync=True) -> None:
+    """Turns the first 2 len(freq) elements of every head of q and k, f32 or bf16 [tokens,
+    heads, head_dim] (k may be None), by positions [tokens] times freq (f64 radians a
+    position, device memory), in place or into q_out and k_out (fe2o3_rotary).
+    inverse turns back, for gradients.  DeviceBuffers take their (heads, head_dim) as
+    q_shape and k_shape and (token, head) strides, dense by default; outputs in
+    DeviceBuffers are dense."""
+    device = _current_device()
+    positions_ptr, tokens = _operand(positions, _INDEX, "positions", device)
+    freq_ptr, pairs = _operand(freq, _DOUBLE, "freq", device)
+    kind = _FLOAT if _FLOAT in _kinds[q.dtype] else _BF16
+    record, shape = _rotary_rows(q, q_out, "q", kind, device, tokens, q_shape, q_strides)
+    rows, other = (shape[0],), None
+    if k is not None:
+        other, k_found = _rotary_rows(k, k_out, "k", kind, device, tokens, k_shape, k_strides)
+        if k_found[2] != shape[2]:
+            raise ValueError(f"head_dim of {shape[2]} in q and {k_found[2]} in k")
+        rows += (k_found[0],)
+        other = C.byref(other)
+    if any(n != tokens for n in rows):
+        raise ValueError(f"{rows} rows and {tokens} positions")
+    _call("fe2o3_rotary", C.byref(record), other, positions_ptr, tokens, freq_ptr, pairs,
+          kind == _BF16, tokens, shape[2], 2 * pairs,
+          ROTARY_INTERLEAVED * bool(interleaved) + ROTARY_INVERSE * bool(inverse), scale,
+          stream=stream, sync=sync)
 
 
 # ---- microscaled 4-bit matrices ----------------------------------------------------------

@@ -456,6 +456,41 @@ int32_t fe2o3_paged_attention_decode(const Fe2o3KvCacheV1 *cache, const uint16_t
                                      uint64_t q_stride, uint32_t window, float scale,
                                      void *stream);
 
+/* ---- rotary positions -----------------------------------------------------------------
+ * Not in the reference.  For token t and each head of Q and of K, the pairs i of the
+ * head's first rotary_dim elements turn by t_i = positions[t] * freq[i] radians:
+ *   (a, b) -> scale (a cos t_i - b sin t_i, b cos t_i + a sin t_i)
+ * pairs (i, i + rotary_dim / 2), or with FE2O3_ROTARY_INTERLEAVED (2 i, 2 i + 1); the
+ * rest of a head is copied.  FE2O3_ROTARY_INVERSE turns by -t_i: the transposed map, for
+ * gradients.  freq: rotary_dim / 2 doubles on the device, any schedule of a stretched
+ * context; angles are taken in 64 bits, products and sums in fp32, rounded once.  A token
+ * at position FE2O3_KV_NO_SLOT (a padded row) is skipped: its outputs keep their bytes.
+ *
+ * Row (t, h) of an array lies at t * token_stride + h * head_stride elements of x, its
+ * result likewise in out; x and out are the same rows (one pointer, the same strides)
+ * or do not overlap.  k may be NULL (q alone).  dtype 0 = f32, 1 = bf16 bits, of all.
+ * Errors in this order: NULL q record FE2O3_ERR_NULL; another dtype or flag, rotary_dim
+ * 0, odd, above head_dim or above 4096, a scale that is not finite, an array of no heads,
+ * heads * (head_dim / 16) of 2^22 or more, or 2^31 tokens FE2O3_ERR_SHAPE; positions_len
+ * or freq_len FE2O3_ERR_LENGTH; strides with which rows share elements FE2O3_ERR_STRIDE
+ * (FE2O3_ERR_OVERFLOW where an extent passes 64 bits); lengths short of the extent
+ * FE2O3_ERR_LENGTH; FE2O3_ERR_NULL; arrays off their elements' alignment
+ * FE2O3_ERR_ALIGNMENT. */
+#define FE2O3_ROTARY_INTERLEAVED 1u
+#define FE2O3_ROTARY_INVERSE 2u
+typedef struct Fe2o3RotaryRowsV1 {
+  const void *x;
+  uint64_t x_len;
+  void *out;
+  uint64_t out_len;
+  uint64_t token_stride, head_stride, out_token_stride, out_head_stride;
+  uint32_t heads, reserved;
+} Fe2o3RotaryRowsV1;
+int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1 *q, const Fe2o3RotaryRowsV1 *k,
+                     const uint32_t *positions, uint64_t positions_len, const double *freq,
+                     uint64_t freq_len, uint32_t dtype, uint32_t tokens, uint32_t head_dim,
+                     uint32_t rotary_dim, uint32_t flags, float scale, void *stream);
+
 /* ---- top-2 MoE ------------------------------------------------------------------------ */
 
 #define FE2O3_DROP_ROUTE 0xffffffffu
