@@ -318,8 +318,7 @@ SIGNATURES = {
         i32, [C.POINTER(Fe2o3KvCacheV1), vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64,
               u32, u32, u32, u32, u64, u32, f32, vp]),
     "fe2o3_rotary": (
-        i32, [C.POINTER(Fe2o3RotaryRowsV1), C.POINTER(Fe2o3RotaryRowsV1), vp, u64, vp, u64, u32,
-              u32, u32, u32, u32, f32, vp]),
+        i32, [vp, vp, vp, u64, vp, u64, u32, u32, u32, u32, u32, f32, vp]),  # two records
     "fe2o3_moe_top2_route_f32_t8_e4_k2_c4_v1": (
         i32, [vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp, u64, vp]),
     "fe2o3_moe_top2_route": (

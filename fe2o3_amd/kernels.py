@@ -22,6 +22,7 @@ until the stream has been synchronized.  The physical argument order is the refe
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import numpy as np
 
@@ -301,6 +302,7 @@ def moe_routing_check(routing: dict, tokens: int, experts: int, capacity: int,
 
 KV_BF16, KV_E4M3, KV_MXFP4 = 0, 1, 4
 KV_NO_SLOT = 0xFFFFFFFF
+MXFP4_BLOCK, MXFP4_PANEL = 32, 256
 PAGED_ATTENTION_MAX_WORKGROUPS = 768
 
 # what an array of each kind may hold: element types of a DeviceBuffer, and of
@@ -326,6 +328,40 @@ class _Kinds(dict):
 
 
 _kinds = _Kinds()
+
+
+class _Is(dict):
+    """element type -> whether it may stand for one kind"""
+
+    def __init__(self, kind):
+        super().__init__()
+        self.kind = kind
+
+    def __missing__(self, dtype):
+        found = self[dtype] = self.kind in _kinds[dtype]
+        return found
+
+
+_is_bf16, _is_codes, _is_index, _is_float, _is_bytes, _is_double = (
+    _Is(kind) for kind in (_BF16, _CODES, _INDEX, _FLOAT, _BYTES, _DOUBLE))
+
+# A call of small arrays takes longer here than on the device, so calls with tensors that
+# are all as they should be go by short ways (the _fast functions), which look at each
+# thing once; these give None, or fail, for everything else (DeviceBuffers, broadcast or
+# wrong operands), and the long way takes it or says what is wrong.
+_NOT_FAST = (AttributeError, TypeError, ValueError, KeyError, IndexError)
+
+
+def _at(x, is_kind, device):
+    """Address of a contiguous tensor of this kind on the device; None of another."""
+    if is_kind[x.dtype] and x.get_device() == device and x.is_contiguous():
+        return x.data_ptr()
+    return None
+
+
+def _fast_count(x, shape, strides):
+    """Elements that a tensor's strides span."""
+    return x.numel() if x.is_contiguous() else _extent(shape, strides, "")
 
 
 def _operand(x, kind, name, device, dense=True):
@@ -411,6 +447,9 @@ def _pair(k, v, dims, kind, device):
     return shape, strides, (k.data_ptr(), count, v.data_ptr(), count)
 
 
+_KV_RECORD = struct.Struct("=11Q6I")  # Fe2o3KvCacheV1
+
+
 class KvCache:
     """A paged key-value cache: K and V rows in slots page * page_size + place: bf16;
     e4m3 codes with f32 scales [pages, kv_heads, page_size]; or microscaled 4-bit
@@ -426,6 +465,14 @@ class KvCache:
     """
 
     def __init__(self, k, v, k_scale=None, v_scale=None, *, shape=None, strides=None):
+        try:
+            record = self._fast(k, v, k_scale, v_scale) if shape is None else None
+        except _NOT_FAST:
+            record = None
+        if record is not None:
+            self.arrays = (k, v, k_scale, v_scale)
+            self.record = _lib.Fe2o3KvCacheV1.from_buffer_copy(record)
+            return
         if (k_scale is None) != (v_scale is None):
             raise ValueError("k_scale and v_scale go together")
         self.device = device = _device_of(k)
@@ -463,6 +510,38 @@ class KvCache:
         self.record = _lib.Fe2o3KvCacheV1(*arrays, *scales, *strides, self.format, pages, page_size,
                                           kv_heads, head_dim, 0)
 
+    def _fast(self, k, v, k_scale, v_scale):
+        shape, found, device = k.shape, k.stride(), k.get_device()
+        if (device < 0 or v.get_device() != device or v.shape != shape or v.stride() != found
+                or (found[3] != 1 and shape[3] != 1)):
+            return None
+        pages, page_size, kv_heads, head_dim = shape
+        count = _fast_count(k, shape, found)
+        ks = vs = scales = 0
+        if k_scale is None:
+            fmt, is_kind = KV_BF16, _is_bf16
+            if v_scale is not None:
+                return None
+        else:
+            want = (pages, kv_heads, page_size)
+            if _is_bytes[k_scale.dtype]:
+                fmt, is_kind, is_scale = KV_MXFP4, _is_bytes, _is_bytes
+                head_dim *= 2
+                want += (head_dim // MXFP4_BLOCK,)
+            else:
+                fmt, is_kind, is_scale = KV_E4M3, _is_codes, _is_float
+            ks, vs = _at(k_scale, is_scale, device), _at(v_scale, is_scale, device)
+            if ks is None or vs is None or k_scale.shape != want or v_scale.shape != want:
+                return None
+            scales = k_scale.numel()
+        if not (is_kind[k.dtype] and is_kind[v.dtype]):
+            return None
+        record = _KV_RECORD.pack(k.data_ptr(), count, v.data_ptr(), count, ks, scales, vs, scales,
+                                 *found[:3], fmt, pages, page_size, kv_heads, head_dim, 0)
+        self.device, self.format = device, fmt
+        self.shape = (pages, page_size, kv_heads, head_dim)
+        return record
+
 
 def _device_of(k):
     if isinstance(k, DeviceBuffer):
@@ -485,7 +564,9 @@ def _on_current_device(cache):
 
 def _current_device():
     current = C.c_int32()
-    check(_lib.lib().fe2o3_rt_get_device(C.byref(current)), "get device")
+    status = _lib.lib().fe2o3_rt_get_device(C.byref(current))
+    if status != 0:
+        check(status, "get device")
     return current.value
 
 
@@ -501,12 +582,38 @@ def _rows(cache, k, v, strides, device):
     return shape[0], found[:2], arrays
 
 
+def _fast_rows(cache, k, v, device):
+    """(tokens, token stride, head stride, address and elements of K and of V) of rows in
+    tensors."""
+    shape, strides = k.shape, k.stride()
+    tokens, kv_heads, head_dim = shape
+    if (kv_heads != cache.shape[2] or head_dim != cache.shape[3] or v.shape != shape
+            or v.stride() != strides or (strides[2] != 1 and head_dim != 1)
+            or k.get_device() != device or v.get_device() != device
+            or not (_is_bf16[k.dtype] and _is_bf16[v.dtype])):
+        return None
+    count = _fast_count(k, shape, strides)
+    return tokens, strides[0], strides[1], k.data_ptr(), count, v.data_ptr(), count
+
+
 def kv_cache_write(cache: KvCache, k, v, slots, *, strides=None, stream=None, sync=True) -> None:
     """Writes rows k, v (bf16 [tokens, kv_heads, head_dim]; DeviceBuffers with
     `strides` (token, head)) into slots[t] of the cache, quantised where it is
     e4m3 or 4-bit.  A slot out of range (KV_NO_SLOT) is skipped; each slot at most once
     a call (fe2o3_kv_cache_write)."""
     device = _on_current_device(cache)
+    rows = None
+    if strides is None:
+        try:
+            rows = _fast_rows(cache, k, v, device)
+            slots_ptr = _at(slots, _is_index, device)
+        except _NOT_FAST:
+            rows = None
+    if rows is not None and slots_ptr is not None and slots.numel() == rows[0]:
+        tokens = rows[0]
+        _call("fe2o3_kv_cache_write", C.byref(cache.record), *rows[3:], slots_ptr, tokens, tokens,
+              rows[1], rows[2], stream=stream, sync=sync)
+        return
     rows, strides, arrays = _rows(cache, k, v, strides, device)
     slots_ptr, tokens = _operand(slots, _INDEX, "slots", device)
     if rows is not None and rows != tokens:
@@ -522,6 +629,21 @@ def kv_cache_read(cache: KvCache, block_table, starts, k, v, *, strides=None, to
     no sequence keep their values (fe2o3_kv_cache_read).  DeviceBuffers take
     `strides` (token, head) and `tokens`."""
     device = _on_current_device(cache)
+    rows = None
+    if strides is None and tokens is None:
+        try:
+            rows = _fast_rows(cache, k, v, device)
+            table_ptr = _at(block_table, _is_index, device)
+            starts_ptr = _at(starts, _is_index, device)
+            (seqs, cols), starts_len = block_table.shape, starts.numel()
+        except _NOT_FAST:
+            rows = None
+    if (rows is not None and table_ptr is not None and starts_ptr is not None
+            and starts_len == seqs + 1):
+        _call("fe2o3_kv_cache_read", C.byref(cache.record), table_ptr, seqs * cols, starts_ptr,
+              starts_len, *rows[3:], seqs, cols, rows[0], rows[1], rows[2], stream=stream,
+              sync=sync)
+        return
     rows, strides, arrays = _rows(cache, k, v, strides, device)
     starts_ptr, starts_len = _operand(starts, _INDEX, "starts", device)
     seqs = starts_len - 1
@@ -542,6 +664,27 @@ def paged_attention_workspace_bytes(q_heads: int, kv_heads: int, head_dim: int) 
     return PAGED_ATTENTION_MAX_WORKGROUPS * 8 * (head_dim + 2) * rows
 
 
+def _fast_decode(cache, q, block_table, lengths, out, lse, workspace, device):
+    """The call's arguments but max_length, window and scale, of tensors; None if they are
+    not as they should be."""
+    shape, strides = q.shape, q.stride()
+    seqs, q_heads, head_dim = shape
+    found_seqs, cols = block_table.shape
+    heads = seqs * q_heads
+    table_at, lengths_at = _at(block_table, _is_index, device), _at(lengths, _is_index, device)
+    out_at, work_at = _at(out, _is_bf16, device), _at(workspace, _is_bytes, device)
+    lse_at = 0 if lse is None else _at(lse, _is_float, device)
+    if (None in (table_at, lengths_at, out_at, work_at, lse_at) or not seqs
+            or found_seqs != seqs or lengths.numel() != seqs or head_dim != cache.shape[3]
+            or (strides[1] != head_dim and q_heads != 1) or (strides[2] != 1 and head_dim != 1)
+            or not _is_bf16[q.dtype] or q.get_device() != device or out.shape != shape
+            or (lse is not None and lse.shape != (seqs, q_heads))):
+        return None
+    return (q.data_ptr(), _fast_count(q, shape, strides), table_at, seqs * cols, lengths_at, seqs,
+            out_at, heads * head_dim, lse_at, 0 if lse is None else heads, work_at,
+            workspace.numel(), seqs, q_heads, cols, strides[0])
+
+
 def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, workspace, *,
                            max_length: int, scale: float, window: int = 0, q_heads=None,
                            q_stride=None, stream=None, sync=True) -> None:
@@ -553,6 +696,15 @@ def paged_attention_decode(cache: KvCache, q, block_table, lengths, out, lse, wo
     overlap.  out and lse may be flat.  DeviceBuffers take q_heads, and q_stride
     between sequences."""
     device = _on_current_device(cache)
+    try:
+        args = (_fast_decode(cache, q, block_table, lengths, out, lse, workspace, device)
+                if q_heads is None and q_stride is None else None)
+    except _NOT_FAST:
+        args = None
+    if args is not None:
+        _call("fe2o3_paged_attention_decode", C.byref(cache.record), *args[:-4], *args[-4:-1],
+              max_length, args[-1], window, scale, stream=stream, sync=sync)
+        return
     head_dim = cache.shape[3]
     lengths_ptr, seqs = _operand(lengths, _INDEX, "lengths", device)
     shape = _dimensions(q, 3, "q")
@@ -643,6 +795,48 @@ def _rotary_rows(x, out, name, kind, device, tokens, shape, strides):
                                   0), found
 
 
+_ROTARY_RECORD = struct.Struct("=8Q2I")  # Fe2o3RotaryRowsV1
+
+
+def _fast_rotary_rows(x, out, is_kind, device):
+    """The packed record of rows in tensors, and their shape."""
+    shape, given = x.shape, x.stride()
+    if not is_kind[x.dtype] or x.get_device() != device or (given[2] != 1 and shape[2] != 1):
+        return None
+    ptr, count = x.data_ptr(), _fast_count(x, shape, given)
+    if out is None:
+        out_ptr, out_count, out_strides = ptr, count, given
+    else:
+        out_strides = out.stride()
+        if (out.shape != shape or not is_kind[out.dtype] or out.get_device() != device
+                or (out_strides[2] != 1 and shape[2] != 1)):
+            return None
+        out_ptr, out_count = out.data_ptr(), _fast_count(out, shape, out_strides)
+    return _ROTARY_RECORD.pack(ptr, count, out_ptr, out_count, given[0], given[1], out_strides[0],
+                               out_strides[1], shape[1], 0), shape
+
+
+def _fast_rotary(q, k, positions, freq, q_out, k_out, device):
+    """The call's arguments before its flags, of tensors."""
+    is_float = _is_float[q.dtype]
+    is_kind = _is_float if is_float else _is_bf16
+    found = _fast_rotary_rows(q, q_out, is_kind, device)
+    other = None if k is None else _fast_rotary_rows(k, k_out, is_kind, device)
+    positions_at, freq_at = _at(positions, _is_index, device), _at(freq, _is_double, device)
+    if found is None or (other is None) != (k is None) or positions_at is None or freq_at is None:
+        return None
+    record, (tokens, _, head_dim) = found
+    pairs = freq.numel()
+    if positions.numel() != tokens:
+        return None
+    if other is not None:
+        other, shape = other
+        if shape[0] != tokens or shape[2] != head_dim:
+            return None
+    return (record, other, positions_at, tokens, freq_at, pairs, 0 if is_float else 1, tokens,
+            head_dim, 2 * pairs)
+
+
 def rotary(q, k, positions, freq, *, q_out=None, k_out=None, interleaved=False, inverse=False,
            scale=1.0, q_shape=None, k_shape=None, q_strides=None, k_strides=None, stream=None,
            sync=True) -> None:
@@ -653,6 +847,14 @@ def rotary(q, k, positions, freq, *, q_out=None, k_out=None, interleaved=False, 
     q_shape and k_shape and (token, head) strides, dense by default; outputs in
     DeviceBuffers are dense."""
     device = _current_device()
+    flags = ROTARY_INTERLEAVED * bool(interleaved) + ROTARY_INVERSE * bool(inverse)
+    try:
+        args = _fast_rotary(q, k, positions, freq, q_out, k_out, device)
+    except _NOT_FAST:
+        args = None
+    if args is not None:
+        _call("fe2o3_rotary", *args, flags, scale, stream=stream, sync=sync)
+        return
     positions_ptr, tokens = _operand(positions, _INDEX, "positions", device)
     freq_ptr, pairs = _operand(freq, _DOUBLE, "freq", device)
     kind = _FLOAT if _FLOAT in _kinds[q.dtype] else _BF16
@@ -667,17 +869,13 @@ def rotary(q, k, positions, freq, *, q_out=None, k_out=None, interleaved=False, 
     if any(n != tokens for n in rows):
         raise ValueError(f"{rows} rows and {tokens} positions")
     _call("fe2o3_rotary", C.byref(record), other, positions_ptr, tokens, freq_ptr, pairs,
-          kind == _BF16, tokens, shape[2], 2 * pairs,
-          ROTARY_INTERLEAVED * bool(interleaved) + ROTARY_INVERSE * bool(inverse), scale,
-          stream=stream, sync=sync)
+          kind == _BF16, tokens, shape[2], 2 * pairs, flags, scale, stream=stream, sync=sync)
 
 
 # ---- microscaled 4-bit matrices ----------------------------------------------------------
 #
 # Arrays are DeviceBuffers or device tensors, on the current device; streams as for the
 # paged cache.
-
-MXFP4_BLOCK, MXFP4_PANEL = 32, 256
 
 
 def mxfp4_shapes(rows: int, cols: int) -> tuple[tuple, tuple]:
@@ -710,12 +908,36 @@ def _dense(x, name, device, rows, cols, stride):
     return _operand(x, kind, name, device, False) + (kind == _BF16, rows, cols, stride)
 
 
+def _fast_packing(x, codes, scales, device):
+    """x, its elements and dtype code, the packed arrays, rows, cols and stride, of tensors."""
+    shape, strides = x.shape, x.stride()
+    rows, cols = shape
+    is_float = _is_float[x.dtype]
+    codes_at, scales_at = _at(codes, _is_bytes, device), _at(scales, _is_bytes, device)
+    panels = (cols + 255) // 256
+    scale_rows = (rows + 15) // 16 * 16
+    if (codes_at is None or scales_at is None or codes.shape != (rows, panels * 128)
+            or scales.shape != (panels, scale_rows, 8) or not (is_float or _is_bf16[x.dtype])
+            or x.get_device() != device or (strides[1] != 1 and cols != 1)):
+        return None
+    return (x.data_ptr(), _fast_count(x, shape, strides), 0 if is_float else 1, codes_at,
+            rows * panels * 128, scales_at, panels * scale_rows * 8, rows, cols, strides[0])
+
+
 def quantize_mxfp4(x, codes, scales, *, rows=None, cols=None, stride=None, stream=None,
                    sync=True) -> None:
     """Packs x, f32 or bf16 [rows, cols] with the last dimension contiguous, into codes and
     scales of mxfp4_shapes(rows, cols) (fe2o3_quantize_mxfp4).  A DeviceBuffer x takes
     rows, cols and the elements between rows."""
     device = _current_device()
+    try:
+        args = (_fast_packing(x, codes, scales, device)
+                if rows is None and cols is None and stride is None else None)
+    except _NOT_FAST:
+        args = None
+    if args is not None:
+        _call("fe2o3_quantize_mxfp4", *args, stream=stream, sync=sync)
+        return
     ptr, count, dtype, rows, cols, stride = _dense(x, "x", device, rows, cols, stride)
     packed = _checked_packed(codes, scales, rows, cols, device)
     _call("fe2o3_quantize_mxfp4", ptr, count, dtype, *packed, rows, cols, stride, stream=stream,
@@ -727,6 +949,14 @@ def dequantize_mxfp4(codes, scales, x, *, rows=None, cols=None, stride=None, str
     """The packed matrix's values into x, f32 or bf16 [rows, cols]
     (fe2o3_dequantize_mxfp4)."""
     device = _current_device()
+    try:
+        args = (_fast_packing(x, codes, scales, device)
+                if rows is None and cols is None and stride is None else None)
+    except _NOT_FAST:
+        args = None
+    if args is not None:
+        _call("fe2o3_dequantize_mxfp4", *args[3:7], *args[:3], *args[7:], stream=stream, sync=sync)
+        return
     ptr, count, dtype, rows, cols, stride = _dense(x, "x", device, rows, cols, stride)
     packed = _checked_packed(codes, scales, rows, cols, device)
     _call("fe2o3_dequantize_mxfp4", *packed, ptr, count, dtype, rows, cols, stride,
@@ -741,11 +971,33 @@ def _checked_packed(codes, scales, rows, cols, device):
     return arrays
 
 
+def _fast_product(a, a_scales, b, b_scales, c, device):
+    """The call's arguments, of tensors."""
+    m, width = a.shape
+    n, other = b.shape
+    panels, a_rows, b_rows = width // 128, (m + 15) // 16 * 16, (n + 15) // 16 * 16
+    a_at, b_at, c_at = _at(a, _is_bytes, device), _at(b, _is_bytes, device), _at(c, _is_bf16, device)
+    as_at, bs_at = _at(a_scales, _is_bytes, device), _at(b_scales, _is_bytes, device)
+    if (a_at is None or b_at is None or c_at is None or as_at is None or bs_at is None
+            or width != other or width % 128 or a_scales.shape != (panels, a_rows, 8)
+            or b_scales.shape != (panels, b_rows, 8) or c.shape != (m, n)):
+        return None
+    return (a_at, m * width, as_at, panels * a_rows * 8, b_at, n * width, bs_at,
+            panels * b_rows * 8, c_at, m * n, m, n, panels * 256)
+
+
 def gemm_mxfp4_nt(a, a_scales, b, b_scales, c, m=None, n=None, k=None, *, stream=None,
                   sync=True) -> None:
     """c (bf16 [m, n]) = A B^T of packed A [m, k] and B [n, k] (fe2o3_gemm_mxfp4_nt).  Sizes
     come from tensors (k in whole panels); DeviceBuffers take m, n, k."""
     device = _current_device()
+    try:
+        args = _fast_product(a, a_scales, b, b_scales, c, device)
+    except _NOT_FAST:
+        args = None
+    if args is not None and m is None and n is None and k is None:
+        _call("fe2o3_gemm_mxfp4_nt", *args, stream=stream, sync=sync)
+        return
     left, (ca, sa) = _packed(a, a_scales, ("a", "a_scales"), device)
     right, (cb, sb) = _packed(b, b_scales, ("b", "b_scales"), device)
     shape = _dimensions(c, 2, "c")
