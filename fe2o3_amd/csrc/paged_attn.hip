@@ -47,6 +47,8 @@
 #include "kv_cache.hpp"
 #include "mxfp4.hpp"
 
+#include <type_traits>
+
 namespace {
 
 using namespace fe2o3;
@@ -56,6 +58,7 @@ using kv_cache::View;
 constexpr uint32_t kBf16 = FE2O3_KV_BF16, kE4m3 = FE2O3_KV_E4M3, kMxfp4 = FE2O3_KV_MXFP4;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;  // of a workgroup, if not said otherwise
 constexpr uint32_t kKeys = 32;              // keys per tile
+constexpr uint32_t kBlockKeys = 128;        // of 4-bit codes, where a wave has one row tile
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
 constexpr uint32_t kWholeTiles = 40;        // of a call without a join
@@ -80,20 +83,22 @@ struct Args {
 struct Span {
   uint32_t first, end, tile0, tiles;
 };
+template <uint32_t KEYS>
 FE2O3_DEVICE Span span_of(const Args& a, uint32_t length) {
   Span s;
   s.end = min(length, a.max_length);
   s.first = a.window != 0u && s.end > a.window ? s.end - a.window : 0u;
-  s.tile0 = s.first / kKeys;
-  s.tiles = max((s.end + kKeys - 1u) / kKeys - s.tile0, 1u);
+  s.tile0 = s.first / KEYS;
+  s.tiles = max((s.end + KEYS - 1u) / KEYS - s.tile0, 1u);
   return s;
 }
 
 // The same of a sequence that the whole wave works on, in scalar registers, so
 // that what follows from it branches as a whole.
 FE2O3_DEVICE uint32_t uniform(uint32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+template <uint32_t KEYS>
 FE2O3_DEVICE Span uniform_span_of(const Args& a, uint32_t seq) {
-  const Span s = span_of(a, a.lengths[seq]);
+  const Span s = span_of<KEYS>(a, a.lengths[seq]);
   return Span{uniform(s.first), uniform(s.end), uniform(s.tile0), uniform(s.tiles)};
 }
 
@@ -177,10 +182,11 @@ constexpr uint32_t waves(int rt) { return kWaves * sharers(rt); }
 // LDS of a workgroup of W waves: their tiles, or two places for tiles that S waves
 // share, which the sums of 16 query rows of each wave take at the end of a run; their
 // tiles' scales; their reference and sum of each query row.
-template <int D, uint32_t F, uint32_t S, uint32_t W>
+template <int D, uint32_t F, uint32_t S, uint32_t W, bool BLOCKS = false>
 struct Lds {
   using T = Tile<D, F == kE4m3 && S == 1 ? kE4m3 : kBf16>;
-  static constexpr uint32_t kTiles = (S == 1 ? 2u : 4u) * T::kBytes;  // of S waves
+  // of S waves; BLOCKS (DecodeBlocks): V rows of 64 D bytes and 8 D of scales
+  static constexpr uint32_t kTiles = BLOCKS ? 72u * D : (S == 1 ? 2u : 4u) * T::kBytes;
   static constexpr uint32_t kSums = S == 1 && kTiles > T::kSumBytes ? kTiles : T::kSumBytes;
   static constexpr uint32_t kOwn = S == 1 ? kSums : kTiles;  // from S waves' to the next
   static constexpr uint32_t kScales = W / S * kOwn > W * kSums ? W / S * kOwn : W * kSums;
@@ -200,7 +206,7 @@ constexpr int per_cu() {
 // D: head_dim.  RW: tiles of 16 query rows of a wave.  S waves, a team, share a tile of
 // keys, or each has its own (1).  WH: KV heads that a workgroup works on at once, of its
 // W waves W / WH on each.
-template <int D, uint32_t F, int RW, uint32_t S, int WH, uint32_t W>
+template <int D, uint32_t F, int RW, uint32_t S, int WH, uint32_t W, bool BLOCKS = false>
 struct Decode {
   // Codes lie in LDS as they are and are widened on the way out, but waves that share
   // a tile would all widen it: they do on the way in, a part each.
@@ -209,7 +215,7 @@ struct Decode {
   static constexpr bool E4M3 = F == kE4m3, kCodes = E4M3 && S == 1;
   using R = Tile<D, F>;                       // as loaded
   using T = Tile<D, kCodes ? kE4m3 : kBf16>;  // in LDS
-  using L = Lds<D, F, S, W>;
+  using L = Lds<D, F, S, W, BLOCKS>;
   static constexpr uint32_t kWiden = T::kRowBytes / R::kRowBytes;  // chunks from one loaded
   static_assert(S == 1 || WH == 1, "waves share a tile of one head");
   static constexpr uint32_t kStep = W / S / WH;  // tiles of a head per round
@@ -660,16 +666,380 @@ struct Decode {
   }
 };
 
+// A 4-bit cache, 16 query heads a KV head at the most.  The codes of 128 keys are the
+// bytes of 32 bf16 keys, so a wave's tile is 128 of them, all in flight, in four subtiles
+// of 32:
+//   * K codes are loaded as the product wants them: lane (l % 16, l / 16) a quarter of a
+//     key's row, widened with its block's scale; the query operand has the same
+//     quarter's d.  Loads of which adjacent lanes take different rows run at a quarter of
+//     the rate, which 4-bit rows leave room for.
+//   * V codes are widened with their scales on the way into LDS, a subtile at a time,
+//     whose registers then take the next tile's.
+//   * With few query heads most lanes of a product hold no query: with at most 16 / C the
+//     scores of C subtiles are moved side by side, C times as many queries to a row of 16
+//     lanes, for the softmax and the probabilities' two bf16 parts, and these moved back
+//     for each subtile's product with V.
+template <int D, int C, int WH, uint32_t W>
+struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
+  using Base = Decode<D, kMxfp4, 1, 1, WH, W, true>;
+  using Base::a;
+  using Base::smem;
+  using Base::wave;
+  static constexpr uint32_t kStep = Base::kStep;
+  static constexpr int kDb = Base::kDb, kFrags = Base::kFrags;
+  static constexpr uint32_t kRowBytes = D / 2, kRowLanes = kRowBytes / 16u;
+  static constexpr uint32_t kRowsPerLoad = 64u / kRowLanes;  // 16 or 32
+  static constexpr int kLoads = kBlockKeys / kRowsPerLoad;   // of K, and of V
+  static constexpr int kSub = 4, kSubLoads = kLoads / kSub;  // subtiles, and their V's loads
+  static constexpr int kSets = kSub / C;                     // softmax registers, 8 each
+  // LDS: V rows of a subtile, K's scales, V's
+  static constexpr uint32_t kVRow = 2u * D;
+  static constexpr uint32_t kScaleAt = kKeys * kVRow, kScaleRow = D / 32u;
+  static constexpr uint32_t kScales = kBlockKeys * kScaleRow;
+  static_assert(kScaleAt + 2u * kScales == 72u * D, "as Lds has it");
+  using ScaleT = std::conditional_t<D == 128, uint32_t, uint16_t>;  // a row's
+  using Quarter = std::conditional_t<D == 128, u32x4_t, u32x2_t>;   // of a row of K
+
+  FE2O3_DEVICE DecodeBlocks(const Args& args, uint8_t* lds) : Base(args, lds) {}
+
+  // V: chunk c of row r lies at c ^ v_swz(r).  The transposing reads take pairs of chunks
+  // of rows 0-3 and 8-11, the writes chunk 4 piece + c of rows 0, 1, 4 and 5 (64 wide:
+  // 0-3 and 8-11).
+  static FE2O3_DEVICE constexpr uint32_t v_swz(uint32_t r) {
+    return D == 128 ? 2u * ((r & 3u) | (r >> 1 & 4u)) | (r >> 2 & 1u)
+                    : 2u * ((r >> 1 & 1u) | (r >> 2 & 2u)) | (r >> 3 & 1u);
+  }
+
+  // v of the lane that is N x `set` on (TO) or back in its row of 16
+  template <int SET>
+  static FE2O3_DEVICE uint32_t beside(uint32_t old, uint32_t v) {  // into set SET
+    constexpr int kShift = 16 / C * SET, kBanks = ((1 << (4 / C)) - 1) << (4 / C * SET);
+    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, 0x110 | kShift, 0xf, kBanks,
+                                                 false);
+  }
+  template <int SET>
+  static FE2O3_DEVICE u32x4_t from_set(u32x4_t v) {
+    if constexpr (SET == 0) {
+      return v;
+    } else {
+      u32x4_t r;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        r[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[i], 0x100 | (16 / C * SET), 0xf,
+                                                     0xf, true);
+      return r;
+    }
+  }
+  // over the lanes of a query in every set
+  static FE2O3_DEVICE float sets_max(float v) {
+    if constexpr (C == 4) v = fmaxf(v, __shfl_xor(v, 4, 64));
+    if constexpr (C > 1) v = fmaxf(v, __shfl_xor(v, 8, 64));
+    return v;
+  }
+  static FE2O3_DEVICE float sets_sum(float v) {
+    if constexpr (C == 4) v += __shfl_xor(v, 4, 64);
+    if constexpr (C > 1) v += __shfl_xor(v, 8, 64);
+    return v;
+  }
+
+  FE2O3_DEVICE void run(uint32_t seq, uint32_t hb0, const Span& sp, uint32_t tile, uint32_t n,
+                        uint32_t slot) {
+    const uint32_t tid = Base::thread(), lane = tid & 63u, lr = lane & 15u, g = lane >> 4;
+    const uint32_t head = WH > 1 ? hb0 + wave / kStep : hb0, rows = a.group;
+    const uint32_t q_head = head * a.group;
+    const uint32_t* table = a.table + (uint64_t)seq * a.table_cols;
+    const uint64_t head_at = head * a.cache.head_stride;
+    const uint32_t pr = lane / kRowLanes, pc = lane % kRowLanes;  // V as loaded: row, piece
+    const uint32_t k_row = 8u * (lr >> 2) + (lr & 3u);            // K, + 32 j + 4 b
+    const uint8_t* kb = a.cache.k + head_at + g * (kRowBytes / 4u);
+    const uint8_t* vb = a.cache.v + head_at + pc * 16u;
+    const ScaleT* kscales = (const ScaleT*)a.cache.k_blocks();
+    const ScaleT* vscales = (const ScaleT*)a.cache.v_blocks();
+
+    const uint32_t end = sp.tile0 + tile + n;
+    uint32_t t = sp.tile0 + tile + wave % kStep;
+    // of the tile whose loads are in flight, lane l's keys l and 64 + l
+    uint32_t page[2];
+    uint64_t valid[2];
+    uint32_t k_scale[2], v_scale[2];
+    // the loads' rows, in 16 bytes from the head's first
+    uint32_t k16[2 * kSub], v16[kLoads];
+    Quarter kx[2 * kSub];  // rows 32 j + 4 b + k_row at 2 j + b
+    u32x4_t vx[kLoads];
+    // the table's entries for tile `at`; none past the run
+    auto entries = [&](uint32_t at) {
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        const uint32_t key = at * kBlockKeys + 64u * h + lane;
+        page[h] = at < end && key >= sp.first && key < sp.end ? table[a.cache.page.div(key)]
+                                                              : 0xffffffffu;
+      }
+    };
+    auto locate = [&](uint32_t at) {
+      uint32_t row16[2];
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        const uint32_t key = at * kBlockKeys + 64u * h + lane;
+        const bool ok = page[h] < a.cache.pages;
+        // a key that is left out reads slot 0, which every cache has, with scales of
+        // 2^-127: its score is -inf all the same, its probability 0 and its V finite
+        const uint32_t p = ok ? page[h] : 0u;
+        const uint32_t place =
+            ok ? key - a.cache.page.div(key) * a.cache.page.divisor : 0u;
+        valid[h] = __ballot(ok);
+        row16[h] = (uint32_t)((p * a.cache.page_stride + place * a.cache.token_stride) >> 4);
+        const uint64_t row = ((uint64_t)p * a.cache.kv_heads + head) * a.cache.page.divisor + place;
+        k_scale[h] = (uint32_t)kscales[row];
+        v_scale[h] = (uint32_t)vscales[row];
+        if (!ok) k_scale[h] = v_scale[h] = 0u;
+      }
+#pragma unroll
+      for (uint32_t i = 0; i < 2u * kSub; ++i)
+        k16[i] = (uint32_t)__shfl((int)row16[i / 4u], (int)(i % 4u * 16u - i % 2u * 12u + k_row), 64);
+#pragma unroll
+      for (uint32_t i = 0; i < (uint32_t)kLoads; ++i)
+        v16[i] = (uint32_t)__shfl((int)row16[i * kRowsPerLoad / 64u],
+                                  (int)(i * kRowsPerLoad % 64u + pr), 64);
+    };
+    auto load_k = [&](uint32_t i) {
+      kx[i] = __builtin_nontemporal_load(
+          reinterpret_cast<const Quarter*>(kb + ((uint64_t)k16[i] << 4)));
+    };
+    auto load_v = [&](uint32_t i) {
+      vx[i] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x4_t*>(vb + ((uint64_t)v16[i] << 4)));
+    };
+
+    entries(t);
+    // the lane's quarter of a row: d D / 4 g + 8 f .. + 7
+    const uint16_t* q = a.q + seq * a.q_stride + (uint64_t)q_head * D +
+                        (lr < rows ? lr : 0u) * D + g * (D / 4u);
+    u32x4_t qf[kFrags];
+    f32x4_t acc[1][kDb];
+    float m_ref[1] = {-__FLT_MAX__}, l_run[1] = {0.0f};
+#pragma unroll
+    for (int f = 0; f < kFrags; ++f) {
+      qf[f] = *reinterpret_cast<const u32x4_t*>(q + 8 * f);
+      if (lr >= rows) qf[f] = u32x4_t{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int db = 0; db < kDb; ++db) acc[0][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    if (t < end) {
+      locate(t);
+      entries(t + kStep);
+#pragma unroll
+      for (uint32_t i = 0; i < 2u * kSub; ++i) load_k(i);
+#pragma unroll
+      for (uint32_t i = 0; i < (uint32_t)kLoads; ++i) load_v(i);
+    }
+
+    uint8_t* own = smem + wave * Base::L::kOwn;
+    const uint32_t v_row = 8u * g + (lr >> 2);
+    // V's row r + 32 j lies a constant further on, and r + 4 also where its swizzle says
+    uint32_t v_put = pr * kVRow + ((4u * pc ^ v_swz(pr)) << 4);
+    uint32_t v_at = v_row * kVRow + ((((lr & 3u) >> 1) ^ v_swz(v_row)) << 4) + (lr & 1u) * 8u;
+    uint32_t ks_at = kScaleAt + k_row * kScaleRow + (D == 128 ? g : g >> 1);
+    uint32_t vs_at = kScaleAt + kScales + pr * kScaleRow + pc;
+
+    for (; t < end; t += kStep) {
+      // other addresses are made from these tile by tile: kept over the loop they would
+      // take the registers of a stage
+      asm volatile("" : "+v"(v_put), "+v"(v_at), "+v"(ks_at), "+v"(vs_at));
+      // the scales to LDS; a wave's LDS operations run in order
+#pragma unroll
+      for (uint32_t h = 0; h < 2u; ++h) {
+        ScaleT* to = reinterpret_cast<ScaleT*>(own + kScaleAt) + 64u * h + lane;
+        to[0] = (ScaleT)k_scale[h];
+        to[kBlockKeys] = (ScaleT)v_scale[h];
+      }
+      asm volatile("" ::: "memory");
+      const uint64_t kept[2] = {valid[0], valid[1]};
+      // behind the run's last tile, slot 0 once more: without a branch but the rescale's,
+      // products, conversions and LDS accesses overlap
+      locate(t + kStep);
+      entries(t + 2u * kStep);
+      // scores: lane's key e (0..7) of subtile j is 32 j + 8 g + e.  Barriers keep the
+      // compiler from reading further ahead than the registers go.
+      float x[kSub][8];
+      uint32_t byte[2 * kSub];
+#pragma unroll
+      for (uint32_t i = 0; i < 2u * kSub; ++i)
+        byte[i] = own[ks_at + (16u * i - 12u * (i % 2u)) * kScaleRow];
+#pragma unroll
+      for (int j = 0; j < kSub; ++j) {
+        f32x4_t s[2] = {};
+#pragma unroll
+        for (int f = 0; f < kFrags; ++f)
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+            s[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                __builtin_bit_cast(bf16x8_t,
+                                   mxfp4::decode8_bf16(kx[2 * j + b][f],
+                                                       mxfp4::scale_float(byte[2 * j + b]))),
+                __builtin_bit_cast(bf16x8_t, qf[f]), s[b], 0, 0, 0);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[j][e] = s[e / 4][e % 4];
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if constexpr (C > 1) {
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            uint32_t y = __float_as_uint(x[s * C][e]);
+            y = beside<1>(y, __float_as_uint(x[s * C + 1][e]));
+            if constexpr (C == 4) {
+              y = beside<2>(y, __float_as_uint(x[s * C + 2][e]));
+              y = beside<3>(y, __float_as_uint(x[s * C + 3][e]));
+            }
+            x[s][e] = __uint_as_float(y);
+          }
+      }
+      if ((kept[0] & kept[1]) != ~UINT64_C(0)) {
+        // set s, subtile C s + lr C / 16 of the lane: its keys' bits
+        const uint32_t words[kSub] = {(uint32_t)kept[0], (uint32_t)(kept[0] >> 32),
+                                      (uint32_t)kept[1], (uint32_t)(kept[1] >> 32)};
+        uint32_t mine = lr, shift = 8u * g;
+        asm volatile("" : "+v"(mine), "+v"(shift));  // no masks kept over the loop
+#pragma unroll
+        for (int s = 0; s < kSets; ++s) {
+          uint32_t word = words[s * C];
+#pragma unroll
+          for (int c = 1; c < C; ++c) word = mine >= 16u / C * c ? words[s * C + c] : word;
+          word >>= shift;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if ((word >> e & 1u) == 0u) x[s][e] = -INFINITY;
+        }
+      }
+      // the next tile's K: its registers are not needed before
+#pragma unroll
+      for (uint32_t i = 0; i < 2u * kSub; ++i) load_k(i);
+      // as Decode's: against a running reference, the same in all sets
+      float p[kSets][8], psum;
+      auto probabilities = [&] {
+        psum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[s][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[s][e], a.scale_log2, -m_ref[0]));
+            psum += p[s][e];
+          }
+        return psum <= kLazyBound;
+      };
+      if (__any(!probabilities())) {
+        float top = x[0][0];
+#pragma unroll
+        for (int s = 0; s < kSets; ++s)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) top = fmaxf(top, x[s][e]);
+        const float m_new = fmaxf(m_ref[0], sets_max(row_max(top * a.scale_log2)));
+        const float alpha = __builtin_amdgcn_exp2f(m_ref[0] - m_new);
+        m_ref[0] = m_new;
+        l_run[0] *= alpha;
+#pragma unroll
+        for (int db = 0; db < kDb; ++db)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[0][db][e] *= alpha;
+        (void)probabilities();
+      }
+      l_run[0] += psum;
+      u32x4_t hi, lo;
+      // V codes of subtile j widened into LDS, its registers to the next tile's
+      auto put_v = [&](auto number) {
+        constexpr int j = decltype(number)::value;
+#pragma unroll
+        for (uint32_t i = 0; i < (uint32_t)kSubLoads; ++i) {
+          const uint32_t r = i * kRowsPerLoad;  // of the subtile, with pr
+          const u32x4_t codes = vx[j * kSubLoads + i];
+          const float scale = mxfp4::scale_float(
+              own[vs_at + (32u * j + r) * kScaleRow]);
+#pragma unroll
+          for (uint32_t c = 0; c < 4u; ++c)
+            *reinterpret_cast<u32x4_t*>(own + (v_put ^ c << 4) + r * kVRow) =
+                mxfp4::decode8_bf16(codes[c], scale);
+          load_v(j * kSubLoads + i);
+        }
+      };
+      auto subtile = [&](auto number) {
+        constexpr int j = decltype(number)::value;
+        if constexpr (j % C == 0) {
+          // two bf16 parts, as Decode's, to the nearest: the write makes no infinite value
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float first = p[j / C][2 * e], second = p[j / C][2 * e + 1];
+            const uint32_t w = pack_bf16x2(first, second);
+            hi[e] = w;
+            lo[e] = pack_bf16x2(first - __uint_as_float(w << 16),
+                                second - __uint_as_float(w & 0xffff0000u));
+          }
+        }
+        const u32x4_t parts[2] = {from_set<j % C>(hi), from_set<j % C>(lo)};
+        // lane i of group g receives d 16 db + i of keys 8 g .. + 7; half of the d at a time
+#pragma unroll
+        for (int d0 = 0; d0 < kDb; d0 += kDb / 2) {
+          bf16x8_t vf[kDb / 2];
+#pragma unroll
+          for (int i = 0; i < kDb / 2; ++i) {
+            bf16x4_t half[2];
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; ++h)
+              half[h] = __builtin_amdgcn_ds_read_tr16_b64_v4bf16(
+                  (lds_bf16x4_t*)(own + (v_at ^ 32u * (d0 + i) ^ v_swz(4u * h) << 4) +
+                                  4u * kVRow * h));
+            vf[i] = __builtin_shufflevector(half[0], half[1], 0, 1, 2, 3, 4, 5, 6, 7);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+          // the next subtile's conversions and writes run beside these products
+          if constexpr (j + 1 < kSub)
+            if (d0 != 0) put_v(std::integral_constant<int, j + 1>{});
+#pragma unroll
+          for (int part = 0; part < 2; ++part)
+#pragma unroll
+            for (int i = 0; i < kDb / 2; ++i)
+              acc[0][d0 + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  vf[i], __builtin_bit_cast(bf16x8_t, parts[part]), acc[0][d0 + i], 0, 0, 0);
+          if (d0 != 0) __builtin_amdgcn_sched_barrier(0);
+        }
+      };
+      __builtin_amdgcn_sched_barrier(0);
+      put_v(std::integral_constant<int, 0>{});
+      __builtin_amdgcn_sched_barrier(0);
+      subtile(std::integral_constant<int, 0>{});
+      subtile(std::integral_constant<int, 1>{});
+      subtile(std::integral_constant<int, 2>{});
+      subtile(std::integral_constant<int, 3>{});
+      asm volatile("" ::: "memory");
+    }
+    l_run[0] = sets_sum(l_run[0]);
+    Base::finish(seq, WH > 1 ? q_head - wave / kStep * a.group : q_head, rows, n == sp.tiles, slot,
+                 acc, m_ref, l_run);
+  }
+};
+
+// How a form works on its tiles: 4-bit codes of one row tile by DecodeBlocks, C subtiles'
+// scores side by side.
+template <uint32_t F, int RT>
+constexpr uint32_t keys_of() {
+  return F == kMxfp4 && RT == 1 ? kBlockKeys : kKeys;
+}
+template <int D, uint32_t F, int RT, uint32_t W>
+using LdsOf = Lds<D, F, sharers(RT), W, F == kMxfp4 && RT == 1>;
+template <int D, uint32_t F, int RT, int C, int WH, uint32_t W>
+using DecodeOf = std::conditional_t<F == kMxfp4 && RT == 1, DecodeBlocks<D, C, WH, W>,
+                                    Decode<D, F, row_tiles(RT), sharers(RT), WH, W>>;
+
 // One workgroup of W waves per sequence and block of query rows, for calls whose
 // sequences are too short to be worth a join.
-template <int D, uint32_t F, int RT, uint32_t W>
+template <int D, uint32_t F, int RT, int C, uint32_t W>
 __global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
-  const Span sp = uniform_span_of(a, seq);
-  Decode<D, F, row_tiles(RT), sharers(RT), 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
+  const Span sp = uniform_span_of<keys_of<F, RT>()>(a, seq);
+  DecodeOf<D, F, RT, C, 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
 }
 
 // The list of all work: sequence, then block of query rows (or WH KV heads), then
@@ -681,7 +1051,7 @@ __global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT>() *
 // four lengths a load, then one scan over the lanes; a place is found among the
 // lanes, then in a chunk.  4096 sequences of 1 to 300 keys, 2 heads: 127 us so, 134
 // by single lengths, 154 with a scan for every 64 sequences.
-template <int RT, int WH>
+template <int RT, int WH, uint32_t KEYS>
 struct Plan {
   static constexpr uint32_t kStep = kWaves / WH, kSetup = RT == 1 ? 1u : 2u;
   const Args& a;
@@ -699,14 +1069,14 @@ struct Plan {
     uint32_t sum = 0;
     if (chunk == 1u) {
       first_length = lane < a.seqs ? a.lengths[lane] : 0u;
-      sum = lane < a.seqs ? rounds(span_of(a, first_length)) : 0u;
+      sum = lane < a.seqs ? rounds(span_of<KEYS>(a, first_length)) : 0u;
     } else {
 #pragma unroll 4
       for (uint32_t i = 0; i < chunk; i += 4u) {
         const uint32_t s = lane * chunk + i, from = min(s, a.seqs - 4u);
         const u32x4_any_t x = *reinterpret_cast<const u32x4_any_t*>(a.lengths + from);
 #pragma unroll
-        for (uint32_t e = 0; e < 4u; ++e) sum += from + e >= s ? rounds(span_of(a, x[e])) : 0u;
+        for (uint32_t e = 0; e < 4u; ++e) sum += from + e >= s ? rounds(span_of<KEYS>(a, x[e])) : 0u;
       }
     }
     chunk_scan = wave_scan(sum);
@@ -716,10 +1086,10 @@ struct Plan {
   // rounds of a block of sequences base .. base + lane, those below limit
   FE2O3_DEVICE uint32_t scan(uint32_t base, uint32_t limit) const {
     const uint32_t s = base + lane;
-    return wave_scan(s < limit ? rounds(span_of(a, a.lengths[s])) : 0u);
+    return wave_scan(s < limit ? rounds(span_of<KEYS>(a, a.lengths[s])) : 0u);
   }
   FE2O3_DEVICE Span span(uint32_t seq) const {
-    return span_of(a, chunk == 1u ? at_lane(first_length, seq) : uniform(a.lengths[seq]));
+    return span_of<KEYS>(a, chunk == 1u ? at_lane(first_length, seq) : uniform(a.lengths[seq]));
   }
   // the sequence that round `at` (below total) falls into, and the rounds of a
   // block before it
@@ -755,10 +1125,10 @@ struct Plan {
   }
 };
 
-template <int D, uint32_t F, int RT, int WH>
+template <int D, uint32_t F, int RT, int C, int WH>
 __global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, F, RT>() * sharers(RT))) paged_split_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
-  using P = Plan<RT, WH>;
+  using P = Plan<RT, WH, keys_of<F, RT>()>;
   const P plan(a);
   uint32_t at = blockIdx.x * plan.run;  // below total + grid: the host keeps it in 32 bits
   const uint32_t end = min(at + plan.run, plan.total);
@@ -769,7 +1139,7 @@ __global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, F, RT>() * sharers(
   Span sp = plan.span(seq);
   uint32_t length = P::rounds(sp);
   uint32_t hb = uniform(rest / length), pos = rest - hb * length;
-  Decode<D, F, row_tiles(RT), sharers(RT), WH, waves(RT)> decode(a, smem);
+  DecodeOf<D, F, RT, C, WH, waves(RT)> decode(a, smem);
   while (true) {
     const uint32_t stop = min(length, pos + (end - at));
     const uint32_t tile = P::kStep * (max(pos, P::kSetup) - P::kSetup);
@@ -796,9 +1166,9 @@ __global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, F, RT>() * sharers(
 // most lie within one (4096 sequences of 1 to 200 keys, 8 heads: 12 us; 213 over
 // the heads, counted 64 by 64).  Bound by latency: the lengths, then the parts (4.6 us after 64
 // sequences, 6 us for the 256 parts of one).
-template <int D, int RT, int WH, int ROWS, int THREADS>
+template <int D, int RT, int WH, uint32_t KEYS, int ROWS, int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_runs) {
-  using P = Plan<RT, WH>;
+  using P = Plan<RT, WH, KEYS>;
   constexpr uint32_t kQuads = D / 4u, kWays = THREADS / (kQuads * ROWS);
   constexpr uint32_t kShared = kWays > 1u ? THREADS / 64u * kQuads * ROWS : 1u;
   __shared__ f32x4_t part_sum[kShared];
@@ -887,11 +1257,12 @@ __global__ void __launch_bounds__(THREADS) paged_join_kernel(Args a, bool by_run
     a.lse[out] = l == 0.0f ? -INFINITY : (m + __log2f(l)) * 0.69314718055994531f;
 }
 
-template <int D, uint32_t F, int RT, int WH>
+template <int D, uint32_t F, int RT, int C, int WH>
 int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
-  constexpr uint32_t kSmem = Lds<D, F, sharers(RT), waves(RT)>::kBytes;
-  using P = Plan<RT, WH>;
-  const auto fn = paged_split_kernel<D, F, RT, WH>;
+  constexpr uint32_t kSmem = LdsOf<D, F, RT, waves(RT)>::kBytes;
+  constexpr uint32_t kTileKeys = keys_of<F, RT>();
+  using P = Plan<RT, WH, kTileKeys>;
+  const auto fn = paged_split_kernel<D, F, RT, C, WH>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   // as many workgroups as are resident at once, and work for each wave
@@ -915,19 +1286,20 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   const bool by_runs = heads > workgroups;
   const uint32_t grid = by_runs ? workgroups : heads;
   if (heads >= workgroups / 8u)
-    paged_join_kernel<D, RT, WH, kRows, kThreads>
+    paged_join_kernel<D, RT, WH, kTileKeys, kRows, kThreads>
         <<<dim3(grid, (rows - 1u) / kRows + 1u), kThreads, 0, s>>>(a, by_runs);
   else if (heads >= workgroups / 64u)
-    paged_join_kernel<D, RT, WH, 1, kThreads><<<dim3(grid, rows), kThreads, 0, s>>>(a, by_runs);
+    paged_join_kernel<D, RT, WH, kTileKeys, 1, kThreads>
+        <<<dim3(grid, rows), kThreads, 0, s>>>(a, by_runs);
   else
-    paged_join_kernel<D, RT, WH, 1, 1024><<<dim3(grid, rows), 1024, 0, s>>>(a, by_runs);
+    paged_join_kernel<D, RT, WH, kTileKeys, 1, 1024><<<dim3(grid, rows), 1024, 0, s>>>(a, by_runs);
   return fe2o3_host::after_launch();
 }
 
-template <int D, uint32_t F, int RT, uint32_t W>
+template <int D, uint32_t F, int RT, int C, uint32_t W>
 int32_t launch_whole(const Args& a, hipStream_t s) {
-  constexpr uint32_t kSmem = Lds<D, F, sharers(RT), W>::kBytes;
-  const auto fn = paged_whole_kernel<D, F, RT, W>;
+  constexpr uint32_t kSmem = LdsOf<D, F, RT, W>::kBytes;
+  const auto fn = paged_whole_kernel<D, F, RT, C, W>;
   static const int32_t lds_rc = fe2o3_host::set_dynamic_lds({(const void*)fn}, (int)kSmem);
   if (lds_rc != FE2O3_OK) return lds_rc;
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head;
@@ -936,8 +1308,15 @@ int32_t launch_whole(const Args& a, hipStream_t s) {
   return fe2o3_host::after_launch();
 }
 
-template <int D, uint32_t F, int RT>
-int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
+// Tiles of the longest span that a call may have.
+uint64_t most_tiles(const Args& a, uint32_t keys) {
+  if (a.window != 0u && a.window < a.max_length) return ((uint64_t)a.window + keys - 1u) / keys + 1u;
+  return ((uint64_t)a.max_length + keys - 1u) / keys;
+}
+
+template <int D, uint32_t F, int RT, int C>
+int32_t launch(const Args& a, uint32_t cus, hipStream_t s) {
+  const uint64_t tiles = most_tiles(a, keys_of<F, RT>());
   const uint64_t heads = (uint64_t)a.seqs * a.cache.kv_heads * a.blocks_per_head;
   // Whether one workgroup a head is enough, without a plan and a join: rounds of
   // tiles on the busiest wave, against an even share of them plus two rounds for
@@ -965,8 +1344,8 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   if (tiles <= kWholeTiles && (rounds_whole > least ? rounds_whole : least) <=
                                   rounds_split + (RT == 1 ? 2u : 4u)) {
     if constexpr (RT == 1)
-      if (wide && tiles > kWaves) return launch_whole<D, F, RT, 8>(a, s);
-    return launch_whole<D, F, RT, waves(RT)>(a, s);
+      if (wide && tiles > kWaves) return launch_whole<D, F, RT, C, 8>(a, s);
+    return launch_whole<D, F, RT, C, waves(RT)>(a, s);
   }
   // Four heads a workgroup read neighbouring rows, but every part that the join adds
   // has the rows of four: worth it where a workgroup has six rounds at least (1 x 130001
@@ -974,44 +1353,55 @@ int32_t launch(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   // group 7: 17.7, 20.0; 1 x 17313 of 4 KV heads, group 16, e4m3: 15.5, 19.4).
   if constexpr (RT == 1)
     if (a.cache.kv_heads % kWaves == 0u && heads / kWaves * tiles >= 6u * resident)
-      return launch_split<D, F, RT, kWaves>(a, tiles, cus, s);
-  return launch_split<D, F, RT, 1>(a, tiles, cus, s);
+      return launch_split<D, F, RT, C, kWaves>(a, tiles, cus, s);
+  return launch_split<D, F, RT, C, 1>(a, tiles, cus, s);
 }
 
 template <int D, uint32_t F>
-int32_t launch_rows(const Args& a, uint64_t tiles, uint32_t cus, hipStream_t s) {
-  if (a.rows <= 16u) return launch<D, F, 1>(a, tiles, cus, s);
-  if (a.rows <= 32u) return launch<D, F, 2>(a, tiles, cus, s);
-  if (a.rows <= 48u) return launch<D, F, 3>(a, tiles, cus, s);
-  return launch<D, F, 4>(a, tiles, cus, s);
+int32_t launch_rows(const Args& a, uint32_t cus, hipStream_t s) {
+  if constexpr (F == kMxfp4) {
+    if (a.rows <= 4u) return launch<D, F, 1, 4>(a, cus, s);
+    if (a.rows <= 8u) return launch<D, F, 1, 2>(a, cus, s);
+  }
+  if (a.rows <= 16u) return launch<D, F, 1, 1>(a, cus, s);
+  if (a.rows <= 32u) return launch<D, F, 2, 1>(a, cus, s);
+  if (a.rows <= 48u) return launch<D, F, 3, 1>(a, cus, s);
+  return launch<D, F, 4, 1>(a, cus, s);
 }
 
 #define FE2O3_KERNEL(NAME, FN, THREADS, LDS) \
   fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", NAME, (const void*)FN, THREADS, LDS})
-#define FE2O3_SPLIT(D, F, RT, WH) \
-  FE2O3_KERNEL("paged_split_kernel<" #D "," #F "," #RT "," #WH ">", (paged_split_kernel<D, F, RT, WH>), waves(RT) * 64u, (Lds<D, F, sharers(RT), waves(RT)>::kBytes))
-#define FE2O3_WHOLE(D, F, RT) \
-  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT ">", (paged_whole_kernel<D, F, RT, waves(RT)>), waves(RT) * 64u, (Lds<D, F, sharers(RT), waves(RT)>::kBytes))
+#define FE2O3_SPLIT(D, F, RT, C, WH) \
+  FE2O3_KERNEL("paged_split_kernel<" #D "," #F "," #RT "," #C "," #WH ">", (paged_split_kernel<D, F, RT, C, WH>), waves(RT) * 64u, (LdsOf<D, F, RT, waves(RT)>::kBytes))
+#define FE2O3_WHOLE(D, F, RT, C, W) \
+  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F "," #RT "," #C "," #W ">", (paged_whole_kernel<D, F, RT, C, W>), (W) * 64u, (LdsOf<D, F, RT, W>::kBytes))
+#define FE2O3_PAGED_ONE(D, F, C)                                                                \
+  FE2O3_SPLIT(D, F, 1, C, 1), FE2O3_SPLIT(D, F, 1, C, 4), FE2O3_WHOLE(D, F, 1, C, 4),           \
+  FE2O3_WHOLE(D, F, 1, C, 8)
 #define FE2O3_PAGED_ALL(D, F)                                                                   \
-  FE2O3_SPLIT(D, F, 1, 1), FE2O3_SPLIT(D, F, 1, 4), FE2O3_SPLIT(D, F, 2, 1),                    \
-  FE2O3_SPLIT(D, F, 3, 1), FE2O3_SPLIT(D, F, 4, 1), FE2O3_WHOLE(D, F, 1),                       \
-  FE2O3_WHOLE(D, F, 2), FE2O3_WHOLE(D, F, 3), FE2O3_WHOLE(D, F, 4),                             \
-  FE2O3_KERNEL("paged_whole_kernel<" #D "," #F ",1,8>", (paged_whole_kernel<D, F, 1, 8>), 512, (Lds<D, F, 1, 8>::kBytes))
-#define FE2O3_JOIN_OF(D, RT, WH, ROWS, THREADS)                                                \
-  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #RT "," #WH "," #ROWS ">", (const void*)paged_join_kernel<D, RT, WH, ROWS, THREADS>, THREADS, 0})
-#define FE2O3_JOIN(D, RT, WH, ROWS) \
-  FE2O3_JOIN_OF(D, RT, WH, ROWS, kThreads), FE2O3_JOIN_OF(D, RT, WH, 1, kThreads), \
-  FE2O3_JOIN_OF(D, RT, WH, 1, 1024)
+  FE2O3_PAGED_ONE(D, F, 1), FE2O3_SPLIT(D, F, 2, 1, 1), FE2O3_SPLIT(D, F, 3, 1, 1),             \
+  FE2O3_SPLIT(D, F, 4, 1, 1), FE2O3_WHOLE(D, F, 2, 1, waves(2)),                                \
+  FE2O3_WHOLE(D, F, 3, 1, waves(3)), FE2O3_WHOLE(D, F, 4, 1, waves(4))
+#define FE2O3_JOIN_OF(D, RT, WH, KEYS, ROWS, THREADS)                                           \
+  fe2o3_host::KernelRegistrar({"fe2o3_paged_attention_decode", "paged_join_kernel<" #D "," #RT "," #WH "," #KEYS "," #ROWS ">", (const void*)paged_join_kernel<D, RT, WH, KEYS, ROWS, THREADS>, THREADS, 0})
+#define FE2O3_JOIN(D, RT, WH, KEYS, ROWS) \
+  FE2O3_JOIN_OF(D, RT, WH, KEYS, ROWS, kThreads), FE2O3_JOIN_OF(D, RT, WH, KEYS, 1, kThreads), \
+  FE2O3_JOIN_OF(D, RT, WH, KEYS, 1, 1024)
 #define FE2O3_JOIN_ALL(D, ROWS) \
-  FE2O3_JOIN(D, 1, 1, ROWS), FE2O3_JOIN(D, 1, 4, ROWS), FE2O3_JOIN(D, 2, 1, ROWS), \
-  FE2O3_JOIN(D, 3, 1, ROWS), FE2O3_JOIN(D, 4, 1, ROWS)
+  FE2O3_JOIN(D, 1, 1, 32, ROWS), FE2O3_JOIN(D, 1, 4, 32, ROWS), FE2O3_JOIN(D, 2, 1, 32, ROWS), \
+  FE2O3_JOIN(D, 3, 1, 32, ROWS), FE2O3_JOIN(D, 4, 1, 32, ROWS), FE2O3_JOIN(D, 1, 1, 128, ROWS), \
+  FE2O3_JOIN(D, 1, 4, 128, ROWS)
 const fe2o3_host::KernelRegistrar kRegistered[] = {
-    FE2O3_PAGED_ALL(64, kBf16),   FE2O3_PAGED_ALL(64, kE4m3),  FE2O3_PAGED_ALL(64, kMxfp4),
-    FE2O3_PAGED_ALL(128, kBf16),  FE2O3_PAGED_ALL(128, kE4m3), FE2O3_PAGED_ALL(128, kMxfp4),
-    FE2O3_JOIN_ALL(64, 16), FE2O3_JOIN_ALL(128, 8)};
+    FE2O3_PAGED_ALL(64, kBf16),       FE2O3_PAGED_ALL(64, kE4m3),
+    FE2O3_PAGED_ALL(64, kMxfp4),      FE2O3_PAGED_ONE(64, kMxfp4, 2),
+    FE2O3_PAGED_ONE(64, kMxfp4, 4),   FE2O3_PAGED_ALL(128, kBf16),
+    FE2O3_PAGED_ALL(128, kE4m3),      FE2O3_PAGED_ALL(128, kMxfp4),
+    FE2O3_PAGED_ONE(128, kMxfp4, 2),  FE2O3_PAGED_ONE(128, kMxfp4, 4),
+    FE2O3_JOIN_ALL(64, 16),           FE2O3_JOIN_ALL(128, 8)};
 #undef FE2O3_KERNEL
 #undef FE2O3_SPLIT
 #undef FE2O3_PAGED_ALL
+#undef FE2O3_PAGED_ONE
 #undef FE2O3_WHOLE
 #undef FE2O3_JOIN
 #undef FE2O3_JOIN_OF
@@ -1090,13 +1480,13 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   hipStream_t s = (hipStream_t)stream;
   switch (cache->format) {
     case kE4m3:
-      return d == 64u ? launch_rows<64, kE4m3>(a, tiles, topo.cus, s)
-                      : launch_rows<128, kE4m3>(a, tiles, topo.cus, s);
+      return d == 64u ? launch_rows<64, kE4m3>(a, topo.cus, s)
+                      : launch_rows<128, kE4m3>(a, topo.cus, s);
     case kMxfp4:
-      return d == 64u ? launch_rows<64, kMxfp4>(a, tiles, topo.cus, s)
-                      : launch_rows<128, kMxfp4>(a, tiles, topo.cus, s);
+      return d == 64u ? launch_rows<64, kMxfp4>(a, topo.cus, s)
+                      : launch_rows<128, kMxfp4>(a, topo.cus, s);
     default:
-      return d == 64u ? launch_rows<64, kBf16>(a, tiles, topo.cus, s)
-                      : launch_rows<128, kBf16>(a, tiles, topo.cus, s);
+      return d == 64u ? launch_rows<64, kBf16>(a, topo.cus, s)
+                      : launch_rows<128, kBf16>(a, topo.cus, s);
   }
 }
