@@ -58,7 +58,7 @@ using kv_cache::View;
 constexpr uint32_t kBf16 = FE2O3_KV_BF16, kE4m3 = FE2O3_KV_E4M3, kMxfp4 = FE2O3_KV_MXFP4;
 constexpr uint32_t kWaves = 4, kThreads = kWaves * 64;  // of a workgroup, if not said otherwise
 constexpr uint32_t kKeys = 32;              // keys per tile
-constexpr uint32_t kBlockKeys = 128;        // of 4-bit codes, where a wave has one row tile
+constexpr uint32_t kBlockKeys = 64;         // of 4-bit codes, where a wave has one row tile
 constexpr float kLazyBound = 256.0f;        // p may reach 2^8 before a rescale
 constexpr uint32_t kMaxWorkgroups = FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS;
 constexpr uint32_t kWholeTiles = 40;        // of a call without a join
@@ -186,7 +186,7 @@ template <int D, uint32_t F, uint32_t S, uint32_t W, bool BLOCKS = false>
 struct Lds {
   using T = Tile<D, F == kE4m3 && S == 1 ? kE4m3 : kBf16>;
   // of S waves; BLOCKS (DecodeBlocks): V rows of 64 D bytes and 8 D of scales
-  static constexpr uint32_t kTiles = BLOCKS ? 72u * D : (S == 1 ? 2u : 4u) * T::kBytes;
+  static constexpr uint32_t kTiles = BLOCKS ? 68u * D : (S == 1 ? 2u : 4u) * T::kBytes;
   static constexpr uint32_t kSums = S == 1 && kTiles > T::kSumBytes ? kTiles : T::kSumBytes;
   static constexpr uint32_t kOwn = S == 1 ? kSums : kTiles;  // from S waves' to the next
   static constexpr uint32_t kScales = W / S * kOwn > W * kSums ? W / S * kOwn : W * kSums;
@@ -197,9 +197,9 @@ struct Lds {
 
 // Workgroups per CU: as many as registers and LDS allow, but two of the widest of one
 // row tile (three of them, e4m3, 64 sequences of 4096 keys: 98.5 -> 105.5 us).
-template <int D, uint32_t F, int RT>
+template <int D, uint32_t F, int RT, int C>
 constexpr int per_cu() {
-  if (RT == 1) return D == 64 ? 3 : 2;
+  if (RT == 1) return D == 64 || (F == kMxfp4 && C == 2) ? 3 : 2;
   return RT == 2 && (D == 64 || F != kBf16) ? 2 : 1;
 }
 
@@ -249,6 +249,12 @@ struct Decode {
     uint32_t t = threadIdx.x;
     asm volatile("" : "+v"(t));
     return t;
+  }
+  // nontemporal, but for 4-bit rows, which share their lines with other heads'
+  static FE2O3_DEVICE u32x4_t load(const uint8_t* p) {
+    const u32x4_t* row = reinterpret_cast<const u32x4_t*>(p);
+    if constexpr (F == kMxfp4) return *row;
+    else return __builtin_nontemporal_load(row);
   }
   FE2O3_DEVICE float* scales(uint32_t w) const {
     return (float*)(smem + L::kScales + w * (2u * kKeys * 4u));
@@ -332,12 +338,11 @@ struct Decode {
       for (uint32_t i = 0; i < R::kLoads; ++i) {
         if constexpr (S == 1) {
           const uint64_t row = shfl64(off, i * R::kRowsPerLoad + pr);
-          st.x[2u * i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(kb + row));
-          st.x[2u * i + 1u] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(vb + row));
+          st.x[2u * i] = load(kb + row);
+          st.x[2u * i + 1u] = load(vb + row);
         } else if (i < kMine && mine(i) < 2u * R::kLoads) {
           const uint64_t row = shfl64(off, mine(i) % R::kLoads * R::kRowsPerLoad + pr);
-          st.x[i] = __builtin_nontemporal_load(
-              reinterpret_cast<const u32x4_t*>((mine(i) < R::kLoads ? kb : vb) + row));
+          st.x[i] = load((mine(i) < R::kLoads ? kb : vb) + row);
         }
       }
     };
@@ -666,19 +671,24 @@ struct Decode {
   }
 };
 
-// A 4-bit cache, 16 query heads a KV head at the most.  The codes of 128 keys are the
-// bytes of 32 bf16 keys, so a wave's tile is 128 of them, all in flight, in four subtiles
-// of 32:
+// A 4-bit cache, 16 query heads a KV head at the most.  A tile is 64 keys, a key a lane
+// where their pages are looked up, in two subtiles of 32:
 //   * K codes are loaded as the product wants them: lane (l % 16, l / 16) a quarter of a
 //     key's row, widened with its block's scale; the query operand has the same
 //     quarter's d.  Loads of which adjacent lanes take different rows run at a quarter of
 //     the rate, which 4-bit rows leave room for.
 //   * V codes are widened with their scales on the way into LDS, a subtile at a time,
 //     whose registers then take the next tile's.
-//   * With few query heads most lanes of a product hold no query: with at most 16 / C the
-//     scores of C subtiles are moved side by side, C times as many queries to a row of 16
-//     lanes, for the softmax and the probabilities' two bf16 parts, and these moved back
-//     for each subtile's product with V.
+//   * With few query heads most lanes of a product hold no query: with at most eight
+//     (C = 2) the scores of both subtiles are moved side by side for the softmax and the
+//     probabilities' two bf16 parts, and these moved back for each product with V.
+//   * A key that is left out reads slot 0, which every cache has, with scales of 2^-127: its
+//     score is set to -inf all the same, its probability is 0 and its V finite.
+// No branch but the rescale's and that of the keys left out, so that products, conversions
+// and LDS accesses overlap.  Loads go by the caches: a head's row is half of a line of 128
+// bytes, whose other half another wave wants (64 sequences of 2 to 8190 keys, 8 heads in
+// token order: 54 us; nontemporal 71, with 1.36 times the bytes).  Three workgroups a CU
+// with tiles of 64 keys; 128 keys, twice the registers and two workgroups: 59 us.
 template <int D, int C, int WH, uint32_t W>
 struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
   using Base = Decode<D, kMxfp4, 1, 1, WH, W, true>;
@@ -690,13 +700,13 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
   static constexpr uint32_t kRowBytes = D / 2, kRowLanes = kRowBytes / 16u;
   static constexpr uint32_t kRowsPerLoad = 64u / kRowLanes;  // 16 or 32
   static constexpr int kLoads = kBlockKeys / kRowsPerLoad;   // of K, and of V
-  static constexpr int kSub = 4, kSubLoads = kLoads / kSub;  // subtiles, and their V's loads
+  static constexpr int kSub = kBlockKeys / 32, kSubLoads = kLoads / kSub;  // subtiles, and their V's loads
   static constexpr int kSets = kSub / C;                     // softmax registers, 8 each
   // LDS: V rows of a subtile, K's scales, V's
   static constexpr uint32_t kVRow = 2u * D;
   static constexpr uint32_t kScaleAt = kKeys * kVRow, kScaleRow = D / 32u;
   static constexpr uint32_t kScales = kBlockKeys * kScaleRow;
-  static_assert(kScaleAt + 2u * kScales == 72u * D, "as Lds has it");
+  static_assert(kScaleAt + 2u * kScales == 68u * D, "as Lds has it");
   using ScaleT = std::conditional_t<D == 128, uint32_t, uint16_t>;  // a row's
   using Quarter = std::conditional_t<D == 128, u32x4_t, u32x2_t>;   // of a row of K
 
@@ -710,37 +720,24 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
                     : 2u * ((r >> 1 & 1u) | (r >> 2 & 2u)) | (r >> 3 & 1u);
   }
 
-  // v of the lane that is N x `set` on (TO) or back in its row of 16
-  template <int SET>
-  static FE2O3_DEVICE uint32_t beside(uint32_t old, uint32_t v) {  // into set SET
-    constexpr int kShift = 16 / C * SET, kBanks = ((1 << (4 / C)) - 1) << (4 / C * SET);
-    return (uint32_t)__builtin_amdgcn_update_dpp((int)old, (int)v, 0x110 | kShift, 0xf, kBanks,
-                                                 false);
+  // C = 2: the upper eight lanes of each row of 16 take v of the lower ones
+  static FE2O3_DEVICE float beside(float low, float v) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+        (int)__float_as_uint(low), (int)__float_as_uint(v), 0x118, 0xf, 0xc, false));  // row_shr:8
   }
-  template <int SET>
-  static FE2O3_DEVICE u32x4_t from_set(u32x4_t v) {
-    if constexpr (SET == 0) {
-      return v;
-    } else {
-      u32x4_t r;
+  // and back: the lower ones take v of the upper
+  static FE2O3_DEVICE u32x4_t from_beside(u32x4_t v) {
+    u32x4_t r;
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        r[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[i], 0x100 | (16 / C * SET), 0xf,
-                                                     0xf, true);
-      return r;
-    }
+    for (int i = 0; i < 4; ++i)  // row_shl:8
+      r[i] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v[i], 0x108, 0xf, 0xf, true);
+    return r;
   }
-  // over the lanes of a query in every set
+  // over the lanes of a query in both subtiles
   static FE2O3_DEVICE float sets_max(float v) {
-    if constexpr (C == 4) v = fmaxf(v, __shfl_xor(v, 4, 64));
-    if constexpr (C > 1) v = fmaxf(v, __shfl_xor(v, 8, 64));
-    return v;
+    return C == 2 ? fmaxf(v, __shfl_xor(v, 8, 64)) : v;
   }
-  static FE2O3_DEVICE float sets_sum(float v) {
-    if constexpr (C == 4) v += __shfl_xor(v, 4, 64);
-    if constexpr (C > 1) v += __shfl_xor(v, 8, 64);
-    return v;
-  }
+  static FE2O3_DEVICE float sets_sum(float v) { return C == 2 ? v + __shfl_xor(v, 8, 64) : v; }
 
   FE2O3_DEVICE void run(uint32_t seq, uint32_t hb0, const Span& sp, uint32_t tile, uint32_t n,
                         uint32_t slot) {
@@ -758,59 +755,48 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
 
     const uint32_t end = sp.tile0 + tile + n;
     uint32_t t = sp.tile0 + tile + wave % kStep;
-    // of the tile whose loads are in flight, lane l's keys l and 64 + l
-    uint32_t page[2];
-    uint64_t valid[2];
-    uint32_t k_scale[2], v_scale[2];
+    // of the tile whose loads are in flight, lane l's key l
+    uint32_t page, place, k_scale, v_scale;
+    uint64_t valid;
     // the loads' rows, in 16 bytes from the head's first
     uint32_t k16[2 * kSub], v16[kLoads];
     Quarter kx[2 * kSub];  // rows 32 j + 4 b + k_row at 2 j + b
     u32x4_t vx[kLoads];
-    // the table's entries for tile `at`; none past the run
-    auto entries = [&](uint32_t at) {
-#pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) {
-        const uint32_t key = at * kBlockKeys + 64u * h + lane;
-        page[h] = at < end && key >= sp.first && key < sp.end ? table[a.cache.page.div(key)]
-                                                              : 0xffffffffu;
-      }
+    // the table's entry for this lane's key of tile `at`; none past the run
+    auto entry = [&](uint32_t at) {
+      const uint32_t key = at * kBlockKeys + lane, col = a.cache.page.div(key);
+      place = key - col * a.cache.page.divisor;
+      page = at < end && key >= sp.first && key < sp.end ? table[col] : 0xffffffffu;
     };
-    auto locate = [&](uint32_t at) {
-      uint32_t row16[2];
-#pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) {
-        const uint32_t key = at * kBlockKeys + 64u * h + lane;
-        const bool ok = page[h] < a.cache.pages;
-        // a key that is left out reads slot 0, which every cache has, with scales of
-        // 2^-127: its score is -inf all the same, its probability 0 and its V finite
-        const uint32_t p = ok ? page[h] : 0u;
-        const uint32_t place =
-            ok ? key - a.cache.page.div(key) * a.cache.page.divisor : 0u;
-        valid[h] = __ballot(ok);
-        row16[h] = (uint32_t)((p * a.cache.page_stride + place * a.cache.token_stride) >> 4);
-        const uint64_t row = ((uint64_t)p * a.cache.kv_heads + head) * a.cache.page.divisor + place;
-        k_scale[h] = (uint32_t)kscales[row];
-        v_scale[h] = (uint32_t)vscales[row];
-        if (!ok) k_scale[h] = v_scale[h] = 0u;
-      }
+    // rows in 32 bits: the host has seen to it
+    const uint32_t page16 = (uint32_t)(a.cache.page_stride >> 4);
+    const uint32_t token16 = (uint32_t)(a.cache.token_stride >> 4);
+    const uint32_t page_rows = a.cache.kv_heads * a.cache.page.divisor;
+    const uint32_t head_rows = head * a.cache.page.divisor;
+    auto locate = [&] {
+      const bool ok = page < a.cache.pages;
+      if (!ok) page = place = 0u;
+      valid = __ballot(ok);
+      const uint32_t row16 = page * page16 + place * token16;
+      const uint32_t row = page * page_rows + head_rows + place;
+      k_scale = (uint32_t)kscales[row];
+      v_scale = (uint32_t)vscales[row];
+      if (!ok) k_scale = v_scale = 0u;
 #pragma unroll
       for (uint32_t i = 0; i < 2u * kSub; ++i)
-        k16[i] = (uint32_t)__shfl((int)row16[i / 4u], (int)(i % 4u * 16u - i % 2u * 12u + k_row), 64);
+        k16[i] = (uint32_t)__shfl((int)row16, (int)(16u * i - 12u * (i % 2u) + k_row), 64);
 #pragma unroll
       for (uint32_t i = 0; i < (uint32_t)kLoads; ++i)
-        v16[i] = (uint32_t)__shfl((int)row16[i * kRowsPerLoad / 64u],
-                                  (int)(i * kRowsPerLoad % 64u + pr), 64);
+        v16[i] = (uint32_t)__shfl((int)row16, (int)(i * kRowsPerLoad + pr), 64);
     };
     auto load_k = [&](uint32_t i) {
-      kx[i] = __builtin_nontemporal_load(
-          reinterpret_cast<const Quarter*>(kb + ((uint64_t)k16[i] << 4)));
+      kx[i] = *reinterpret_cast<const Quarter*>(kb + ((uint64_t)k16[i] << 4));
     };
     auto load_v = [&](uint32_t i) {
-      vx[i] = __builtin_nontemporal_load(
-          reinterpret_cast<const u32x4_t*>(vb + ((uint64_t)v16[i] << 4)));
+      vx[i] = *reinterpret_cast<const u32x4_t*>(vb + ((uint64_t)v16[i] << 4));
     };
 
-    entries(t);
+    entry(t);
     // the lane's quarter of a row: d D / 4 g + 8 f .. + 7
     const uint16_t* q = a.q + seq * a.q_stride + (uint64_t)q_head * D +
                         (lr < rows ? lr : 0u) * D + g * (D / 4u);
@@ -825,8 +811,8 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
 #pragma unroll
     for (int db = 0; db < kDb; ++db) acc[0][db] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     if (t < end) {
-      locate(t);
-      entries(t + kStep);
+      locate();
+      entry(t + kStep);
 #pragma unroll
       for (uint32_t i = 0; i < 2u * kSub; ++i) load_k(i);
 #pragma unroll
@@ -846,18 +832,14 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
       // take the registers of a stage
       asm volatile("" : "+v"(v_put), "+v"(v_at), "+v"(ks_at), "+v"(vs_at));
       // the scales to LDS; a wave's LDS operations run in order
-#pragma unroll
-      for (uint32_t h = 0; h < 2u; ++h) {
-        ScaleT* to = reinterpret_cast<ScaleT*>(own + kScaleAt) + 64u * h + lane;
-        to[0] = (ScaleT)k_scale[h];
-        to[kBlockKeys] = (ScaleT)v_scale[h];
-      }
+      ScaleT* to = reinterpret_cast<ScaleT*>(own + kScaleAt) + lane;
+      to[0] = (ScaleT)k_scale;
+      to[kBlockKeys] = (ScaleT)v_scale;
       asm volatile("" ::: "memory");
-      const uint64_t kept[2] = {valid[0], valid[1]};
-      // behind the run's last tile, slot 0 once more: without a branch but the rescale's,
-      // products, conversions and LDS accesses overlap
-      locate(t + kStep);
-      entries(t + 2u * kStep);
+      const uint64_t kept = valid;
+      // behind the run's last tile, slot 0 once more
+      locate();
+      entry(t + 2u * kStep);
       // scores: lane's key e (0..7) of subtile j is 32 j + 8 g + e.  Barriers keep the
       // compiler from reading further ahead than the registers go.
       float x[kSub][8];
@@ -881,32 +863,18 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
         for (int e = 0; e < 8; ++e) x[j][e] = s[e / 4][e % 4];
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (C > 1) {
+      if constexpr (C == 2) {
 #pragma unroll
-        for (int s = 0; s < kSets; ++s)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            uint32_t y = __float_as_uint(x[s * C][e]);
-            y = beside<1>(y, __float_as_uint(x[s * C + 1][e]));
-            if constexpr (C == 4) {
-              y = beside<2>(y, __float_as_uint(x[s * C + 2][e]));
-              y = beside<3>(y, __float_as_uint(x[s * C + 3][e]));
-            }
-            x[s][e] = __uint_as_float(y);
-          }
+        for (int e = 0; e < 8; ++e) x[0][e] = beside(x[0][e], x[1][e]);
       }
-      if ((kept[0] & kept[1]) != ~UINT64_C(0)) {
-        // set s, subtile C s + lr C / 16 of the lane: its keys' bits
-        const uint32_t words[kSub] = {(uint32_t)kept[0], (uint32_t)(kept[0] >> 32),
-                                      (uint32_t)kept[1], (uint32_t)(kept[1] >> 32)};
+      if (kept != ~UINT64_C(0)) {
         uint32_t mine = lr, shift = 8u * g;
         asm volatile("" : "+v"(mine), "+v"(shift));  // no masks kept over the loop
 #pragma unroll
         for (int s = 0; s < kSets; ++s) {
-          uint32_t word = words[s * C];
-#pragma unroll
-          for (int c = 1; c < C; ++c) word = mine >= 16u / C * c ? words[s * C + c] : word;
-          word >>= shift;
+          // the lane's subtile of set s
+          const uint32_t low = (uint32_t)kept, high = (uint32_t)(kept >> 32);
+          const uint32_t word = (C == 2 ? (mine >= 8u ? high : low) : s == 0 ? low : high) >> shift;
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if ((word >> e & 1u) == 0u) x[s][e] = -INFINITY;
@@ -975,7 +943,8 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
                                 second - __uint_as_float(w & 0xffff0000u));
           }
         }
-        const u32x4_t parts[2] = {from_set<j % C>(hi), from_set<j % C>(lo)};
+        constexpr bool kBeside = j % C != 0;
+        const u32x4_t parts[2] = {kBeside ? from_beside(hi) : hi, kBeside ? from_beside(lo) : lo};
         // lane i of group g receives d 16 db + i of keys 8 g .. + 7; half of the d at a time
 #pragma unroll
         for (int d0 = 0; d0 < kDb; d0 += kDb / 2) {
@@ -1008,8 +977,6 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
       __builtin_amdgcn_sched_barrier(0);
       subtile(std::integral_constant<int, 0>{});
       subtile(std::integral_constant<int, 1>{});
-      subtile(std::integral_constant<int, 2>{});
-      subtile(std::integral_constant<int, 3>{});
       asm volatile("" ::: "memory");
     }
     l_run[0] = sets_sum(l_run[0]);
@@ -1033,7 +1000,7 @@ using DecodeOf = std::conditional_t<F == kMxfp4 && RT == 1, DecodeBlocks<D, C, W
 // One workgroup of W waves per sequence and block of query rows, for calls whose
 // sequences are too short to be worth a join.
 template <int D, uint32_t F, int RT, int C, uint32_t W>
-__global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
+__global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT, C>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
   const uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
@@ -1126,7 +1093,7 @@ struct Plan {
 };
 
 template <int D, uint32_t F, int RT, int C, int WH>
-__global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, F, RT>() * sharers(RT))) paged_split_kernel(Args a) {
+__global__ void __launch_bounds__(waves(RT) * 64, (per_cu<D, F, RT, C>() * sharers(RT))) paged_split_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   using P = Plan<RT, WH, keys_of<F, RT>()>;
   const P plan(a);
@@ -1268,7 +1235,7 @@ int32_t launch_split(Args a, uint64_t tiles, uint32_t cus, hipStream_t s) {
   // as many workgroups as are resident at once, and work for each wave
   const uint32_t heads = a.seqs * a.cache.kv_heads * a.blocks_per_head / WH;
   const uint64_t most = heads * ((tiles + P::kStep - 1u) / P::kStep + P::kSetup);
-  uint32_t workgroups = per_cu<D, F, RT>() * cus;
+  uint32_t workgroups = per_cu<D, F, RT, C>() * cus;
   if (workgroups > kMaxWorkgroups) workgroups = kMaxWorkgroups;
   if (workgroups > most) workgroups = (uint32_t)most;
   a.workgroups = workgroups;
@@ -1335,7 +1302,7 @@ int32_t launch(const Args& a, uint32_t cus, hipStream_t s) {
   // join, and a head its own rounds at least (48 rows, one KV head):
   //   48 x 170 14.0, 9.5    48 x 1000 16.4, 21.9    8 x 500   13.6, 13.1
   //   64 x 500 16.0, 14.2   200 x 500 24.6, 15.9    300 x 500 32.5, 29.0
-  const uint32_t resident = (per_cu<D, F, RT>() == 1 ? 1u : 2u) * cus;
+  const uint32_t resident = (per_cu<D, F, RT, C>() == 1 ? 1u : 2u) * cus;
   const bool wide = RT == 1 && heads <= cus;
   const uint64_t rounds_whole =
       wide ? (tiles + 7u) / 8u : ((tiles + 3u) / 4u * heads + resident - 1u) / resident;
@@ -1360,7 +1327,6 @@ int32_t launch(const Args& a, uint32_t cus, hipStream_t s) {
 template <int D, uint32_t F>
 int32_t launch_rows(const Args& a, uint32_t cus, hipStream_t s) {
   if constexpr (F == kMxfp4) {
-    if (a.rows <= 4u) return launch<D, F, 1, 4>(a, cus, s);
     if (a.rows <= 8u) return launch<D, F, 1, 2>(a, cus, s);
   }
   if (a.rows <= 16u) return launch<D, F, 1, 1>(a, cus, s);
@@ -1389,14 +1355,14 @@ int32_t launch_rows(const Args& a, uint32_t cus, hipStream_t s) {
   FE2O3_JOIN_OF(D, RT, WH, KEYS, 1, 1024)
 #define FE2O3_JOIN_ALL(D, ROWS) \
   FE2O3_JOIN(D, 1, 1, 32, ROWS), FE2O3_JOIN(D, 1, 4, 32, ROWS), FE2O3_JOIN(D, 2, 1, 32, ROWS), \
-  FE2O3_JOIN(D, 3, 1, 32, ROWS), FE2O3_JOIN(D, 4, 1, 32, ROWS), FE2O3_JOIN(D, 1, 1, 128, ROWS), \
-  FE2O3_JOIN(D, 1, 4, 128, ROWS)
+  FE2O3_JOIN(D, 3, 1, 32, ROWS), FE2O3_JOIN(D, 4, 1, 32, ROWS), FE2O3_JOIN(D, 1, 1, 64, ROWS), \
+  FE2O3_JOIN(D, 1, 4, 64, ROWS)
 const fe2o3_host::KernelRegistrar kRegistered[] = {
     FE2O3_PAGED_ALL(64, kBf16),       FE2O3_PAGED_ALL(64, kE4m3),
     FE2O3_PAGED_ALL(64, kMxfp4),      FE2O3_PAGED_ONE(64, kMxfp4, 2),
-    FE2O3_PAGED_ONE(64, kMxfp4, 4),   FE2O3_PAGED_ALL(128, kBf16),
+       FE2O3_PAGED_ALL(128, kBf16),
     FE2O3_PAGED_ALL(128, kE4m3),      FE2O3_PAGED_ALL(128, kMxfp4),
-    FE2O3_PAGED_ONE(128, kMxfp4, 2),  FE2O3_PAGED_ONE(128, kMxfp4, 4),
+    FE2O3_PAGED_ONE(128, kMxfp4, 2),  
     FE2O3_JOIN_ALL(64, 16),           FE2O3_JOIN_ALL(128, 8)};
 #undef FE2O3_KERNEL
 #undef FE2O3_SPLIT
@@ -1477,6 +1443,14 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.max_length = max_length;
   a.window = window;
   a.scale_log2 = scale_log2;
+  // DecodeBlocks has rows in 32 bits, 16 bytes each
+  if (cache->format == kMxfp4) {
+    uint64_t last = 0;
+    if (!kv_cache::reach(a.cache.pages, a.cache.page_stride, &last) ||
+        !kv_cache::reach(cache->page_size, a.cache.token_stride, &last) ||
+        last >= (UINT64_C(1) << 36))
+      return FE2O3_ERR_SHAPE;
+  }
   hipStream_t s = (hipStream_t)stream;
   switch (cache->format) {
     case kE4m3:
