@@ -9,6 +9,8 @@
 #include "kv_cache.hpp"
 #include "mxfp4.hpp"
 
+#include <type_traits>
+
 namespace {
 
 using namespace fe2o3;
@@ -45,16 +47,6 @@ struct Eight<uint16_t> {
     for (uint32_t i = 0; i < 7u; ++i)
       if (i < n) v[i / 2u] |= (uint32_t)p[i] << (16u * (i & 1u));
   }
-  FE2O3_DEVICE void decode(uint32_t q, float scale) { v = mxfp4::decode8_bf16(q, scale); }
-  FE2O3_DEVICE void store(uint16_t* p, uint32_t n) const {
-    if (n >= 8u) {
-      __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any_t*>(p));
-      return;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 7u; ++i)
-      if (i < n) p[i] = (uint16_t)(v[i / 2u] >> (16u * (i & 1u)));
-  }
 };
 template <>
 struct Eight<float> {
@@ -72,19 +64,6 @@ struct Eight<float> {
     }
 #pragma unroll
     for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? p[i] : 0.0f;
-  }
-  FE2O3_DEVICE void decode(uint32_t q, float scale) { mxfp4::decode8_f32(q, scale, v); }
-  FE2O3_DEVICE void store(float* p, uint32_t n) const {
-    if (n >= 8u) {
-      __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]},
-                                  reinterpret_cast<f32x4_any_t*>(p));
-      __builtin_nontemporal_store(f32x4_t{v[4], v[5], v[6], v[7]},
-                                  reinterpret_cast<f32x4_any_t*>(p + 4));
-      return;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 7u; ++i)
-      if (i < n) p[i] = v[i];
   }
 };
 
@@ -126,24 +105,57 @@ __global__ void __launch_bounds__(kThreads) mxfp4_quantize_kernel(Args a) {
   }
 }
 
+// A store covers whole lines: 16 bytes a lane of neighbouring columns, eight of bf16, four of
+// f32 in either half of the panel (eight of f32 a lane, two stores 32 bytes apart: 14336 x
+// 4096 88 us, so 49).
 template <class T, int U>
 __global__ void __launch_bounds__(kThreads) mxfp4_dequantize_kernel(Args a) {
+  constexpr uint32_t kParts = sizeof(T) / 2u, kEach = 8u / kParts;  // stores, columns of one
+  using Codes = std::conditional_t<kParts == 1u, uint32_t, uint16_t>;
   const Place at(a, U * kPass);
-  uint32_t q[U], byte[U];
+  uint32_t q[U][kParts], byte[U][kParts];
 #pragma unroll
   for (uint32_t u = 0; u < (uint32_t)U; ++u) {
     const uint32_t row = min(at.row + u * kPass, a.rows - 1u);
-    q[u] = *reinterpret_cast<const uint32_t*>(
-        a.q + ((uint64_t)row * a.panels.divisor + at.panel) * mxfp4::kRowBytes + 4u * at.lane);
-    byte[u] = a.scales[at.panel * a.scale_panel + (uint64_t)row * 8u + at.lane / 4u];
+    const uint8_t* codes =
+        a.q + ((uint64_t)row * a.panels.divisor + at.panel) * mxfp4::kRowBytes;
+    const uint8_t* scales = a.scales + at.panel * a.scale_panel + (uint64_t)row * 8u;
+#pragma unroll
+    for (uint32_t h = 0; h < kParts; ++h) {
+      const uint32_t first = 128u * h + kEach * at.lane;
+      q[u][h] = *reinterpret_cast<const Codes*>(codes + first / 2u);
+      byte[u][h] = scales[first / mxfp4::kBlock];
+    }
   }
 #pragma unroll
   for (uint32_t u = 0; u < (uint32_t)U; ++u) {
     const uint32_t row = at.row + u * kPass;
     if (row >= a.rows) return;
-    Eight<T> x;
-    x.decode(q[u], mxfp4::scale_float(byte[u]));
-    if (at.left != 0u) x.store((T*)a.out + row * a.stride + at.col, at.left);
+#pragma unroll
+    for (uint32_t h = 0; h < kParts; ++h) {
+      const uint32_t col = at.panel * mxfp4::kPanel + 128u * h + kEach * at.lane;
+      const uint32_t n = col < a.cols ? min(a.cols - col, kEach) : 0u;
+      T* out = (T*)a.out + row * a.stride + col;
+      const float scale = mxfp4::scale_float(byte[u][h]);
+      if constexpr (kParts == 1u) {
+        const u32x4_t v = mxfp4::decode8_bf16(q[u][h], scale);
+        if (n == kEach) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any_t*>(out));
+        else
+#pragma unroll
+          for (uint32_t i = 0; i < kEach - 1u; ++i)
+            if (i < n) out[i] = (T)(v[i / 2u] >> (16u * (i & 1u)));
+      } else {
+        float v[4];
+        mxfp4::decode4_f32(q[u][h], scale, v);
+        if (n == kEach)
+          __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]},
+                                      reinterpret_cast<f32x4_any_t*>(out));
+        else
+#pragma unroll
+          for (uint32_t i = 0; i < kEach - 1u; ++i)
+            if (i < n) out[i] = v[i];
+      }
+    }
   }
 }
 

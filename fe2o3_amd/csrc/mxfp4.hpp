@@ -86,13 +86,14 @@ FE2O3_DEVICE u32x4_t decode8_bf16(uint32_t q, float scale) {
   x[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, scale, 3));
   return x;
 }
-FE2O3_DEVICE void decode8_f32(uint32_t q, float scale, float (&x)[8]) {
+// Of four codes, in f32.
+FE2O3_DEVICE void decode4_f32(uint32_t q, float scale, float (&x)[4]) {
   const fe2o3::f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 0);
   const fe2o3::f32x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 1);
-  const fe2o3::f32x2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 2);
-  const fe2o3::f32x2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(q, scale, 3);
-  x[0] = a[0]; x[1] = a[1]; x[2] = b[0]; x[3] = b[1];
-  x[4] = c[0]; x[5] = c[1]; x[6] = d[0]; x[7] = d[1];
+  x[0] = a[0];
+  x[1] = a[1];
+  x[2] = b[0];
+  x[3] = b[1];
 }
 
 // The largest magnitude's bits of eight values.

@@ -75,7 +75,7 @@ struct Args {
   float* sums;   // and weighted V, [workgroup][2][rows][head_dim]
   uint64_t q_stride;
   uint32_t seqs, q_heads, group, blocks_per_head, rows;  // rows: per block, at most kBlockRows
-  uint32_t table_cols, max_length, window, workgroups;
+  uint32_t table_cols, max_length, window, workgroups, xcds;
   float scale_log2;
 };
 
@@ -1003,7 +1003,15 @@ template <int D, uint32_t F, int RT, int C, uint32_t W>
 __global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT, C>() * sharers(RT) : 2)) paged_whole_kernel(Args a) {
   extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
   const uint32_t blocks = a.cache.kv_heads * a.blocks_per_head;
-  const uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x, seq = id / blocks, hb = id - seq * blocks;
+  uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x;
+  // 4-bit rows of neighbouring heads share their lines: such workgroups on one XCD, which
+  // workgroups are dealt to in turn (64 x 500 keys, 8 heads: 11.0 us, in turn 15.7; 64 x
+  // 2000: 28.8, 45.9)
+  if constexpr (F == kMxfp4) {
+    const uint32_t total = a.seqs * blocks;
+    if (total % a.xcds == 0u) id = id % a.xcds * (total / a.xcds) + id / a.xcds;
+  }
+  const uint32_t seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
   const Span sp = uniform_span_of<keys_of<F, RT>()>(a, seq);
   DecodeOf<D, F, RT, C, 1, W>(a, smem).run(seq, hb, sp, 0u, sp.tiles, 0u);
@@ -1302,6 +1310,11 @@ int32_t launch(const Args& a, uint32_t cus, hipStream_t s) {
   // join, and a head its own rounds at least (48 rows, one KV head):
   //   48 x 170 14.0, 9.5    48 x 1000 16.4, 21.9    8 x 500   13.6, 13.1
   //   64 x 500 16.0, 14.2   200 x 500 24.6, 15.9    300 x 500 32.5, 29.0
+  // 4-bit rows, tiles of 64 keys, in the same rounds (8 KV heads of 128 in token order):
+  //   1 x 500   8.5,  6.5   1 x 2000   8.7, 13.6    4 x 2000  10.2, 13.7
+  //   16 x 2000 17.7, 14.7  64 x 500  18.1, 11.0    64 x 2000 35.3, 28.8
+  //   200 x 500 32.6, 25.5  64 x 1..2000 24.4, 22.6 30 x 1..2000 18.0, 14.6
+  //   8 x 3000  17.0, 18.3  64 x 1..4000 36.3, 38.6 64 x 1000 (64 wide) 16.9, 10.7
   const uint32_t resident = (per_cu<D, F, RT, C>() == 1 ? 1u : 2u) * cus;
   const bool wide = RT == 1 && heads <= cus;
   const uint64_t rounds_whole =
@@ -1317,9 +1330,13 @@ int32_t launch(const Args& a, uint32_t cus, hipStream_t s) {
   // Four heads a workgroup read neighbouring rows, but every part that the join adds
   // has the rows of four: worth it where a workgroup has six rounds at least (1 x 130001
   // 91.8, 88.7 with four; 4 x 16000 49.6, 47.7; 1 x 40000 34.5, 35.4; 8 x 1200..2400,
-  // group 7: 17.7, 20.0; 1 x 17313 of 4 KV heads, group 16, e4m3: 15.5, 19.4).
+  // group 7: 17.7, 20.0; 1 x 17313 of 4 KV heads, group 16, e4m3: 15.5, 19.4).  4-bit rows
+  // of four heads in token order are two lines, which single heads read twice: from two
+  // rounds on (1 x 40000 23.8, 21.8; 4 x 16000 30.9, 24.2; 64 x 2000 50.3, 36.0; but 4 x
+  // 2000 10.3, 11.3; 8 x 1200..2400, group 7: 13.5, 15.2).
   if constexpr (RT == 1)
-    if (a.cache.kv_heads % kWaves == 0u && heads / kWaves * tiles >= 6u * resident)
+    if (a.cache.kv_heads % kWaves == 0u &&
+        heads / kWaves * tiles >= (F == kMxfp4 ? 2u : 6u) * resident)
       return launch_split<D, F, RT, C, kWaves>(a, tiles, cus, s);
   return launch_split<D, F, RT, C, 1>(a, tiles, cus, s);
 }
@@ -1443,6 +1460,7 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.max_length = max_length;
   a.window = window;
   a.scale_log2 = scale_log2;
+  a.xcds = topo.xcds ? topo.xcds : 1u;
   // DecodeBlocks has rows in 32 bits, 16 bytes each
   if (cache->format == kMxfp4) {
     uint64_t last = 0;
