@@ -1437,6 +1437,14 @@ extern "C" int32_t fe2o3_paged_attention_decode(
       (seqs > 1u && q_stride % 8u != 0u) ||
       (((uintptr_t)lse | (uintptr_t)block_table | (uintptr_t)lengths) & 3u) != 0u)
     return FE2O3_ERR_ALIGNMENT;
+  // DecodeBlocks has rows in 32 bits, 16 bytes each
+  if (cache->format == kMxfp4) {
+    uint64_t last = 0;
+    if (!kv_cache::reach(a.cache.pages, a.cache.page_stride, &last) ||
+        !kv_cache::reach(cache->page_size, a.cache.token_stride, &last) ||
+        last >= (UINT64_C(1) << 36))
+      return FE2O3_ERR_SHAPE;
+  }
   if (workspace_bytes < FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES(q_heads, kv_heads, d))
     return FE2O3_ERR_WORKSPACE;
   tile_plan::Topology topo;
@@ -1461,14 +1469,6 @@ extern "C" int32_t fe2o3_paged_attention_decode(
   a.window = window;
   a.scale_log2 = scale_log2;
   a.xcds = topo.xcds ? topo.xcds : 1u;
-  // DecodeBlocks has rows in 32 bits, 16 bytes each
-  if (cache->format == kMxfp4) {
-    uint64_t last = 0;
-    if (!kv_cache::reach(a.cache.pages, a.cache.page_stride, &last) ||
-        !kv_cache::reach(cache->page_size, a.cache.token_stride, &last) ||
-        last >= (UINT64_C(1) << 36))
-      return FE2O3_ERR_SHAPE;
-  }
   hipStream_t s = (hipStream_t)stream;
   switch (cache->format) {
     case kE4m3:

@@ -349,7 +349,7 @@ _is_bf16, _is_codes, _is_index, _is_float, _is_bytes, _is_double = (
 # are all as they should be go by short ways (the _fast functions), which look at each
 # thing once; these give None, or fail, for everything else (DeviceBuffers, broadcast or
 # wrong operands), and the long way takes it or says what is wrong.
-_NOT_FAST = (AttributeError, TypeError, ValueError, KeyError, IndexError)
+_NOT_FAST = (AttributeError, TypeError, ValueError, KeyError, IndexError, struct.error)
 
 
 def _at(x, is_kind, device):

@@ -341,7 +341,8 @@ int32_t fe2o3_flash_attention_fwd(const uint16_t *q, uint64_t q_len,
  * v_scale [pages, kv_heads, page_size, head_dim / 32] (uint8_t arrays, their
  * pointers cast).  k_len, v_len and the strides count bytes of codes, the scale
  * lengths bytes; head_dim is a multiple of 32.  A block with a NaN or an infinity
- * reads back as NaN.
+ * reads back as NaN.  Scale bytes of 253 and 254, which the write never makes, have
+ * infinite values: attention over them may give NaN.
  *
  * The record is checked in this order: NULL record FE2O3_ERR_NULL; another
  * format, a size of 0, slots or head_dim of 2^31 or more, or a head_dim that the
@@ -434,7 +435,8 @@ int32_t fe2o3_kv_cache_read(const Fe2o3KvCacheV1 *cache, const uint32_t *block_t
  * FE2O3_ERR_SHAPE; q_stride below q_heads * head_dim FE2O3_ERR_STRIDE; lengths
  * FE2O3_ERR_LENGTH (q_len covers the extent); NULL FE2O3_ERR_NULL; cache rows,
  * q rows, o or workspace off 16 bytes, the others off 4 FE2O3_ERR_ALIGNMENT;
- * a scale that is not positive, or not finite times log2 e, FE2O3_ERR_SHAPE; a
+ * a scale that is not positive, or not finite times log2 e, FE2O3_ERR_SHAPE; an
+ * MXFP4 cache whose slots span 2^36 bytes or more of one array FE2O3_ERR_SHAPE; a
  * short workspace FE2O3_ERR_WORKSPACE. */
 #define FE2O3_PAGED_ATTENTION_MAX_WORKGROUPS 768u
 /* query rows of one workgroup's sums: of one KV head, or of four at once */

@@ -102,3 +102,17 @@ def test_format_from_the_scales():
     with pytest.raises(TypeError):
         kernels.KvCache(b, b, s(4, 2, 16, 2), s(4, 2, 16, 2))
     assert C.sizeof(c.record) == 112
+
+
+def test_decode_of_a_cache_past_its_span(L):  # noqa: F811
+    """Slots that span 2^36 bytes are past decode attention's row numbers; the write and
+    the read take them."""
+    pages = (1 << 20) + 1
+    row = 64 * 8
+    far = dict(pages=pages, page_size=128, kv_heads=8, head_dim=64, page_stride=128 * row,
+               token_stride=row, head_stride=64, k_len=1 << 40, v_len=1 << 40,
+               k_scale_len=pages * 128 * 8 * 2, v_scale_len=pages * 128 * 8 * 2)
+    assert _decode(L, _cache(**far)) == SHAPE
+    assert _write(L, _cache(**far), k=None, token_stride=1024, head_stride=128,
+                  k_len=1 << 20, v_len=1 << 20) == NULL
+    assert _decode(L, _cache(**dict(far, k=P + 8))) == ALIGNMENT
