@@ -1009,7 +1009,7 @@ __global__ void __launch_bounds__(W * 64, (W == waves(RT) ? per_cu<D, F, RT, C>(
   // 2000: 28.8, 45.9)
   if constexpr (F == kMxfp4) {
     const uint32_t total = a.seqs * blocks;
-    if (total % a.xcds == 0u) id = id % a.xcds * (total / a.xcds) + id / a.xcds;
+    if (total % a.xcds == 0u && id < total) id = id % a.xcds * (total / a.xcds) + id / a.xcds;
   }
   const uint32_t seq = id / blocks, hb = id - seq * blocks;
   if (seq >= a.seqs) return;  // the last row of a grid of two dimensions
@@ -1377,9 +1377,9 @@ int32_t launch_rows(const Args& a, uint32_t cus, hipStream_t s) {
 const fe2o3_host::KernelRegistrar kRegistered[] = {
     FE2O3_PAGED_ALL(64, kBf16),       FE2O3_PAGED_ALL(64, kE4m3),
     FE2O3_PAGED_ALL(64, kMxfp4),      FE2O3_PAGED_ONE(64, kMxfp4, 2),
-       FE2O3_PAGED_ALL(128, kBf16),
+    FE2O3_PAGED_ALL(128, kBf16),
     FE2O3_PAGED_ALL(128, kE4m3),      FE2O3_PAGED_ALL(128, kMxfp4),
-    FE2O3_PAGED_ONE(128, kMxfp4, 2),  
+    FE2O3_PAGED_ONE(128, kMxfp4, 2),
     FE2O3_JOIN_ALL(64, 16),           FE2O3_JOIN_ALL(128, 8)};
 #undef FE2O3_KERNEL
 #undef FE2O3_SPLIT
@@ -1437,12 +1437,14 @@ extern "C" int32_t fe2o3_paged_attention_decode(
       (seqs > 1u && q_stride % 8u != 0u) ||
       (((uintptr_t)lse | (uintptr_t)block_table | (uintptr_t)lengths) & 3u) != 0u)
     return FE2O3_ERR_ALIGNMENT;
-  // DecodeBlocks has rows in 32 bits, 16 bytes each
+  // DecodeBlocks has rows' numbers, and their places in 16 bytes, in 32 bits
   if (cache->format == kMxfp4) {
-    uint64_t last = 0;
+    uint64_t last = 0, n;
     if (!kv_cache::reach(a.cache.pages, a.cache.page_stride, &last) ||
         !kv_cache::reach(cache->page_size, a.cache.token_stride, &last) ||
-        last >= (UINT64_C(1) << 36))
+        last >= (UINT64_C(1) << 36) ||
+        !kv_cache::mul_ok((uint64_t)cache->pages * cache->page_size, kv_heads, &n) ||
+        n >= (UINT64_C(1) << 32))
       return FE2O3_ERR_SHAPE;
   }
   if (workspace_bytes < FE2O3_PAGED_ATTENTION_WORKSPACE_BYTES(q_heads, kv_heads, d))

@@ -7,8 +7,8 @@
 // with the same m it is the transposed map, which takes a gradient back.
 //
 // An angle reaches 10^6 radians, where 32 bits are off by 0.06, so it is taken in turns:
-// position * (freq / 2 pi) in 64 bits, less its nearest whole number, is exact to 2^-30
-// of a turn at the largest position; sine and cosine of what is left are f32.
+// position * (freq / 2 pi) in 64 bits, less its nearest whole number, is off by 2^-52 of
+// the turns (2^-34 of one at 10^6 radians); sine and cosine of what is left are f32.
 //
 // Bound by memory: x is read once and written once.  A workgroup takes a few tokens, each
 // pair's sine and cosine is computed once for all heads and kept in LDS, and a lane turns

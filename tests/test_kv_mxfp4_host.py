@@ -116,3 +116,13 @@ def test_decode_of_a_cache_past_its_span(L):  # noqa: F811
     assert _write(L, _cache(**far), k=None, token_stride=1024, head_stride=128,
                   k_len=1 << 20, v_len=1 << 20) == NULL
     assert _decode(L, _cache(**dict(far, k=P + 8))) == ALIGNMENT
+
+
+def test_decode_of_a_cache_of_too_many_rows(L):  # noqa: F811
+    """One page, the heads outermost: slots span little, and there are 2^32 rows."""
+    slots, heads = 1 << 30, 4
+    many = dict(pages=1, page_size=slots, kv_heads=heads, head_dim=64, token_stride=32,
+                head_stride=32 * slots, page_stride=0, k_len=1 << 40, v_len=1 << 40,
+                k_scale_len=slots * heads * 2, v_scale_len=slots * heads * 2)
+    assert _decode(L, _cache(**many)) == SHAPE
+    assert _decode(L, _cache(**dict(many, k=P + 8))) == ALIGNMENT
