@@ -12,6 +12,12 @@
 // MFMA.  What is added is the scales: a stage's are 8 bytes a row, contiguous for the
 // tile's rows (2 KiB for 256), copied behind the stage's codes.  A lane reads a row's
 // eight with one ds_read_b64 and keeps its block's of both substeps in one register.
+//
+// Measured: 8192 x 8192 x 8192 221 us = 4.98 PFLOP/s.  The instruction alone, from registers,
+// sustains 7.1 on codes of normal values, where power limits it (9.6 on zeros, on which this
+// kernel reaches 6.5); the loop keeps the matrix core busy for three quarters of its cycles.
+// 16 x 14336 x 4096 9.0 us with the weights from memory (3.5 TB/s), 5.6 from the caches;
+// 4096 x 4096 x 4096 37.6.
 #include "common.hpp"
 #include "gemm_core.hpp"
 #include "gemm_direct.hpp"
@@ -42,8 +48,18 @@ struct ScaleRows {
   uint32_t bytes;
 };
 
+// Stage t of a tile: where the codes of its rows begin, and the scales that this wave copies.
+struct From {
+  const uint8_t *a, *b, *scales;
+  uint32_t t;
+  FE2O3_DEVICE From stage(uint32_t to) const {
+    return From{a, b, scales, (uint32_t)__builtin_amdgcn_readfirstlane(to)};
+  }
+};
+
 // A tile of 32 RB rows of A by 32 CB rows of B: four waves, 2 x 2, of RB x CB MFMA tiles.
-template <int RB, int CB, int STAGES>
+// EVEN: no row is clamped, so that a wave's copies lie 32 rows apart.
+template <int RB, int CB, int STAGES, bool EVEN = false>
 struct Tile {
   static constexpr int kMfma = RB * CB;  // per substep of 128 k
   static constexpr int kARows = 32 * RB, kBRows = 32 * CB;
@@ -93,30 +109,37 @@ struct Tile {
     ln.pick = 0x0c0c0400u + g * 0x0101u;  // bytes g and 4 + g, zeros above
   }
 
-  FE2O3_DEVICE uint32_t stage(uint32_t t) const {  // clamped to the last
-    return __builtin_amdgcn_readfirstlane(t < steps ? t : steps - 1u);
+  FE2O3_DEVICE From tile() const {  // the one that the rows were made for
+    return From{(const uint8_t*)ar.base[0], (const uint8_t*)br.base[0], own.base, 0u};
+  }
+  FE2O3_DEVICE From at(const From& from, uint32_t t) const {  // clamped to the last
+    return from.stage(t < steps ? t : steps - 1u);
   }
 
-  // copy C of stage t into buffer buf: B's codes, the scales, then A's codes
+  template <int J>
+  FE2O3_DEVICE uint32_t at_row(const From& from) const {
+    return from.t * (uint32_t)kRow + (EVEN ? J * 32u * kRow * steps : 0u);
+  }
+  // copy C of a stage into buffer buf: B's codes, the scales, then A's codes
   template <int C>
-  FE2O3_DEVICE void copy(uint32_t t, int buf) const {
+  FE2O3_DEVICE void copy(const From& from, int buf) const {
     if constexpr (C < NB) {
-      gemm_pipe::b2l_b128(gemm_pipe::rsrc(br.base[C], br.bytes),
-                          smem + L::b_region + L::b(buf) + (4u * C + wave) * 1024u, br.voff[C],
-                          t * (uint32_t)kRow);
+      gemm_pipe::b2l_b128(gemm_pipe::rsrc(from.b, br.bytes),
+                          smem + L::b_region + L::b(buf) + (4u * C + wave) * 1024u,
+                          br.voff[EVEN ? 0 : C], at_row<C>(from));
     } else if constexpr (C == NB) {
       // a quarter of the tile's scales, 16 bytes a lane
       constexpr uint32_t kPart = kScaleTile / 4u;
       const uint32_t lane = threadIdx.x & 63u;
       if (kPart == 1024u || lane < kPart / 16u)
-        gemm_pipe::b2l_b128(gemm_pipe::rsrc(own.base + t * own.step, own.bytes),
+        gemm_pipe::b2l_b128(gemm_pipe::rsrc(from.scales + from.t * own.step, own.bytes),
                             smem + kScaleRegion + buf * kScaleTile + wave * kPart,
                             (wave & 1u) * kPart + lane * 16u, 0u);
     } else {
       constexpr int j = C - NB - 1;
-      gemm_pipe::b2l_b128(gemm_pipe::rsrc(ar.base[j], ar.bytes),
-                          smem + L::a(buf) + (4u * j + wave) * 1024u, ar.voff[j],
-                          t * (uint32_t)kRow);
+      gemm_pipe::b2l_b128(gemm_pipe::rsrc(from.a, ar.bytes),
+                          smem + L::a(buf) + (4u * j + wave) * 1024u, ar.voff[EVEN ? 0 : j],
+                          at_row<j>(from));
     }
   }
 
@@ -151,10 +174,14 @@ struct Tile {
   // for its reason.  What the compiler then does not provide: the accumulators are
   // zeroed before the first copies are waited for, scale registers are written at least
   // two MFMAs before their first use, and finish() waits before the epilogue reads.
-  template <int S, int I>
+  template <int S, int I, bool ZERO>
   static FE2O3_DEVICE void mfma(Acc& acc, const Frags& f, const Scales& s) {
     constexpr int i = I / CB, j = I % CB;
-    if constexpr (S == 0)
+    if constexpr (ZERO && S == 0)  // a sum's first
+      asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, 0, %3, %4 "
+                   "op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
+                   : "=a"(acc.v[i][j]) : "v"(f.b[j]), "v"(f.a[i]), "v"(s.b[j]), "v"(s.a[i]));
+    else if constexpr (S == 0)
       asm volatile("v_mfma_scale_f32_16x16x128_f8f6f4 %0, %1, %2, %0, %3, %4 "
                    "op_sel:[0,0,0] op_sel_hi:[0,0,0] cbsz:4 blgp:4"
                    : "+a"(acc.v[i][j]) : "v"(f.b[j]), "v"(f.a[i]), "v"(s.b[j]), "v"(s.a[i]));
@@ -177,17 +204,23 @@ struct Tile {
   static constexpr int kEarly = NB + 1, kLate = NA;
   static constexpr int kBarrier = kMfma / 2;
   static constexpr int kPickFrom = kBarrier + kMfma / 8;
-  template <int P, int S, int I = 0>
-  FE2O3_DEVICE void slots(uint32_t next, uint32_t next2, Frags (&f)[2], const Scales& now,
+  // KIND, of tiles one after another (run_all): a tile's first step finds stage 1 copied
+  // before the last tile's stores, which it does not wait for, and starts the sums; its last
+  // step copies all of the next tile's stage 1.
+  static constexpr int kFirst = 1, kLast = 2;
+  static constexpr int kStores = RB * CB / 2;  // at least, of a wave's outputs, 16 bytes a lane
+  template <int P, int S, int KIND, int I = 0>
+  FE2O3_DEVICE void slots(const From& next, const From& next2, Frags (&f)[2], const Scales& now,
                           Scales& then, u32x2_t (&raw)[kReads], Acc& acc) const {
     if constexpr (I < kMfma) {
       if constexpr (S == 1 && I == kBarrier) {
-        __builtin_amdgcn_s_waitcnt(gemm_pipe::waitcnt_imm((STAGES - 2) * NC, 0));
+        __builtin_amdgcn_s_waitcnt(
+            gemm_pipe::waitcnt_imm((KIND & kFirst) != 0 ? kStores : (STAGES - 2) * NC, 0));
         __builtin_amdgcn_s_barrier();
       }
-      mfma<S, I>(acc, f[S], now);
+      mfma<S, I, (KIND & kFirst) != 0>(acc, f[S], now);
       if constexpr (S == 1) {
-        Spread<kEarly, kBarrier, kMfma>::template at<I>(
+        Spread<(KIND & kLast) != 0 ? NC : kEarly, kBarrier, kMfma>::template at<I>(
             [&](auto n) { copy<decltype(n)::value>(next2, P); });
         Spread<kReads, kBarrier, kMfma>::template at<I>([&](auto n) {
           constexpr int PN = (P + 1) % STAGES;
@@ -197,50 +230,57 @@ struct Tile {
         Spread<kReads, kPickFrom, kMfma>::template at<I>(
             [&](auto n) { pick_scale<decltype(n)::value>(raw, then); });
       } else {
-        Spread<kLate, 0, kMfma>::template at<I>([&](auto n) {
-          copy<kEarly + decltype(n)::value>(next, (P + STAGES - 1) % STAGES);
-        });
+        if constexpr ((KIND & kFirst) == 0)
+          Spread<kLate, 0, kMfma>::template at<I>([&](auto n) {
+            copy<kEarly + decltype(n)::value>(next, (P + STAGES - 1) % STAGES);
+          });
         Spread<kReads, kMfma / 8, kMfma - kMfma / 8>::template at<I>(
             [&](auto n) { read<P, 1, decltype(n)::value>(f[1]); });
       }
       __builtin_amdgcn_sched_barrier(0);
-      slots<P, S, I + 1>(next, next2, f, now, then, raw, acc);
+      slots<P, S, KIND, I + 1>(next, next2, f, now, then, raw, acc);
     }
   }
   // Steps t .. of a round, U of kRound: buffers and the two sets of scale registers
   // alternate by U, so that no register is copied.
   static constexpr int kRound = STAGES % 2 == 0 ? STAGES : 2 * STAGES;
   template <int U, bool TAIL>
-  FE2O3_DEVICE void step(uint32_t t, Frags (&f)[2], Scales (&s)[2], Acc& acc) const {
+  FE2O3_DEVICE void step(const From& from, uint32_t t, Frags (&f)[2], Scales (&s)[2],
+                         Acc& acc) const {
     if (TAIL && t >= steps) return;
-    const uint32_t next = stage(t + STAGES - 1), next2 = stage(t + STAGES);
+    const From next = at(from, t + STAGES - 1), next2 = at(from, t + STAGES);
     u32x2_t raw[kReads];
     __builtin_amdgcn_sched_barrier(0);
-    slots<U % STAGES, 0>(next, next2, f, s[U & 1], s[~U & 1], raw, acc);
-    slots<U % STAGES, 1>(next, next2, f, s[U & 1], s[~U & 1], raw, acc);
-    if constexpr (U + 1 < kRound) step<U + 1, TAIL>(t + 1u, f, s, acc);
+    slots<U % STAGES, 0, 0>(next, next2, f, s[U & 1], s[~U & 1], raw, acc);
+    slots<U % STAGES, 1, 0>(next, next2, f, s[U & 1], s[~U & 1], raw, acc);
+    if constexpr (U + 1 < kRound) step<U + 1, TAIL>(from, t + 1u, f, s, acc);
+  }
+  // Steps t and t + 1 of a tile with two stages, `then` being the next one (or it).
+  template <int KIND>
+  FE2O3_DEVICE void pair(const From& from, const From& then, uint32_t t, Frags (&f)[2],
+                         Scales (&s)[2], Acc& acc) const {
+    static_assert(STAGES == 2, "a buffer a step");
+    constexpr bool kEnd = (KIND & kLast) != 0;
+    const From one = from.stage(t + 1u);
+    const From two = kEnd ? then.stage(0u) : from.stage(t + 2u);
+    const From three = kEnd ? then.stage(1u) : from.stage(t + 3u);
+    u32x2_t raw[kReads];
+    __builtin_amdgcn_sched_barrier(0);
+    slots<0, 0, KIND & kFirst>(one, two, f, s[0], s[1], raw, acc);
+    slots<0, 1, KIND & kFirst>(one, two, f, s[0], s[1], raw, acc);
+    slots<1, 0, KIND & kLast>(two, three, f, s[1], s[0], raw, acc);
+    slots<1, 1, KIND & kLast>(two, three, f, s[1], s[0], raw, acc);
   }
   template <int C, int END>
-  FE2O3_DEVICE void copies(uint32_t t, int buf) const {
+  FE2O3_DEVICE void copies(const From& from, int buf) const {
     if constexpr (C < END) {
-      copy<C>(t, buf);
-      copies<C + 1, END>(t, buf);
+      copy<C>(from, buf);
+      copies<C + 1, END>(from, buf);
     }
   }
 
-  FE2O3_DEVICE void run(Acc& acc) const {
-#pragma unroll
-    for (int i = 0; i < RB; ++i)
-#pragma unroll
-      for (int j = 0; j < CB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    pin(acc);
-#pragma unroll
-    for (int st = 0; st + 1 < STAGES; ++st) copies<0, NC>(stage(st), st);
-    copies<0, kEarly>(stage(STAGES - 1), STAGES - 1);
-    __builtin_amdgcn_s_waitcnt(gemm_pipe::waitcnt_imm((STAGES - 2) * NC + kEarly, 0));
-    __builtin_amdgcn_s_barrier();
-    Frags f[2];
-    Scales s[2];
+  // step 0's fragments and scales; the copies of stage 0 have landed
+  FE2O3_DEVICE void read_first(Frags (&f)[2], Scales (&s)[2]) const {
     u32x2_t raw[kReads];
     Spread<kReads, 0, 1>::template at<0>([&](auto n) { read_scale<0, decltype(n)::value>(raw); });
     Spread<kReads, 0, 1>::template at<0>([&](auto n) { pick_scale<decltype(n)::value>(raw, s[0]); });
@@ -249,16 +289,69 @@ struct Tile {
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
-    uint32_t t = 0;
-    for (; t + kRound <= steps; t += kRound) step<0, false>(t, f, s, acc);
-    if (t < steps) step<0, true>(t, f, s, acc);
+  }
+  // the last MFMA's result is written before the epilogue reads it
+  FE2O3_DEVICE void finish(Acc& acc) const {
     __builtin_amdgcn_sched_barrier(0);
-    // copies past the last stage land before the workgroup's LDS is another's; the last
-    // MFMA's result is written before the epilogue reads it
-    __builtin_amdgcn_s_waitcnt(gemm_pipe::kWaitVm0Lgkm0);
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
     pin(acc);
     __builtin_amdgcn_sched_barrier(0);
+  }
+
+  FE2O3_DEVICE void run(Acc& acc) const {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < CB; ++j) acc.v[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    pin(acc);
+    const From from = tile();
+#pragma unroll
+    for (int st = 0; st + 1 < STAGES; ++st) copies<0, NC>(at(from, st), st);
+    copies<0, kEarly>(at(from, STAGES - 1), STAGES - 1);
+    __builtin_amdgcn_s_waitcnt(gemm_pipe::waitcnt_imm((STAGES - 2) * NC + kEarly, 0));
+    __builtin_amdgcn_s_barrier();
+    Frags f[2];
+    Scales s[2];
+    read_first(f, s);
+    uint32_t t = 0;
+    for (; t + kRound <= steps; t += kRound) step<0, false>(from, t, f, s, acc);
+    if (t < steps) step<0, true>(from, t, f, s, acc);
+    __builtin_amdgcn_sched_barrier(0);
+    // copies past the last stage land before the workgroup's LDS is another's
+    __builtin_amdgcn_s_waitcnt(gemm_pipe::kWaitVm0Lgkm0);
+    finish(acc);
+  }
+  // Tiles one after another, of an even number of steps each: a tile's last steps copy the
+  // first two stages of the next, which is under way while the sums are stored.
+  // next(&from): whether there is one; store(acc): a tile's sums, kStores stores at least.
+  template <class Next, class Store>
+  FE2O3_DEVICE void run_all(From from, Next next, Store store) const {
+    copies<0, NC>(from.stage(0u), 0);
+    copies<0, NC>(from.stage(1u), 1);
+    // all of both: the first step counts on stores behind them, of which there are none yet
+    __builtin_amdgcn_s_waitcnt(gemm_pipe::kWaitVm0Lgkm0);
+    __builtin_amdgcn_s_barrier();
+    Frags f[2];
+    Scales s[2];
+    read_first(f, s);
+    while (true) {
+      From then = from;
+      const bool more = next(&then);
+      Acc acc;
+      if (steps == 2u) {
+        pair<kFirst | kLast>(from, then, 0u, f, s, acc);
+      } else {
+        pair<kFirst>(from, then, 0u, f, s, acc);
+        for (uint32_t t = 2u; t + 2u < steps; t += 2u) pair<0>(from, then, t, f, s, acc);
+        pair<kLast>(from, then, steps - 2u, f, s, acc);
+      }
+      finish(acc);
+      store(acc);
+      if (!more) break;
+      from = then;
+    }
+    // copies of the tile that `then` was at the end
+    __builtin_amdgcn_s_waitcnt(gemm_pipe::kWaitVm0Lgkm0);
   }
 };
 
@@ -307,6 +400,55 @@ __global__ void __launch_bounds__(256, 1) gemm_mxfp4_kernel(Operand a, Operand b
   if constexpr (EDGE) gemm_pipe::store_bf16_edge(acc, c_tile, n, rows_a, rows_b, wave);
   else if constexpr (STAGED) gemm_pipe::store_bf16_staged(acc, smem, c_tile, n, wave);
   else gemm_pipe::store_bf16(acc, c_tile, n, wave);
+}
+
+// 256 x 256 tiles of the list entries blockIdx.x + i gridDim.x, one workgroup a CU.  A tile
+// of its own costs 8 us besides its products: its start, its first loads from memory, its
+// stores, which all tiles begin together, and the next workgroup's start.  Here the first
+// stages of a tile arrive while the one before is stored, and the stores drain during the
+// first steps (us, a workgroup a tile against this):
+//   8192 x 8192 x 512 44.4, 38.0    x 1024 61.5, 51.5   x 2048 84.3, 75.6   x 4096 131.2, 123.0
+//   x 8192 231.0, 221.9   x 16384 430.4, 418.9   5120 x 5120 x 4096 60.4, 59.1
+//   4096 x 8192 x 4096 68.6, 63.7   16384 x 16384 x 4096 548, 520   6144 x 6144 x 1024 40.8, 38.8
+// But where the stores go through LDS (staged_epilogue) they cannot overlap, and that is
+// worth more: 1024 x 57344 x 8192 220, 226; 4096 x 57344 x 8192 786, 801.
+// Whole tiles, an even number of panels.
+__global__ void __launch_bounds__(256, 1) gemm_mxfp4_rounds_kernel(Operand a, Operand b,
+                                                                   uint16_t* __restrict__ c,
+                                                                   uint32_t m, uint32_t n,
+                                                                   uint32_t panels, uint32_t xcds,
+                                                                   uint32_t tiles) {
+  extern __shared__ __attribute__((aligned(1024))) uint8_t smem[];
+  const uint32_t wave = gemm_pipe::wave_id();
+  const Operand& own = wave < 2u ? a : b;
+  uint32_t id = blockIdx.x, tm, tn;
+  auto place = [&](From* from) {
+    gemm_core::xcd_tile_order(id, m / 256u, n / 256u, xcds, &tm, &tn);
+    const uint64_t row_a = tm * 256u, row_b = tn * 256u;
+    from->a = a.codes + row_a * panels * kRow;
+    from->b = b.codes + row_b * panels * kRow;
+    from->scales = own.scales + (wave < 2u ? row_a : row_b) * 8u;
+  };
+  From from{};
+  place(&from);
+  const auto ar = code_rows<256>(a, 0u, 256u, panels), br = code_rows<256>(b, 0u, 256u, panels);
+  const Tile<8, 8, 2, true> tile(ar, br, scale_rows<256>(a, 0u), scale_rows<256>(b, 0u), panels,
+                                 smem);
+  uint16_t* c_tile = c + (uint64_t)tm * 256u * n + (uint64_t)tn * 256u;
+  tile.run_all(
+      from,
+      [&](From* to) {
+        id += gridDim.x;
+        if (id >= tiles) return false;
+        place(to);
+        return true;
+      },
+      [&](const Big::Acc& acc) {
+        uint32_t ld = n;
+        asm volatile("" : "+s"(ld));  // no addresses kept over the loop
+        gemm_pipe::store_bf16(acc, c_tile, ld, wave);
+        c_tile = c + (uint64_t)tm * 256u * n + (uint64_t)tn * 256u;
+      });
 }
 
 // 128 x 128 tiles: small grids, and (TAIL) the quarters of a last round (tile_plan.hpp).
@@ -367,7 +509,7 @@ int32_t set_tile_lds() {
   static const int32_t rc = [] {
     int32_t r = fe2o3_host::set_dynamic_lds(
         {(const void*)gemm_mxfp4_kernel<false, false>, (const void*)gemm_mxfp4_kernel<true, false>,
-         (const void*)gemm_mxfp4_kernel<false, true>},
+         (const void*)gemm_mxfp4_kernel<false, true>, (const void*)gemm_mxfp4_rounds_kernel},
         (int)Big::kSmem);
     if (r == FE2O3_OK)
       r = fe2o3_host::set_dynamic_lds({(const void*)gemm_mxfp4_128_kernel<2, true, false>,
@@ -412,9 +554,12 @@ int32_t launch_tiles(const Operand& a, const Operand& b, uint16_t* c, uint32_t m
     return plan.stages == 2 ? small(Two{}, std::false_type{}, plan.grid, 0u)
                             : small(Three{}, std::false_type{}, plan.grid, 0u);
   const unsigned big = (unsigned)plan.grid;
-  if (!whole)
+  const bool staged = gemm_core::staged_epilogue(((uint64_t)m + n) * panels * kRow);
+  if (whole && !staged && panels % 2u == 0u && big > topo.cus)
+    gemm_mxfp4_rounds_kernel<<<topo.cus, 256, Big::kSmem, s>>>(a, b, c, m, n, panels, topo.xcds, big);
+  else if (!whole)
     gemm_mxfp4_kernel<false, true><<<big, 256, Big::kSmem, s>>>(a, b, c, m, n, panels, topo.xcds);
-  else if (gemm_core::staged_epilogue(((uint64_t)m + n) * panels * kRow))
+  else if (staged)
     gemm_mxfp4_kernel<true, false><<<big, 256, Big::kSmem, s>>>(a, b, c, m, n, panels, topo.xcds);
   else
     gemm_mxfp4_kernel<false, false><<<big, 256, Big::kSmem, s>>>(a, b, c, m, n, panels, topo.xcds);
@@ -431,6 +576,7 @@ int32_t launch_tiles(const Operand& a, const Operand& b, uint16_t* c, uint32_t m
 const fe2o3_host::KernelRegistrar kRegistered[] = {
     FE2O3_MX("gemm_mxfp4_kernel", (gemm_mxfp4_kernel<false, false>), 256, Big::kSmem),
     FE2O3_MX("gemm_mxfp4_kernel<staged>", (gemm_mxfp4_kernel<true, false>), 256, Big::kSmem),
+    FE2O3_MX("gemm_mxfp4_rounds_kernel", gemm_mxfp4_rounds_kernel, 256, Big::kSmem),
     FE2O3_MX("gemm_mxfp4_kernel<edge>", (gemm_mxfp4_kernel<false, true>), 256, Big::kSmem),
     FE2O3_MX_128(2, true, false), FE2O3_MX_128(2, false, false), FE2O3_MX_128(2, true, true),
     FE2O3_MX_128(2, false, true), FE2O3_MX_128(3, true, false), FE2O3_MX_128(3, false, false),

@@ -245,6 +245,13 @@ def test_product_of_every_number_of_panels(gpu, m, n, panels):
     _check_product(gpu, m, n, 256 * panels)
 
 
+@pytest.mark.parametrize("m,n,k", [(5120, 5120, 512), (8192, 4096, 1024), (5120, 4864, 768)])
+def test_product_in_rounds(gpu, m, n, k):
+    """More whole tiles than a device has CUs, the last round part full or not; stages of k
+    that a round hands to the next, and (768) that it does not."""
+    _check_product(gpu, m, n, k)
+
+
 @pytest.mark.parametrize("m,n,k", [(20, 40, 600), (200, 300, 600), (2500, 2000, 512)])
 def test_product_scales_of_every_size(gpu, m, n, k):
     """Scales down to 2^-127 beside others, whose products are subnormal or vanish."""
