@@ -487,6 +487,19 @@ __global__ void __launch_bounds__(gemm_direct::kThreads, WIDE ? 2 : 4) gemm_mxfp
                                                   panels * (uint32_t)kRow, 1.0f, xcds, smem, s);
 }
 
+// Whether the direct kernel takes a product: by the rule of the other types, and few rows (of
+// k from eight units on) also whatever k is, once what they stream is more than a round of
+// tiles (us, the streamed operand from memory, tile against direct):
+//   16 x 40000 x 2048 18.4, 14.8    16 x 65536 x 2048 23.3, 22.7   x 4096 40.3, 35.2
+//   16 x 128256 x 2048 43.8, 37.7   x 4096 77.0, 62.9   1 x 128256 x 4096 73.8, 58.9
+//   32 x 128256 x 4096 75.6, 70.6   65536 x 16 x 4096 43.8, 33.7
+bool prefer_direct(uint32_t m, uint32_t n, uint32_t kbytes, uint32_t cus) {
+  const uint32_t rows = m > n ? m : n, few = m > n ? n : m;
+  return gemm_direct::prefer(m, n, kbytes, 1u, cus) ||
+         (few <= 32u && kbytes >= gemm_direct::kWaves * gemm_direct::kUnit &&
+          ((uint64_t)rows + 127u) / 128u > cus);
+}
+
 int32_t launch_direct(const gemm_direct::Launch& l, const Operand& a, const Operand& b,
                       uint16_t* c, uint32_t m, uint32_t n, uint32_t panels,
                       const tile_plan::Topology& topo, hipStream_t s) {
@@ -611,7 +624,7 @@ extern "C" int32_t fe2o3_gemm_mxfp4_nt(const uint8_t* a, uint64_t a_len, const u
   const Operand oa{a, a_scales, pa.scale_rows}, ob{b, b_scales, pb.scale_rows};
   if (k == 0u) return launch_direct(gemm_direct::plan_fill(c_len), oa, ob, c, m, n, 0u, topo, s);
   const uint32_t kbytes = pa.panels * (uint32_t)kRow;
-  if (gemm_direct::prefer(m, n, kbytes, 1u, topo.cus))
+  if (prefer_direct(m, n, kbytes, topo.cus))
     return launch_direct(gemm_direct::plan(m, n, kbytes, 1u, topo.cus), oa, ob, c, m, n, pa.panels,
                          topo, s);
   return launch_tiles(oa, ob, c, m, n, pa.panels, topo, s);

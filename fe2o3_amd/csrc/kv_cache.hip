@@ -1,10 +1,11 @@
 // kv_cache.hip -- a paged key-value cache on gfx950: new rows written into
 // their slots, copied, quantised to e4m3 with a scale per token and head, or to
-// microscaled 4-bit blocks of 32 (mxfp4.hpp), and cached rows of several sequences read back as packed bf16.
+// microscaled 4-bit blocks of 32 (mxfp4.hpp); and cached rows of several
+// sequences read back as packed bf16.
 //
 // Both are one pass over the rows, bound by memory: 32768 tokens of 8 heads, 128
-// wide, bf16 51 us = 5.2 TB/s, e4m3 41 us = 5.0; 16 sequences of 1 to 4097 read
-// back from e4m3 34 us = 6.0.  A row (token, head) of K and the same of V belong
+// wide, bf16 51 us = 5.2 TB/s, e4m3 41 us = 5.0, 4-bit 28 us = 6.0; 16 sequences
+// of 1 to 4097 read back from e4m3 34 us = 6.0, 8 of 4096 from 4-bit 28 us = 6.0.  A row (token, head) of K and the same of V belong
 // to a group of `lanes` adjacent lanes, a power of two, 8 elements each: 16 bytes
 // of bf16, 8 bytes of codes.  Adjacent groups take adjacent heads of a token, so
 // that a wave reads and writes runs of whole cache lines wherever heads are

@@ -1,9 +1,13 @@
 // mxfp4.hip -- matrices into the packed microscaled 4-bit form (mxfp4.hpp) and back.
 //
 // Both are one pass, bound by memory: a piece is a row's panel of 256 columns, 32 lanes
-// of eight columns, four lanes to a block of 32.  A workgroup takes 8 rows at a time of
+// of eight columns, four lanes to a block of 32.  A workgroup takes 8 or 16 rows of
 // one panel, so that the scales of neighbouring rows, which lie beside each other, come
 // from one workgroup; a wave's accesses of x are runs of 512 bytes (bf16).
+//
+// Measured: 14336 x 4096 of f32 into 4 bits 46 us = 5.8 TB/s, back 38 us = 7.0 (part of the
+// codes cached); 16384 x 4096 of bf16 28 us = 6.1 and 25 us = 6.9; 33 x 4096 2.1 each, as
+// any launch.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -81,19 +85,27 @@ struct Place {
   }
 };
 
-// U passes of 8 rows with all their loads in flight.
-template <class T, int U>
+// Rows of a workgroup: 32 bytes of x a thread in flight.  Of bf16 half or twice that takes
+// longer, of f32 twice (16384 x 4096 bf16: 30.8 | 28.1 | 28.4 us; 14336 x 4096 f32: 46.0 |
+// 49.7); only of few rows less (33 x 4096 bf16: 2.1 | 2.2).
+template <class T>
+constexpr uint32_t quantize_rows() {
+  return kPass * 4u / sizeof(T);
+}
+
+template <class T>
 __global__ void __launch_bounds__(kThreads) mxfp4_quantize_kernel(Args a) {
-  const Place at(a, U * kPass);
-  Eight<T> x[U];
+  constexpr uint32_t kRows = quantize_rows<T>(), kEach = kRows / kPass;
+  const Place at(a, kRows);
+  Eight<T> x[kEach];
 #pragma unroll
-  for (uint32_t u = 0; u < (uint32_t)U; ++u) {
+  for (uint32_t u = 0; u < kEach; ++u) {
     const uint32_t row = at.row + u * kPass;
     x[u].load((const T*)a.x + (row < a.rows ? row : 0u) * a.stride + at.col,
               row < a.rows ? at.left : 0u);
   }
 #pragma unroll
-  for (uint32_t u = 0; u < (uint32_t)U; ++u) {
+  for (uint32_t u = 0; u < kEach; ++u) {
     const uint32_t row = at.row + u * kPass;
     const uint32_t byte = mxfp4::scale_byte(mxfp4::quad_max(mxfp4::top8(x[u].v)));
     const uint32_t q = mxfp4::encode8(x[u].v, mxfp4::scale_float(byte));
@@ -107,76 +119,58 @@ __global__ void __launch_bounds__(kThreads) mxfp4_quantize_kernel(Args a) {
 
 // A store covers whole lines: 16 bytes a lane of neighbouring columns, eight of bf16, four of
 // f32 in either half of the panel (eight of f32 a lane, two stores 32 bytes apart: 14336 x
-// 4096 88 us, so 49).
-template <class T, int U>
+// 4096 88 us).  8 rows a workgroup (16, 32 rows: 38.1, 38.2, 40.7).
+template <class T>
 __global__ void __launch_bounds__(kThreads) mxfp4_dequantize_kernel(Args a) {
   constexpr uint32_t kParts = sizeof(T) / 2u, kEach = 8u / kParts;  // stores, columns of one
   using Codes = std::conditional_t<kParts == 1u, uint32_t, uint16_t>;
-  const Place at(a, U * kPass);
-  uint32_t q[U][kParts], byte[U][kParts];
+  const Place at(a, kPass);
+  if (at.row >= a.rows) return;
+  const uint8_t* codes =
+      a.q + ((uint64_t)at.row * a.panels.divisor + at.panel) * mxfp4::kRowBytes;
+  const uint8_t* scales = a.scales + at.panel * a.scale_panel + (uint64_t)at.row * 8u;
+  uint32_t q[kParts], byte[kParts];
 #pragma unroll
-  for (uint32_t u = 0; u < (uint32_t)U; ++u) {
-    const uint32_t row = min(at.row + u * kPass, a.rows - 1u);
-    const uint8_t* codes =
-        a.q + ((uint64_t)row * a.panels.divisor + at.panel) * mxfp4::kRowBytes;
-    const uint8_t* scales = a.scales + at.panel * a.scale_panel + (uint64_t)row * 8u;
-#pragma unroll
-    for (uint32_t h = 0; h < kParts; ++h) {
-      const uint32_t first = 128u * h + kEach * at.lane;
-      q[u][h] = *reinterpret_cast<const Codes*>(codes + first / 2u);
-      byte[u][h] = scales[first / mxfp4::kBlock];
-    }
+  for (uint32_t h = 0; h < kParts; ++h) {
+    const uint32_t first = 128u * h + kEach * at.lane;
+    q[h] = *reinterpret_cast<const Codes*>(codes + first / 2u);
+    byte[h] = scales[first / mxfp4::kBlock];
   }
 #pragma unroll
-  for (uint32_t u = 0; u < (uint32_t)U; ++u) {
-    const uint32_t row = at.row + u * kPass;
-    if (row >= a.rows) return;
+  for (uint32_t h = 0; h < kParts; ++h) {
+    const uint32_t col = at.panel * mxfp4::kPanel + 128u * h + kEach * at.lane;
+    const uint32_t n = col < a.cols ? min(a.cols - col, kEach) : 0u;
+    T* out = (T*)a.out + at.row * a.stride + col;
+    const float scale = mxfp4::scale_float(byte[h]);
+    if constexpr (kParts == 1u) {
+      const u32x4_t v = mxfp4::decode8_bf16(q[h], scale);
+      if (n == kEach) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any_t*>(out));
+      else
 #pragma unroll
-    for (uint32_t h = 0; h < kParts; ++h) {
-      const uint32_t col = at.panel * mxfp4::kPanel + 128u * h + kEach * at.lane;
-      const uint32_t n = col < a.cols ? min(a.cols - col, kEach) : 0u;
-      T* out = (T*)a.out + row * a.stride + col;
-      const float scale = mxfp4::scale_float(byte[u][h]);
-      if constexpr (kParts == 1u) {
-        const u32x4_t v = mxfp4::decode8_bf16(q[u][h], scale);
-        if (n == kEach) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any_t*>(out));
-        else
+        for (uint32_t i = 0; i < kEach - 1u; ++i)
+          if (i < n) out[i] = (T)(v[i / 2u] >> (16u * (i & 1u)));
+    } else {
+      float v[4];
+      mxfp4::decode4_f32(q[h], scale, v);
+      if (n == kEach)
+        __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]},
+                                    reinterpret_cast<f32x4_any_t*>(out));
+      else
 #pragma unroll
-          for (uint32_t i = 0; i < kEach - 1u; ++i)
-            if (i < n) out[i] = (T)(v[i / 2u] >> (16u * (i & 1u)));
-      } else {
-        float v[4];
-        mxfp4::decode4_f32(q[u][h], scale, v);
-        if (n == kEach)
-          __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]},
-                                      reinterpret_cast<f32x4_any_t*>(out));
-        else
-#pragma unroll
-          for (uint32_t i = 0; i < kEach - 1u; ++i)
-            if (i < n) out[i] = v[i];
-      }
+        for (uint32_t i = 0; i < kEach - 1u; ++i)
+          if (i < n) out[i] = v[i];
     }
   }
 }
 
-constexpr uint32_t kManyPasses = 4;
-
 template <class T>
-void launch(bool quantize, const Args& a, uint32_t grid_of_one, uint32_t cus, hipStream_t s) {
-  const auto grid = [](uint64_t n) {
-    const kv_cache::Grid g = kv_cache::Grid::of((uint32_t)n);
-    return dim3(g.x, g.y);
-  };
-  const uint64_t many = (((uint64_t)a.rows + kManyPasses * kPass - 1u) / (kManyPasses * kPass)) *
-                        a.panels.divisor;
-  // four passes a workgroup once these fill the device twice
-  if (many >= 2u * cus) {
-    if (quantize) mxfp4_quantize_kernel<T, kManyPasses><<<grid(many), kThreads, 0, s>>>(a);
-    else mxfp4_dequantize_kernel<T, kManyPasses><<<grid(many), kThreads, 0, s>>>(a);
-  } else {
-    if (quantize) mxfp4_quantize_kernel<T, 1><<<grid(grid_of_one), kThreads, 0, s>>>(a);
-    else mxfp4_dequantize_kernel<T, 1><<<grid(grid_of_one), kThreads, 0, s>>>(a);
-  }
+void launch(bool quantize, const Args& a, hipStream_t s) {
+  const uint32_t rows = quantize ? quantize_rows<T>() : kPass;
+  const kv_cache::Grid g =
+      kv_cache::Grid::of((uint32_t)(((uint64_t)a.rows + rows - 1u) / rows) * a.panels.divisor);
+  const dim3 grid(g.x, g.y);
+  if (quantize) mxfp4_quantize_kernel<T><<<grid, kThreads, 0, s>>>(a);
+  else mxfp4_dequantize_kernel<T><<<grid, kThreads, 0, s>>>(a);
 }
 
 int32_t run(bool quantize, const void* x, void* out, uint64_t x_len, uint32_t dtype, uint8_t* q,
@@ -198,9 +192,6 @@ int32_t run(bool quantize, const void* x, void* out, uint64_t x_len, uint32_t dt
   if (((uintptr_t)dense & (dtype == 0u ? 3u : 1u)) != 0u ||
       (((uintptr_t)q | (uintptr_t)scales) & 15u) != 0u)
     return FE2O3_ERR_ALIGNMENT;
-  tile_plan::Topology topo;
-  const int32_t rc = fe2o3_host::device_topology(&topo);
-  if (rc != FE2O3_OK) return rc;
   Args a;
   a.x = x;
   a.out = out;
@@ -211,21 +202,18 @@ int32_t run(bool quantize, const void* x, void* out, uint64_t x_len, uint32_t dt
   a.panels = FastDiv::of(p.panels);
   a.rows = rows;
   a.cols = cols;
-  if (dtype == 0u) launch<float>(quantize, a, (uint32_t)groups, topo.cus, s);
-  else launch<uint16_t>(quantize, a, (uint32_t)groups, topo.cus, s);
+  if (dtype == 0u) launch<float>(quantize, a, s);
+  else launch<uint16_t>(quantize, a, s);
   return fe2o3_host::after_launch();
 }
 
-#define FE2O3_MX(ENTRY, K, T, U) \
-  fe2o3_host::KernelRegistrar({ENTRY, #K "<" #T "," #U ">", (const void*)K<T, U>, kThreads, 0})
-#define FE2O3_MX_ALL(ENTRY, K) \
-  FE2O3_MX(ENTRY, K, float, 1), FE2O3_MX(ENTRY, K, float, 4), FE2O3_MX(ENTRY, K, uint16_t, 1), \
-  FE2O3_MX(ENTRY, K, uint16_t, 4)
+#define FE2O3_MX(ENTRY, K) \
+  fe2o3_host::KernelRegistrar({ENTRY, #K "<f32>", (const void*)K<float>, kThreads, 0}), \
+  fe2o3_host::KernelRegistrar({ENTRY, #K "<bf16>", (const void*)K<uint16_t>, kThreads, 0})
 const fe2o3_host::KernelRegistrar kRegistered[] = {
-    FE2O3_MX_ALL("fe2o3_quantize_mxfp4", mxfp4_quantize_kernel),
-    FE2O3_MX_ALL("fe2o3_dequantize_mxfp4", mxfp4_dequantize_kernel)};
+    FE2O3_MX("fe2o3_quantize_mxfp4", mxfp4_quantize_kernel),
+    FE2O3_MX("fe2o3_dequantize_mxfp4", mxfp4_dequantize_kernel)};
 #undef FE2O3_MX
-#undef FE2O3_MX_ALL
 
 }  // namespace
 

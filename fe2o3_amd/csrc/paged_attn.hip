@@ -41,7 +41,9 @@
 // 6.6 TB/s, and 4.6 of the join; 130001 keys of one sequence, 8 heads: 82 us and
 // 6; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 88 us = 6.3 TB/s, 4.8; 500
 // keys of one: 7.7 us.  48 query heads on one KV head, 48 sequences of 100 to 6000
-// keys: 21 us and 4.0, half of it starting, adding and ending.
+// keys: 21 us and 4.0, half of it starting, adding and ending.  4-bit rows (DecodeBlocks):
+// 64 sequences of 2 to 8190 keys, 32 heads on 8: 54 us = 5.2 TB/s, 5.0; 500 keys of one:
+// 6.7 us; 40 windows of 1024, 64 wide, 24 heads on 8: 10.6 us.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"

@@ -12,7 +12,9 @@
 //
 // Bound by memory: x is read once and written once.  A workgroup takes a few tokens, each
 // pair's sine and cosine is computed once for all heads and kept in LDS, and a lane turns
-// eight pairs, 16 bytes of bf16 on each side.
+// eight pairs, 16 bytes of bf16 on each side.  Measured: 16384 tokens of 32 + 8 heads of
+// 128, bf16, into other rows 60.5 us = 5.5 TB/s; 32 tokens 4.1, the chain of position,
+// frequency, sine, table and rows.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -252,14 +254,18 @@ extern "C" int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1* q, const Fe2o3RotaryRow
   a.turned = turned;
   a.cos_scale = scale;
   a.sin_scale = (flags & FE2O3_ROTARY_INVERSE) != 0u ? -scale : scale;
-  // a pair for every thread where the tokens still fill the device twice
+  // Tokens of a workgroup: two tasks for every thread, as far as a pair each and the device
+  // filled twice allow (us, a token | this | as many as have a pair for every thread):
+  //   2048 tokens of 32 + 8 heads, d 128 8.1 | 8.1 | 9.9   16384 of them 60.5 | 60.5 | 62.3
+  //   16384 of 8 + 1, d 64, 32 turned 18.7 | 9.9 | 9.9     16384 of 16 + 2, d 64 19.4 | 13.8 | 13.8
   tile_plan::Topology topo;
   rc = fe2o3_host::device_topology(&topo);
   if (rc != FE2O3_OK) return rc;
-  uint32_t per_wg = pairs < kThreads ? kThreads / pairs : 1u;
-  const uint32_t most = tokens / (2u * topo.cus);
-  if (per_wg > most) per_wg = most > 1u ? most : 1u;
-  a.per_wg = per_wg;
+  const uint32_t most[] = {kThreads / pairs, 2u * kThreads / (uint32_t)tasks,
+                           tokens / (2u * topo.cus)};
+  uint32_t per_wg = most[0];
+  for (const uint32_t n : most) per_wg = n < per_wg ? n : per_wg;
+  a.per_wg = per_wg = per_wg > 1u ? per_wg : 1u;
   const kv_cache::Grid g = kv_cache::Grid::of((tokens - 1u) / per_wg + 1u);
   const dim3 grid(g.x, g.y);
   hipStream_t s = (hipStream_t)stream;

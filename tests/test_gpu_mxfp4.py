@@ -245,6 +245,11 @@ def test_product_of_every_number_of_panels(gpu, m, n, panels):
     _check_product(gpu, m, n, 256 * panels)
 
 
+@pytest.mark.parametrize("m,n,k", [(20, 40000, 2048), (1, 66000, 2300), (36000, 17, 2048)])
+def test_product_streams_more_than_a_round(gpu, m, n, k):
+    _check_product(gpu, m, n, k)
+
+
 @pytest.mark.parametrize("m,n,k", [(5120, 5120, 512), (8192, 4096, 1024), (5120, 4864, 768)])
 def test_product_in_rounds(gpu, m, n, k):
     """More whole tiles than a device has CUs, the last round part full or not; stages of k
