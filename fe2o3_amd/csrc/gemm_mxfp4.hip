@@ -168,6 +168,7 @@ struct Tile {
   FE2O3_DEVICE void pick_scale(const u32x2_t (&raw)[kReads], Scales& s) const {
     uint32_t& to = R >= 1 && R <= CB ? s.b[R - 1] : s.a[R == 0 ? 0 : R - CB];
     to = __builtin_amdgcn_perm(raw[R][1], raw[R][0], ln.pick);
+    asm volatile("" : "+v"(to));  // here: moved to its use, it would be too near (mfma)
   }
 
   // Inline asm with the accumulator tied to the destination, as gemm_pipe::Bf16Mma's, and
