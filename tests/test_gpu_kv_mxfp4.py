@@ -524,3 +524,38 @@ def test_layer_steps_in_a_graph(gpu):
             mean = np.einsum("hgn,nhd->hgd", p, np.abs(x[:, 1])).reshape(heads, d)
             got = eager[0]["out"][s].double().cpu().numpy()
             assert np.all(np.abs(got - o) <= mean * 2.0 ** -7), turn
+
+
+def test_grid_of_two_dimensions(gpu):
+    """More workgroups than a grid's row has, one a head, against the same sequences in parts."""
+    torch = pytest.importorskip("torch")
+    k = _k()
+    seqs, heads, d, pages, page, cols = (1 << 18) + 3, 8, 64, 64, 16, 16
+    gen = torch.Generator(device="cuda").manual_seed(2)
+
+    def byte(*shape, low=0, high=256):
+        return torch.randint(low, high, shape, dtype=torch.uint8, device="cuda", generator=gen)
+
+    cache = k.KvCache(byte(pages, page, heads, d // 2), byte(pages, page, heads, d // 2),
+                      byte(pages, heads, page, d // 32, low=120, high=128),
+                      byte(pages, heads, page, d // 32, low=120, high=128))
+    q = torch.randn(seqs, heads, d, device="cuda", generator=gen).to(torch.bfloat16)
+    table = torch.randint(0, pages, (seqs, cols), dtype=torch.int32, device="cuda", generator=gen)
+    lengths = torch.randint(0, 41, (seqs,), dtype=torch.int32, device="cuda", generator=gen)
+    work = torch.empty(k.paged_attention_workspace_bytes(heads, heads, d), dtype=torch.uint8,
+                       device="cuda")
+    results = []
+    for step in (seqs, 1 << 17):
+        out = torch.full_like(q, 3.0)
+        lse = torch.full((seqs, heads), 3.0, device="cuda")
+        for at in range(0, seqs, step):
+            to = min(seqs, at + step)
+            # the last part by itself would be a call of one workgroup of eight waves a head
+            at = max(0, min(at, to - 1024))
+            k.paged_attention_decode(cache, q[at:to], table[at:to], lengths[at:to], out[at:to],
+                                     lse[at:to], work, max_length=page * cols, scale=0.125)
+        results.append((out, lse))
+    assert torch.equal(results[0][0], results[1][0]) and torch.equal(results[0][1], results[1][1])
+    empty = lengths == 0
+    assert not bool(results[0][0][empty].any())
+    assert bool(torch.isneginf(results[0][1][empty]).all())

@@ -353,3 +353,27 @@ def test_linear_on_tensors_streams_and_graphs(gpu):
         c.zero_()
         graph.replay()
         check()
+
+
+def test_packing_in_a_grid_of_two_dimensions(gpu):
+    """More workgroups than a grid's row has, against the same rows in parts."""
+    torch = pytest.importorskip("torch")
+    k = _k()
+    rows = 16 * (1 << 21) + 37
+    x = torch.randn(rows, 1, device="cuda").to(torch.bfloat16)
+    whole = [torch.full(s, 7, dtype=torch.uint8, device="cuda") for s in k.mxfp4_shapes(rows, 1)]
+    back = torch.empty_like(x)
+    k.quantize_mxfp4(x, *whole)
+    k.dequantize_mxfp4(*whole, back)
+    at = 0
+    while at < rows:
+        n = min(rows - at, 1 << 23)
+        part = [torch.empty(s, dtype=torch.uint8, device="cuda") for s in k.mxfp4_shapes(n, 1)]
+        values = torch.empty(n, 1, dtype=torch.bfloat16, device="cuda")
+        k.quantize_mxfp4(x[at:at + n], *part)
+        k.dequantize_mxfp4(*part, values)
+        assert torch.equal(part[0], whole[0][at:at + n])
+        assert torch.equal(part[1][:, :n], whole[1][:, at:at + n])
+        assert torch.equal(values, back[at:at + n])
+        at += n
+    assert bool((whole[1][:, rows:] == 7).all())

@@ -253,3 +253,19 @@ def test_more_tokens_than_a_grid_row(gpu):
     k.rotary(x, None, pos, freq)
     assert bool((x[:-77] == 1).all())
     assert torch.equal(x[-77:, 0].float().cpu(), torch.tensor([[-1.0, 1.0]]).repeat(77, 1))
+
+
+def test_grid_of_two_dimensions(gpu):
+    """More workgroups than a grid's row has, against the same tokens in parts."""
+    torch = pytest.importorskip("torch")
+    k = _k()
+    tokens, d = (1 << 21) + 37, 512
+    x = torch.randn(tokens, 1, d, device="cuda").to(torch.bfloat16)
+    positions = torch.randint(0, 1 << 20, (tokens,), dtype=torch.int32, device="cuda")
+    freq = torch.from_numpy(k.rotary_frequencies(d)[0]).cuda()
+    whole, part = torch.empty_like(x), torch.empty_like(x)
+    k.rotary(x, None, positions, freq, q_out=whole)
+    for at in range(0, tokens, 1 << 20):
+        to = min(tokens, at + (1 << 20))
+        k.rotary(x[at:to], None, positions[at:to], freq, q_out=part[at:to])
+    assert torch.equal(whole, part)
