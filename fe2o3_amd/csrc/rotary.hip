@@ -19,6 +19,8 @@
 #include "internal.hpp"
 #include "kv_cache.hpp"
 
+#include <type_traits>
+
 namespace {
 
 using namespace fe2o3;
@@ -28,7 +30,8 @@ constexpr int kThreads = 256;
 constexpr uint32_t kMaxPairs = 2048;
 constexpr uint32_t kTable = 2048;  // sines and cosines in LDS, 8 bytes each
 typedef uint32_t u32x4_any_t __attribute__((ext_vector_type(4), aligned(2)));
-typedef float f32x4_any_t __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_any_t __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32_any_t __attribute__((aligned(2)));
 
 // Rows of one of the two arrays, strides in elements.
 struct Rows {
@@ -45,85 +48,99 @@ struct Args {
   FastDiv heads;   // of both arrays
   FastDiv chunks;  // of a head: eight pairs each, then 16 copied elements each
   FastDiv pairs;
-  uint32_t tokens, per_wg, head_dim, turned;  // turned: chunks of pairs
+  FastDiv parts;   // workgroups that share a token's tasks
+  uint32_t tokens, per_wg, part_tasks, head_dim, turned;  // turned: chunks of pairs
   float cos_scale, sin_scale;  // the inverse has another sign of the sine
 };
 
-template <class T>
-struct Eight;
-template <>
-struct Eight<uint16_t> {
-  // the bits, those of a NaN too
-  static FE2O3_DEVICE void copy(const uint16_t* p, uint32_t n, uint16_t* out) {
-    if (n >= 8u) {
-      *reinterpret_cast<u32x4_any_t*>(out) = *reinterpret_cast<const u32x4_any_t*>(p);
-      return;
-    }
+// N elements (a power of two to 8) at any alignment of theirs, as 32-bit words; a single bf16
+// in the low half of one.
+template <class T, uint32_t N>
+struct Piece {
+  static constexpr uint32_t kBytes = N * sizeof(T), kWords = (kBytes + 3u) / 4u;
+  uint32_t w[kWords];
+  FE2O3_DEVICE void load(const T* p) {
+    if constexpr (kBytes == 2u) {
+      w[0] = *reinterpret_cast<const uint16_t*>(p);
+    } else if constexpr (kBytes == 4u) {
+      w[0] = *reinterpret_cast<const u32_any_t*>(p);
+    } else if constexpr (kBytes == 8u) {
+      const u32x2_t x = *reinterpret_cast<const u32x2_any_t*>(p);
+      w[0] = x[0];
+      w[1] = x[1];
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 7u; ++i)
-      if (i < n) out[i] = p[i];
-  }
-  static FE2O3_DEVICE void load(const uint16_t* p, uint32_t n, float (&v)[8]) {
-    if (n >= 8u) {
-      const u32x4_t w = *reinterpret_cast<const u32x4_any_t*>(p);
+      for (uint32_t i = 0; i < kWords; i += 4u) {
+        const u32x4_t x = reinterpret_cast<const u32x4_any_t*>(p)[i / 4u];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        v[i] = __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
-      return;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? f32_from_bf16_bits(p[i]) : 0.0f;
-  }
-  static FE2O3_DEVICE void store(uint16_t* p, uint32_t n, const float (&v)[8]) {
-    if (n >= 8u) {
-      *reinterpret_cast<u32x4_any_t*>(p) =
-          u32x4_t{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                  pack_bf16x2(v[6], v[7])};
-      return;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < 7u; ++i)
-      if (i < n) p[i] = bf16_bits_from_f32(v[i]);
-  }
-};
-template <>
-struct Eight<float> {
-  static FE2O3_DEVICE void copy(const float* p, uint32_t n, float* out) {
-    float v[8];
-    load(p, n, v);
-    store(out, n, v);
-  }
-  static FE2O3_DEVICE void load(const float* p, uint32_t n, float (&v)[8]) {
-    if (n >= 8u) {
-      const f32x4_t a = *reinterpret_cast<const f32x4_any_t*>(p);
-      const f32x4_t b = *reinterpret_cast<const f32x4_any_t*>(p + 4);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = a[i];
-        v[4 + i] = b[i];
+        for (uint32_t e = 0; e < 4u; ++e) w[i + e] = x[e];
       }
-      return;
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 8u; ++i) v[i] = i < n ? p[i] : 0.0f;
   }
-  static FE2O3_DEVICE void store(float* p, uint32_t n, const float (&v)[8]) {
-    if (n >= 8u) {
-      *reinterpret_cast<f32x4_any_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
-      *reinterpret_cast<f32x4_any_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
-      return;
-    }
+  FE2O3_DEVICE void store(T* p) const {
+    if constexpr (kBytes == 2u) {
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    } else if constexpr (kBytes == 4u) {
+      *reinterpret_cast<u32_any_t*>(p) = w[0];
+    } else if constexpr (kBytes == 8u) {
+      *reinterpret_cast<u32x2_any_t*>(p) = u32x2_t{w[0], w[1]};
+    } else {
 #pragma unroll
-    for (uint32_t i = 0; i < 7u; ++i)
-      if (i < n) p[i] = v[i];
+      for (uint32_t i = 0; i < kWords; i += 4u)
+        reinterpret_cast<u32x4_any_t*>(p)[i / 4u] = u32x4_t{w[i], w[i + 1], w[i + 2], w[i + 3]};
+    }
   }
 };
+template <uint32_t N, class T>
+FE2O3_DEVICE void load(const T* p, float* v) {
+  Piece<T, N> x;
+  x.load(p);
+#pragma unroll
+  for (uint32_t i = 0; i < N; ++i) {
+    if constexpr (sizeof(T) == 4u) v[i] = __uint_as_float(x.w[i]);
+    else v[i] = __uint_as_float(i & 1u ? x.w[i / 2u] & 0xffff0000u : x.w[i / 2u] << 16);
+  }
+}
+template <uint32_t N, class T>
+FE2O3_DEVICE void store(T* p, const float* v) {
+  Piece<T, N> x;
+#pragma unroll
+  for (uint32_t i = 0; i < Piece<T, N>::kWords; ++i) {
+    if constexpr (sizeof(T) == 4u) x.w[i] = __float_as_uint(v[i]);
+    else if constexpr (N == 1u) x.w[i] = bf16_bits_from_f32(v[0]);
+    else x.w[i] = pack_bf16x2(v[2u * i], v[2u * i + 1u]);
+  }
+  x.store(p);
+}
+template <uint32_t N, class T>
+FE2O3_DEVICE void copy(const T* p, T* out) {  // the bits, those of a NaN too
+  Piece<T, N> x;
+  x.load(p);
+  x.store(out);
+}
+
+// What a task calls for n of eight pairs, or elements: at<N>(place, first) for a piece of N
+// from the `first` one on, which are places place .. of eight; a part of eight goes in
+// pieces of four, two and one, in fixed registers.
+template <class At>
+FE2O3_DEVICE void pieces(uint32_t n, At at) {
+  using std::integral_constant;
+  if (n >= 8u) {
+    at(integral_constant<uint32_t, 8>{}, integral_constant<uint32_t, 0>{}, 0u);
+    return;
+  }
+  if ((n & 4u) != 0u) at(integral_constant<uint32_t, 4>{}, integral_constant<uint32_t, 0>{}, 0u);
+  if ((n & 2u) != 0u) at(integral_constant<uint32_t, 2>{}, integral_constant<uint32_t, 4>{}, n & 4u);
+  if ((n & 1u) != 0u) at(integral_constant<uint32_t, 1>{}, integral_constant<uint32_t, 6>{}, n & 6u);
+}
 
 template <class T, bool INTERLEAVED>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
   __shared__ __attribute__((aligned(16))) float2 table[kTable];
   __shared__ uint32_t skipped[kThreads];
-  const uint32_t first = (blockIdx.y * kv_cache::kGridWidth + blockIdx.x) * a.per_wg;
+  const uint32_t id = blockIdx.y * kv_cache::kGridWidth + blockIdx.x;
+  const uint32_t group = a.parts.div(id), part = id - group * a.parts.divisor;
+  const uint32_t first = group * a.per_wg;
   if (first >= a.tokens) return;  // the last row of a grid of two dimensions
   const uint32_t count = min(a.per_wg, a.tokens - first);
   const uint32_t pairs = a.pairs.divisor;
@@ -139,8 +156,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
   }
   __syncthreads();
   const uint32_t heads = a.heads.divisor, chunks = a.chunks.divisor;
-  const uint32_t tasks = count * heads * chunks;
-  for (uint32_t i = threadIdx.x; i < tasks; i += kThreads) {
+  const uint32_t end = min(count * heads * chunks, (part + 1u) * a.part_tasks);
+  for (uint32_t i = part * a.part_tasks + threadIdx.x; i < end; i += kThreads) {
     const uint32_t row = a.chunks.div(i), chunk = i - row * chunks;
     const uint32_t t = a.heads.div(row), h = row - t * heads;
     if (skipped[t]) continue;
@@ -149,41 +166,61 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(Args a) {
     const uint32_t head = second ? h - a.rows[0].heads : h;
     const T* x = (const T*)r.x + (first + t) * r.token_stride + head * r.head_stride;
     T* out = (T*)r.out + (first + t) * r.out_token_stride + head * r.out_head_stride;
-    float u[8], v[8];
     if (chunk < a.turned) {
-      const uint32_t p0 = 8u * chunk, n = min(pairs - p0, 8u);
-      // interleaved: elements 2 p0 .. + 15; halves: eight of each
-      const uint32_t at = INTERLEAVED ? 2u * p0 : p0, bt = INTERLEAVED ? at + 8u : pairs + p0;
-      const uint32_t na = INTERLEAVED ? min(2u * n, 8u) : n, nb = INTERLEAVED ? 2u * n - na : n;
-      Eight<T>::load(x + at, na, u);
-      Eight<T>::load(x + bt, nb, v);
-      float uo[8], vo[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float2 cs = table[t * pairs + min(p0 + j, pairs - 1u)];
-        if constexpr (INTERLEAVED) {
-          const float p = j < 4 ? u[2 * j & 7] : v[2 * j & 7];
-          const float q = j < 4 ? u[2 * j + 1 & 7] : v[2 * j + 1 & 7];
-          const float po = p * cs.x - q * cs.y, qo = q * cs.x + p * cs.y;
-          if (j < 4) {
-            uo[2 * j & 7] = po;
-            uo[2 * j + 1 & 7] = qo;
+      const uint32_t p0 = 8u * chunk;
+      auto turn = [&](auto number) {
+        const uint32_t n = number;
+        // the pairs' elements: of the halves eight each, or interleaved
+        float x_in[16] = {}, x_out[16];
+        pieces(n, [&](auto size, auto place, uint32_t from) {
+          constexpr uint32_t N = decltype(size)::value, P = decltype(place)::value;
+          if constexpr (INTERLEAVED && N == 8u) {
+            load<8>(x + 2u * p0, x_in);
+            load<8>(x + 2u * p0 + 8u, x_in + 8);
+          } else if constexpr (INTERLEAVED) {
+            load<2u * N>(x + 2u * (p0 + from), x_in + 2u * P);
           } else {
-            vo[2 * j & 7] = po;
-            vo[2 * j + 1 & 7] = qo;
+            load<N>(x + p0 + from, x_in + P);
+            load<N>(x + pairs + p0 + from, x_in + 8u + P);
           }
-        } else {
-          uo[j] = u[j] * cs.x - v[j] * cs.y;
-          vo[j] = v[j] * cs.x + u[j] * cs.y;
+          // keeps the pieces apart: merged, their registers would become an array in memory
+          asm volatile("; %0" : : "n"(N));
+        });
+        // the pair at place 4, and at 6
+        const uint32_t four = n >= 8u ? 4u : n & 4u, six = n >= 8u ? 6u : n & 6u;
+        const float2* turns = table + t * pairs + p0;
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; ++j) {
+          const uint32_t pair = min(j < 4u ? j : j < 6u ? four + j - 4u : six + j - 6u, n - 1u);
+          const float2 cs = turns[pair];
+          const uint32_t i0 = INTERLEAVED ? 2u * j : j, i1 = INTERLEAVED ? 2u * j + 1u : 8u + j;
+          const float p = x_in[i0], q = x_in[i1];
+          x_out[i0] = p * cs.x - q * cs.y;
+          x_out[i1] = q * cs.x + p * cs.y;
         }
-      }
-      Eight<T>::store(out + at, na, uo);
-      Eight<T>::store(out + bt, nb, vo);
+        pieces(n, [&](auto size, auto place, uint32_t from) {
+          constexpr uint32_t N = decltype(size)::value, P = decltype(place)::value;
+          if constexpr (INTERLEAVED && N == 8u) {
+            store<8>(out + 2u * p0, x_out);
+            store<8>(out + 2u * p0 + 8u, x_out + 8);
+          } else if constexpr (INTERLEAVED) {
+            store<2u * N>(out + 2u * (p0 + from), x_out + 2u * P);
+          } else {
+            store<N>(out + p0 + from, x_out + P);
+            store<N>(out + pairs + p0 + from, x_out + 8u + P);
+          }
+        });
+      };
+      if (pairs - p0 >= 8u) turn(std::integral_constant<uint32_t, 8>{});
+      else turn(pairs - p0);
     } else if (x != out) {
       const uint32_t at = 2u * pairs + 16u * (chunk - a.turned), n = min(a.head_dim - at, 16u);
-      const uint32_t na = min(n, 8u), nb = n - na;
-      Eight<T>::copy(x + at, na, out + at);
-      Eight<T>::copy(x + at + 8u, nb, out + at + 8u);
+#pragma unroll
+      for (uint32_t h = 0; h < 16u; h += 8u)
+        pieces(n > h ? min(n - h, 8u) : 0u, [&](auto size, auto, uint32_t from) {
+          constexpr uint32_t N = decltype(size)::value;
+          copy<N>(x + at + h + from, out + at + h + from);
+        });
     }
   }
 }
@@ -266,7 +303,15 @@ extern "C" int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1* q, const Fe2o3RotaryRow
   uint32_t per_wg = most[0];
   for (const uint32_t n : most) per_wg = n < per_wg ? n : per_wg;
   a.per_wg = per_wg = per_wg > 1u ? per_wg : 1u;
-  const kv_cache::Grid g = kv_cache::Grid::of((tokens - 1u) / per_wg + 1u);
+  // few tokens: their heads over as many workgroups as have tasks for all threads
+  // (SPLIT)
+  uint32_t parts = 2u * topo.cus / tokens;
+  const uint32_t most_parts = ((uint32_t)tasks - 1u) / kThreads + 1u;
+  parts = parts < most_parts ? parts : most_parts;
+  parts = parts > 1u ? parts : 1u;
+  a.parts = FastDiv::of(parts);
+  a.part_tasks = parts > 1u ? ((uint32_t)tasks - 1u) / parts + 1u : ~0u;
+  const kv_cache::Grid g = kv_cache::Grid::of(((tokens - 1u) / per_wg + 1u) * parts);
   const dim3 grid(g.x, g.y);
   hipStream_t s = (hipStream_t)stream;
   if ((flags & FE2O3_ROTARY_INTERLEAVED) != 0u) {
