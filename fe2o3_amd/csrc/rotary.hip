@@ -13,8 +13,8 @@
 // Bound by memory: x is read once and written once.  A workgroup takes a few tokens, each
 // pair's sine and cosine is computed once for all heads and kept in LDS, and a lane turns
 // eight pairs, 16 bytes of bf16 on each side.  Measured: 16384 tokens of 32 + 8 heads of
-// 128, bf16, into other rows 60.5 us = 5.5 TB/s; 32 tokens 4.1, the chain of position,
-// frequency, sine, table and rows.
+// 128, bf16, into other rows 59 us = 5.7 TB/s; 32 tokens 2.9, the chain of position,
+// frequency, sine, table and rows.  18 pairs of such a head, which end in a part of eight, 94.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -293,8 +293,8 @@ extern "C" int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1* q, const Fe2o3RotaryRow
   a.sin_scale = (flags & FE2O3_ROTARY_INVERSE) != 0u ? -scale : scale;
   // Tokens of a workgroup: two tasks for every thread, as far as a pair each and the device
   // filled twice allow (us, a token | this | as many as have a pair for every thread):
-  //   2048 tokens of 32 + 8 heads, d 128 8.1 | 8.1 | 9.9   16384 of them 60.5 | 60.5 | 62.3
-  //   16384 of 8 + 1, d 64, 32 turned 18.7 | 9.9 | 9.9     16384 of 16 + 2, d 64 19.4 | 13.8 | 13.8
+  //   2048 tokens of 32 + 8 heads, d 128 7.8 | 7.8 | 8.7   16384 of them 59.0 | 59.3 | 62.0
+  //   16384 of 8 + 1, d 64, 32 turned 16.4 | 9.4 | 9.7     16384 of 16 + 2, d 64 17.5 | 13.3 | 13.4
   tile_plan::Topology topo;
   rc = fe2o3_host::device_topology(&topo);
   if (rc != FE2O3_OK) return rc;
@@ -303,8 +303,9 @@ extern "C" int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1* q, const Fe2o3RotaryRow
   uint32_t per_wg = most[0];
   for (const uint32_t n : most) per_wg = n < per_wg ? n : per_wg;
   a.per_wg = per_wg = per_wg > 1u ? per_wg : 1u;
-  // few tokens: their heads over as many workgroups as have tasks for all threads
-  // (SPLIT)
+  // few tokens: their heads over as many workgroups as have tasks for all threads (us, one a
+  // token and this: 1 token of 160 heads, d 128 17.1, 3.5; 32 of 40 4.1, 2.9; 111 of 256
+  // 13.3, 5.0)
   uint32_t parts = 2u * topo.cus / tokens;
   const uint32_t most_parts = ((uint32_t)tasks - 1u) / kThreads + 1u;
   parts = parts < most_parts ? parts : most_parts;
