@@ -77,3 +77,11 @@ def test_whole_rounds_and_a_tail(gpu, m, n, k):
     """Two whole rounds, and two with a last part round as quarters (three stages or two);
     k that ends within a panel."""
     _check_exact(m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", [(512, 24576, 16384), (1024, 24576, 16384), (24576, 768, 16128)])
+def test_staged_stores(gpu, m, n, k):
+    """Operands of 192 MiB and more, whose tiles store C through LDS: less than a round, and a
+    round with a tail of two stages, and of three under a tall C and an odd number of panels."""
+    assert (m + n) * (-(-k // 256) * 128) >= 192 << 20
+    _check_exact(m, n, k)
