@@ -85,3 +85,93 @@ def test_staged_stores(gpu, m, n, k):
     round with a tail of two stages, and of three under a tall C and an odd number of panels."""
     assert (m + n) * (-(-k // 256) * 128) >= 192 << 20
     _check_exact(m, n, k)
+
+
+# more than 128 tiles of 256 x 256, where they run as such: whole tiles, and edges on both sides
+ONE_ROUND = [(3328, 2816), (3300, 2801)]
+
+
+@pytest.mark.parametrize("k", [256, 512, 700, 1280, 1536, 2304, 3328])
+@pytest.mark.parametrize("m,n", ONE_ROUND)
+def test_one_round(gpu, m, n, k):
+    _check_exact(m, n, k)
+
+
+@pytest.mark.parametrize("m,n", [*ONE_ROUND, (5120, 5120), (8192, 4096)])
+@pytest.mark.parametrize("offset", [1, 4, 8])
+def test_c_at_any_element_of_large_tiles(gpu, m, n, offset):
+    """Whole tiles whose C is not at 16 bytes (8 elements are) end as edge tiles do."""
+    _check_exact(m, n, 1024, offset)
+
+
+# and in rounds with quarters behind or not, on small tiles, and split over a workgroup's waves
+# (the last three: few tiles, a few rows of a wide C, a few columns of a tall one)
+EVERY_WAY = [*ONE_ROUND, (5120, 5120), (6144, 6144), (1300, 1200), (300, 1100), (20, 4096),
+             (4096, 17)]
+
+
+@pytest.mark.parametrize("m,n", EVERY_WAY)
+def test_nan_scales_of_large_tiles(gpu, m, n):
+    """A NaN block makes NaN of its row or column and of nothing else: in the first, a middle
+    and the last panel, in every block of a panel."""
+    panels = 4
+    a, b = _operand(m, 256 * panels, 1), _operand(n, 256 * panels, 2)
+    gen = torch.Generator(device="cpu").manual_seed(m)
+    rows = torch.randperm(m, generator=gen)[:min(m // 2, 24)].tolist() + [0, m - 1]
+    cols = torch.randperm(n, generator=gen)[:min(n // 2, 24)].tolist() + [n - 1]
+    for i, row in enumerate(rows):
+        a[1][i % panels, row, i // 3 % 8] = 255
+    for i, col in enumerate(cols):
+        b[1][(i + 1) % panels, col, i // 3 % 8] = 255
+    got = torch.isnan(_product(a, b))
+    want = torch.zeros_like(got)
+    want[rows] = True
+    want[:, cols] = True
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("m,n", EVERY_WAY)
+def test_scales_of_every_size_of_large_tiles(gpu, m, n):
+    """Scales down to 2^-127 beside others up to 2^125, whose products are subnormal or vanish.
+    The bound: half a bf16 step of the result, for each of k additions 2^-24 of the sum of
+    magnitudes, and what vanishes below the normal range."""
+    k = 1024
+    a, b = _operand(m, k, 3, 60, 190), _operand(n, k, 4, 60, 190)
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    low, high = a[1][:, :m // 2], b[1][:, :n // 2]
+    low.copy_(torch.randint(0, 3, low.shape, generator=gen, device="cuda"))
+    high.copy_(torch.randint(120, 253, high.shape, generator=gen, device="cuda"))
+    x, y = _unpack(*a), _unpack(*b)
+    got = _product(a, b).double()
+    want = torch.matmul(x, y.T.contiguous())
+    total = torch.matmul(x.abs(), y.abs().T.contiguous())
+    bound = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -7) + total * k * 2.0 ** -24 + 2.0 ** -126
+    fine = total < 2.0 ** 127  # others may overflow on the way
+    assert float(fine.double().mean()) > 0.5
+    assert bool((~fine | ((got - want).abs() <= bound)).all())
+
+
+def test_every_tile_has_the_same_bits(gpu):
+    """Rows of one product in tiles one after another with a last round of quarters, and the
+    same rows of smaller products: in rounds alone, in one round of whole tiles and of edge
+    tiles, in quarters' tiles of two stages and of three.  Scales of 14 octaves, so that sums
+    round on the way and another order would show."""
+    k = 2048
+    a, b = _operand(8192, k, 5, 118, 132), _operand(5120, k, 6, 118, 132)
+    whole = _product(a, b)
+
+    def rows(x, first, count):
+        up = (count + 15) // 16 * 16
+        return x[0][first:first + count].contiguous(), x[1][:, first:first + up].contiguous()
+
+    x, y = _unpack(*rows(a, 0, 256)), _unpack(*b)
+    want = torch.matmul(x, y.T.contiguous())
+    total = torch.matmul(x.abs(), y.abs().T.contiguous())
+    bound = want.abs() * 2.0 ** -8 * (1 + 2.0 ** -7) + total * k * 2.0 ** -24
+    assert bool(((whole[:256].double() - want).abs() <= bound).all())
+    for first, count, cols in [(0, 5120, 5120), (4096, 4096, 5120), (1024, 1792, 5120),
+                               (16, 1790, 5001), (6896, 1296, 5120), (7888, 300, 5120),
+                               (32, 301, 4999)]:
+        got = _product(rows(a, first, count), rows(b, 0, cols))
+        same = got.view(torch.int16) == whole[first:first + count, :cols].view(torch.int16)
+        assert bool(same.all()), (first, count, cols, int((~same).sum()))
