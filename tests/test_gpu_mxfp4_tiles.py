@@ -175,3 +175,11 @@ def test_every_tile_has_the_same_bits(gpu):
         got = _product(rows(a, first, count), rows(b, 0, cols))
         same = got.view(torch.int16) == whole[first:first + count, :cols].view(torch.int16)
         assert bool(same.all()), (first, count, cols, int((~same).sum()))
+
+
+@pytest.mark.parametrize("m,n,k", [(4300, 4900, 700), (4300, 4100, 1300), (4480, 4864, 1280),
+                                   (4224, 4224, 512)])
+def test_edges_and_a_tail(gpu, m, n, k):
+    """A round of edge tiles and a last round of quarters, of two stages or three; the last two
+    have whole quarters all the same."""
+    _check_exact(m, n, k)
