@@ -9,10 +9,11 @@
 //   code of x: the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 to |x| / scale, ties to the
 //   even code, 6 at most, and x's sign in bit 3.
 //
-// gfx950's conversions compute both directions: over all 2^16 bf16 values, the f32
-// values beside them and every scale exponent, 0 (2^-127) among them, their codes and
-// values are the formula's, and scale byte 255 in a float's exponent field gives NaN.
-// They read a float's exponent field alone, so a scale byte takes one shift.
+// gfx950's conversions compute both directions, and the tests go through what decides a
+// code: all bf16 values under each largest exponent, so on every scale, 2^-127 among them;
+// of f32 the three values on either side of each border on every scale; and back, every
+// code on every scale byte, of which 255 in a float's exponent field gives NaN.  They read
+// a float's exponent field alone, so a scale byte takes one shift.
 #pragma once
 
 #include <stdint.h>
