@@ -522,7 +522,9 @@ inline bool in_order(uint32_t m, uint32_t n, uint32_t k, uint32_t elem_bytes) {
 }
 
 // 64 rows of K within 32-bit byte offsets, as the chosen forms need
-inline bool k_fits(uint32_t k, uint32_t elem_bytes) { return 64ull * k * elem_bytes < (1ull << 32); }
+constexpr bool k_fits(uint32_t k, uint32_t elem_bytes) {
+  return 64ull * k * elem_bytes < (1ull << 32);
+}
 
 constexpr uint32_t smem_of(uint32_t mb, uint32_t nb) {
   return kWaves * 1024u * (mb * nb > 2u * (mb + nb) ? mb * nb : 2u * (mb + nb));
@@ -587,7 +589,9 @@ FE2O3_DEVICE void run_form(int form, const uint8_t* a, const uint8_t* b, uint16_
       case 5: FE2O3_DIRECT(4, 1, 3);
       case 6: FE2O3_DIRECT(2, 4, T::kDeep);
       case 7: FE2O3_DIRECT(4, 2, T::kDeep);
-      case kInOrder:  // this and the last for operands at any alignment, of any K
+      // this and the last for operands at any alignment, of any K: no plan of a type of
+      // blocks has them, whose K fits (gemm_mxfp4.hip)
+      case kInOrder:
         if constexpr (!T::kBlocks)
           block<T, 2, 2, 2, uint32_t, true>(a, b, c, m, n, k, scale, xcds, smem);
         return;

@@ -501,6 +501,10 @@ bool prefer_direct(uint32_t m, uint32_t n, uint32_t kbytes, uint32_t cus) {
           ((uint64_t)rows + 127u) / 128u > cus);
 }
 
+// The forms for any K leave C as it is for this type: every k has to fit the others.
+static_assert(gemm_direct::k_fits(mxfp4::kMaxPanels * (uint32_t)kRow, 1u),
+              "more panels would plan a form that this type lacks");
+
 int32_t launch_direct(const gemm_direct::Launch& l, const Operand& a, const Operand& b,
                       uint16_t* c, uint32_t m, uint32_t n, uint32_t panels,
                       const tile_plan::Topology& topo, hipStream_t s) {
