@@ -264,11 +264,9 @@ extern "C" int32_t fe2o3_rotary(const Fe2o3RotaryRowsV1* q, const Fe2o3RotaryRow
     return FE2O3_ERR_SHAPE;
   if (q->heads == 0u || (k && k->heads == 0u)) return FE2O3_ERR_SHAPE;
   const uint32_t turned = (pairs + 7u) / 8u;
-  const uint64_t chunks = turned + ((uint64_t)(head_dim - rotary_dim) + 15u) / 16u;
-  uint64_t tasks;  // of one token
-  if (!kv_cache::mul_ok(heads, chunks, &tasks) || tasks >= (UINT64_C(1) << 22) ||
-      tokens >= (1u << 31))
-    return FE2O3_ERR_SHAPE;
+  const uint64_t chunks = FE2O3_ROTARY_PIECES(1u, head_dim, rotary_dim);
+  const uint64_t tasks = heads * chunks;  // of one token: below 2^33 times 2^29
+  if (tasks >= (UINT64_C(1) << 22) || tokens >= (1u << 31)) return FE2O3_ERR_SHAPE;
   if (positions_len != tokens || freq_len != pairs) return FE2O3_ERR_LENGTH;
   if (tokens == 0u) return FE2O3_OK;
   Args a{};

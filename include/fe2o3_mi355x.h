@@ -473,13 +473,18 @@ int32_t fe2o3_paged_attention_decode(const Fe2o3KvCacheV1 *cache, const uint16_t
  * or do not overlap.  k may be NULL (q alone).  dtype 0 = f32, 1 = bf16 bits, of all.
  * Errors in this order: NULL q record FE2O3_ERR_NULL; another dtype or flag, rotary_dim
  * 0, odd, above head_dim or above 4096, a scale that is not finite, an array of no heads,
- * heads * (head_dim / 16) of 2^22 or more, or 2^31 tokens FE2O3_ERR_SHAPE; positions_len
+ * FE2O3_ROTARY_PIECES of 2^22 or more (the heads of Q and K together), or 2^31 tokens
+ * FE2O3_ERR_SHAPE; positions_len
  * or freq_len FE2O3_ERR_LENGTH; strides with which rows share elements FE2O3_ERR_STRIDE
  * (FE2O3_ERR_OVERFLOW where an extent passes 64 bits); lengths short of the extent
  * FE2O3_ERR_LENGTH; FE2O3_ERR_NULL; arrays off their elements' alignment
  * FE2O3_ERR_ALIGNMENT. */
 #define FE2O3_ROTARY_INTERLEAVED 1u
 #define FE2O3_ROTARY_INVERSE 2u
+/* pieces of a token: eight pairs of a head each, then 16 copied elements each */
+#define FE2O3_ROTARY_PIECES(heads, head_dim, rotary_dim) \
+  ((uint64_t)(heads) * (((uint64_t)(rotary_dim) + 15u) / 16u + \
+                        ((uint64_t)(head_dim) - (rotary_dim) + 15u) / 16u))
 typedef struct Fe2o3RotaryRowsV1 {
   const void *x;
   uint64_t x_len;
