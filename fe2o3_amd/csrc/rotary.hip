@@ -8,7 +8,10 @@
 //
 // An angle reaches 10^6 radians, where 32 bits are off by 0.06, so it is taken in turns:
 // position * (freq / 2 pi) in 64 bits, less its nearest whole number, is off by 2^-52 of
-// the turns (2^-34 of one at 10^6 radians); sine and cosine of what is left are f32.
+// the turns (2^-34 of one at 10^6 radians).  Sine and cosine of what is left, times the
+// scale, are f32: a few units of 2^-24 off, far below a bf16 output's rounding.  f32 outputs
+// are off by 6e-8 (rms, of 64 bits), where the rounding alone would be 2.5e-8, and by 1.8e-7
+// of their pair's magnitudes at the most (three ranges of positions up to 10^6).
 //
 // Bound by memory: x is read once and written once.  A workgroup takes a few tokens, each
 // pair's sine and cosine is computed once for all heads and kept in LDS, and a lane turns

@@ -465,8 +465,10 @@ int32_t fe2o3_paged_attention_decode(const Fe2o3KvCacheV1 *cache, const uint16_t
  * pairs (i, i + rotary_dim / 2), or with FE2O3_ROTARY_INTERLEAVED (2 i, 2 i + 1); the
  * rest of a head is copied.  FE2O3_ROTARY_INVERSE turns by -t_i: the transposed map, for
  * gradients.  freq: rotary_dim / 2 doubles on the device, any schedule of a stretched
- * context; angles are taken in 64 bits, products and sums in fp32, rounded once.  A token
- * at position FE2O3_KV_NO_SLOT (a padded row) is skipped: its outputs keep their bytes.
+ * context.  Angles are taken in 64 bits; their sine and cosine times scale, the products
+ * and the sum are fp32, off by at most 2^-21 |scale| (|a| + |b|) together, and the result
+ * is rounded once.  A token at position FE2O3_KV_NO_SLOT (a padded row) is skipped: its
+ * outputs keep their bytes.
  *
  * Row (t, h) of an array lies at t * token_stride + h * head_stride elements of x, its
  * result likewise in out; x and out are the same rows (one pointer, the same strides)
