@@ -748,7 +748,10 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, *, factor: float 
                   fastest keeps its speed
       "by_turns"  pairs of fast_turns and more over original_length keep their speed,
                   those of slow_turns and fewer are factor times slower, a straight line
-                  between; the scale is 0.1 ln(factor) + 1
+                  in the turns between, as Peng, Quesnelle, Fan and Shippole publish it
+                  (YaRN, 2023); the scale is 0.1 ln(factor) + 1.  A model whose program
+                  draws that line over the pairs' numbers has other angles: make their
+                  table as it does, rotary() takes any
     """
     if rotary_dim <= 0 or rotary_dim % 2:
         raise ValueError("rotary_dim must be positive and even")

@@ -2,10 +2,12 @@
 macro says, compiled as a C program's.  A size below it fails on the length given."""
 from __future__ import annotations
 
+import math
 import os
 import shutil
 import subprocess
 
+import numpy as np
 import pytest
 
 from test_rotary_host import LENGTH, ROOT, SHAPE, _call, _rows
@@ -45,3 +47,22 @@ def test_largest_token(pieces, head_dim, rotary_dim):
     assert _call(lib, q=_rows(heads=0xFFFFFFFF), k=_rows(heads=0xFFFFFFFF), **size) == SHAPE
     assert _call(lib, q=_rows(heads=0xFFFFFFFF), k=_rows(heads=0xFFFFFFFF), head_dim=0xFFFFFFFF,
                  rotary_dim=2, freq_len=2) == SHAPE
+
+
+@pytest.mark.parametrize("slow,fast", [(1.0, 32.0), (0.0, 4.0), (2.0, 64.0)])
+def test_a_line_in_turns(slow, fast):
+    """Between slow_turns and fast_turns a pair's speed is a straight line in its turns, not in
+    its number."""
+    from fe2o3_amd import kernels
+    plain = kernels.rotary_frequencies(128)[0]
+    got = kernels.rotary_frequencies(128, factor=8.0, schedule="by_turns", slow_turns=slow,
+                                     fast_turns=fast)[0]
+    turns = 4096 * plain / (2 * math.pi)
+    inner = (turns > slow) & (turns < fast)
+    assert inner.sum() > 3
+    share = (got - plain / 8) / (plain - plain / 8)  # of the plain speed
+    assert np.allclose(share[inner], (turns[inner] - slow) / (fast - slow), rtol=1e-12, atol=1e-12)
+    number = np.arange(64)[inner]
+    along = (number[-1] - number) / (number[-1] - number[0])
+    assert np.abs(share[inner] - along * (share[inner][0] - share[inner][-1])
+                  - share[inner][-1]).max() > 0.05
