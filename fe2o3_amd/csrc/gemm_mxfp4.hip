@@ -13,11 +13,20 @@
 // tile's rows (2 KiB for 256), copied behind the stage's codes.  A lane reads a row's
 // eight with one ds_read_b64 and keeps its block's of both substeps in one register.
 //
-// Measured: 8192 x 8192 x 8192 221 us = 4.98 PFLOP/s.  The instruction alone, from registers,
-// sustains 7.1 on codes of normal values, where power limits it (9.6 on zeros, on which this
-// kernel reaches 6.5); the loop keeps the matrix core busy for three quarters of its cycles.
+// Measured: 8192 x 8192 x 8192 210-225 us in calls and replays = 4.9-5.2 PFLOP/s, by the box
+// and its power (237 over wider values, median of a traced run 242).  The instruction alone,
+// from registers, sustains 6.3-7.4 by the box on codes of normal values, where power limits
+// it, and 9.6 on zeros, on which this kernel takes 169 us: three quarters of it in the loop
+// either way (8192 k more take 198 us of 149, on zeros 151 of 114), and 4 us a round of tiles
+// besides.  The loop waits for its copies: waves spend 19% of their time at the wait and the
+// barrier for the next stage, of which LDS holds two (68 KiB each), and 25% waiting to issue.
+// LDS is no limit: busy 21%, no conflicts, and without the reads of scales 207-209 us for 213.
 // 16 x 14336 x 4096 9.0 us with the weights from memory (3.5 TB/s), 5.6 from the caches;
-// 4096 x 4096 x 4096 37.6.
+// 4096 x 4096 x 4096 33-38.
+//
+// A tile's steps follow one another, so that few tiles take the steps' time whatever their
+// number: 128 and 256 rows by 8192 x 8192 24 us (64 and 128 workgroups of 32 steps of 0.58 us,
+// 0.2 of it products), from the caches 18; 512 rows 25 (0.8 a step).
 #include "common.hpp"
 #include "gemm_core.hpp"
 #include "gemm_direct.hpp"
@@ -494,6 +503,16 @@ __global__ void __launch_bounds__(gemm_direct::kThreads, WIDE ? 2 : 4) gemm_mxfp
 //   16 x 40000 x 2048 18.4, 14.8    16 x 65536 x 2048 23.3, 22.7   x 4096 40.3, 35.2
 //   16 x 128256 x 2048 43.8, 37.7   x 4096 77.0, 62.9   1 x 128256 x 4096 73.8, 58.9
 //   32 x 128256 x 4096 75.6, 70.6   65536 x 16 x 4096 43.8, 33.7
+// The other types' rule (gemm_direct::prefer) on 4-bit operands, so measured, by cost:
+//   2  1 x 4096 x 4096 11.1, 4.5    4  64 x 4096 x 1024 6.1, 4.1    x 4096 11.4, 5.9
+//   4  32 x 8192 x 8192 19.8, 11.5  4  64 x 4096 x 16384 35.2, 15.1
+//   5  16 x 14336 x 4096 14.1, 10.0 6  64 x 8192 x 1024 6.3, 4.8    x 8192 20.6, 14.9
+//   6  256 x 2048 x 4096 11.6, 7.2  6  128 x 4096 x 16384 40.7, 20.0
+//   9  16 x 20000 x 512 5.5, 5.2    x 4096 15.2, 12.0
+//   10 16 x 28672 x 4096 17.1, 17.5 x 1024 7.3, 8.8 (goes to direct)
+//   12 128 x 8192 x 1024 6.9, 7.3   x 4096 14.6, 15.1   x 16384 42.5, 37.0 (goes to the tile)
+//   12 32 x 20000 x 4096 15.3, 17.0 32 x 28672 x 1024 7.2, 8.9   x 4096 17.1, 19.3
+//   12 64 x 14336 x 4096 14.5, 16.4 512 x 2048 x 4096 11.8, 12.2   8192 x 128 x 4096 14.4, 17.3
 bool prefer_direct(uint32_t m, uint32_t n, uint32_t kbytes, uint32_t cus) {
   const uint32_t rows = m > n ? m : n, few = m > n ? n : m;
   return gemm_direct::prefer(m, n, kbytes, 1u, cus) ||
@@ -548,6 +567,12 @@ int32_t set_tile_lds() {
 
 int32_t launch_tiles(const Operand& a, const Operand& b, uint16_t* c, uint32_t m, uint32_t n,
                      uint32_t panels, const tile_plan::Topology& topo, hipStream_t s) {
+  // The plan's lines on 4-bit operands (us, all in tiles of 128, in tiles of 256 in rounds, and
+  // as planned where that is neither):
+  //   2048 x 2048 x 4096 15.5, 27.7   2816 x 2816 x 1024 11.2, 15.2   x 8192 39.9, 50.1
+  //   1024 x 8192 x 8192 46, 52       1024 x 9216 x 8192 72, 55
+  //   3328 x 2816 x 1024 15.1, 15.3   x 4096 35.4, 31.4   4096 x 2560 x 4096 35.3, 31.4
+  //   4352 x 4096 x 1024 21.5, 24.1, a round and quarters 22.0   x 4096 54.4, 56.2, 46.9
   const tile_plan::Plan plan = tile_plan::plan(m, n, topo);
   if (plan.grid > 0x7fffffffu || plan.tail_grid > 0x7fffffffu) return FE2O3_ERR_SHAPE;
   const int32_t lds_rc = set_tile_lds();

@@ -42,8 +42,9 @@
 // 6; 64 sequences of 2 to 8190 keys, 8 heads, e4m3: 88 us = 6.3 TB/s, 4.8; 500
 // keys of one: 7.7 us.  48 query heads on one KV head, 48 sequences of 100 to 6000
 // keys: 21 us and 4.0, half of it starting, adding and ending.  4-bit rows (DecodeBlocks):
-// 64 sequences of 2 to 8190 keys, 32 heads on 8: 54 us = 5.2 TB/s, 5.0; 500 keys of one:
-// 6.7 us; 40 windows of 1024, 64 wide, 24 heads on 8: 10.6 us.
+// 64 sequences of 2 to 8190 keys, 32 heads on 8: 54 us = 5.2 TB/s, 5.0 (65 and 6 over caches
+// that the last call did not read); 500 keys of one: 6.7 us; 40 windows of 1024, 64 wide, 24
+// heads on 8: 10.6 us.
 #include "common.hpp"
 #include "internal.hpp"
 #include "kv_cache.hpp"
@@ -988,7 +989,12 @@ struct DecodeBlocks : Decode<D, kMxfp4, 1, 1, WH, W, true> {
 };
 
 // How a form works on its tiles: 4-bit codes of one row tile by DecodeBlocks, C subtiles'
-// scores side by side.
+// scores side by side.  More query heads go the way of a bf16 cache, widened into LDS, one KV
+// head a workgroup: of heads in token order it takes whole lines of 128 bytes for rows that
+// are half of one, or 64 wide a quarter (64 sequences of 2 to 8190 keys, 8 KV heads: 560 MB
+// for 290, or 147).  Times with the join over caches that alternate, by query heads a KV head,
+// 128 wide and 64: 8 78 and 46 us, 16 84 and 48, 17 106 and 88, 32 110 and 89, 48 137 and 104,
+// 64 154 and 108 (there the conversions count as well, VALU 62-66%).
 template <uint32_t F, int RT>
 constexpr uint32_t keys_of() {
   return F == kMxfp4 && RT == 1 ? kBlockKeys : kKeys;
