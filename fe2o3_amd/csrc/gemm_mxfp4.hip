@@ -13,10 +13,10 @@
 // tile's rows (2 KiB for 256), copied behind the stage's codes.  A lane reads a row's
 // eight with one ds_read_b64 and keeps its block's of both substeps in one register.
 //
-// Measured: 8192 x 8192 x 8192 210-225 us in calls and replays = 4.9-5.2 PFLOP/s, by the box
-// and its power (237 over wider values, median of a traced run 242).  The instruction alone,
-// from registers, sustains 6.3-7.4 by the box on codes of normal values, where power limits
-// it, and 9.6 on zeros, on which this kernel takes 169 us: three quarters of it in the loop
+// Measured: 8192 x 8192 x 8192 210-237 us in calls and replays = 4.6-5.2 PFLOP/s, by the card
+// and its power (median of a traced run 242).  The instruction alone, from registers, sustains
+// 6.3-7.4 by the card on codes of normal values, where power limits it, and 9.6 on zeros, on
+// which this kernel takes 169-176 us: three quarters of it in the loop
 // either way (8192 k more take 198 us of 149, on zeros 151 of 114), and 4 us a round of tiles
 // besides.  The loop waits for its copies: waves spend 19% of their time at the wait and the
 // barrier for the next stage, of which LDS holds two (68 KiB each), and 25% waiting to issue.
